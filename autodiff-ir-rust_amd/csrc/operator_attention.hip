@@ -1,0 +1,232 @@
+// Attention on device arrays: checks of arguments, workspace, the choice of kernels.
+#include "operator_attention.hpp"
+
+#include <cmath>
+
+namespace adhip {
+namespace {
+
+using attn::Params;
+
+// Smallest and largest document of every kRange positions, so that a tile whose documents cannot meet is passed over
+// without a look at its positions: a wavefront for two entries.
+__global__ __launch_bounds__(256) void document_ranges_kernel(const int* q, int64_t qb, int64_t ql, int Lq, int2* qr, int qn, const int* k,
+                                                              int64_t kb, int64_t kl, int Lk, int2* kr, int kn) {
+    const int blocks = (qn + kn + 7) / 8, lane = threadIdx.x & 31;
+    const int64_t b = blockIdx.x / blocks;
+    const int entry = (int)(blockIdx.x - b * blocks) * 8 + (threadIdx.x >> 5);
+    const bool of_keys = entry >= qn;
+    const int e = of_keys ? entry - qn : entry;
+    if (of_keys && e >= kn) return;
+    const int i = e * attn::kRange + lane;
+    const int d = i >= (of_keys ? Lk : Lq) ? -1 : of_keys ? k[b * kb + i * kl] : q[b * qb + i * ql];
+    int lo = d >= 0 ? d : 0x7fffffff, hi = d;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+        lo = min(lo, __shfl_xor(lo, s));
+        hi = max(hi, __shfl_xor(hi, s));
+    }
+    if (lane == 0) (of_keys ? kr + (int64_t)b * kn : qr + (int64_t)b * qn)[e] = int2{lo, max(hi, -1)};
+}
+
+attn::Tensor tensor_of(const adhip_array& a) {
+    const int chunk = 16 / type_bytes(a.type);
+    attn::Tensor t = {a.data, a.strides[0], a.strides[1], a.strides[2], 0};
+    t.vec = vector_elements(a, chunk) == chunk && a.dims[3] % chunk == 0;
+    return t;
+}
+
+size_t rounded(size_t n) { return (n + 255) & ~size_t(255); }
+
+// How a call is cut up, and where its workspace's parts begin.
+struct Layout {
+    bool few_rows;
+    int row_tile, tiles, splits;
+    size_t qrange, krange, part, part_ml, delta, bytes;
+};
+
+Layout layout_of(const adhip_attention_args& g, bool backward) {
+    Layout y = {};
+    const int64_t B = g.q.dims[0], Lq = g.q.dims[1], H = g.q.dims[2], D = g.q.dims[3], Lk = g.k.dims[1], Hk = g.k.dims[2];
+    const int64_t R = Hk > 0 ? Lq * (H / Hk) : 0;
+    // One wavefront's 32 columns hold all rows of a key head: the wavefronts of a workgroup go along the keys.
+    y.few_rows = R <= 32;
+    y.row_tile = y.few_rows ? 32 : 128;
+    y.tiles = (int)((R + y.row_tile - 1) / y.row_tile);
+    // Ranges of keys: as many as give every compute unit two workgroups, none shorter than two tiles of keys.
+    const int64_t blocks = (int64_t)y.tiles * Hk * B, keys = y.few_rows ? 128 : 64;
+    y.splits = 1;
+    if (blocks > 0 && blocks < 256) {
+        const int64_t want = (512 + blocks - 1) / blocks, most = (Lk + 2 * keys - 1) / (2 * keys);
+        y.splits = (int)std::max<int64_t>(1, std::min(std::min(want, most), (int64_t)256));
+    }
+    size_t at = 0;
+    // (whether documents are given or not: what a call needs goes by shapes alone)
+    y.qrange = at;
+    at += rounded((size_t)(B * ((Lq + attn::kRange - 1) / attn::kRange)) * sizeof(int2));
+    y.krange = at;
+    at += rounded((size_t)(B * ((Lk + attn::kRange - 1) / attn::kRange)) * sizeof(int2));
+    size_t forward = at, back = at;
+    if (y.splits > 1) {
+        y.part = forward;
+        forward += rounded((size_t)(y.splits * B * Hk * R * D) * 4);
+        y.part_ml = forward;
+        forward += rounded((size_t)(y.splits * B * Hk * R * 2) * 4);
+    }
+    y.delta = back;
+    if (backward) back += rounded((size_t)(B * Hk * R) * 4);
+    y.bytes = std::max(forward, back);
+    return y;
+}
+
+void check_sizes(const char* op, const adhip_attention_args& g) {
+    ADHIP_CHECK(g.q.type == ADHIP_F32 || g.q.type == ADHIP_BF16, "%s: q is %s, f32 or bf16 is wanted", op, type_name(g.q.type));
+    check_array(op, "q", g.q, g.q.type, 4);
+    check_array(op, "k", g.k, g.q.type, 4);
+    check_array(op, "v", g.v, g.q.type, 4);
+    const int64_t B = g.q.dims[0], Lq = g.q.dims[1], H = g.q.dims[2], D = g.q.dims[3], Lk = g.k.dims[1], Hk = g.k.dims[2];
+    check_dims(op, "k", g.k, {B, Lk, Hk, D});
+    check_dims(op, "v", g.v, {B, Lk, Hk, D});
+    ADHIP_CHECK(D >= 1 && D <= 256, "%s: heads of %lld features, 1 to 256 are supported", op, (long long)D);
+    ADHIP_CHECK(Hk >= 1 && H >= 1 && H % Hk == 0, "%s: %lld heads cannot share %lld key heads", op, (long long)H, (long long)Hk);
+    // positions and rows in 32 bits, with room for a window on either side
+    constexpr int64_t kMost = int64_t(1) << 28;
+    ADHIP_CHECK(Lq <= kMost && Lk <= kMost && Lq * (H / Hk) <= kMost && B * H <= kMost, "%s: q %s and k %s are too large", op, array_str(g.q).c_str(),
+                array_str(g.k).c_str());
+    ADHIP_CHECK(B * Hk * ((Lq * (H / Hk) + 31) / 32 + (Lk + 31) / 32) <= kMost, "%s: q %s and k %s are too large", op, array_str(g.q).c_str(),
+                array_str(g.k).c_str());
+}
+
+Params checked(const char* op, const adhip_attention_args& g, const Layout& y, bool backward) {
+    const int64_t B = g.q.dims[0], Lq = g.q.dims[1], H = g.q.dims[2], D = g.q.dims[3], Lk = g.k.dims[1], Hk = g.k.dims[2];
+    auto tensor = [&](const char* name, const adhip_array& a, std::initializer_list<int64_t> dims, bool output) {
+        check_array(op, name, a, g.q.type, 4);
+        check_dims(op, name, a, dims);
+        check_packed_rows(op, name, a);
+        if (output) check_distinct(op, name, a);
+        return tensor_of(a);
+    };
+    Params p = {};
+    p.q = tensor("q", g.q, {B, Lq, H, D}, false);
+    p.k = tensor("k", g.k, {B, Lk, Hk, D}, false);
+    p.v = tensor("v", g.v, {B, Lk, Hk, D}, false);
+    p.out = tensor("out", g.out, {B, Lq, H, D}, !backward);
+    check_array(op, "lse", g.lse, ADHIP_F32, 3);
+    check_dims(op, "lse", g.lse, {B, Lq, H});
+    if (!backward) check_distinct(op, "lse", g.lse);
+    p.lse = (float*)g.lse.data;
+    p.lse_b = g.lse.strides[0], p.lse_l = g.lse.strides[1], p.lse_h = g.lse.strides[2];
+    if (backward) {
+        p.dout = tensor("out_grad", g.out_grad, {B, Lq, H, D}, false);
+        p.dq = tensor("q_grad", g.q_grad, {B, Lq, H, D}, true);
+        p.dk = tensor("k_grad", g.k_grad, {B, Lk, Hk, D}, true);
+        p.dv = tensor("v_grad", g.v_grad, {B, Lk, Hk, D}, true);
+    }
+    if (g.slopes.data) {
+        check_array(op, "slopes", g.slopes, ADHIP_F32, 1);
+        check_dims(op, "slopes", g.slopes, {H});
+        p.slopes = (const float*)g.slopes.data;
+        p.slope_stride = g.slopes.strides[0];
+    }
+    if (g.lengths.data) {
+        check_array(op, "lengths", g.lengths, ADHIP_I32, 1);
+        check_dims(op, "lengths", g.lengths, {B});
+        p.lengths = (const int*)g.lengths.data;
+        p.lengths_s = g.lengths.strides[0];
+    }
+    if (g.prefix.data) {
+        check_array(op, "prefix", g.prefix, ADHIP_I32, 1);
+        check_dims(op, "prefix", g.prefix, {B});
+        p.prefix = (const int*)g.prefix.data;
+        p.prefix_s = g.prefix.strides[0];
+    }
+    const bool documents = g.query_documents.data || g.key_documents.data;
+    if (documents) {
+        check_array(op, "query_documents", g.query_documents, ADHIP_I32, 2);
+        check_array(op, "key_documents", g.key_documents, ADHIP_I32, 2);
+        check_dims(op, "query_documents", g.query_documents, {B, Lq});
+        check_dims(op, "key_documents", g.key_documents, {B, Lk});
+        p.qdoc = (const int*)g.query_documents.data;
+        p.kdoc = (const int*)g.key_documents.data;
+        p.qdoc_b = g.query_documents.strides[0], p.qdoc_l = g.query_documents.strides[1];
+        p.kdoc_b = g.key_documents.strides[0], p.kdoc_l = g.key_documents.strides[1];
+    }
+    ADHIP_CHECK(std::isfinite(g.scale), "%s: the scale is not finite", op);
+    ADHIP_CHECK(std::isfinite(g.cap) && g.cap >= 0.f, "%s: the cap must be 0 (none) or positive, and finite", op);
+    ADHIP_CHECK(g.window >= 0, "%s: the window must be 0 (none) or positive", op);
+    ADHIP_CHECK(g.workspace_bytes >= y.bytes && (g.workspace || y.bytes == 0), "%s: a workspace of %zu bytes is given, %zu are needed", op,
+                g.workspace ? (size_t)g.workspace_bytes : (size_t)0, y.bytes);
+    ADHIP_CHECK((uintptr_t)g.workspace % 256 == 0, "%s: the workspace is not aligned to 256 bytes", op);
+    char* const room = (char*)g.workspace;
+    if (documents) {
+        p.qrange = (const int2*)(room + y.qrange);
+        p.krange = (const int2*)(room + y.krange);
+        p.qranges = (int)((Lq + attn::kRange - 1) / attn::kRange);
+        p.kranges = (int)((Lk + attn::kRange - 1) / attn::kRange);
+    }
+    p.B = (int)B, p.Lq = (int)Lq, p.Lk = (int)Lk, p.Hk = (int)Hk, p.G = (int)(H / Hk), p.D = (int)D, p.R = (int)(Lq * (H / Hk));
+    p.scale = g.scale;
+    p.cap = g.cap;
+    p.causal = g.causal != 0;
+    p.window = (int)std::min<int64_t>(g.window, int64_t(1) << 30);
+    p.tiles = y.tiles;
+    p.splits = y.splits;
+    p.part = (float*)(room + y.part);
+    p.part_ml = (float*)(room + y.part_ml);
+    p.delta = (float*)(room + y.delta);
+    return p;
+}
+
+void document_ranges(const Params& p, hipStream_t stream) {
+    const int entries = p.qranges + p.kranges;
+    if (!p.qdoc || entries == 0 || p.B == 0) return;
+    document_ranges_kernel<<<(unsigned)((entries + 7) / 8 * p.B), 256, 0, stream>>>(
+        p.qdoc, p.qdoc_b, p.qdoc_l, p.Lq, (int2*)p.qrange, p.qranges, p.kdoc, p.kdoc_b, p.kdoc_l, p.Lk, (int2*)p.krange, p.kranges);
+    check_launch("adhip_attention");
+}
+
+}  // namespace
+}  // namespace adhip
+
+using namespace adhip;
+
+extern "C" {
+
+int adhip_attention_workspace(adhip_ctx* ctx, const adhip_attention_args* args, int backward, size_t* bytes) {
+    return context_guarded(ctx, [&] {
+        const char* op = "adhip_attention_workspace";
+        ADHIP_CHECK(args && bytes, "%s: no arguments", op);
+        check_sizes(op, *args);
+        *bytes = layout_of(*args, backward != 0).bytes;
+    });
+}
+
+int adhip_attention(adhip_ctx* ctx, const adhip_attention_args* args, void* stream) {
+    return context_guarded(ctx, [&] {
+        const char* op = "adhip_attention";
+        ADHIP_CHECK(args, "%s: no arguments", op);
+        check_sizes(op, *args);
+        const Layout y = layout_of(*args, false);
+        const Params p = checked(op, *args, y, false);
+        if (p.R == 0 || p.B == 0) return;
+        document_ranges(p, (hipStream_t)stream);
+        if (args->q.type == ADHIP_BF16) attn::forward_bf16(p, y.few_rows, (hipStream_t)stream);
+        else attn::forward_f32(p, y.few_rows, (hipStream_t)stream);
+    });
+}
+
+int adhip_attention_backward(adhip_ctx* ctx, const adhip_attention_args* args, void* stream) {
+    return context_guarded(ctx, [&] {
+        const char* op = "adhip_attention_backward";
+        ADHIP_CHECK(args, "%s: no arguments", op);
+        check_sizes(op, *args);
+        const Layout y = layout_of(*args, true);
+        const Params p = checked(op, *args, y, true);
+        if (p.B == 0) return;
+        document_ranges(p, (hipStream_t)stream);
+        if (args->q.type == ADHIP_BF16) attn::backward_bf16(p, (hipStream_t)stream);
+        else attn::backward_f32(p, (hipStream_t)stream);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,358 @@
+// Attention forward: softmax in one pass over the keys with a running maximum and sum (Milakov and Gimelshein 2018; Dao et
+// al. 2022), the scores never leave the registers.
+//
+// A wavefront owns 32 rows and multiplies keys by rows (S^T = K Q^T) and values by probabilities (O^T = V^T P^T), so that a
+// lane holds one row of the softmax, 16 keys of every 32: its maximum takes one exchange between the lane's halves, its
+// sum none until the end, and its rescaling is one factor a lane.
+//
+// WQ wavefronts along the rows, WK along the keys of a tile of BK.  Many rows: four wavefronts own 128 rows and share each
+// tile of keys.  Few rows (one token a sequence): four wavefronts share 32 rows and split each tile of keys, the keys are
+// split over workgroups beside that, and the parts are joined, with their maxima and sums, in LDS and by a second kernel.
+#pragma once
+#include "operator_attention.hpp"
+
+namespace adhip {
+namespace attn {
+
+// AHEAD 0: a tile is loaded when it is needed; 1: one tile ahead in registers, one LDS tile; 2: one ahead, two LDS tiles
+template <class T, int DP, int WQ_, int WK_, int BK_, int AHEAD_>
+struct ForwardConfig {
+    static constexpr int WQ = WQ_, WK = WK_, BK = BK_, AHEAD = AHEAD_;
+    static constexpr int NT = 64 * WQ * WK, BQ = 32 * WQ, KB = BK / (32 * WK);
+    static constexpr int kTile = BK * Lds<T, DP>::kPitch;
+    static constexpr int kBufs = AHEAD == 2 ? 2 : 1;
+    static constexpr int kMerge = WK > 1 ? WK * 32 * (DP + 4) * 4 + WK * 64 * 4 : 0;
+    static constexpr int kLoop = kBufs * (2 * kTile * (int)sizeof(T) + BK * 4);
+    static constexpr int kBytes = kLoop > kMerge ? kLoop : kMerge;
+};
+
+template <class T, int DP, class C>
+__global__ __launch_bounds__(C::NT) void forward_kernel(const Params p) {
+    typedef Matrix<T> M;
+    typedef typename M::Frag Frag;
+    __shared__ __attribute__((aligned(16))) char lds[C::kBytes];
+    T* const ks = (T*)lds;                                         // [bufs][BK][pitch]
+    T* const vs = ks + C::kBufs * C::kTile;
+    int* const docs = (int*)(vs + C::kBufs * C::kTile);            // [bufs][BK]
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = wave % C::WQ, wk = wave / C::WQ;
+
+    // this workgroup's tile of rows (the last ones, which see most keys, first), key head, sequence and range of keys
+    const int total = p.tiles * p.splits * p.Hk * p.B;
+    int id = by_die(blockIdx.x, total);
+    if ((int)(blockIdx.x >> 3) >= (total + 7) / 8 || id >= total) return;
+    const int tile = p.tiles - 1 - id % p.tiles;
+    id /= p.tiles;
+    const int split = id % p.splits;
+    id /= p.splits;
+    const int c = id % p.Hk, b = id / p.Hk;
+
+    const int n = sequence_length(p, b), offset = n - p.Lq;
+    const int prefix = p.prefix ? min(max(p.prefix[b * p.prefix_s], 0), n) : 0;
+    const Band band(p);
+    const Scoring sc(p);
+    const int row0 = tile * C::BQ, row1 = min(row0 + C::BQ, p.R) - 1;
+    const int first = row0 / p.G, last = row1 / p.G;  // tokens of the tile
+
+    // the lane's row
+    const int row = row0 + wq * 32 + (lane & 31);
+    const bool valid = row < p.R;
+    const int token = valid ? row / p.G : 0, head = c * p.G + (valid ? row - token * p.G : 0);
+    const int at = token + offset;
+    int lo = at - band.below, hi = at + band.above, pre = prefix;
+    const int doc = p.qdoc && valid ? p.qdoc[b * p.qdoc_b + token * p.qdoc_l] : 0;
+    if (!valid || doc < 0) lo = 1, hi = 0, pre = 0;
+    const float slope = p.slopes && valid ? p.slopes[head * p.slope_stride] * kLog2e : 0.f;
+
+    Frag qf[DP / 16];
+    {
+        const T* q = (const T*)p.q.data + b * p.q.b + token * p.q.l + head * p.q.h;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) qf[s] = load_frag(q, s * 16 + half * 8, p.D, p.q.vec, valid);
+    }
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) o[d] = zero16();
+    float m = -__builtin_inff(), l = 0.f;
+
+    // tiles of keys that some row of this workgroup sees
+    const int n_tiles = (n + C::BK - 1) / C::BK, per = (n_tiles + p.splits - 1) / p.splits;
+    const int t_begin = split * per, t_end = min(t_begin + per, n_tiles);
+    const int hi_all = last + offset + band.above, lo_all = first + offset - band.below;
+    const int2* const kr = p.krange ? p.krange + (int64_t)b * p.kranges : nullptr;
+    int2 mine = {0, 0};
+    if (kr) mine = document_range(p.qrange + (int64_t)b * p.qranges, first, last);
+    auto needed = [&](int t) {
+        const int j0 = t * C::BK, j1 = min(j0 + C::BK, n) - 1;
+        if (j0 >= prefix && (j0 > hi_all || j1 < lo_all)) return false;
+        if (!kr) return true;
+        const int2 theirs = document_range(kr, j0, j1);
+        return theirs.x <= mine.y && mine.x <= theirs.y;
+    };
+    Tiles<decltype(needed)> tiles(needed, t_begin, t_end);
+
+    const T* const kb = (const T*)p.k.data + b * p.k.b + c * p.k.h;
+    const T* const vb = (const T*)p.v.data + b * p.v.b + c * p.v.h;
+    const int* const kd = p.kdoc ? p.kdoc + b * p.kdoc_b : nullptr;
+    Stage<T, DP, C::BK, C::NT> sk, sv;
+    int sd = 0;
+    // keys behind the sequence or of no document are zero, whatever the arrays hold there
+    auto used = [&](int j) { return j < n && !(kd && kd[j * p.kdoc_l] < 0); };
+    auto load_k = [&](int j0) { sk.load([&](int i) { return used(j0 + i) ? kb + (j0 + i) * p.k.l : (const T*)nullptr; }, p.D, p.k.vec, tid); };
+    auto load_v = [&](int j0) { sv.load([&](int i) { return used(j0 + i) ? vb + (j0 + i) * p.v.l : (const T*)nullptr; }, p.D, p.v.vec, tid); };
+    auto load_d = [&](int j0) { if (kd && tid < C::BK) sd = j0 + tid < n ? kd[(j0 + tid) * p.kdoc_l] : -1; };
+    auto load = [&](int t) {
+        load_k(t * C::BK);
+        load_v(t * C::BK);
+        load_d(t * C::BK);
+    };
+    static_assert(C::NT >= C::BK, "one thread a key for the documents");
+    auto store_d = [&](int buf) { if (kd && tid < C::BK) docs[buf * C::BK + tid] = sd; };
+    auto store = [&](int buf) {
+        sk.store(ks + buf * C::kTile, tid);
+        sv.store(vs + buf * C::kTile, tid);
+        store_d(buf);
+    };
+
+    int t = tiles.next(lane), buf = 0;
+    if (C::AHEAD && t >= 0) load(t);
+    if (C::AHEAD == 2) {
+        if (t >= 0) store(0);
+        __syncthreads();
+    }
+    while (t >= 0) {
+        const int next = tiles.next(lane);
+        if (C::AHEAD == 2) {
+            if (next >= 0) load(next);
+        } else if (C::AHEAD == 1) {
+            __syncthreads();
+            store(0);
+            __syncthreads();
+            if (next >= 0) load(next);
+        } else {
+            __syncthreads();
+            load_k(t * C::BK);
+            sk.store(ks, tid);
+            load_v(t * C::BK);
+            sv.store(vs, tid);
+            load_d(t * C::BK);
+            store_d(0);
+            __syncthreads();
+        }
+        const T* kt = ks + buf * C::kTile;
+        const T* vt = vs + buf * C::kTile;
+        const int* dt = docs + buf * C::BK;
+        f32x16 s[C::KB];
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int x = 0; x < C::KB; ++x) {
+            const int key0 = (wk * C::KB + x) * 32;
+            s[x] = zero16();
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) s[x] = M::mma(rows_frag<T, DP>(kt, key0, k, lane), qf[k], s[x]);
+            const int j0 = t * C::BK + key0, jl = j0 + 4 * half;
+            if (p.cap > 0.f) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[x][i] = tanh_of(s[x][i] * sc.cap_in) * sc.cap_out;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[x][i] *= sc.scale2;
+            }
+            if (p.slopes) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[x][i] -= slope * fabsf((float)(at - jl - c_row(i)));
+            }
+            // masks only where some row of the wavefront does not see all 32 keys
+            if (kd || !__all(j0 + 31 < n && ((lo <= j0 && j0 + 31 <= hi) || j0 + 31 < pre))) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int j = jl + c_row(i);
+                    bool sees = j < n && (j < pre || (lo <= j && j <= hi));
+                    if (kd) sees = sees && dt[key0 + 4 * half + c_row(i)] == doc;
+                    s[x][i] = sees ? s[x][i] : -__builtin_inff();
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][i]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float m_new = fmaxf(m, top), base = m_new == -__builtin_inff() ? 0.f : m_new;
+        if (__any(m_new > m)) {
+            const float a = __builtin_amdgcn_exp2f(m - base);
+            l *= a;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= a;
+            m = m_new;
+        }
+#pragma unroll
+        for (int x = 0; x < C::KB; ++x) {
+            const int key0 = (wk * C::KB + x) * 32;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[x][i] = __builtin_amdgcn_exp2f(s[x][i] - base);
+                l += s[x][i];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                Frag f;
+                to_frag(s[x], h, f);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) o[d] = M::mma(cols_frag<DP>(vt, key0 + 16 * h, d * 32, lane), f, o[d]);
+            }
+        }
+        if (C::AHEAD == 2) {
+            buf ^= 1;
+            if (next >= 0) store(buf);
+            __syncthreads();
+        }
+        t = next;
+    }
+    l += __shfl_xor(l, 32);
+
+    const int64_t rows_before = (((int64_t)split * p.B + b) * p.Hk + c) * p.R;
+    if (C::WK == 1) {
+        if (!valid) return;
+        if (p.splits > 1) {
+            float* part = p.part + (rows_before + row) * p.D;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float f[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+                    store4(part, d * 32 + 8 * g + 4 * half, p.D, (p.D & 3) == 0, f);
+                }
+            if (half == 0) {
+                p.part_ml[(rows_before + row) * 2] = m;
+                p.part_ml[(rows_before + row) * 2 + 1] = l;
+            }
+            return;
+        }
+        const float r = l > 0.f || l != l ? 1.f / l : 0.f;
+        T* out = (T*)p.out.data + b * p.out.b + token * p.out.l + head * p.out.h;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float f[4] = {o[d][4 * g] * r, o[d][4 * g + 1] * r, o[d][4 * g + 2] * r, o[d][4 * g + 3] * r};
+                store4(out, d * 32 + 8 * g + 4 * half, p.D, p.out.vec, f);
+            }
+        if (half == 0) p.lse[b * p.lse_b + token * p.lse_l + head * p.lse_h] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+        return;
+    }
+    // join the wavefronts' parts: every one scales its own to the common maximum, then all add up
+    __syncthreads();
+    float* const so = (float*)lds;                                // [WK][32][DP + 4]
+    float* const sm = so + C::WK * 32 * (DP + 4);                 // [WK][32] maxima, [WK][32] sums
+    if (half == 0) sm[wk * 32 + lane] = m;
+    __syncthreads();
+    float all = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < C::WK; ++w) all = fmaxf(all, sm[w * 32 + (lane & 31)]);
+    const float a = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - all);
+    if (half == 0) sm[C::WK * 32 + wk * 32 + lane] = l * a;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float* to = so + (wk * 32 + (lane & 31)) * (DP + 4) + d * 32 + 8 * g + 4 * half;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[e] = o[d][4 * g + e] * a;
+        }
+    __syncthreads();
+    for (int i = tid; i < 32 * (DP / 4); i += C::NT) {
+        const int rr = i / (DP / 4), d = i % (DP / 4) * 4, gr = row0 + rr;
+        if (gr >= p.R) break;
+        float f[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f, mm = -__builtin_inff();
+#pragma unroll
+        for (int w = 0; w < C::WK; ++w) {
+            const float* from = so + (w * 32 + rr) * (DP + 4) + d;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] += from[e];
+            sum += sm[C::WK * 32 + w * 32 + rr];
+            mm = fmaxf(mm, sm[w * 32 + rr]);
+        }
+        if (p.splits > 1) {
+            store4(p.part + (rows_before + gr) * p.D, d, p.D, (p.D & 3) == 0, f);
+            if (d == 0) {
+                p.part_ml[(rows_before + gr) * 2] = mm;
+                p.part_ml[(rows_before + gr) * 2 + 1] = sum;
+            }
+            continue;
+        }
+        const int tk = gr / p.G, hd = c * p.G + gr - tk * p.G;
+        const float r = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] *= r;
+        store4((T*)p.out.data + b * p.out.b + tk * p.out.l + hd * p.out.h, d, p.D, p.out.vec, f);
+        if (d == 0) p.lse[b * p.lse_b + tk * p.lse_l + hd * p.lse_h] = (mm + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+}
+
+// Joins the ranges of keys: a wavefront a row.
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(const Params p) {
+    const int64_t rows = (int64_t)p.B * p.Hk * p.R, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (at >= rows) return;
+    float m = -__builtin_inff();
+    for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, p.part_ml[(s * rows + at) * 2]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    const float base = m == -__builtin_inff() ? 0.f : m;
+    float sum = 0.f;
+    for (int s = lane; s < p.splits; s += 64) sum += p.part_ml[(s * rows + at) * 2 + 1] * __builtin_amdgcn_exp2f(p.part_ml[(s * rows + at) * 2] - base);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    const int64_t bc = at / p.R;
+    const int row = (int)(at - bc * p.R), c = (int)(bc % p.Hk), token = row / p.G, head = c * p.G + row - token * p.G;
+    const int64_t b = bc / p.Hk;
+    const float r = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    T* out = (T*)p.out.data + b * p.out.b + token * p.out.l + head * p.out.h;
+    for (int d = lane; d < p.D; d += 64) {
+        float f = 0.f;
+        for (int s = 0; s < p.splits; ++s) f += p.part[(s * rows + at) * p.D + d] * __builtin_amdgcn_exp2f(p.part_ml[(s * rows + at) * 2] - base);
+        out[d] = (T)(f * r);
+    }
+    if (lane == 0) p.lse[b * p.lse_b + token * p.lse_l + head * p.lse_h] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+template <class T, int DP>
+struct ForwardMany {
+    // f32 at 128 features and more: 32 keys a tile, or two tiles of keys and values would not fit LDS twice
+    typedef ForwardConfig<T, DP, 4, 1, sizeof(T) == 2 ? 64 : 32, 2> C;
+};
+template <class T, int DP>
+struct ForwardFew {
+    static constexpr int kRowBytes = DP * (int)sizeof(T);
+    // as many wavefronts along the keys as fit LDS; above 512 bytes a row no registers are left to load ahead
+    static constexpr int WK = kRowBytes <= 256 ? 4 : kRowBytes <= 512 ? 2 : 1;
+    typedef ForwardConfig<T, DP, 1, WK, 32 * WK, kRowBytes <= 512 ? 1 : 0> C;
+};
+
+template <class T, int DP, class C>
+void launch_forward(const Params& p, hipStream_t stream) {
+    forward_kernel<T, DP, C><<<die_grid((int64_t)p.tiles * p.splits * p.Hk * p.B), C::NT, 0, stream>>>(p);
+    check_launch("adhip_attention");
+    if (p.splits > 1) {
+        join_kernel<T><<<(unsigned)(((int64_t)p.B * p.Hk * p.R + 3) / 4), 256, 0, stream>>>(p);
+        check_launch("adhip_attention");
+    }
+}
+
+template <class T>
+void forward(const Params& p, bool few_rows, hipStream_t stream) {
+    switch (padded_size(p.D)) {
+#define ADHIP_CASE(DP)                                                                                   \
+    case DP:                                                                                             \
+        if (few_rows) launch_forward<T, DP, typename ForwardFew<T, DP>::C>(p, stream);                   \
+        else launch_forward<T, DP, typename ForwardMany<T, DP>::C>(p, stream);                           \
+        break;
+        ADHIP_CASE(32) ADHIP_CASE(64) ADHIP_CASE(96) ADHIP_CASE(128) ADHIP_CASE(192) ADHIP_CASE(256)
+#undef ADHIP_CASE
+    }
+}
+
+}  // namespace attn
+}  // namespace adhip

@@ -31,6 +31,7 @@
 #include "ir.hpp"
 #include "lower.hpp"
 #include "plan.hpp"
+#include "runtime.hpp"
 
 using namespace adhip;
 
@@ -196,6 +197,7 @@ struct adhip_program {
     std::vector<std::pair<int, std::pair<hipEvent_t, hipEvent_t>>> pending;  // stat index, (start, stop)
     std::vector<hipEvent_t> event_pool;
     std::string description;
+    std::map<std::string, std::vector<uint64_t>> result_dims;  // what adhip_program_buffer handed out
 };
 
 namespace {
@@ -980,6 +982,17 @@ int guarded(adhip_ctx* ctx, F&& f) {
 
 }  // namespace
 
+int adhip::context_guarded(adhip_ctx* ctx, const std::function<void()>& f) {
+    if (!ctx) {
+        g_tls_error = "no context";
+        return 2;
+    }
+    return guarded(ctx, [&] {
+        HIP_OK(hipSetDevice(ctx->device));
+        f();
+    });
+}
+
 extern "C" {
 
 const char* adhip_version(void) { return "adhip 0.1 (gfx950)"; }
@@ -1200,6 +1213,58 @@ int adhip_program_readback(adhip_program* p) {
 }
 
 void adhip_program_destroy(adhip_program* p) { program_free(p); }
+
+int adhip_program_buffer(adhip_program* p, const char* id, void** data, const uint64_t** dims, size_t* ndim) {
+    if (!p || !id || !data || !dims || !ndim) return 2;
+    int rc = 0;
+    const int failed = guarded(p->ctx, [&] {
+        auto it = p->plan->results.find(id);
+        if (it == p->plan->results.end()) {
+            rc = 1;
+            return;
+        }
+        std::vector<uint64_t>& d = p->result_dims[it->first];
+        d.assign(it->second.shape.begin(), it->second.shape.end());
+        *data = p->buf_ptr[(size_t)it->second.buf];
+        *dims = d.data();
+        *ndim = d.size();
+    });
+    return failed ? failed : rc;
+}
+
+int adhip_alloc(adhip_ctx* ctx, size_t bytes, void** out) {
+    if (!out) return 2;
+    *out = nullptr;
+    return context_guarded(ctx, [&] { HIP_OK(hipMalloc(out, std::max<size_t>(bytes, 1))); });
+}
+
+int adhip_free(adhip_ctx* ctx, void* data) {
+    return context_guarded(ctx, [&] { HIP_OK(hipFree(data)); });
+}
+
+int adhip_copy_in(adhip_ctx* ctx, void* device, const void* host, size_t bytes) {
+    return context_guarded(ctx, [&] {
+        ADHIP_CHECK(bytes == 0 || (device && host), "adhip_copy_in: null pointer");
+        if (bytes == 0) return;
+        HIP_OK(hipMemcpyAsync(device, host, bytes, hipMemcpyHostToDevice, ctx->stream));
+        HIP_OK(hipStreamSynchronize(ctx->stream));
+    });
+}
+
+int adhip_copy_out(adhip_ctx* ctx, void* host, const void* device, size_t bytes) {
+    return context_guarded(ctx, [&] {
+        ADHIP_CHECK(bytes == 0 || (device && host), "adhip_copy_out: null pointer");
+        if (bytes == 0) return;
+        HIP_OK(hipMemcpyAsync(host, device, bytes, hipMemcpyDeviceToHost, ctx->stream));
+        HIP_OK(hipStreamSynchronize(ctx->stream));
+    });
+}
+
+void* adhip_stream(adhip_ctx* ctx) { return ctx ? (void*)ctx->stream : nullptr; }
+
+int adhip_sync(adhip_ctx* ctx) {
+    return context_guarded(ctx, [&] { HIP_OK(hipStreamSynchronize(ctx->stream)); });
+}
 
 int adhip_program_set_profiling(adhip_program* p, int enabled) {
     if (!p) return 2;

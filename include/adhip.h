@@ -118,6 +118,114 @@ int adhip_lower_describe(const uint8_t* program, size_t program_len, const char*
 int adhip_compile_check(const uint8_t* program, size_t program_len, const char* const* dep_ids, size_t n_dep_ids,
                         const char* arch, char* out, size_t out_cap);
 
+/* ---- operators on device arrays -----------------------------------------------------------------------
+ * What training and running a decoder takes beside programs: rotary positions, attention with masks, capped scores,
+ * distance bias and shared heads (forward, backward, single tokens against a cache) and AdamW over many tensors.  They
+ * have no counterpart in the reference.  They work on device memory that the caller holds -- the buffers of a resident
+ * program (adhip_program_buffer), arrays from adhip_alloc, or any other HIP allocation on the context's device -- and
+ * queue their kernels on `stream` (a hipStream_t; NULL is HIP's default stream, adhip_stream(ctx) the context's own):
+ * they allocate nothing, keep nothing and do not wait, so they may be captured into a graph.  Arguments are checked
+ * before anything is queued; what a kernel cannot check (addresses) is the caller's.  Outputs must not overlap inputs
+ * except where it is said. */
+
+enum { ADHIP_F32 = 0, ADHIP_BF16 = 1, ADHIP_I32 = 2, ADHIP_E4M3 = 3 };
+
+/* An array in device memory: element (i0, i1, ...) is at data + sum(i * strides) elements.  Attention and rotary arrays
+ * need a last stride of 1; strides may be 0 or negative on inputs only where it is said (broadcast), and an output's
+ * elements must be distinct.  data = NULL: not given. */
+typedef struct adhip_array {
+    void* data;
+    int32_t type; /* ADHIP_F32 ... */
+    int32_t rank; /* 1 to 4 */
+    int64_t dims[4];
+    int64_t strides[4]; /* in elements */
+} adhip_array;
+
+/* Device memory of a context (freed by adhip_free or with the process, not with the context). */
+int adhip_alloc(adhip_ctx* ctx, size_t bytes, void** out);
+int adhip_free(adhip_ctx* ctx, void* data);
+/* Copies between host and device memory on the context's stream; they return when the copy is done. */
+int adhip_copy_in(adhip_ctx* ctx, void* device, const void* host, size_t bytes);
+int adhip_copy_out(adhip_ctx* ctx, void* host, const void* device, size_t bytes);
+/* The context's own stream (a hipStream_t), and a wait for everything queued on it. */
+void* adhip_stream(adhip_ctx* ctx);
+int adhip_sync(adhip_ctx* ctx);
+
+/* The device buffer of a kept id of a resident program (dims as adhip_get_tensor gives them; dims memory is the
+ * program's): where its value is after a run, and, for a CreateMat outside of loops and branches, where the next run
+ * reads it from, so an operator may write there what the next run is to use.  The buffer holds packed floats and lives
+ * as long as the program.  Returns 1 if `id` is not a kept id of the program. */
+int adhip_program_buffer(adhip_program* p, const char* id, void** data, const uint64_t** dims, size_t* ndim);
+
+/* Rotary positions.  x and out are [batch, length, heads, size], cos and sin f32 tables [rows, pairs] with packed rows,
+ * positions int32 [batch, length]; 2 pairs <= size features of every head are turned, the others copied:
+ *     (a, b) -> (a cos - b sin, a sin + b cos),   cos, sin of row positions[b, l], column i
+ * with a, b the features i and i + pairs, or 2 i and 2 i + 1 where `interleaved`.  `inverse` turns the other way, which
+ * is the gradient's rule.  second / second_out (data NULL: none) is another array of the same batch, length, size and
+ * type that is turned by the same angles in the same launch (a step's keys beside its queries).  out may be x itself.
+ * A position outside of the table gives NaN in the turned features. */
+typedef struct adhip_rotary_args {
+    adhip_array x, out, second, second_out;
+    adhip_array cos, sin, positions;
+    int32_t interleaved, inverse;
+} adhip_rotary_args;
+int adhip_rotary(adhip_ctx* ctx, const adhip_rotary_args* args, void* stream);
+
+/* AdamW over many tensors: one step on each, in as few launches as their number allows.
+ *     g = grad_scale gradient;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g g
+ *     p = p (1 - rate decay) - rate / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * in 32 bits, rounded once where p is bf16.  p and g are ADHIP_F32 or ADHIP_BF16 of `count` packed elements, m and v
+ * either f32 (state_type ADHIP_F32) or ADHIP_E4M3: blocks of 256 elements, the last one padded to 256 with zeros, codes
+ * [blocks, 256] and one f32 scale a block; m = code scale, sqrt(v) = code scale, scale = max(largest, 2^-100) / 448, and a
+ * v that is not zero never gets the code zero.  The *_out pointers may be the inputs themselves (a step in place). */
+#define ADHIP_ADAMW_BLOCK 256
+typedef struct adhip_adamw_tensor {
+    const void *p, *g, *m, *v;
+    const float *m_scale, *v_scale; /* ADHIP_E4M3 only */
+    void *p_out, *m_out, *v_out;
+    float *m_scale_out, *v_scale_out;
+    int64_t count;
+} adhip_adamw_tensor;
+typedef struct adhip_adamw_args {
+    const adhip_adamw_tensor* tensors; /* host memory, read before the call returns */
+    int64_t n_tensors;
+    int32_t p_type, g_type, state_type;
+    int32_t step; /* 1 for the first */
+    double rate, beta1, beta2, eps, decay, grad_scale;
+} adhip_adamw_args;
+int adhip_adamw(adhip_ctx* ctx, const adhip_adamw_args* args, void* stream);
+
+/* Attention.  q and out are [batch, queries, heads, size], k and v [batch, keys, key heads, size] (f32 or bf16, one type),
+ * heads a multiple of the key heads (head h reads key head h / (heads / key heads)), size at most 256.  Query i of
+ * sequence b stands at position  at = i + lengths[b] - queries  (the last query at the last key), sees key j where
+ *     j < lengths[b],
+ *     j < prefix[b], or j <= at (causal) and, with a window, |at - j| < window,
+ *     query_documents[b, i] == key_documents[b, j] >= 0 (where documents are given),
+ * and scores it with
+ *     z = cap tanh(scale q.k / cap) - slopes[h] |at - j|      (cap 0: scale q.k uncapped; no slopes: no second term).
+ * out = softmax(z) v over what it sees, lse = log(sum(exp(z))) (f32, [batch, queries, heads]).  A query that sees nothing
+ * gives out = 0 and lse = -infinity; keys and values that no query may see (behind lengths, documents below 0) are not
+ * used, whatever they hold.  lengths (int32 [batch]; default: keys) is clamped to 0 .. keys.
+ * workspace: device memory of at least adhip_attention_workspace() bytes, aligned to 256, used until the call's kernels
+ * are done. */
+typedef struct adhip_attention_args {
+    adhip_array q, k, v, out, lse;
+    adhip_array slopes, lengths, prefix, query_documents, key_documents; /* slopes f32 [heads], the others int32 */
+    /* backward only: gradient of out, gradients of q, k and v (of the arrays' own shapes and type) */
+    adhip_array out_grad, q_grad, k_grad, v_grad;
+    float scale, cap;
+    int32_t causal;
+    int64_t window; /* 0: none */
+    void* workspace;
+    size_t workspace_bytes;
+} adhip_attention_args;
+/* What a call on arrays of these shapes needs: only the shapes and types of q, k and v are looked at. */
+int adhip_attention_workspace(adhip_ctx* ctx, const adhip_attention_args* args, int backward, size_t* bytes);
+int adhip_attention(adhip_ctx* ctx, const adhip_attention_args* args, void* stream);
+/* Gradients of q, k and v from what adhip_attention gave (out, lse) and the gradient of out.  The order of additions
+ * is fixed: the same inputs give the same bits. */
+int adhip_attention_backward(adhip_ctx* ctx, const adhip_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
