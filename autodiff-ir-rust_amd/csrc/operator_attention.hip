@@ -1,6 +1,7 @@
 // Attention on device arrays: checks of arguments, workspace, the choice of kernels.
 #include "operator_attention.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace adhip {
@@ -19,20 +20,22 @@ __global__ __launch_bounds__(256) void document_ranges_kernel(const int* q, int6
     const int e = of_keys ? entry - qn : entry;
     if (of_keys && e >= kn) return;
     const int i = e * attn::kRange + lane;
-    const int d = i >= (of_keys ? Lk : Lq) ? -1 : of_keys ? k[b * kb + i * kl] : q[b * qb + i * ql];
-    int lo = d >= 0 ? d : 0x7fffffff, hi = d;
+    const bool there = i < (of_keys ? Lk : Lq);
+    const int d = !there ? 0 : max(of_keys ? k[b * kb + i * kl] : q[b * qb + i * ql], -1);
+    int lo = there ? d : 0x7fffffff, hi = there ? d : -2;
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) {
         lo = min(lo, __shfl_xor(lo, s));
         hi = max(hi, __shfl_xor(hi, s));
     }
-    if (lane == 0) (of_keys ? kr + (int64_t)b * kn : qr + (int64_t)b * qn)[e] = int2{lo, max(hi, -1)};
+    if (lane == 0) (of_keys ? kr + (int64_t)b * kn : qr + (int64_t)b * qn)[e] = int2{lo, hi};
 }
 
 attn::Tensor tensor_of(const adhip_array& a) {
     const int chunk = 16 / type_bytes(a.type);
     attn::Tensor t = {a.data, a.strides[0], a.strides[1], a.strides[2], 0};
-    t.vec = vector_elements(a, chunk) == chunk && a.dims[3] % chunk == 0;
+    // (a tile's offsets, up to 128 rows, are to fit 31 bits)
+    t.vec = vector_elements(a, chunk) == chunk && a.dims[3] % chunk == 0 && (a.dims[1] <= 1 || a.strides[1] < (int64_t(1) << 31) / 4 / 128 - 256);
     return t;
 }
 
@@ -41,8 +44,8 @@ size_t rounded(size_t n) { return (n + 255) & ~size_t(255); }
 // How a call is cut up, and where its workspace's parts begin.
 struct Layout {
     bool few_rows;
-    int row_tile, tiles, splits;
-    size_t qrange, krange, part, part_ml, delta, bytes;
+    int row_tile, tiles, splits, dq_splits, dk_splits;
+    size_t qrange, krange, part, part_ml, delta, part_dq, part_dk, part_dv, bytes;
 };
 
 Layout layout_of(const adhip_attention_args& g, bool backward) {
@@ -73,8 +76,30 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
         y.part_ml = forward;
         forward += rounded((size_t)(y.splits * B * Hk * R * 2) * 4);
     }
-    y.delta = back;
-    if (backward) back += rounded((size_t)(B * Hk * R) * 4);
+    y.dq_splits = y.dk_splits = 1;
+    if (backward) {
+        y.delta = back;
+        back += rounded((size_t)(B * Hk * R) * 4);
+        // Parts of the backward walks: as many as give every compute unit four workgroups, which evens out a causal mask's
+        // uneven ones, none shorter than four tiles.
+        auto parts = [](int64_t blocks, int64_t tiles) {
+            if (blocks <= 0 || blocks >= 1024) return 1;
+            return (int)std::max<int64_t>(1, std::min<int64_t>((1024 + blocks - 1) / blocks, tiles / 4));
+        };
+        const int64_t rows = (R + 127) / 128 * Hk * B, keys = (Lk + 127) / 128 * Hk * B;
+        y.dq_splits = parts(rows, (Lk + 63) / 64);
+        y.dk_splits = parts(keys, (R + 63) / 64);
+        if (y.dq_splits > 1) {
+            y.part_dq = back;
+            back += rounded((size_t)(y.dq_splits * B * Hk * R * D) * 4);
+        }
+        if (y.dk_splits > 1) {
+            y.part_dk = back;
+            back += rounded((size_t)(y.dk_splits * B * Hk * Lk * D) * 4);
+            y.part_dv = back;
+            back += rounded((size_t)(y.dk_splits * B * Hk * Lk * D) * 4);
+        }
+    }
     y.bytes = std::max(forward, back);
     return y;
 }
@@ -174,6 +199,11 @@ Params checked(const char* op, const adhip_attention_args& g, const Layout& y, b
     p.part = (float*)(room + y.part);
     p.part_ml = (float*)(room + y.part_ml);
     p.delta = (float*)(room + y.delta);
+    p.dq_splits = y.dq_splits;
+    p.dk_splits = y.dk_splits;
+    p.part_dq = (float*)(room + y.part_dq);
+    p.part_dk = (float*)(room + y.part_dk);
+    p.part_dv = (float*)(room + y.part_dv);
     return p;
 }
 

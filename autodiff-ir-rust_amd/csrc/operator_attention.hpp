@@ -22,7 +22,7 @@ constexpr int kRange = 32;  // positions that share an entry of the document ran
 struct Tensor {
     const void* data;
     int64_t b, l, h;  // strides in elements
-    int vec;          // 16 bytes can be read at a time
+    int vec;          // rows begin at multiples of 16 bytes and hold whole pieces of 16 bytes
 };
 
 struct Params {
@@ -33,14 +33,16 @@ struct Params {
     int64_t slope_stride;
     const int *lengths, *prefix, *qdoc, *kdoc;
     int64_t lengths_s, prefix_s, qdoc_b, qdoc_l, kdoc_b, kdoc_l;
-    const int2 *qrange, *krange;  // smallest and largest document (of those >= 0) of every kRange positions
+    const int2 *qrange, *krange;  // smallest and largest document of every kRange positions, those below 0 as -1
     int qranges, kranges;         // entries of a sequence
     int B, Lq, Lk, Hk, G, D, R;   // R = Lq G rows
     float scale, cap;
     int causal, window;
     int tiles, splits;            // row tiles (or key tiles); ranges that the keys (or rows) are split into
     float *part, *part_ml;        // forward, split: [split][b][c][row][D], [..][row][2]
-    float* delta;                 // backward: [b][c][row]
+    float* delta;                 // backward: [b][head][query]
+    float *part_dq, *part_dk, *part_dv;  // backward, split: [split] of what the gradients are, packed [b][c][row or key][D]
+    int dq_splits, dk_splits;
 };
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -69,10 +71,22 @@ struct Matrix<float> {
     }
 };
 
+// Tiles in LDS: rows of DP features in pieces of 16 bytes, whose places within a row are exchanged by an exclusive or
+// with bits of the row's number.  16 rows at one piece (an operand whose rows are rows of the tile) then lie in all 64
+// banks, and so do 4 rows at four pieces (the transposing reads): 230 and 200 bytes a clock, where rows padded by 16 bytes
+// give the first 230 and the second 62, unpadded ones 16 and less.  The exchange costs one instruction an address, and
+// pieces keep places of 16 bytes, so that loads can go to LDS without passing through registers.
 template <class T, int DP>
 struct Lds {
-    // 16 bytes behind every row: eight rows of a fragment start in different banks
-    static constexpr int kPitch = DP + 16 / (int)sizeof(T);
+    static constexpr int kPieces = DP * (int)sizeof(T) / 16;
+    static constexpr int kPlaces = kPieces == 12 ? 16 : kPieces;  // the exchange wants a power of two in each row
+    static constexpr int kPitch = kPlaces * 16;                   // bytes
+    static __device__ __forceinline__ int swap(int row) {
+        if (kPlaces % 16 == 0) return (row & 3) << 2 | (row >> 2 & 3);
+        if (kPlaces % 8 == 0) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+        return row >> 2 & 3;
+    }
+    static __device__ __forceinline__ int at(int row, int piece) { return row * kPitch + (piece ^ swap(row)) * 16; }
 };
 
 __device__ __forceinline__ f32x16 zero16() {
@@ -82,31 +96,39 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
-// A (or B) operand whose rows are rows of the tile: rows row0 .. + 31, features 16 step .. + 15
+// A (or B) operand whose rows are rows of the tile: rows row0 .. + 31 (row0 a multiple of 16), features 16 step .. + 15
 template <class T, int DP>
-__device__ __forceinline__ typename Matrix<T>::Frag rows_frag(const T* tile, int row0, int step, int lane) {
-    return *(const typename Matrix<T>::Frag*)(tile + (row0 + (lane & 31)) * Lds<T, DP>::kPitch + step * 16 + (lane >> 5) * 8);
+__device__ __forceinline__ typename Matrix<T>::Frag rows_frag(const char* tile, int row0, int step, int lane) {
+    typedef typename Matrix<T>::Frag Frag;
+    constexpr int N = sizeof(Frag) / 16;
+    Frag f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        ((uint4*)&f)[i] = *(const uint4*)(tile + row0 * Lds<T, DP>::kPitch + Lds<T, DP>::at(lane & 31, (2 * step + (lane >> 5)) * N + i));
+    return f;
 }
 
-// A operand whose rows are features d0 .. + 31 of the tile and whose k are its rows k0 .. + 15, in the order of C's registers
+// A operand whose rows are features d0 .. + 31 of the tile and whose k are its rows k0 .. + 15 (a multiple of 16), in the order
+// of C's registers
 template <int DP>
-__device__ __forceinline__ bf16x8 cols_frag(const bf16* tile, int k0, int d0, int lane) {
+__device__ __forceinline__ bf16x8 cols_frag(const bf16*, const char* tile, int k0, int d0, int lane) {
     typedef __attribute__((address_space(3))) s16x4* Ptr;
-    const bf16* a = tile + (k0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * Lds<bf16, DP>::kPitch + d0 + (lane & 16) + 4 * (lane & 3);
-    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)a);
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(a + 8 * Lds<bf16, DP>::kPitch));
+    typedef Lds<bf16, DP> L;
+    const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), piece = d0 / 8 + (lane >> 4 & 1) * 2 + (lane >> 1 & 1);
+    const char* base = tile + k0 * L::kPitch + 8 * (lane & 1);
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(base + L::at(row, piece)));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(base + L::at(row + 8, piece)));
     const s16x8 r = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(bf16x8, r);
 }
 template <int DP>
-__device__ __forceinline__ f32x8 cols_frag(const float* tile, int k0, int d0, int lane) {
-    const float* a = tile + (k0 + 4 * (lane >> 5)) * Lds<float, DP>::kPitch + d0 + (lane & 31);
+__device__ __forceinline__ f32x8 cols_frag(const float*, const char* tile, int k0, int d0, int lane) {
+    typedef Lds<float, DP> L;
+    const int piece = d0 / 4 + ((lane & 31) >> 2);
+    const char* base = tile + k0 * L::kPitch + 4 * (lane & 3);
     f32x8 r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        r[e] = a[e * Lds<float, DP>::kPitch];
-        r[e + 4] = a[(e + 8) * Lds<float, DP>::kPitch];
-    }
+    for (int e = 0; e < 8; ++e) r[e] = *(const float*)(base + L::at(4 * (lane >> 5) + (e & 3) + 2 * (e & 4), piece));
     return r;
 }
 
@@ -121,11 +143,12 @@ __device__ __forceinline__ void to_frag(const f32x16& c, int s, f32x8& f) {
     for (int e = 0; e < 8; ++e) f[e] = c[8 * s + e];
 }
 
-// 16 bytes of a row of D features from d on; what lies behind the row's end is zero
-template <class T>
-__device__ __forceinline__ uint4 load_chunk(const T* row, int d, int D, int vec) {
+// 16 bytes of a row of D features from d on; what lies behind the row's end is zero.  VEC: rows begin at multiples of 16
+// bytes and hold whole pieces of 16 bytes; otherwise element by element.
+template <bool VEC, class T>
+__device__ __forceinline__ uint4 load_chunk(const T* row, int d, int D) {
     uint4 r = {0, 0, 0, 0};
-    if (vec) {
+    if (VEC) {
         if (d < D) r = *(const uint4*)(row + d);
     } else {
         T t[Matrix<T>::kChunk];
@@ -137,13 +160,13 @@ __device__ __forceinline__ uint4 load_chunk(const T* row, int d, int D, int vec)
 }
 
 // the stationary operand of a product: eight features of one row of an array
-template <class T>
-__device__ __forceinline__ typename Matrix<T>::Frag load_frag(const T* row, int d, int D, int vec, bool valid) {
+template <bool VEC, class T>
+__device__ __forceinline__ typename Matrix<T>::Frag load_frag(const T* row, int d, int D, bool valid) {
     typename Matrix<T>::Frag f;
     uint4* u = (uint4*)&f;
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(f) / 16); ++i)
-        u[i] = valid ? load_chunk(row, d + i * Matrix<T>::kChunk, D, vec) : uint4{0, 0, 0, 0};
+        u[i] = valid ? load_chunk<VEC>(row, d + i * Matrix<T>::kChunk, D) : uint4{0, 0, 0, 0};
     return f;
 }
 
@@ -170,16 +193,15 @@ __device__ __forceinline__ float tanh_of(float x) {
     return 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
 }
 
-// Scores in units of log 2 from raw products, without masks; `bent` gets tanh where scores are capped.
-// far: position of the query minus key of register 0 (or key minus position: only its magnitude counts), step: +1 / -1 per row
+// row of register i of a C tile
+__device__ __forceinline__ constexpr int c_row(int i) { return 8 * (i >> 2) + (i & 3); }
+
+// Scores in units of log 2 from raw products
 struct Scoring {
     float scale2, cap_in, cap_out;  // scale log2 e; scale / cap, cap log2 e
     __device__ __forceinline__ explicit Scoring(const Params& p)
         : scale2(p.scale * kLog2e), cap_in(p.cap > 0.f ? p.scale / p.cap : 0.f), cap_out(p.cap * kLog2e) {}
 };
-
-// row of register i of a C tile
-__device__ __forceinline__ constexpr int c_row(int i) { return 8 * (i >> 2) + (i & 3); }
 
 // Positions that a query sees: j < n and (j < prefix or lo <= j <= hi).  lo and hi by the query's own position.
 struct Band {
@@ -196,9 +218,9 @@ __device__ __forceinline__ int sequence_length(const Params& p, int b) {
     return min(max(n, 0), p.Lk);
 }
 
-// smallest and largest document of positions first .. last from the table of ranges
+// smallest and largest document of positions first .. last from the table of ranges (-1: some belong to none)
 __device__ __forceinline__ int2 document_range(const int2* ranges, int first, int last) {
-    int2 r = {0x7fffffff, -1};
+    int2 r = {0x7fffffff, -2};
     for (int i = first / kRange; i <= last / kRange; ++i) {
         const int2 x = ranges[i];
         r.x = min(r.x, x.x);
@@ -236,33 +258,143 @@ __device__ __forceinline__ int by_die(int block, int total) {
 }
 inline unsigned die_grid(int64_t total) { return (unsigned)((total + 7) / 8 * 8); }
 
-// The tile that a workgroup copies from an array's rows into LDS: NT threads, ROWS rows of DP features.
-template <class T, int DP, int ROWS, int NT>
-struct Stage {
-    static constexpr int kPerRow = DP / Matrix<T>::kChunk;
-    static constexpr int kChunks = (ROWS * kPerRow + NT - 1) / NT;
-    static constexpr bool kEven = ROWS * kPerRow % NT == 0;
-    uint4 r[kChunks];
-    // row(i) gives the address of tile row i, or null for a row of zeros
-    template <class Row>
-    __device__ __forceinline__ void load(const Row& row, int D, int vec, int tid) {
+// Waits for this wavefront's loads to LDS.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Copies of tiles from an array's rows (a fixed stride apart) into LDS by a workgroup of NT threads: ROWS rows of DP
+// features.  Where rows allow it (VEC) the loads write LDS themselves, 16 bytes a lane, in the order of the tile's places;
+// which piece of which row that is decides each lane's address.  A place without a piece (behind the head's features or
+// the last row) is read at an offset behind the resource's end, which gives zeros.  Other rows take the way through
+// registers, element by element.
+template <class T, int DP, int ROWS, int NT, bool VEC>
+struct Copy {
+    typedef Lds<T, DP> L;
+    static constexpr int kTotal = ROWS * L::kPlaces, kEach = (kTotal + NT - 1) / NT;
+    static constexpr unsigned kNowhere = 0xffffffffu;
+    static_assert(kTotal % 64 == 0, "whole wavefronts copy");
+    unsigned offset[kEach];
+    int wave;
+    static __device__ __forceinline__ int row(int c, int tid) { return (tid + c * NT) / L::kPlaces; }
+    __device__ __forceinline__ Copy(int64_t stride, int D, int tid) : wave(__builtin_amdgcn_readfirstlane(tid >> 6)) {
+        if (!VEC) return;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int at = tid + c * NT, i = at / kPerRow, d = at % kPerRow * Matrix<T>::kChunk;
-            r[c] = uint4{0, 0, 0, 0};
-            if (kEven || i < ROWS) {
-                const T* x = row(i);
-                if (x) r[c] = load_chunk(x, d, D, vec);
+        for (int c = 0; c < kEach; ++c) {
+            const int i = row(c, tid), piece = (tid + c * NT) % L::kPlaces ^ L::swap(i), d = piece * Matrix<T>::kChunk;
+            offset[c] = d < D ? (unsigned)(i * stride + d) * (unsigned)sizeof(T) : kNowhere;
+        }
+    }
+    // from: the first row; rows: how many there are (at least one)
+    __device__ __forceinline__ void start(char* tile, const T* from, int64_t stride, int rows, int D, int tid) const {
+        if (VEC) {
+            const __amdgpu_buffer_rsrc_t source = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, 0x7fffffff, 0x00020000);
+            typedef __attribute__((address_space(3))) void* To;
+            const bool whole = rows >= ROWS;
+#pragma unroll
+            for (int c = 0; c < kEach; ++c) {
+                if (kTotal % NT != 0 && (wave * 64 + c * NT) >= kTotal) break;
+                const unsigned o = whole || row(c, tid) < rows ? offset[c] : kNowhere;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(source, (To)(tile + (wave * 64 + c * NT) * 16), 16, o, 0, 0, 0);
+            }
+        } else {
+#pragma unroll 1
+            for (int at = tid; at < kTotal; at += NT) {
+                const int i = at / L::kPlaces, d = (at % L::kPlaces ^ L::swap(i)) * Matrix<T>::kChunk;
+                T t[Matrix<T>::kChunk];
+#pragma unroll
+                for (int e = 0; e < Matrix<T>::kChunk; ++e) t[e] = i < rows && d + e < D ? from[i * stride + d + e] : (T)0.f;
+                *(uint4*)(tile + at * 16) = *(uint4*)t;
             }
         }
     }
-    __device__ __forceinline__ void store(T* tile, int tid) const {
+    // rows for which none(row) holds become zeros; behind the copy and a barrier
+    template <class None>
+    static __device__ __forceinline__ void clear(char* tile, const None& none, int tid) {
+#pragma unroll 1
+        for (int at = tid; at < kTotal; at += NT)
+            if (none(at / L::kPlaces)) *(uint4*)(tile + at * 16) = uint4{0, 0, 0, 0};
+    }
+};
+
+// Tiles of keys and values on their way from memory to LDS, one ahead of the products where LDS holds two, with what
+// decides about them: shared by the kernels that own rows.  Keys behind the sequence or of no document are zero, whatever
+// the arrays hold there.
+template <class T, int DP, class C, bool VEC>
+struct KeyTiles {
+    typedef Copy<T, DP, C::BK, C::NT, VEC> S;
+    static_assert(C::NT >= C::BK, "one thread a key for the documents");
+    static constexpr int kTile = C::BK * Lds<T, DP>::kPitch;
+    static constexpr int kBytes = C::kBufs * (2 * kTile + C::BK * 4);
+    const Params& p;
+    const T *kb, *vb;
+    const int* kd;
+    const int2* kr;
+    char* lds;
+    int n, tid, key0;
+    S k, v;
+    int doc;
+    int2 range[C::KB];  // documents of the 32 keys of each of the wavefront's products: of the tile that is under way ..
+    int2 now[C::KB];    // .. and of the one in LDS
+    bool unclean;       // the tile under way has keys of no document
+    __device__ __forceinline__ KeyTiles(const Params& p_, int b, int c, int n_, int tid_, int key0_, char* lds_)
+        : p(p_), lds(lds_), n(n_), tid(tid_), key0(key0_), k(p_.k.l, p_.D, tid_), v(p_.v.l, p_.D, tid_), doc(0), unclean(false) {
+        kb = (const T*)p.k.data + b * p.k.b + c * p.k.h;
+        vb = (const T*)p.v.data + b * p.v.b + c * p.v.h;
+        kd = p.kdoc ? p.kdoc + b * p.kdoc_b : nullptr;
+        kr = p.krange ? p.krange + (int64_t)b * p.kranges : nullptr;
+    }
+    __device__ __forceinline__ char* keys(int buf) const { return lds + buf * 2 * kTile; }
+    __device__ __forceinline__ char* values(int buf) const { return lds + buf * 2 * kTile + kTile; }
+    __device__ __forceinline__ int* docs(int buf) const { return (int*)(lds + C::kBufs * 2 * kTile) + buf * C::BK; }
+    __device__ __forceinline__ void start(int t, int buf) {
+        const int64_t j0 = (int64_t)t * C::BK;
+        const int left = n - (int)j0;
+        k.start(keys(buf), kb + j0 * p.k.l, p.k.l, left, p.D, tid);
+        v.start(values(buf), vb + j0 * p.v.l, p.v.l, left, p.D, tid);
+        if (!kd) return;
+        if (tid < C::BK) doc = kd[min((int)j0 + tid, n - 1) * p.kdoc_l];
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int at = tid + c * NT, i = at / kPerRow, d = at % kPerRow * Matrix<T>::kChunk;
-            if (kEven || i < ROWS) *(uint4*)(tile + i * Lds<T, DP>::kPitch + d) = r[c];
+        for (int x = 0; x < C::KB; ++x) range[x] = kr[min((int)j0 + key0 + 32 * x, n - 1) / kRange];
+        unclean = document_range(kr, (int)j0, min((int)j0 + C::BK, n) - 1).x < 0;
+    }
+    __device__ __forceinline__ void finish(int buf) {
+        wait_loads();
+        if (kd) {
+            if (tid < C::BK) docs(buf)[tid] = doc;
+#pragma unroll
+            for (int x = 0; x < C::KB; ++x) now[x] = range[x];
+        }
+        __syncthreads();
+        if (kd && unclean) {
+            const int* of = docs(buf);
+            S::clear(keys(buf), [&](int i) { return of[i] < 0; }, tid);
+            S::clear(values(buf), [&](int i) { return of[i] < 0; }, tid);
+            __syncthreads();
         }
     }
+    __device__ __forceinline__ void begin(int t) {
+        if (C::kBufs == 2 && t >= 0) {
+            start(t, 0);
+            finish(0);
+        }
+    }
+    // before a tile's products: the next one gets under way
+    __device__ __forceinline__ void fetch(int t, int next, int buf) {
+        if (C::kBufs == 2) {
+            if (next >= 0) start(next, buf ^ 1);
+        } else {
+            __syncthreads();
+            start(t, 0);
+            finish(0);
+        }
+    }
+    // behind them: it has arrived
+    __device__ __forceinline__ void advance(int next, int& buf) {
+        if (C::kBufs != 2 || next < 0) return;
+        buf ^= 1;
+        finish(buf);
+    }
+    // all 32 keys of product x are of the document `mine`
+    __device__ __forceinline__ bool one_document(int x, int mine) const { return !kd || (now[x].x == mine && now[x].y == mine); }
 };
 
 // DP: the head's features, rounded up to what the kernels are built for

@@ -5,6 +5,9 @@
 // owns keys and walks the rows of all heads that share them (dk, dv).  That is seven products where one kernel with dq in
 // atomic additions would take five, but nothing is added in an order that changes from run to run, dq takes no memory in
 // f32, and heads that share keys add up in registers.
+//
+// Where there are too few workgroups for the card, or too few for the uneven work of a causal mask to even out, each walk
+// is split and the parts are added, in order, by a third kernel.
 #pragma once
 #include "operator_attention.hpp"
 
@@ -13,29 +16,27 @@ namespace attn {
 
 // ---- dq: the forward kernel's walk ------------------------------------------------------------------------------------
 
-template <class T, int DP, int BK_, int AHEAD_>
+template <class T, int DP, int BK_, int BUFS, int WAVES_>
 struct QueryConfig {
-    static constexpr int BK = BK_, AHEAD = AHEAD_, NT = 256, BQ = 128, KB = BK / 32;
-    static constexpr int kTile = BK * Lds<T, DP>::kPitch, kBufs = AHEAD == 2 ? 2 : 1;
-    static constexpr int kBytes = kBufs * (2 * kTile * (int)sizeof(T) + BK * 4);
+    static constexpr int BK = BK_, kBufs = BUFS, WAVES = WAVES_, NT = 256, BQ = 128, KB = BK / 32;
 };
 
-template <class T, int DP, class C>
-__global__ __launch_bounds__(C::NT) void query_gradient_kernel(const Params p) {
+template <class T, int DP, bool VEC, class C>
+__global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const Params p) {
     typedef Matrix<T> M;
     typedef typename M::Frag Frag;
-    __shared__ __attribute__((aligned(16))) char lds[C::kBytes];
-    T* const ks = (T*)lds;
-    T* const vs = ks + C::kBufs * C::kTile;
-    int* const docs = (int*)(vs + C::kBufs * C::kTile);
+    typedef KeyTiles<T, DP, C, VEC> Keys;
+    __shared__ __attribute__((aligned(1024))) char lds[Keys::kBytes];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    const int total = p.tiles * p.Hk * p.B;
+    const int total = p.tiles * p.dq_splits * p.Hk * p.B;
     int id = by_die(blockIdx.x, total);
     if (id >= total) return;
-    const int tile = p.tiles - 1 - id % p.tiles;
+    const int tile = p.tiles - 1 - id % p.tiles;  // the last ones, which see most keys, first
     id /= p.tiles;
+    const int split = id % p.dq_splits;
+    id /= p.dq_splits;
     const int c = id % p.Hk, b = id / p.Hk;
 
     const int n = sequence_length(p, b), offset = n - p.Lq;
@@ -67,20 +68,23 @@ __global__ __launch_bounds__(C::NT) void query_gradient_kernel(const Params p) {
         const T* o = (const T*)p.out.data + b * p.out.b + token * p.out.l + head * p.out.h;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
-            qf[s] = load_frag(q, s * 16 + half * 8, p.D, p.q.vec, valid);
-            df[s] = load_frag(d, s * 16 + half * 8, p.D, p.dout.vec, valid);
-            const Frag of = load_frag(o, s * 16 + half * 8, p.D, p.out.vec, valid);
+            qf[s] = load_frag<VEC>(q, s * 16 + half * 8, p.D, valid);
+            df[s] = load_frag<VEC>(d, s * 16 + half * 8, p.D, valid);
+            const Frag of = load_frag<VEC>(o, s * 16 + half * 8, p.D, valid);
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta += (float)df[s][e] * (float)of[e];
         }
     }
     delta += __shfl_xor(delta, 32);
-    if (inside && half == 0) p.delta[((int64_t)b * p.Hk + c) * p.R + row] = delta;
+    if (inside && half == 0 && split == 0) p.delta[((int64_t)b * p.Hk * p.G + head) * p.Lq + token] = delta;
     f32x16 dq[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) dq[d] = zero16();
 
     const int hi_all = last + offset + band.above, lo_all = first + offset - band.below;
+    const int t_first = prefix > 0 ? 0 : max(lo_all, 0) / C::BK, t_stop = (min(n, max(hi_all + 1, prefix)) + C::BK - 1) / C::BK;
+    const int per = max(0, t_stop - t_first + p.dq_splits - 1) / p.dq_splits;
+    const int t_begin = t_first + split * per, t_end = min(t_begin + per, t_stop);
     const int2* const kr = p.krange ? p.krange + (int64_t)b * p.kranges : nullptr;
     int2 mine = {0, 0};
     if (kr) mine = document_range(p.qrange + (int64_t)b * p.qranges, first, last);
@@ -91,140 +95,111 @@ __global__ __launch_bounds__(C::NT) void query_gradient_kernel(const Params p) {
         const int2 theirs = document_range(kr, j0, j1);
         return theirs.x <= mine.y && mine.x <= theirs.y;
     };
-    Tiles<decltype(needed)> tiles(needed, 0, (n + C::BK - 1) / C::BK);
+    Tiles<decltype(needed)> tiles(needed, t_begin, t_end);
 
-    const T* const kb = (const T*)p.k.data + b * p.k.b + c * p.k.h;
-    const T* const vb = (const T*)p.v.data + b * p.v.b + c * p.v.h;
-    const int* const kd = p.kdoc ? p.kdoc + b * p.kdoc_b : nullptr;
-    Stage<T, DP, C::BK, C::NT> sk, sv;
-    int sd = 0;
-    auto used = [&](int j) { return j < n && !(kd && kd[j * p.kdoc_l] < 0); };
-    auto load_k = [&](int j0) { sk.load([&](int i) { return used(j0 + i) ? kb + (j0 + i) * p.k.l : (const T*)nullptr; }, p.D, p.k.vec, tid); };
-    auto load_v = [&](int j0) { sv.load([&](int i) { return used(j0 + i) ? vb + (j0 + i) * p.v.l : (const T*)nullptr; }, p.D, p.v.vec, tid); };
-    auto load_d = [&](int j0) { if (kd && tid < C::BK) sd = j0 + tid < n ? kd[(j0 + tid) * p.kdoc_l] : -1; };
-    auto load = [&](int t) {
-        load_k(t * C::BK);
-        load_v(t * C::BK);
-        load_d(t * C::BK);
-    };
-    static_assert(C::NT >= C::BK, "one thread a key for the documents");
-    auto store_d = [&](int buf) { if (kd && tid < C::BK) docs[buf * C::BK + tid] = sd; };
-    auto store = [&](int buf) {
-        sk.store(ks + buf * C::kTile, tid);
-        sv.store(vs + buf * C::kTile, tid);
-        store_d(buf);
-    };
-
+    Keys kt(p, b, c, n, tid, 0, lds);
     int t = tiles.next(lane), buf = 0;
-    if (C::AHEAD == 2) {
-        if (t >= 0) {
-            load(t);
-            store(0);
-        }
-        __syncthreads();
-    }
+    kt.begin(t);
     while (t >= 0) {
         const int next = tiles.next(lane);
-        if (C::AHEAD == 2) {
-            if (next >= 0) load(next);
-        } else {
-            __syncthreads();
-            load_k(t * C::BK);
-            sk.store(ks, tid);
-            load_v(t * C::BK);
-            sv.store(vs, tid);
-            load_d(t * C::BK);
-            store_d(0);
-            __syncthreads();
-        }
-        const T* kt = ks + buf * C::kTile;
-        const T* vt = vs + buf * C::kTile;
-        const int* dt = docs + buf * C::BK;
+        kt.fetch(t, next, buf);
+        const char* ks = kt.keys(buf);
+        const char* vs = kt.values(buf);
+        const int* docs = kt.docs(buf);
 #pragma unroll
         for (int x = 0; x < C::KB; ++x) {
             const int key0 = x * 32;
             f32x16 s = zero16(), g = zero16();
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) s = M::mma(rows_frag<T, DP>(kt, key0, k, lane), qf[k], s);
+            for (int k = 0; k < DP / 16; ++k) s = M::mma(rows_frag<T, DP>(ks, key0, k, lane), qf[k], s);
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) g = M::mma(rows_frag<T, DP>(vt, key0, k, lane), df[k], g);
+            for (int k = 0; k < DP / 16; ++k) g = M::mma(rows_frag<T, DP>(vs, key0, k, lane), df[k], g);
             const int j0 = t * C::BK + key0, jl = j0 + 4 * half;
-            const bool masked = kd || !__all(j0 + 31 < n && ((lo <= j0 && j0 + 31 <= hi) || j0 + 31 < pre));
+            const bool masked = !__all(j0 + 31 < n && ((lo <= j0 && j0 + 31 <= hi) || j0 + 31 < pre) && kt.one_document(x, doc));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float z, bend = 1.f;
-                if (p.cap > 0.f) {
+            for (int i = 0; i < 16; ++i) g[i] -= delta;
+            if (p.cap > 0.f) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
                     const float y = tanh_of(s[i] * sc.cap_in);
-                    z = y * sc.cap_out;
-                    bend = 1.f - y * y;
-                } else {
-                    z = s[i] * sc.scale2;
+                    s[i] = y * sc.cap_out;
+                    g[i] *= 1.f - y * y;
                 }
-                if (p.slopes) z -= slope * fabsf((float)(at - jl - c_row(i)));
-                const float w = __builtin_amdgcn_exp2f(z - lse2);
-                float ds = w * (g[i] - delta) * bend;
-                if (masked) {
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] *= sc.scale2;
+            }
+            if (p.slopes) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] -= slope * fabsf((float)(at - jl - c_row(i)));
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] - lse2) * g[i];
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
                     const int j = jl + c_row(i);
                     bool sees = j < n && (j < pre || (lo <= j && j <= hi));
-                    if (kd) sees = sees && dt[key0 + 4 * half + c_row(i)] == doc;
-                    ds = sees ? ds : 0.f;
+                    if (kt.kd) sees = sees && docs[key0 + 4 * half + c_row(i)] == doc;
+                    s[i] = sees ? s[i] : 0.f;
                 }
-                s[i] = ds;
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 Frag f;
                 to_frag(s, h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dq[d] = M::mma(cols_frag<DP>(kt, key0 + 16 * h, d * 32, lane), f, dq[d]);
+                for (int d = 0; d < DP / 32; ++d) dq[d] = M::mma(cols_frag<DP>((const T*)0, ks, key0 + 16 * h, d * 32, lane), f, dq[d]);
             }
         }
-        if (C::AHEAD == 2) {
-            buf ^= 1;
-            if (next >= 0) store(buf);
-            __syncthreads();
-        }
+        kt.advance(next, buf);
         t = next;
     }
     if (!inside) return;
-    T* out = (T*)p.dq.data + b * p.dq.b + token * p.dq.l + head * p.dq.h;
+    float* const part = p.dq_splits > 1 ? p.part_dq + ((((int64_t)split * p.B + b) * p.Hk + c) * p.R + row) * p.D : nullptr;
+    T* const out = (T*)p.dq.data + b * p.dq.b + token * p.dq.l + head * p.dq.h;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const float f[4] = {dq[d][4 * g] * p.scale, dq[d][4 * g + 1] * p.scale, dq[d][4 * g + 2] * p.scale, dq[d][4 * g + 3] * p.scale};
-            store4(out, d * 32 + 8 * g + 4 * half, p.D, p.dq.vec, f);
+            if (part) store4(part, d * 32 + 8 * g + 4 * half, p.D, (p.D & 3) == 0, f);
+            else store4(out, d * 32 + 8 * g + 4 * half, p.D, p.dq.vec, f);
         }
 }
 
 // ---- dk, dv -------------------------------------------------------------------------------------------------------------
 
-// NW wavefronts own 32 keys each and walk tiles of BR rows.  V_LDS: the values are read from LDS, where registers hold no
-// more than keys and two sums.
-template <class T, int DP, int NW_, int BR_, int AHEAD_, bool V_LDS_>
+// KG wavefronts own 32 keys each, RG of them share the keys and take every RG-th 32 rows of a tile of BR.
+// K_LDS, V_LDS: the keys or values are read from LDS, where the two sums leave no registers for them.
+template <class T, int DP, int KG_, int RG_, int BUFS, bool K_LDS_, bool V_LDS_, int WAVES_>
 struct KeyConfig {
-    static constexpr int NW = NW_, BR = BR_, AHEAD = AHEAD_, NT = 64 * NW, BKEYS = 32 * NW;
-    static constexpr bool V_LDS = V_LDS_;
-    static constexpr int kTile = BR * Lds<T, DP>::kPitch, kBufs = AHEAD == 2 ? 2 : 1;
-    static constexpr int kValues = V_LDS ? BKEYS * Lds<T, DP>::kPitch : 0;
-    static constexpr int kBytes = (kBufs * 2 * kTile + kValues) * (int)sizeof(T) + kBufs * BR * 5 * 4;
+    static constexpr int KG = KG_, RG = RG_, BR = 32 * RG, kBufs = BUFS, NT = 64 * KG * RG, BKEYS = 32 * KG, WAVES = WAVES_;
+    static constexpr bool K_LDS = K_LDS_, V_LDS = V_LDS_;
+    static constexpr int kTile = BR * Lds<T, DP>::kPitch, kOwn = BKEYS * Lds<T, DP>::kPitch;
+    static constexpr int kRows = kBufs * 2 * kTile + (K_LDS ? kOwn : 0) + (V_LDS ? kOwn : 0);
+    static constexpr int kLoop = kRows + kBufs * BR * 5 * 4;
+    static constexpr int kMerge = RG > 1 ? (RG - 1) * BKEYS * (DP + 4) * 4 : 0;
+    static constexpr int kBytes = kLoop > kMerge ? kLoop : kMerge;
 };
 
-template <class T, int DP, class C>
-__global__ __launch_bounds__(C::NT) void key_gradient_kernel(const Params p) {
+template <class T, int DP, bool VEC, class C>
+__global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Params p) {
     typedef Matrix<T> M;
     typedef typename M::Frag Frag;
-    __shared__ __attribute__((aligned(16))) char lds[C::kBytes];
-    T* const qs = (T*)lds;                       // [bufs][BR][pitch]
-    T* const gs = qs + C::kBufs * C::kTile;      // dout
-    T* const vs = gs + C::kBufs * C::kTile;      // [BKEYS][pitch] where V_LDS
-    float* const rows = (float*)(vs + C::kValues);  // [bufs][5][BR]: lse, delta, position, slope, document
+    typedef Lds<T, DP> L;
+    __shared__ __attribute__((aligned(1024))) char lds[C::kBytes];
+    char* const k_own = lds + C::kBufs * 2 * C::kTile;
+    char* const v_own = k_own + (C::K_LDS ? C::kOwn : 0);
+    float* const rows = (float*)(lds + C::kRows);  // [bufs][5][BR]: lse, delta, position, slope, document
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave % C::KG, rg = wave / C::KG;
 
-    const int total = p.tiles * p.Hk * p.B;
+    const int total = p.tiles * p.dk_splits * p.Hk * p.B;
     int id = by_die(blockIdx.x, total);
     if (id >= total) return;
+    const int split = id % p.dk_splits;
+    id /= p.dk_splits;
     const int tile = id % p.tiles;  // the first ones, which most rows see, first
     id /= p.tiles;
     const int c = id % p.Hk, b = id / p.Hk;
@@ -234,7 +209,7 @@ __global__ __launch_bounds__(C::NT) void key_gradient_kernel(const Params p) {
     const Band band(p);
     const Scoring sc(p);
     const int key_first = tile * C::BKEYS, key_last = min(key_first + C::BKEYS, n) - 1;
-    const int key = key_first + wave * 32 + (lane & 31);
+    const int key = key_first + kg * 32 + (lane & 31);
     const int doc = p.kdoc && key < n ? p.kdoc[b * p.kdoc_b + key * p.kdoc_l] : 0;
     const bool valid = key < n && doc >= 0;
     // rows at positions from .. to see this key (limits of the sequence aside), all rows where it is in the prefix
@@ -242,207 +217,300 @@ __global__ __launch_bounds__(C::NT) void key_gradient_kernel(const Params p) {
     if (key < prefix) from = -0x7fffffff, to = 0x7fffffff;
     if (!valid) from = 1, to = 0;
 
-    Frag kf[DP / 16], vf[C::V_LDS ? 1 : DP / 16];
+    Frag kf[C::K_LDS ? 1 : DP / 16], vf[C::V_LDS ? 1 : DP / 16];
     {
         const T* k = (const T*)p.k.data + b * p.k.b + key * p.k.l + c * p.k.h;
         const T* v = (const T*)p.v.data + b * p.v.b + key * p.v.l + c * p.v.h;
+        constexpr int N = sizeof(Frag) / 16;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
-            kf[s] = load_frag(k, s * 16 + half * 8, p.D, p.k.vec, valid);
-            const Frag f = load_frag(v, s * 16 + half * 8, p.D, p.v.vec, valid);
-            if (C::V_LDS) *(Frag*)(vs + (wave * 32 + (lane & 31)) * Lds<T, DP>::kPitch + s * 16 + half * 8) = f;
-            else vf[s] = f;
+            const Frag x = load_frag<VEC>(k, s * 16 + half * 8, p.D, valid), y = load_frag<VEC>(v, s * 16 + half * 8, p.D, valid);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int at = L::at(kg * 32 + (lane & 31), (2 * s + half) * N + i);
+                if (C::K_LDS && rg == 0) *(uint4*)(k_own + at) = ((const uint4*)&x)[i];
+                if (C::V_LDS && rg == 0) *(uint4*)(v_own + at) = ((const uint4*)&y)[i];
+            }
+            if (!C::K_LDS) kf[s] = x;
+            if (!C::V_LDS) vf[s] = y;
         }
     }
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) dk[d] = zero16(), dv[d] = zero16();
 
+    // Tiles of rows: BR queries of one head of the group.  Those that some key's band reaches, `len` a head, are numbered
+    // head by head; a split takes a run of the numbers.
+    const int i_first = key_first < prefix ? 0 : max(key_first - band.above - offset, 0);
+    const int i_last = key_first < prefix ? p.Lq - 1 : min(key_last + band.below - offset, p.Lq - 1);
+    const int t_first = i_first / C::BR, len = key_last >= key_first && i_last >= i_first ? i_last / C::BR + 1 - t_first : 0;
+    const int all = len * p.G, per = (all + p.dk_splits - 1) / p.dk_splits;
     const int2* const qr = p.qrange ? p.qrange + (int64_t)b * p.qranges : nullptr;
     int2 mine = {0, 0};
-    if (qr && key_last >= key_first) mine = document_range(p.krange + (int64_t)b * p.kranges, key_first, key_last);
-    auto needed = [&](int t) {
-        const int i0 = t * C::BR / p.G, i1 = (min((t + 1) * C::BR, p.R) - 1) / p.G;
-        if (key_first >= prefix && (i1 + offset < key_first - band.above || i0 + offset > key_last + band.below)) return false;
+    if (qr && len > 0) mine = document_range(p.krange + (int64_t)b * p.kranges, key_first, key_last);
+    auto needed = [&](int u) {
         if (!qr) return true;
-        const int2 theirs = document_range(qr, i0, i1);
+        const int i0 = (t_first + u % len) * C::BR;
+        const int2 theirs = document_range(qr, i0, min(i0 + C::BR, p.Lq) - 1);
         return theirs.x <= mine.y && mine.x <= theirs.y;
     };
-    Tiles<decltype(needed)> tiles(needed, 0, key_last >= key_first ? (p.R + C::BR - 1) / C::BR : 0);
+    Tiles<decltype(needed)> tiles(needed, split * per, min((split + 1) * per, all));
 
-    const T* const qb = (const T*)p.q.data + b * p.q.b + (int64_t)c * p.G * p.q.h;
-    const T* const gb = (const T*)p.dout.data + b * p.dout.b + (int64_t)c * p.G * p.dout.h;
-    const float* const lb = p.lse + b * p.lse_b + (int64_t)c * p.G * p.lse_h;
-    const float* const eb = p.delta + ((int64_t)b * p.Hk + c) * p.R;
-    Stage<T, DP, C::BR, C::NT> sq, sg;
+    typedef Copy<T, DP, C::BR, C::NT, VEC> Rows;
+    const Rows copy_q(p.q.l, p.D, tid), copy_g(p.dout.l, p.D, tid);
+    static_assert(C::NT >= C::BR, "one thread a row for what rows have beside features");
     float r_lse = 0.f, r_delta = 0.f, r_slope = 0.f;
     int r_at = 0, r_doc = 0;
-    // the row's log-sum, or -inf where it sees nothing: such rows are zero, whatever the arrays hold there
-    auto row_lse = [&](int r, int i, int g) { return r < p.R ? lb[i * p.lse_l + g * p.lse_h] : -__builtin_inff(); };
-    auto load_q = [&](int r0) {
-        sq.load([&](int x) {
-            const int r = r0 + x, i = r / p.G, g = r - i * p.G;
-            return row_lse(r, i, g) != -__builtin_inff() ? qb + i * p.q.l + g * p.q.h : (const T*)nullptr;
-        }, p.D, p.q.vec, tid);
+    int2 range = {0, 0}, now = {0, 0};
+    auto start = [&](int u, int buf) {
+        const int g = u / len, i0 = (t_first + u - g * len) * C::BR, h = c * p.G + g, left = p.Lq - i0;
+        char* const to_q = lds + buf * 2 * C::kTile;
+        copy_q.start(to_q, (const T*)p.q.data + b * p.q.b + i0 * p.q.l + h * p.q.h, p.q.l, left, p.D, tid);
+        copy_g.start(to_q + C::kTile, (const T*)p.dout.data + b * p.dout.b + i0 * p.dout.l + h * p.dout.h, p.dout.l, left, p.D, tid);
+        if (qr) range = document_range(qr, i0 + rg * 32, min(i0 + rg * 32 + 31, p.Lq - 1));
+        r_slope = p.slopes ? p.slopes[h * p.slope_stride] * kLog2e : 0.f;
+        if (tid < C::BR) {
+            const int i = min(i0 + tid, p.Lq - 1);
+            r_lse = tid < left ? p.lse[b * p.lse_b + i * p.lse_l + h * p.lse_h] : -__builtin_inff();
+            r_delta = p.delta[((int64_t)b * p.Hk * p.G + h) * p.Lq + i];
+            r_at = i + offset;
+            if (p.qdoc) r_doc = p.qdoc[b * p.qdoc_b + i * p.qdoc_l];
+        }
     };
-    auto load_g = [&](int r0) {
-        sg.load([&](int x) {
-            const int r = r0 + x, i = r / p.G, g = r - i * p.G;
-            return row_lse(r, i, g) != -__builtin_inff() ? gb + i * p.dout.l + g * p.dout.h : (const T*)nullptr;
-        }, p.D, p.dout.vec, tid);
-    };
-    static_assert(C::NT >= C::BR, "one thread a row for what rows have beside features");
-    auto load_r = [&](int r0) {
-        if (tid >= C::BR) return;
-        const int r = r0 + tid, i = r / p.G, g = r - i * p.G;
-        const float x = row_lse(r, i, g);
-        const bool some = x != -__builtin_inff();
-        r_lse = some ? x * kLog2e : __builtin_inff();  // p = exp2(z - inf) = 0
-        r_delta = some ? eb[r] : 0.f;
-        r_at = i + offset;
-        r_slope = p.slopes && some ? p.slopes[(c * p.G + g) * p.slope_stride] * kLog2e : 0.f;
-        r_doc = p.qdoc && some ? p.qdoc[b * p.qdoc_b + i * p.qdoc_l] : -1;
-    };
-    auto store_r = [&](int buf) {
-        if (tid >= C::BR) return;
-        float* to_rows = rows + buf * 5 * C::BR + tid;
-        to_rows[0] = r_lse;
-        to_rows[C::BR] = r_delta;
-        to_rows[2 * C::BR] = __int_as_float(r_at);
-        to_rows[3 * C::BR] = r_slope;
-        to_rows[4 * C::BR] = __int_as_float(r_doc);
+    auto finish = [&](int buf) {
+        wait_loads();
+        now = range;
+        float* const of = rows + buf * 5 * C::BR;
+        // A row that sees nothing (its log-sum is -inf) is zero, whatever the arrays hold there.
+        const bool none = tid < C::BR && r_lse == -__builtin_inff();
+        if (tid < C::BR) {
+            of[tid] = none ? __builtin_inff() : r_lse * kLog2e;  // p = exp2(z - inf) = 0
+            of[C::BR + tid] = none ? 0.f : r_delta;
+            of[2 * C::BR + tid] = __int_as_float(r_at);
+            of[3 * C::BR + tid] = r_slope;
+            of[4 * C::BR + tid] = __int_as_float(none ? -1 : r_doc);
+        }
+        if (__syncthreads_or(none)) {
+            char* const q = lds + buf * 2 * C::kTile;
+            Rows::clear(q, [&](int i) { return of[i] == __builtin_inff(); }, tid);
+            Rows::clear(q + C::kTile, [&](int i) { return of[i] == __builtin_inff(); }, tid);
+            __syncthreads();
+        }
     };
 
     int t = tiles.next(lane), buf = 0;
-    if (C::AHEAD == 2) {
-        if (t >= 0) {
-            load_q(t * C::BR);
-            load_g(t * C::BR);
-            load_r(t * C::BR);
-            sq.store(qs, tid);
-            sg.store(gs, tid);
-            store_r(0);
-        }
-        __syncthreads();
+    if (C::kBufs == 2 && t >= 0) {
+        start(t, 0);
+        finish(0);
     }
     while (t >= 0) {
         const int next = tiles.next(lane);
-        if (C::AHEAD == 2) {
-            if (next >= 0) {
-                load_q(next * C::BR);
-                load_g(next * C::BR);
-                load_r(next * C::BR);
-            }
+        if (C::kBufs == 2) {
+            if (next >= 0) start(next, buf ^ 1);
         } else {
             __syncthreads();
-            load_q(t * C::BR);
-            sq.store(qs, tid);
-            load_g(t * C::BR);
-            sg.store(gs, tid);
-            load_r(t * C::BR);
-            store_r(0);
-            __syncthreads();
+            start(t, 0);
+            finish(0);
         }
-        const T* qt = qs + buf * C::kTile;
-        const T* gt = gs + buf * C::kTile;
-        const float* rt = rows + buf * 5 * C::BR;
-#pragma unroll
-        for (int x = 0; x < C::BR / 32; ++x) {
-            const int q0 = x * 32, first_at = (t * C::BR + q0) / p.G + offset, last_at = (t * C::BR + q0 + 31) / p.G + offset;
-            const bool masked = p.qdoc || !__all(from <= first_at && last_at <= to);
+        const char* qt = lds + buf * 2 * C::kTile;
+        const char* gt = qt + C::kTile;
+        const int q0 = rg * 32;
+        const float* of = rows + buf * 5 * C::BR + q0 + 4 * half;  // what the rows of registers 4 g .. have: of[array BR + 8 g + e]
+        {
+            const int first_at = (t_first + t % len) * C::BR + q0 + offset;
+            const bool masked = !__all(from <= first_at && first_at + 31 <= to && (!p.qdoc || (now.x == doc && now.y == doc)));
             f32x16 s = zero16();
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) s = M::mma(rows_frag<T, DP>(qt, q0, k, lane), kf[k], s);
-            f32x16 bend;
-            const float* own = rt + q0 + 4 * half;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float z;
-                if (p.cap > 0.f) {
-                    const float y = tanh_of(s[i] * sc.cap_in);
-                    z = y * sc.cap_out;
-                    bend[i] = 1.f - y * y;
-                } else {
-                    z = s[i] * sc.scale2;
-                    bend[i] = 1.f;
-                }
-                const int at = __float_as_int(own[2 * C::BR + c_row(i)]);
-                if (p.slopes) z -= own[3 * C::BR + c_row(i)] * fabsf((float)(at - key));
-                float w = __builtin_amdgcn_exp2f(z - own[c_row(i)]);
-                if (masked) {
-                    bool sees = from <= at && at <= to;
-                    if (p.qdoc) sees = sees && __float_as_int(own[4 * C::BR + c_row(i)]) == doc;
-                    w = sees ? w : 0.f;
-                    bend[i] = sees ? bend[i] : 0.f;
-                }
-                s[i] = w;
-            }
+            for (int k = 0; k < DP / 16; ++k)
+                s = M::mma(rows_frag<T, DP>(qt, q0, k, lane), C::K_LDS ? rows_frag<T, DP>(k_own, kg * 32, k, lane) : kf[C::K_LDS ? 0 : k], s);
             f32x16 g = zero16();
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                if (C::V_LDS) g = M::mma(rows_frag<T, DP>(gt, q0, k, lane), rows_frag<T, DP>(vs, wave * 32, k, lane), g);
-                else g = M::mma(rows_frag<T, DP>(gt, q0, k, lane), vf[C::V_LDS ? 0 : k], g);
+            for (int k = 0; k < DP / 16; ++k)
+                g = M::mma(rows_frag<T, DP>(gt, q0, k, lane), C::V_LDS ? rows_frag<T, DP>(v_own, kg * 32, k, lane) : vf[C::V_LDS ? 0 : k], g);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4 delta = *(const f32x4*)(of + C::BR + c_row(i));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) g[i + e] -= delta[e];
+            }
+            if (p.cap > 0.f) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float y = tanh_of(s[i] * sc.cap_in);
+                    s[i] = y * sc.cap_out;
+                    g[i] *= 1.f - y * y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] *= sc.scale2;
+            }
+            if (p.slopes) {
+                const float slope = of[3 * C::BR];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] -= slope * fabsf((float)(first_at + 4 * half + c_row(i) - key));
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4 lse = *(const f32x4*)(of + c_row(i));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i + e] = __builtin_amdgcn_exp2f(s[i + e] - lse[e]);
+            }
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int at = first_at + 4 * half + c_row(i);
+                    bool sees = from <= at && at <= to;
+                    if (p.qdoc) sees = sees && __float_as_int(of[4 * C::BR + c_row(i)]) == doc;
+                    s[i] = sees ? s[i] : 0.f;
+                    g[i] = sees ? g[i] : 0.f;
+                }
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 Frag f;
                 to_frag(s, h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dv[d] = M::mma(cols_frag<DP>(gt, q0 + 16 * h, d * 32, lane), f, dv[d]);
+                for (int d = 0; d < DP / 32; ++d) dv[d] = M::mma(cols_frag<DP>((const T*)0, gt, q0 + 16 * h, d * 32, lane), f, dv[d]);
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = s[i] * (g[i] - own[C::BR + c_row(i)]) * bend[i];
+            for (int i = 0; i < 16; ++i) s[i] *= g[i];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 Frag f;
                 to_frag(s, h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dk[d] = M::mma(cols_frag<DP>(qt, q0 + 16 * h, d * 32, lane), f, dk[d]);
+                for (int d = 0; d < DP / 32; ++d) dk[d] = M::mma(cols_frag<DP>((const T*)0, qt, q0 + 16 * h, d * 32, lane), f, dk[d]);
             }
         }
-        if (C::AHEAD == 2) {
+        if (C::kBufs == 2 && next >= 0) {
             buf ^= 1;
-            if (next >= 0) {
-                sq.store(qs + buf * C::kTile, tid);
-                sg.store(gs + buf * C::kTile, tid);
-                store_r(buf);
-            }
-            __syncthreads();
+            finish(buf);
         }
         t = next;
     }
+    if (C::RG > 1) {
+        // the wavefronts that share keys add up, one sum after the other
+        float* const mine_f = (float*)lds + (kg * 32 + (lane & 31)) * (DP + 4) + 4 * half;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+            if (rg > 0) {
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        f32x4 x;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = which ? dv[d][4 * g + e] : dk[d][4 * g + e];
+                        *(f32x4*)(mine_f + (rg - 1) * C::BKEYS * (DP + 4) + d * 32 + 8 * g) = x;
+                    }
+            }
+            __syncthreads();
+            if (rg == 0) {
+#pragma unroll
+                for (int r = 0; r < C::RG - 1; ++r)
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const f32x4 x = *(const f32x4*)(mine_f + r * C::BKEYS * (DP + 4) + d * 32 + 8 * g);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) (which ? dv[d] : dk[d])[4 * g + e] += x[e];
+                        }
+            }
+        }
+        if (rg > 0) return;
+    }
     if (key >= p.Lk) return;
+    const int64_t part_at = ((((int64_t)split * p.B + b) * p.Hk + c) * p.Lk + key) * p.D;
     T* ko = (T*)p.dk.data + b * p.dk.b + key * p.dk.l + c * p.dk.h;
     T* vo = (T*)p.dv.data + b * p.dv.b + key * p.dv.l + c * p.dv.h;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
+            const int at = d * 32 + 8 * g + 4 * half;
             const float f[4] = {dk[d][4 * g] * p.scale, dk[d][4 * g + 1] * p.scale, dk[d][4 * g + 2] * p.scale, dk[d][4 * g + 3] * p.scale};
             const float e[4] = {dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
-            store4(ko, d * 32 + 8 * g + 4 * half, p.D, p.dk.vec, f);
-            store4(vo, d * 32 + 8 * g + 4 * half, p.D, p.dv.vec, e);
+            if (p.dk_splits > 1) {
+                store4(p.part_dk + part_at, at, p.D, (p.D & 3) == 0, f);
+                store4(p.part_dv + part_at, at, p.D, (p.D & 3) == 0, e);
+            } else {
+                store4(ko, at, p.D, p.dk.vec, f);
+                store4(vo, at, p.D, p.dv.vec, e);
+            }
         }
+}
+
+// Adds the parts of split walks: [splits][B][Hk][L G][D] to an array [B, L, Hk G, D], an element a thread at a time.
+template <class T>
+__global__ __launch_bounds__(256) void add_parts_kernel(const float* part, int splits, Tensor out, int B, int Hk, int L, int G, int D) {
+    const int64_t count = (int64_t)B * Hk * L * G * D;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < count; at += (int64_t)gridDim.x * 256) {
+        float f = 0.f;
+        for (int s = 0; s < splits; ++s) f += part[s * count + at];
+        const int64_t row = at / D;
+        const int d = (int)(at - row * D), r = (int)(row % ((int64_t)L * G)), i = r / G;
+        const int64_t bc = row / ((int64_t)L * G), b = bc / Hk;
+        ((T*)out.data)[b * out.b + i * out.l + ((bc - b * Hk) * G + r - i * G) * out.h + d] = (T)f;
+    }
 }
 
 template <class T, int DP>
 struct BackwardConfig {
     static constexpr int kRowBytes = DP * (int)sizeof(T);
-    typedef QueryConfig<T, DP, sizeof(T) == 2 ? 64 : 32, kRowBytes <= 512 ? 2 : 0> Q;
-    typedef KeyConfig<T, DP, kRowBytes <= 512 ? 4 : 2, 32, kRowBytes <= 512 ? 2 : 0, (kRowBytes > 512)> K;
+    // dq: rows and their gradients stay in registers; two workgroups a compute unit up to 128 features in bf16
+    typedef QueryConfig<T, DP, kRowBytes <= 256 ? 64 : 32, kRowBytes <= 768 ? 2 : 1, kRowBytes <= 256 && sizeof(T) == 2 ? 2 : 1> Q;
 };
+// keys and values in registers where the sums leave room for them, sums of 256 features and more with one wavefront a SIMD
+template <class T, int DP>
+struct KeyChoice { typedef KeyConfig<T, DP, 4, 1, 2, false, false, 1> K; };
+template <>
+struct KeyChoice<bf16, 32> { typedef KeyConfig<bf16, 32, 4, 2, 2, false, false, 2> K; };
+template <>
+struct KeyChoice<bf16, 64> { typedef KeyConfig<bf16, 64, 4, 2, 2, false, false, 2> K; };
+template <>
+struct KeyChoice<bf16, 96> { typedef KeyConfig<bf16, 96, 4, 2, 2, false, true, 2> K; };
+template <>
+struct KeyChoice<bf16, 128> { typedef KeyConfig<bf16, 128, 4, 2, 2, true, true, 2> K; };
+template <>
+struct KeyChoice<bf16, 256> { typedef KeyConfig<bf16, 256, 4, 1, 2, false, true, 1> K; };
+template <>
+struct KeyChoice<float, 128> { typedef KeyConfig<float, 128, 4, 1, 2, false, false, 1> K; };
+template <>
+struct KeyChoice<float, 192> { typedef KeyConfig<float, 192, 2, 1, 1, false, true, 1> K; };
+template <>
+struct KeyChoice<float, 256> { typedef KeyConfig<float, 256, 2, 1, 1, false, true, 1> K; };
+
+template <class T>
+void add_parts(const float* part, int splits, const Tensor& out, int B, int Hk, int L, int G, int D, hipStream_t stream) {
+    const int64_t count = (int64_t)B * Hk * L * G * D;
+    const unsigned blocks = (unsigned)std::min<int64_t>((count + 255) / 256, 4096);
+    if (blocks) add_parts_kernel<T><<<blocks, 256, 0, stream>>>(part, splits, out, B, Hk, L, G, D);
+    check_launch("adhip_attention_backward");
+}
 
 template <class T, int DP>
 void launch_backward(const Params& p, hipStream_t stream) {
     typedef typename BackwardConfig<T, DP>::Q Q;
-    typedef typename BackwardConfig<T, DP>::K K;
+    typedef typename KeyChoice<T, DP>::K K;
     Params x = p;
+    const bool vec = p.q.vec && p.k.vec && p.v.vec && p.out.vec && p.dout.vec;
     x.tiles = (p.R + Q::BQ - 1) / Q::BQ;
-    if (x.tiles > 0) query_gradient_kernel<T, DP, Q><<<die_grid((int64_t)x.tiles * p.Hk * p.B), Q::NT, 0, stream>>>(x);
+    unsigned grid = die_grid((int64_t)x.tiles * p.dq_splits * p.Hk * p.B);
+    if (grid > 0 && vec) query_gradient_kernel<T, DP, true, Q><<<grid, Q::NT, 0, stream>>>(x);
+    else if (grid > 0) query_gradient_kernel<T, DP, false, Q><<<grid, Q::NT, 0, stream>>>(x);
     check_launch("adhip_attention_backward");
+    if (p.dq_splits > 1) add_parts<T>(p.part_dq, p.dq_splits, p.dq, p.B, p.Hk, p.Lq, p.G, p.D, stream);
     x.tiles = (p.Lk + K::BKEYS - 1) / K::BKEYS;
-    if (x.tiles > 0) key_gradient_kernel<T, DP, K><<<die_grid((int64_t)x.tiles * p.Hk * p.B), K::NT, 0, stream>>>(x);
+    grid = die_grid((int64_t)x.tiles * p.dk_splits * p.Hk * p.B);
+    if (grid > 0 && vec) key_gradient_kernel<T, DP, true, K><<<grid, K::NT, 0, stream>>>(x);
+    else if (grid > 0) key_gradient_kernel<T, DP, false, K><<<grid, K::NT, 0, stream>>>(x);
     check_launch("adhip_attention_backward");
+    if (p.dk_splits > 1) {
+        add_parts<T>(p.part_dk, p.dk_splits, p.dk, p.B, p.Hk, p.Lk, 1, p.D, stream);
+        add_parts<T>(p.part_dv, p.dk_splits, p.dv, p.B, p.Hk, p.Lk, 1, p.D, stream);
+    }
 }
 
 template <class T>

@@ -14,26 +14,21 @@
 namespace adhip {
 namespace attn {
 
-// AHEAD 0: a tile is loaded when it is needed; 1: one tile ahead in registers, one LDS tile; 2: one ahead, two LDS tiles
-template <class T, int DP, int WQ_, int WK_, int BK_, int AHEAD_>
+// BUFS: tiles of keys in LDS; with two, one is under way while the other is worked on.
+// WAVES: wavefronts of a SIMD that registers must leave room for.
+template <class T, int DP, int WQ_, int WK_, int BK_, int BUFS, int WAVES_>
 struct ForwardConfig {
-    static constexpr int WQ = WQ_, WK = WK_, BK = BK_, AHEAD = AHEAD_;
+    static constexpr int WQ = WQ_, WK = WK_, BK = BK_, kBufs = BUFS, WAVES = WAVES_;
     static constexpr int NT = 64 * WQ * WK, BQ = 32 * WQ, KB = BK / (32 * WK);
-    static constexpr int kTile = BK * Lds<T, DP>::kPitch;
-    static constexpr int kBufs = AHEAD == 2 ? 2 : 1;
     static constexpr int kMerge = WK > 1 ? WK * 32 * (DP + 4) * 4 + WK * 64 * 4 : 0;
-    static constexpr int kLoop = kBufs * (2 * kTile * (int)sizeof(T) + BK * 4);
-    static constexpr int kBytes = kLoop > kMerge ? kLoop : kMerge;
 };
 
-template <class T, int DP, class C>
-__global__ __launch_bounds__(C::NT) void forward_kernel(const Params p) {
+template <class T, int DP, bool VEC, class C>
+__global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p) {
     typedef Matrix<T> M;
     typedef typename M::Frag Frag;
-    __shared__ __attribute__((aligned(16))) char lds[C::kBytes];
-    T* const ks = (T*)lds;                                         // [bufs][BK][pitch]
-    T* const vs = ks + C::kBufs * C::kTile;
-    int* const docs = (int*)(vs + C::kBufs * C::kTile);            // [bufs][BK]
+    typedef KeyTiles<T, DP, C, VEC> Keys;
+    __shared__ __attribute__((aligned(1024))) char lds[Keys::kBytes > C::kMerge ? Keys::kBytes : C::kMerge];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = wave % C::WQ, wk = wave / C::WQ;
 
@@ -68,7 +63,7 @@ __global__ __launch_bounds__(C::NT) void forward_kernel(const Params p) {
     {
         const T* q = (const T*)p.q.data + b * p.q.b + token * p.q.l + head * p.q.h;
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) qf[s] = load_frag(q, s * 16 + half * 8, p.D, p.q.vec, valid);
+        for (int s = 0; s < DP / 16; ++s) qf[s] = load_frag<VEC>(q, s * 16 + half * 8, p.D, valid);
     }
     f32x16 o[DP / 32];
 #pragma unroll
@@ -76,9 +71,10 @@ __global__ __launch_bounds__(C::NT) void forward_kernel(const Params p) {
     float m = -__builtin_inff(), l = 0.f;
 
     // tiles of keys that some row of this workgroup sees
-    const int n_tiles = (n + C::BK - 1) / C::BK, per = (n_tiles + p.splits - 1) / p.splits;
-    const int t_begin = split * per, t_end = min(t_begin + per, n_tiles);
     const int hi_all = last + offset + band.above, lo_all = first + offset - band.below;
+    const int t_first = prefix > 0 ? 0 : max(lo_all, 0) / C::BK, t_stop = (min(n, max(hi_all + 1, prefix)) + C::BK - 1) / C::BK;
+    const int per = max(0, t_stop - t_first + p.splits - 1) / p.splits;
+    const int t_begin = t_first + split * per, t_end = min(t_begin + per, t_stop);
     const int2* const kr = p.krange ? p.krange + (int64_t)b * p.kranges : nullptr;
     int2 mine = {0, 0};
     if (kr) mine = document_range(p.qrange + (int64_t)b * p.qranges, first, last);
@@ -91,57 +87,15 @@ __global__ __launch_bounds__(C::NT) void forward_kernel(const Params p) {
     };
     Tiles<decltype(needed)> tiles(needed, t_begin, t_end);
 
-    const T* const kb = (const T*)p.k.data + b * p.k.b + c * p.k.h;
-    const T* const vb = (const T*)p.v.data + b * p.v.b + c * p.v.h;
-    const int* const kd = p.kdoc ? p.kdoc + b * p.kdoc_b : nullptr;
-    Stage<T, DP, C::BK, C::NT> sk, sv;
-    int sd = 0;
-    // keys behind the sequence or of no document are zero, whatever the arrays hold there
-    auto used = [&](int j) { return j < n && !(kd && kd[j * p.kdoc_l] < 0); };
-    auto load_k = [&](int j0) { sk.load([&](int i) { return used(j0 + i) ? kb + (j0 + i) * p.k.l : (const T*)nullptr; }, p.D, p.k.vec, tid); };
-    auto load_v = [&](int j0) { sv.load([&](int i) { return used(j0 + i) ? vb + (j0 + i) * p.v.l : (const T*)nullptr; }, p.D, p.v.vec, tid); };
-    auto load_d = [&](int j0) { if (kd && tid < C::BK) sd = j0 + tid < n ? kd[(j0 + tid) * p.kdoc_l] : -1; };
-    auto load = [&](int t) {
-        load_k(t * C::BK);
-        load_v(t * C::BK);
-        load_d(t * C::BK);
-    };
-    static_assert(C::NT >= C::BK, "one thread a key for the documents");
-    auto store_d = [&](int buf) { if (kd && tid < C::BK) docs[buf * C::BK + tid] = sd; };
-    auto store = [&](int buf) {
-        sk.store(ks + buf * C::kTile, tid);
-        sv.store(vs + buf * C::kTile, tid);
-        store_d(buf);
-    };
-
+    Keys kt(p, b, c, n, tid, wk * C::KB * 32, lds);
     int t = tiles.next(lane), buf = 0;
-    if (C::AHEAD && t >= 0) load(t);
-    if (C::AHEAD == 2) {
-        if (t >= 0) store(0);
-        __syncthreads();
-    }
+    kt.begin(t);
     while (t >= 0) {
         const int next = tiles.next(lane);
-        if (C::AHEAD == 2) {
-            if (next >= 0) load(next);
-        } else if (C::AHEAD == 1) {
-            __syncthreads();
-            store(0);
-            __syncthreads();
-            if (next >= 0) load(next);
-        } else {
-            __syncthreads();
-            load_k(t * C::BK);
-            sk.store(ks, tid);
-            load_v(t * C::BK);
-            sv.store(vs, tid);
-            load_d(t * C::BK);
-            store_d(0);
-            __syncthreads();
-        }
-        const T* kt = ks + buf * C::kTile;
-        const T* vt = vs + buf * C::kTile;
-        const int* dt = docs + buf * C::BK;
+        kt.fetch(t, next, buf);
+        const char* ks = kt.keys(buf);
+        const char* vs = kt.values(buf);
+        const int* docs = kt.docs(buf);
         f32x16 s[C::KB];
         float top = -__builtin_inff();
 #pragma unroll
@@ -149,7 +103,7 @@ __global__ __launch_bounds__(C::NT) void forward_kernel(const Params p) {
             const int key0 = (wk * C::KB + x) * 32;
             s[x] = zero16();
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) s[x] = M::mma(rows_frag<T, DP>(kt, key0, k, lane), qf[k], s[x]);
+            for (int k = 0; k < DP / 16; ++k) s[x] = M::mma(rows_frag<T, DP>(ks, key0, k, lane), qf[k], s[x]);
             const int j0 = t * C::BK + key0, jl = j0 + 4 * half;
             if (p.cap > 0.f) {
 #pragma unroll
@@ -163,12 +117,12 @@ __global__ __launch_bounds__(C::NT) void forward_kernel(const Params p) {
                 for (int i = 0; i < 16; ++i) s[x][i] -= slope * fabsf((float)(at - jl - c_row(i)));
             }
             // masks only where some row of the wavefront does not see all 32 keys
-            if (kd || !__all(j0 + 31 < n && ((lo <= j0 && j0 + 31 <= hi) || j0 + 31 < pre))) {
+            if (!__all(j0 + 31 < n && ((lo <= j0 && j0 + 31 <= hi) || j0 + 31 < pre) && kt.one_document(x, doc))) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int j = jl + c_row(i);
                     bool sees = j < n && (j < pre || (lo <= j && j <= hi));
-                    if (kd) sees = sees && dt[key0 + 4 * half + c_row(i)] == doc;
+                    if (kt.kd) sees = sees && docs[key0 + 4 * half + c_row(i)] == doc;
                     s[x][i] = sees ? s[x][i] : -__builtin_inff();
                 }
             }
@@ -199,14 +153,10 @@ __global__ __launch_bounds__(C::NT) void forward_kernel(const Params p) {
                 Frag f;
                 to_frag(s[x], h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) o[d] = M::mma(cols_frag<DP>(vt, key0 + 16 * h, d * 32, lane), f, o[d]);
+                for (int d = 0; d < DP / 32; ++d) o[d] = M::mma(cols_frag<DP>((const T*)0, vs, key0 + 16 * h, d * 32, lane), f, o[d]);
             }
         }
-        if (C::AHEAD == 2) {
-            buf ^= 1;
-            if (next >= 0) store(buf);
-            __syncthreads();
-        }
+        kt.advance(next, buf);
         t = next;
     }
     l += __shfl_xor(l, 32);
@@ -320,20 +270,24 @@ __global__ __launch_bounds__(256) void join_kernel(const Params p) {
 
 template <class T, int DP>
 struct ForwardMany {
-    // f32 at 128 features and more: 32 keys a tile, or two tiles of keys and values would not fit LDS twice
-    typedef ForwardConfig<T, DP, 4, 1, sizeof(T) == 2 ? 64 : 32, 2> C;
+    // 64 keys a tile; 32 where two tiles of 64 would not leave room for a second workgroup or, at 512 bytes a feature row and
+    // more, not fit
+    static constexpr int kRowBytes = DP * (int)sizeof(T);
+    typedef ForwardConfig<T, DP, 4, 1, kRowBytes <= 256 ? 64 : 32, 2, kRowBytes <= 256 ? 2 : 1> C;
 };
 template <class T, int DP>
 struct ForwardFew {
     static constexpr int kRowBytes = DP * (int)sizeof(T);
-    // as many wavefronts along the keys as fit LDS; above 512 bytes a row no registers are left to load ahead
+    // as many wavefronts along the keys as LDS holds tiles for twice
     static constexpr int WK = kRowBytes <= 256 ? 4 : kRowBytes <= 512 ? 2 : 1;
-    typedef ForwardConfig<T, DP, 1, WK, 32 * WK, kRowBytes <= 512 ? 1 : 0> C;
+    typedef ForwardConfig<T, DP, 1, WK, 32 * WK, 2, 1> C;
 };
 
 template <class T, int DP, class C>
 void launch_forward(const Params& p, hipStream_t stream) {
-    forward_kernel<T, DP, C><<<die_grid((int64_t)p.tiles * p.splits * p.Hk * p.B), C::NT, 0, stream>>>(p);
+    const unsigned grid = die_grid((int64_t)p.tiles * p.splits * p.Hk * p.B);
+    if (p.q.vec && p.k.vec && p.v.vec) forward_kernel<T, DP, true, C><<<grid, C::NT, 0, stream>>>(p);
+    else forward_kernel<T, DP, false, C><<<grid, C::NT, 0, stream>>>(p);
     check_launch("adhip_attention");
     if (p.splits > 1) {
         join_kernel<T><<<(unsigned)(((int64_t)p.B * p.Hk * p.R + 3) / 4), 256, 0, stream>>>(p);
