@@ -3,8 +3,8 @@
 are behind the C ABI (`adhip_rotary`, `adhip_attention`, `adhip_attention_backward`, `adhip_adamw` in include/adhip.h,
 where the formulas stand); they have no counterpart in the reference.
 
-An array is a `DeviceArray` (`DeviceArray.empty`, `DeviceArray.of`, `program_array`) or anything with `data_ptr()`,
-`shape`, `stride()` and `dtype` on the device's memory, such as a torch tensor.  Every call queues its kernels on `stream`
+An array is a `DeviceArray` (`DeviceArray.empty`, `DeviceArray.of`, `program_array`) or anything on the device's memory with
+`data_ptr()`, `shape`, `stride()` and `dtype` (for AdamW also `numel()` and `is_contiguous()`), such as a torch tensor.  Every call queues its kernels on `stream`
 (a hipStream_t as an integer, for instance `torch.cuda.current_stream().cuda_stream`; the device's own stream where it is
 not given) and returns: results are there when the stream has got to them, and arrays and workspaces must live and keep
 still until then.  Nothing is allocated and nothing is kept between calls.
@@ -58,6 +58,12 @@ class DeviceArray:
 
     def data_ptr(self) -> int:
         return self._data
+
+    def numel(self) -> int:
+        return math.prod(self.shape)
+
+    def is_contiguous(self) -> bool:
+        return True
 
     def stride(self):
         out, n = [], 1
@@ -121,24 +127,43 @@ def synchronize(dev) -> None:
 # ---- the C structs, packed without a ctypes object per field: a call's own cost counts where one token is decoded ----
 
 _ARRAY = struct.Struct("=Qii8q")
+_PACK_ARRAY = _ARRAY.pack
 _NONE = bytes(_ARRAY.size)
 _ZEROS = (0, 0, 0, 0)
 _PADS = [(0,) * (4 - n) for n in range(5)]
 _ROTARY_TAIL = struct.Struct("=ii")
 _ATTENTION_TAIL = struct.Struct("=ffiiqQQ")
-_ADAMW_TENSOR = struct.Struct("=12q")
 _ADAMW = struct.Struct("=Qqiiii6d")
+_NO_MORE = _NONE * 11 + bytes(_ATTENTION_TAIL.size)
+
+
+_kinds = {}  # type objects met so far -> our number of the type
+
+
+def _kind(dtype) -> int:
+    kind = _kinds.get(dtype)
+    if kind is None:
+        kind = _TYPES.get(str(dtype))
+        if kind is None:
+            raise ValueError(f"arrays of type {dtype} are not supported")
+        _kinds[dtype] = kind
+    return kind
 
 
 def _array(a) -> bytes:
     if a is None:
         return _NONE
-    kind = _TYPES.get(str(a.dtype))
-    shape = tuple(a.shape)
-    if kind is None or len(shape) > 4:
-        raise ValueError(f"arrays of type {a.dtype} and {len(shape)} dims are not supported")
-    pad = _PADS[len(shape)]
-    return _ARRAY.pack(a.data_ptr(), kind, len(shape), *shape, *pad, *a.stride(), *pad)
+    shape = a.shape
+    n = len(shape)
+    kind = _kinds.get(a.dtype)
+    if kind is None:
+        kind = _kind(a.dtype)
+    if n == 4:
+        return _PACK_ARRAY(a.data_ptr(), kind, 4, *shape, *a.stride())
+    if n > 4:
+        raise ValueError(f"arrays of {n} dims are not supported")
+    pad = _PADS[n]
+    return _PACK_ARRAY(a.data_ptr(), kind, n, *shape, *pad, *a.stride(), *pad)
 
 
 def _declared(lib):
@@ -165,7 +190,8 @@ def _declared(lib):
 
 
 def _lib(dev):
-    return _declared(dev._lib)
+    lib = dev._lib
+    return lib if getattr(lib, "_adhip_operators", False) else _declared(lib)
 
 
 def _check(dev, rc: int, what: str) -> None:
@@ -232,15 +258,18 @@ def _attention_args(q, k, v, out=None, lse=None, out_grad=None, q_grad=None, k_g
     room, room_bytes = 0, 0
     if workspace is not None:
         room, room_bytes = workspace.data_ptr(), workspace.nbytes
-    return (_array(q) + _array(k) + _array(v) + _array(out) + _array(lse) + _array(slopes) + _array(lengths) + _array(prefix)
-            + _array(query_documents) + _array(key_documents) + _array(out_grad) + _array(q_grad) + _array(k_grad) + _array(v_grad)
+    return (_array(q) + _array(k) + _array(v) + _array(out) + _array(lse)
+            + (_NONE * 5 if slopes is lengths is prefix is query_documents is key_documents is None else
+               b"".join([_array(a) for a in (slopes, lengths, prefix, query_documents, key_documents)]))
+            + (_NONE * 4 if out_grad is q_grad is k_grad is v_grad is None else
+               b"".join([_array(a) for a in (out_grad, q_grad, k_grad, v_grad)]))
             + _ATTENTION_TAIL.pack(scale, cap, bool(causal), 0, window, room, room_bytes))
 
 
 def attention_workspace(dev, q, k, v, *, backward: bool = False) -> int:
     """Bytes of workspace that `attention`, and with `backward` also `attention_backward`, take on arrays of these shapes."""
     need = ctypes.c_size_t()
-    args = _attention_args(q, k, v)
+    args = _array(q) + _array(k) + _array(v) + _NO_MORE
     _check(dev, _lib(dev).adhip_attention_workspace(dev._ctx, args, bool(backward), ctypes.byref(need)), "adhip_attention_workspace")
     return need.value
 
@@ -270,20 +299,21 @@ def attention_backward(dev, q, k, v, out, lse, out_grad, q_grad, k_grad, v_grad,
 # ---- AdamW ----------------------------------------------------------------------------------------------------------
 
 
-def _is_packed(a) -> bool:
-    n = 1
-    for d, s in zip(reversed(tuple(a.shape)), reversed(tuple(a.stride()))):
-        if d != 1 and s != n:
-            return False
-        n *= d
-    return True
-
-
-def _one_type(name, arrays, allowed) -> int:
-    kinds = {_TYPES.get(str(a.dtype)) for a in arrays}
+def _one_kind(name, arrays, allowed) -> int:
+    kinds = {_kind(t) for t in {a.dtype for a in arrays}}
     if len(kinds) != 1 or not kinds <= allowed:
         raise ValueError(f"{name} must all have one supported type, not {sorted({str(a.dtype) for a in arrays})}")
     return kinds.pop()
+
+
+def _addresses(name, arrays, counts) -> List[int]:
+    """Where the packed arrays begin, of these numbers of elements."""
+    if [a.numel() for a in arrays] != counts or not all([a.is_contiguous() for a in arrays]):
+        if len(arrays) != len(counts):
+            raise ValueError(f"{len(arrays)} {name} for {len(counts)} parameters")
+        i = next(i for i, (a, n) in enumerate(zip(arrays, counts)) if a.numel() != n or not a.is_contiguous())
+        raise ValueError(f"{name}[{i}] is {list(arrays[i].shape)}: {counts[i]} packed elements are wanted")
+    return [a.data_ptr() for a in arrays]
 
 
 def adamw(dev, parameters: List, gradients: List, first: List, second: List, *, step: int, rate: float, beta1: float = 0.9,
@@ -294,43 +324,37 @@ def adamw(dev, parameters: List, gradients: List, first: List, second: List, *, 
     """One AdamW step on every tensor of the list: parameters and gradients f32 or bf16, moments `first` and `second` f32 of
     the parameters' sizes, or float8_e4m3fn codes [blocks, 256] with f32 scales [blocks] (`adamw_blocks`).  In place where
     no *_out list is given.  Arrays are packed."""
-    outs = (parameters_out or parameters, first_out or first, second_out or second)
-    lists = {"parameters": parameters, "gradients": gradients, "first": first, "second": second, "parameters_out": outs[0],
-             "first_out": outs[1], "second_out": outs[2]}
     n = len(parameters)
     if n == 0:
         return
-    p_type = _one_type("parameters", list(parameters) + list(outs[0]), {F32, BF16})
-    g_type = _one_type("gradients", gradients, {F32, BF16})
-    state = _one_type("moments", list(first) + list(second) + list(outs[1]) + list(outs[2]), {F32, E4M3})
-    scales = []
+    counts = [p.numel() for p in parameters]
+    p_type = _one_kind("parameters", parameters, {F32, BF16})
+    g_type = _one_kind("gradients", gradients, {F32, BF16})
+    state = _one_kind("moments", [*first, *second], {F32, E4M3})
+    blocks = [-(-c // ADAMW_BLOCK) for c in counts]
+    held = counts if state == F32 else [b * ADAMW_BLOCK for b in blocks]
+    none = [0] * n
+    columns = [_addresses("parameters", parameters, counts), _addresses("gradients", gradients, counts),
+               _addresses("first", first, held), _addresses("second", second, held)]
+    scales = [none, none]
     if state == E4M3:
         if first_scales is None or second_scales is None:
             raise ValueError("moments in 8 bits want first_scales and second_scales")
-        scales = [first_scales, second_scales, first_scales_out or first_scales, second_scales_out or second_scales]
-        for name, s in zip(("first_scales", "second_scales", "first_scales_out", "second_scales_out"), scales):
-            _one_type(name, s, {F32})
-            lists[name] = s
-    for name, arrays in lists.items():
-        if len(arrays) != n:
-            raise ValueError(f"{len(arrays)} {name} for {n} parameters")
-    counts = [math.prod(p.shape) for p in parameters]
-    for name, arrays in lists.items():
-        for i, a in enumerate(arrays):
-            want, blocks = counts[i], -(-counts[i] // ADAMW_BLOCK)
-            if "scales" in name:
-                want = blocks
-            elif state == E4M3 and name in ("first", "second", "first_out", "second_out"):
-                want = blocks * ADAMW_BLOCK
-            if math.prod(a.shape) != want or not _is_packed(a):
-                raise ValueError(f"{name}[{i}] is {list(a.shape)}: {want} packed elements are wanted")
-    tensors = bytearray()
-    for i in range(n):
-        s = [x[i].data_ptr() for x in scales] if scales else _ZEROS
-        tensors += _ADAMW_TENSOR.pack(parameters[i].data_ptr(), gradients[i].data_ptr(), first[i].data_ptr(), second[i].data_ptr(), s[0], s[1],
-                                      outs[0][i].data_ptr(), outs[1][i].data_ptr(), outs[2][i].data_ptr(), s[2], s[3], counts[i])
-    held = ctypes.create_string_buffer(bytes(tensors), len(tensors))
-    args = _ADAMW.pack(ctypes.addressof(held), n, p_type, g_type, state, step, rate, beta1, beta2, eps, decay, grad_scale)
+        _one_kind("scales", [*first_scales, *second_scales], {F32})
+        scales = [_addresses("first_scales", first_scales, blocks), _addresses("second_scales", second_scales, blocks)]
+    outs = []
+    for name, arrays, own, size, kind in (("parameters_out", parameters_out, columns[0], counts, p_type),
+                                          ("first_out", first_out, columns[2], held, state), ("second_out", second_out, columns[3], held, state),
+                                          ("first_scales_out", first_scales_out if state == E4M3 else None, scales[0], blocks, F32),
+                                          ("second_scales_out", second_scales_out if state == E4M3 else None, scales[1], blocks, F32)):
+        if arrays is not None:
+            _one_kind(name, arrays, {kind})
+            own = _addresses(name, arrays, size)
+        outs.append(own)
+    flat = [x for row in zip(*columns, *scales, *outs, counts) for x in row]
+    tensors = struct.pack(f"={12 * n}q", *flat)
+    held_bytes = ctypes.c_char_p(tensors)
+    args = _ADAMW.pack(ctypes.cast(held_bytes, ctypes.c_void_p).value, n, p_type, g_type, state, step, rate, beta1, beta2, eps, decay, grad_scale)
     _check(dev, _lib(dev).adhip_adamw(dev._ctx, args, _stream(dev, stream)), "adhip_adamw")
 
 

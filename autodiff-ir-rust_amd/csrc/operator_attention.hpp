@@ -187,20 +187,21 @@ __device__ __forceinline__ void store4(T* row, int d, int D, int vec, const floa
     }
 }
 
-// tanh to about 2e-7 of one: what a capped score takes, in units of the cap
-__device__ __forceinline__ float tanh_of(float x) {
-    const float e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e));
-    return 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+// tanh(x) from y = 2 x log2 e, to about 2e-7: what a capped score takes, in units of the cap
+__device__ __forceinline__ float tanh_of(float y) {
+    const float e = __builtin_amdgcn_exp2f(y);
+    return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
 }
 
 // row of register i of a C tile
 __device__ __forceinline__ constexpr int c_row(int i) { return 8 * (i >> 2) + (i & 3); }
 
-// Scores in units of log 2 from raw products
+// How raw products become scores in units of log 2: tanh(raw bend) where they are capped, then times unit, then the
+// distance's part.
 struct Scoring {
-    float scale2, cap_in, cap_out;  // scale log2 e; scale / cap, cap log2 e
+    float bend, unit;  // 2 log2 e scale / cap; cap log2 e, or scale log2 e
     __device__ __forceinline__ explicit Scoring(const Params& p)
-        : scale2(p.scale * kLog2e), cap_in(p.cap > 0.f ? p.scale / p.cap : 0.f), cap_out(p.cap * kLog2e) {}
+        : bend(p.cap > 0.f ? 2.f * kLog2e * p.scale / p.cap : 0.f), unit((p.cap > 0.f ? p.cap : p.scale) * kLog2e) {}
 };
 
 // Positions that a query sees: j < n and (j < prefix or lo <= j <= hi).  lo and hi by the query's own position.
@@ -229,20 +230,27 @@ __device__ __forceinline__ int2 document_range(const int2* ranges, int first, in
     return r;
 }
 
-// Walks the tiles that a block needs, 64 candidates at a time: each lane decides on one, all wavefronts alike.
+// Walks the tiles begin .. stop - 1 that a block needs, 64 candidates at a time: each lane decides on one, all wavefronts
+// alike.  Of those needed, split s of S takes numbers s, s + S, ..: the splits' shares are even whatever the masks leave.
 template <class Needed>
 struct Tiles {
     const Needed& needed;
-    int base, end;
+    int base, end, split, splits, seen = 0;
     unsigned long long mask = 0;
-    __device__ __forceinline__ Tiles(const Needed& f, int begin, int stop) : needed(f), base(begin - 64), end(stop) {}
+    __device__ __forceinline__ Tiles(const Needed& f, int begin, int stop, int split_, int splits_)
+        : needed(f), base(begin - 64), end(stop), split(split_), splits(splits_) {}
     // the next tile, or -1
     __device__ __forceinline__ int next(int lane) {
         while (!mask) {
             base += 64;
             if (base >= end) return -1;
-            const int t = base + lane;
-            mask = __ballot(t < end && needed(t));
+            const bool mine = base + lane < end && needed(base + lane);
+            mask = __ballot(mine);
+            if (splits > 1) {
+                const int number = seen + __popcll(mask & ((1ull << lane) - 1));
+                seen += __popcll(mask);
+                mask = __ballot(mine && number % splits == split);
+            }
         }
         const int t = base + __builtin_ctzll(mask);
         mask &= mask - 1;
@@ -250,14 +258,35 @@ struct Tiles {
     }
 };
 
-// Consecutive workgroups go to the eight dies in turn; this gives each die a run of consecutive numbers instead, so that
-// tiles that share keys share an L2.  The grid is rounded up to a multiple of eight; numbers from `total` on do nothing.
-__device__ __forceinline__ int by_die(int block, int total) {
-    const int each = (total + 7) / 8;
-    return (block & 7) * each + (block >> 3);
-}
-inline unsigned die_grid(int64_t total) { return (unsigned)((total + 7) / 8 * 8); }
+// What a workgroup works on.  Workgroups are given out in the order of their numbers, to the eight dies in turn: numbers run
+// over key heads and sequences first, so that a key head stays on as few dies as their count allows (one, where it is a
+// multiple of eight) and its keys in their L2, and over tiles from the longest walk to the shortest, so that the short ones
+// fill the end.
+struct Place {
+    int tile, split, c, b;
+    __device__ __forceinline__ Place(const Params& p, int splits) {
+        unsigned id = blockIdx.x;
+        const unsigned pairs = p.Hk * p.B, pair = id % pairs;
+        id /= pairs;
+        b = pair / p.Hk;
+        c = pair % p.Hk;
+        split = id % splits;
+        tile = id / splits;
+    }
+};
 
+// A load of 16 bytes a lane that writes LDS by itself: lane i's go to `to` + 16 i, from `base` (of the whole wavefront) and the
+// lane's offset; an offset behind the resource's end gives zeros.  It stands here as the instruction because the compiler
+// orders every later read of LDS behind the one it knows of, and so would wait for a tile that is not needed before the
+// next step; wait_loads() and a barrier stand where it is.  No register is written, so none can be written late.
+__device__ __forceinline__ void load_to_lds(const void* base, unsigned offset, char* to) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    const uintptr_t a = (uintptr_t)base;
+    const u32x4 source = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a),
+                          (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)) & 0xffffu, 0x7fffffffu, 0x00020000u};
+    const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)to);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(source) : "memory");
+}
 // Waits for this wavefront's loads to LDS.
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -286,14 +315,12 @@ struct Copy {
     // from: the first row; rows: how many there are (at least one)
     __device__ __forceinline__ void start(char* tile, const T* from, int64_t stride, int rows, int D, int tid) const {
         if (VEC) {
-            const __amdgpu_buffer_rsrc_t source = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, 0x7fffffff, 0x00020000);
-            typedef __attribute__((address_space(3))) void* To;
             const bool whole = rows >= ROWS;
 #pragma unroll
             for (int c = 0; c < kEach; ++c) {
                 if (kTotal % NT != 0 && (wave * 64 + c * NT) >= kTotal) break;
                 const unsigned o = whole || row(c, tid) < rows ? offset[c] : kNowhere;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(source, (To)(tile + (wave * 64 + c * NT) * 16), 16, o, 0, 0, 0);
+                load_to_lds(from, o, tile + (wave * 64 + c * NT) * 16);
             }
         } else {
 #pragma unroll 1

@@ -30,19 +30,14 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    const int total = p.tiles * p.dq_splits * p.Hk * p.B;
-    int id = by_die(blockIdx.x, total);
-    if (id >= total) return;
-    const int tile = p.tiles - 1 - id % p.tiles;  // the last ones, which see most keys, first
-    id /= p.tiles;
-    const int split = id % p.dq_splits;
-    id /= p.dq_splits;
-    const int c = id % p.Hk, b = id / p.Hk;
+    const Place place(p, p.dq_splits);
+    const int tile = p.tiles - 1 - place.tile, split = place.split, c = place.c, b = place.b;  // the last ones see most keys
 
     const int n = sequence_length(p, b), offset = n - p.Lq;
     const int prefix = p.prefix ? min(max(p.prefix[b * p.prefix_s], 0), n) : 0;
     const Band band(p);
     const Scoring sc(p);
+    const float unit = p.slopes ? 1.f : sc.unit;
     const int row0 = tile * C::BQ, row1 = min(row0 + C::BQ, p.R) - 1;
     const int first = row0 / p.G, last = row1 / p.G;
 
@@ -83,8 +78,6 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
 
     const int hi_all = last + offset + band.above, lo_all = first + offset - band.below;
     const int t_first = prefix > 0 ? 0 : max(lo_all, 0) / C::BK, t_stop = (min(n, max(hi_all + 1, prefix)) + C::BK - 1) / C::BK;
-    const int per = max(0, t_stop - t_first + p.dq_splits - 1) / p.dq_splits;
-    const int t_begin = t_first + split * per, t_end = min(t_begin + per, t_stop);
     const int2* const kr = p.krange ? p.krange + (int64_t)b * p.kranges : nullptr;
     int2 mine = {0, 0};
     if (kr) mine = document_range(p.qrange + (int64_t)b * p.qranges, first, last);
@@ -95,7 +88,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
         const int2 theirs = document_range(kr, j0, j1);
         return theirs.x <= mine.y && mine.x <= theirs.y;
     };
-    Tiles<decltype(needed)> tiles(needed, t_begin, t_end);
+    Tiles<decltype(needed)> tiles(needed, t_first, t_stop, split, p.dq_splits);
 
     Keys kt(p, b, c, n, tid, 0, lds);
     int t = tiles.next(lane), buf = 0;
@@ -109,32 +102,28 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
 #pragma unroll
         for (int x = 0; x < C::KB; ++x) {
             const int key0 = x * 32;
-            f32x16 s = zero16(), g = zero16();
+            f32x16 s = zero16(), g;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) g[i] = -delta;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) s = M::mma(rows_frag<T, DP>(ks, key0, k, lane), qf[k], s);
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) g = M::mma(rows_frag<T, DP>(vs, key0, k, lane), df[k], g);
             const int j0 = t * C::BK + key0, jl = j0 + 4 * half;
             const bool masked = !__all(j0 + 31 < n && ((lo <= j0 && j0 + 31 <= hi) || j0 + 31 < pre) && kt.one_document(x, doc));
-#pragma unroll
-            for (int i = 0; i < 16; ++i) g[i] -= delta;
             if (p.cap > 0.f) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float y = tanh_of(s[i] * sc.cap_in);
-                    s[i] = y * sc.cap_out;
-                    g[i] *= 1.f - y * y;
+                    s[i] = tanh_of(s[i] * sc.bend);
+                    g[i] *= 1.f - s[i] * s[i];
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] *= sc.scale2;
             }
             if (p.slopes) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] -= slope * fabsf((float)(at - jl - c_row(i)));
+                for (int i = 0; i < 16; ++i) s[i] = s[i] * sc.unit - slope * fabsf((float)(at - jl - c_row(i)));
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] - lse2) * g[i];
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], unit, -lse2)) * g[i];
             if (masked) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -178,7 +167,7 @@ struct KeyConfig {
     static constexpr bool K_LDS = K_LDS_, V_LDS = V_LDS_;
     static constexpr int kTile = BR * Lds<T, DP>::kPitch, kOwn = BKEYS * Lds<T, DP>::kPitch;
     static constexpr int kRows = kBufs * 2 * kTile + (K_LDS ? kOwn : 0) + (V_LDS ? kOwn : 0);
-    static constexpr int kLoop = kRows + kBufs * BR * 5 * 4;
+    static constexpr int kLoop = kRows + kBufs * BR * 4 * 4;
     static constexpr int kMerge = RG > 1 ? (RG - 1) * BKEYS * (DP + 4) * 4 : 0;
     static constexpr int kBytes = kLoop > kMerge ? kLoop : kMerge;
 };
@@ -191,23 +180,18 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
     __shared__ __attribute__((aligned(1024))) char lds[C::kBytes];
     char* const k_own = lds + C::kBufs * 2 * C::kTile;
     char* const v_own = k_own + (C::K_LDS ? C::kOwn : 0);
-    float* const rows = (float*)(lds + C::kRows);  // [bufs][5][BR]: lse, delta, position, slope, document
+    float* const rows = (float*)(lds + C::kRows);  // [bufs][4][BR]: lse, -delta, slope, document
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave % C::KG, rg = wave / C::KG;
 
-    const int total = p.tiles * p.dk_splits * p.Hk * p.B;
-    int id = by_die(blockIdx.x, total);
-    if (id >= total) return;
-    const int split = id % p.dk_splits;
-    id /= p.dk_splits;
-    const int tile = id % p.tiles;  // the first ones, which most rows see, first
-    id /= p.tiles;
-    const int c = id % p.Hk, b = id / p.Hk;
+    const Place place(p, p.dk_splits);
+    const int tile = place.tile, split = place.split, c = place.c, b = place.b;  // the first ones are seen by most rows
 
     const int n = sequence_length(p, b), offset = n - p.Lq;
     const int prefix = p.prefix ? min(max(p.prefix[b * p.prefix_s], 0), n) : 0;
     const Band band(p);
     const Scoring sc(p);
+    const float unit = p.slopes ? 1.f : sc.unit;
     const int key_first = tile * C::BKEYS, key_last = min(key_first + C::BKEYS, n) - 1;
     const int key = key_first + kg * 32 + (lane & 31);
     const int doc = p.kdoc && key < n ? p.kdoc[b * p.kdoc_b + key * p.kdoc_l] : 0;
@@ -240,11 +224,10 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
     for (int d = 0; d < DP / 32; ++d) dk[d] = zero16(), dv[d] = zero16();
 
     // Tiles of rows: BR queries of one head of the group.  Those that some key's band reaches, `len` a head, are numbered
-    // head by head; a split takes a run of the numbers.
+    // head by head.
     const int i_first = key_first < prefix ? 0 : max(key_first - band.above - offset, 0);
     const int i_last = key_first < prefix ? p.Lq - 1 : min(key_last + band.below - offset, p.Lq - 1);
     const int t_first = i_first / C::BR, len = key_last >= key_first && i_last >= i_first ? i_last / C::BR + 1 - t_first : 0;
-    const int all = len * p.G, per = (all + p.dk_splits - 1) / p.dk_splits;
     const int2* const qr = p.qrange ? p.qrange + (int64_t)b * p.qranges : nullptr;
     int2 mine = {0, 0};
     if (qr && len > 0) mine = document_range(p.krange + (int64_t)b * p.kranges, key_first, key_last);
@@ -254,13 +237,13 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         const int2 theirs = document_range(qr, i0, min(i0 + C::BR, p.Lq) - 1);
         return theirs.x <= mine.y && mine.x <= theirs.y;
     };
-    Tiles<decltype(needed)> tiles(needed, split * per, min((split + 1) * per, all));
+    Tiles<decltype(needed)> tiles(needed, 0, len * p.G, split, p.dk_splits);
 
     typedef Copy<T, DP, C::BR, C::NT, VEC> Rows;
     const Rows copy_q(p.q.l, p.D, tid), copy_g(p.dout.l, p.D, tid);
     static_assert(C::NT >= C::BR, "one thread a row for what rows have beside features");
     float r_lse = 0.f, r_delta = 0.f, r_slope = 0.f;
-    int r_at = 0, r_doc = 0;
+    int r_doc = 0;
     int2 range = {0, 0}, now = {0, 0};
     auto start = [&](int u, int buf) {
         const int g = u / len, i0 = (t_first + u - g * len) * C::BR, h = c * p.G + g, left = p.Lq - i0;
@@ -273,22 +256,20 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
             const int i = min(i0 + tid, p.Lq - 1);
             r_lse = tid < left ? p.lse[b * p.lse_b + i * p.lse_l + h * p.lse_h] : -__builtin_inff();
             r_delta = p.delta[((int64_t)b * p.Hk * p.G + h) * p.Lq + i];
-            r_at = i + offset;
             if (p.qdoc) r_doc = p.qdoc[b * p.qdoc_b + i * p.qdoc_l];
         }
     };
     auto finish = [&](int buf) {
         wait_loads();
         now = range;
-        float* const of = rows + buf * 5 * C::BR;
+        float* const of = rows + buf * 4 * C::BR;
         // A row that sees nothing (its log-sum is -inf) is zero, whatever the arrays hold there.
         const bool none = tid < C::BR && r_lse == -__builtin_inff();
         if (tid < C::BR) {
             of[tid] = none ? __builtin_inff() : r_lse * kLog2e;  // p = exp2(z - inf) = 0
-            of[C::BR + tid] = none ? 0.f : r_delta;
-            of[2 * C::BR + tid] = __int_as_float(r_at);
-            of[3 * C::BR + tid] = r_slope;
-            of[4 * C::BR + tid] = __int_as_float(none ? -1 : r_doc);
+            of[C::BR + tid] = none ? 0.f : -r_delta;
+            of[2 * C::BR + tid] = r_slope;
+            of[3 * C::BR + tid] = __int_as_float(none ? -1 : r_doc);
         }
         if (__syncthreads_or(none)) {
             char* const q = lds + buf * 2 * C::kTile;
@@ -315,7 +296,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         const char* qt = lds + buf * 2 * C::kTile;
         const char* gt = qt + C::kTile;
         const int q0 = rg * 32;
-        const float* of = rows + buf * 5 * C::BR + q0 + 4 * half;  // what the rows of registers 4 g .. have: of[array BR + 8 g + e]
+        const float* of = rows + buf * 4 * C::BR + q0 + 4 * half;  // what the rows of registers 4 g .. have: of[array BR + 8 g + e]
         {
             const int first_at = (t_first + t % len) * C::BR + q0 + offset;
             const bool masked = !__all(from <= first_at && first_at + 31 <= to && (!p.qdoc || (now.x == doc && now.y == doc)));
@@ -323,44 +304,40 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
                 s = M::mma(rows_frag<T, DP>(qt, q0, k, lane), C::K_LDS ? rows_frag<T, DP>(k_own, kg * 32, k, lane) : kf[C::K_LDS ? 0 : k], s);
-            f32x16 g = zero16();
+            f32x16 g;
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4 x = *(const f32x4*)(of + C::BR + c_row(i));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) g[i + e] = x[e];
+            }
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
                 g = M::mma(rows_frag<T, DP>(gt, q0, k, lane), C::V_LDS ? rows_frag<T, DP>(v_own, kg * 32, k, lane) : vf[C::V_LDS ? 0 : k], g);
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const f32x4 delta = *(const f32x4*)(of + C::BR + c_row(i));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) g[i + e] -= delta[e];
-            }
             if (p.cap > 0.f) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float y = tanh_of(s[i] * sc.cap_in);
-                    s[i] = y * sc.cap_out;
-                    g[i] *= 1.f - y * y;
+                    s[i] = tanh_of(s[i] * sc.bend);
+                    g[i] *= 1.f - s[i] * s[i];
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] *= sc.scale2;
             }
             if (p.slopes) {
-                const float slope = of[3 * C::BR];
+                const float slope = of[2 * C::BR];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] -= slope * fabsf((float)(first_at + 4 * half + c_row(i) - key));
+                for (int i = 0; i < 16; ++i) s[i] = s[i] * sc.unit - slope * fabsf((float)(first_at + 4 * half + c_row(i) - key));
             }
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const f32x4 lse = *(const f32x4*)(of + c_row(i));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[i + e] = __builtin_amdgcn_exp2f(s[i + e] - lse[e]);
+                for (int e = 0; e < 4; ++e) s[i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + e], unit, -lse[e]));
             }
             if (masked) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int at = first_at + 4 * half + c_row(i);
                     bool sees = from <= at && at <= to;
-                    if (p.qdoc) sees = sees && __float_as_int(of[4 * C::BR + c_row(i)]) == doc;
+                    if (p.qdoc) sees = sees && __float_as_int(of[3 * C::BR + c_row(i)]) == doc;
                     s[i] = sees ? s[i] : 0.f;
                     g[i] = sees ? g[i] : 0.f;
                 }
@@ -497,13 +474,13 @@ void launch_backward(const Params& p, hipStream_t stream) {
     Params x = p;
     const bool vec = p.q.vec && p.k.vec && p.v.vec && p.out.vec && p.dout.vec;
     x.tiles = (p.R + Q::BQ - 1) / Q::BQ;
-    unsigned grid = die_grid((int64_t)x.tiles * p.dq_splits * p.Hk * p.B);
+    unsigned grid = (unsigned)((int64_t)x.tiles * p.dq_splits * p.Hk * p.B);
     if (grid > 0 && vec) query_gradient_kernel<T, DP, true, Q><<<grid, Q::NT, 0, stream>>>(x);
     else if (grid > 0) query_gradient_kernel<T, DP, false, Q><<<grid, Q::NT, 0, stream>>>(x);
     check_launch("adhip_attention_backward");
     if (p.dq_splits > 1) add_parts<T>(p.part_dq, p.dq_splits, p.dq, p.B, p.Hk, p.Lq, p.G, p.D, stream);
     x.tiles = (p.Lk + K::BKEYS - 1) / K::BKEYS;
-    grid = die_grid((int64_t)x.tiles * p.dk_splits * p.Hk * p.B);
+    grid = (unsigned)((int64_t)x.tiles * p.dk_splits * p.Hk * p.B);
     if (grid > 0 && vec) key_gradient_kernel<T, DP, true, K><<<grid, K::NT, 0, stream>>>(x);
     else if (grid > 0) key_gradient_kernel<T, DP, false, K><<<grid, K::NT, 0, stream>>>(x);
     check_launch("adhip_attention_backward");

@@ -32,20 +32,17 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = wave % C::WQ, wk = wave / C::WQ;
 
-    // this workgroup's tile of rows (the last ones, which see most keys, first), key head, sequence and range of keys
-    const int total = p.tiles * p.splits * p.Hk * p.B;
-    int id = by_die(blockIdx.x, total);
-    if ((int)(blockIdx.x >> 3) >= (total + 7) / 8 || id >= total) return;
-    const int tile = p.tiles - 1 - id % p.tiles;
-    id /= p.tiles;
-    const int split = id % p.splits;
-    id /= p.splits;
-    const int c = id % p.Hk, b = id / p.Hk;
+    // this workgroup's tile of rows (the last ones see most keys), range of keys, key head and sequence
+    const Place place(p, p.splits);
+    const int tile = p.tiles - 1 - place.tile, split = place.split, c = place.c, b = place.b;
 
     const int n = sequence_length(p, b), offset = n - p.Lq;
     const int prefix = p.prefix ? min(max(p.prefix[b * p.prefix_s], 0), n) : 0;
     const Band band(p);
+    // the running maximum wants a positive unit: the scale's sign goes to the queries
+    const float sign = p.scale < 0.f ? -1.f : 1.f;
     const Scoring sc(p);
+    const float unit = p.slopes ? 1.f : p.scale == 0.f ? 1.f : sign * sc.unit;
     const int row0 = tile * C::BQ, row1 = min(row0 + C::BQ, p.R) - 1;
     const int first = row0 / p.G, last = row1 / p.G;  // tokens of the tile
 
@@ -63,7 +60,12 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
     {
         const T* q = (const T*)p.q.data + b * p.q.b + token * p.q.l + head * p.q.h;
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) qf[s] = load_frag<VEC>(q, s * 16 + half * 8, p.D, valid);
+        for (int s = 0; s < DP / 16; ++s) {
+            qf[s] = load_frag<VEC>(q, s * 16 + half * 8, p.D, valid && p.scale != 0.f);
+            if (sign < 0.f)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qf[s][e] = -qf[s][e];
+        }
     }
     f32x16 o[DP / 32];
 #pragma unroll
@@ -73,8 +75,6 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
     // tiles of keys that some row of this workgroup sees
     const int hi_all = last + offset + band.above, lo_all = first + offset - band.below;
     const int t_first = prefix > 0 ? 0 : max(lo_all, 0) / C::BK, t_stop = (min(n, max(hi_all + 1, prefix)) + C::BK - 1) / C::BK;
-    const int per = max(0, t_stop - t_first + p.splits - 1) / p.splits;
-    const int t_begin = t_first + split * per, t_end = min(t_begin + per, t_stop);
     const int2* const kr = p.krange ? p.krange + (int64_t)b * p.kranges : nullptr;
     int2 mine = {0, 0};
     if (kr) mine = document_range(p.qrange + (int64_t)b * p.qranges, first, last);
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         const int2 theirs = document_range(kr, j0, j1);
         return theirs.x <= mine.y && mine.x <= theirs.y;
     };
-    Tiles<decltype(needed)> tiles(needed, t_begin, t_end);
+    Tiles<decltype(needed)> tiles(needed, t_first, t_stop, split, p.splits);
 
     Keys kt(p, b, c, n, tid, wk * C::KB * 32, lds);
     int t = tiles.next(lane), buf = 0;
@@ -97,42 +97,51 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         const char* vs = kt.values(buf);
         const int* docs = kt.docs(buf);
         f32x16 s[C::KB];
-        float top = -__builtin_inff();
 #pragma unroll
         for (int x = 0; x < C::KB; ++x) {
-            const int key0 = (wk * C::KB + x) * 32;
             s[x] = zero16();
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) s[x] = M::mma(rows_frag<T, DP>(ks, key0, k, lane), qf[k], s[x]);
-            const int j0 = t * C::BK + key0, jl = j0 + 4 * half;
-            if (p.cap > 0.f) {
+            for (int k = 0; k < DP / 16; ++k) s[x] = M::mma(rows_frag<T, DP>(ks, (wk * C::KB + x) * 32, k, lane), qf[k], s[x]);
+        }
+        const int j0 = t * C::BK + wk * C::KB * 32, jl = j0 + 4 * half;  // register i of s[x] has key jl + 32 x + c_row(i)
+        if (p.cap > 0.f) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[x][i] = tanh_of(s[x][i] * sc.cap_in) * sc.cap_out;
-            } else {
+            for (int x = 0; x < C::KB; ++x)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[x][i] *= sc.scale2;
-            }
-            if (p.slopes) {
+                for (int i = 0; i < 16; ++i) s[x][i] = tanh_of(s[x][i] * (sign * sc.bend));
+        }
+        if (p.slopes) {
+            const float inner = p.cap > 0.f ? sc.unit : sign * sc.unit;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[x][i] -= slope * fabsf((float)(at - jl - c_row(i)));
-            }
-            // masks only where some row of the wavefront does not see all 32 keys
-            if (!__all(j0 + 31 < n && ((lo <= j0 && j0 + 31 <= hi) || j0 + 31 < pre) && kt.one_document(x, doc))) {
+            for (int x = 0; x < C::KB; ++x)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[x][i] = s[x][i] * inner - slope * fabsf((float)(at - jl - 32 * x - c_row(i)));
+        }
+        // masks only where some row of the wavefront does not see all its keys of the tile
+        bool all = j0 + 32 * C::KB <= n && ((lo <= j0 && j0 + 32 * C::KB - 1 <= hi) || j0 + 32 * C::KB <= pre);
+#pragma unroll
+        for (int x = 0; x < C::KB; ++x) all = all && kt.one_document(x, doc);
+        if (!__all(all)) {
+#pragma unroll
+            for (int x = 0; x < C::KB; ++x)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int j = jl + c_row(i);
+                    const int j = jl + 32 * x + c_row(i);
                     bool sees = j < n && (j < pre || (lo <= j && j <= hi));
-                    if (kt.kd) sees = sees && docs[key0 + 4 * half + c_row(i)] == doc;
+                    if (kt.kd) sees = sees && docs[(wk * C::KB + x) * 32 + 4 * half + c_row(i)] == doc;
                     s[x][i] = sees ? s[x][i] : -__builtin_inff();
                 }
-            }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int x = 0; x < C::KB; ++x)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][i]);
-        }
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float m_new = fmaxf(m, top), base = m_new == -__builtin_inff() ? 0.f : m_new;
-        if (__any(m_new > m)) {
-            const float a = __builtin_amdgcn_exp2f(m - base);
+        // The sums are rescaled when the maximum has grown by more than 2^8, not at each of its first, small steps: they and
+        // the probabilities have the same relative precision below that as below one.
+        if (__any(top * unit > m * unit + 8.f)) {
+            const float m_new = fmaxf(m, top), a = m_new == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * unit);
             l *= a;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
@@ -140,12 +149,12 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
                 for (int i = 0; i < 16; ++i) o[d][i] *= a;
             m = m_new;
         }
+        const float base = m == -__builtin_inff() ? 0.f : m * unit;
 #pragma unroll
         for (int x = 0; x < C::KB; ++x) {
-            const int key0 = (wk * C::KB + x) * 32;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[x][i] = __builtin_amdgcn_exp2f(s[x][i] - base);
+                s[x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], unit, -base));
                 l += s[x][i];
             }
 #pragma unroll
@@ -153,13 +162,14 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
                 Frag f;
                 to_frag(s[x], h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) o[d] = M::mma(cols_frag<DP>((const T*)0, vs, key0 + 16 * h, d * 32, lane), f, o[d]);
+                for (int d = 0; d < DP / 32; ++d) o[d] = M::mma(cols_frag<DP>((const T*)0, vs, (wk * C::KB + x) * 32 + 16 * h, d * 32, lane), f, o[d]);
             }
         }
         kt.advance(next, buf);
         t = next;
     }
     l += __shfl_xor(l, 32);
+    m *= unit;
 
     const int64_t rows_before = (((int64_t)split * p.B + b) * p.Hk + c) * p.R;
     if (C::WK == 1) {
@@ -273,7 +283,7 @@ struct ForwardMany {
     // 64 keys a tile; 32 where two tiles of 64 would not leave room for a second workgroup or, at 512 bytes a feature row and
     // more, not fit
     static constexpr int kRowBytes = DP * (int)sizeof(T);
-    typedef ForwardConfig<T, DP, 4, 1, kRowBytes <= 256 ? 64 : 32, 2, kRowBytes <= 256 ? 2 : 1> C;
+    typedef ForwardConfig<T, DP, 4, 1, kRowBytes <= 256 ? 64 : 32, 2, kRowBytes <= 128 ? 3 : kRowBytes <= 256 ? 2 : 1> C;
 };
 template <class T, int DP>
 struct ForwardFew {
@@ -285,7 +295,7 @@ struct ForwardFew {
 
 template <class T, int DP, class C>
 void launch_forward(const Params& p, hipStream_t stream) {
-    const unsigned grid = die_grid((int64_t)p.tiles * p.splits * p.Hk * p.B);
+    const unsigned grid = (unsigned)((int64_t)p.tiles * p.splits * p.Hk * p.B);
     if (p.q.vec && p.k.vec && p.v.vec) forward_kernel<T, DP, true, C><<<grid, C::NT, 0, stream>>>(p);
     else forward_kernel<T, DP, false, C><<<grid, C::NT, 0, stream>>>(p);
     check_launch("adhip_attention");

@@ -30,7 +30,7 @@ int main(void) {
     subprocess.run(["gcc", "-std=c99", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
     c = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
     a = ops._ARRAY.size
-    mine = [a, 16, 48, 7 * a + ops._ROTARY_TAIL.size, 7 * a + 4, ops._ADAMW_TENSOR.size, 48, 88, ops._ADAMW.size, 28, 72,
+    mine = [a, 16, 48, 7 * a + ops._ROTARY_TAIL.size, 7 * a + 4, 12 * 8, 6 * 8, 11 * 8, ops._ADAMW.size, 28, 72,
             14 * a + ops._ATTENTION_TAIL.size, 5 * a, 10 * a, 14 * a, 14 * a + 8, 14 * a + 16, 14 * a + 32]
     assert c == mine
 
