@@ -193,6 +193,16 @@ __device__ __forceinline__ float tanh_of(float y) {
     return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
 }
 
+// The larger (the sum) of a lane's value and that of the lane 32 away, in both.
+__device__ __forceinline__ float max_of_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // row of register i of a C tile
 __device__ __forceinline__ constexpr int c_row(int i) { return 8 * (i >> 2) + (i & 3); }
 
@@ -361,9 +371,8 @@ struct KeyTiles {
     int doc;
     int2 range[C::KB];  // documents of the 32 keys of each of the wavefront's products: of the tile that is under way ..
     int2 now[C::KB];    // .. and of the one in LDS
-    bool unclean;       // the tile under way has keys of no document
     __device__ __forceinline__ KeyTiles(const Params& p_, int b, int c, int n_, int tid_, int key0_, char* lds_)
-        : p(p_), lds(lds_), n(n_), tid(tid_), key0(key0_), k(p_.k.l, p_.D, tid_), v(p_.v.l, p_.D, tid_), doc(0), unclean(false) {
+        : p(p_), lds(lds_), n(n_), tid(tid_), key0(key0_), k(p_.k.l, p_.D, tid_), v(p_.v.l, p_.D, tid_), doc(0) {
         kb = (const T*)p.k.data + b * p.k.b + c * p.k.h;
         vb = (const T*)p.v.data + b * p.v.b + c * p.v.h;
         kd = p.kdoc ? p.kdoc + b * p.kdoc_b : nullptr;
@@ -375,23 +384,24 @@ struct KeyTiles {
     __device__ __forceinline__ void start(int t, int buf) {
         const int64_t j0 = (int64_t)t * C::BK;
         const int left = n - (int)j0;
+        if (kd) {  // before the tiles: loads return in order
+            if (tid < C::BK) doc = kd[min((int)j0 + tid, n - 1) * p.kdoc_l];
+#pragma unroll
+            for (int x = 0; x < C::KB; ++x) range[x] = kr[min((int)j0 + key0 + 32 * x, n - 1) / kRange];
+        }
         k.start(keys(buf), kb + j0 * p.k.l, p.k.l, left, p.D, tid);
         v.start(values(buf), vb + j0 * p.v.l, p.v.l, left, p.D, tid);
-        if (!kd) return;
-        if (tid < C::BK) doc = kd[min((int)j0 + tid, n - 1) * p.kdoc_l];
-#pragma unroll
-        for (int x = 0; x < C::KB; ++x) range[x] = kr[min((int)j0 + key0 + 32 * x, n - 1) / kRange];
-        unclean = document_range(kr, (int)j0, min((int)j0 + C::BK, n) - 1).x < 0;
     }
     __device__ __forceinline__ void finish(int buf) {
         wait_loads();
-        if (kd) {
-            if (tid < C::BK) docs(buf)[tid] = doc;
-#pragma unroll
-            for (int x = 0; x < C::KB; ++x) now[x] = range[x];
+        if (!kd) {
+            __syncthreads();
+            return;
         }
-        __syncthreads();
-        if (kd && unclean) {
+        if (tid < C::BK) docs(buf)[tid] = doc;
+#pragma unroll
+        for (int x = 0; x < C::KB; ++x) now[x] = range[x];
+        if (__syncthreads_or(tid < C::BK && doc < 0)) {
             const int* of = docs(buf);
             S::clear(keys(buf), [&](int i) { return of[i] < 0; }, tid);
             S::clear(values(buf), [&](int i) { return of[i] < 0; }, tid);

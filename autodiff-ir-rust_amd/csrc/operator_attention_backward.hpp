@@ -70,7 +70,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
             for (int e = 0; e < 8; ++e) delta += (float)df[s][e] * (float)of[e];
         }
     }
-    delta += __shfl_xor(delta, 32);
+    delta = sum_of_halves(delta);
     if (inside && half == 0 && split == 0) p.delta[((int64_t)b * p.Hk * p.G + head) * p.Lq + token] = delta;
     f32x16 dq[DP / 32];
 #pragma unroll
@@ -247,10 +247,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
     int2 range = {0, 0}, now = {0, 0};
     auto start = [&](int u, int buf) {
         const int g = u / len, i0 = (t_first + u - g * len) * C::BR, h = c * p.G + g, left = p.Lq - i0;
-        char* const to_q = lds + buf * 2 * C::kTile;
-        copy_q.start(to_q, (const T*)p.q.data + b * p.q.b + i0 * p.q.l + h * p.q.h, p.q.l, left, p.D, tid);
-        copy_g.start(to_q + C::kTile, (const T*)p.dout.data + b * p.dout.b + i0 * p.dout.l + h * p.dout.h, p.dout.l, left, p.D, tid);
-        if (qr) range = document_range(qr, i0 + rg * 32, min(i0 + rg * 32 + 31, p.Lq - 1));
+        if (qr) range = qr[min(i0 + rg * 32, p.Lq - 1) / kRange];
         r_slope = p.slopes ? p.slopes[h * p.slope_stride] * kLog2e : 0.f;
         if (tid < C::BR) {
             const int i = min(i0 + tid, p.Lq - 1);
@@ -258,6 +255,9 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
             r_delta = p.delta[((int64_t)b * p.Hk * p.G + h) * p.Lq + i];
             if (p.qdoc) r_doc = p.qdoc[b * p.qdoc_b + i * p.qdoc_l];
         }
+        char* const to_q = lds + buf * 2 * C::kTile;
+        copy_q.start(to_q, (const T*)p.q.data + b * p.q.b + i0 * p.q.l + h * p.q.h, p.q.l, left, p.D, tid);
+        copy_g.start(to_q + C::kTile, (const T*)p.dout.data + b * p.dout.b + i0 * p.dout.l + h * p.dout.h, p.dout.l, left, p.D, tid);
     };
     auto finish = [&](int buf) {
         wait_loads();

@@ -137,7 +137,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         for (int x = 0; x < C::KB; ++x)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[x][i]);
-        top = fmaxf(top, __shfl_xor(top, 32));
+        top = max_of_halves(top);
         // The sums are rescaled when the maximum has grown by more than 2^8, not at each of its first, small steps: they and
         // the probabilities have the same relative precision below that as below one.
         if (__any(top * unit > m * unit + 8.f)) {
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         kt.advance(next, buf);
         t = next;
     }
-    l += __shfl_xor(l, 32);
+    l = sum_of_halves(l);
     m *= unit;
 
     const int64_t rows_before = (((int64_t)split * p.B + b) * p.Hk + c) * p.R;
