@@ -45,7 +45,7 @@ size_t rounded(size_t n) { return (n + 255) & ~size_t(255); }
 struct Layout {
     bool few_rows;
     int row_tile, tiles, splits, dq_splits, dk_splits;
-    size_t qrange, krange, part, part_ml, delta, part_dq, part_dk, part_dv, bytes;
+    size_t qrange, krange, part, part_ml, stats, part_dq, part_dk, part_dv, bytes;
 };
 
 Layout layout_of(const adhip_attention_args& g, bool backward) {
@@ -78,8 +78,8 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
     }
     y.dq_splits = y.dk_splits = 1;
     if (backward) {
-        y.delta = back;
-        back += rounded((size_t)(B * Hk * R) * 4);
+        y.stats = back;
+        back += rounded((size_t)(B * Hk * R) * 2 * 4);
         // Parts of the backward walks: as many as give every compute unit four workgroups, which evens out a causal mask's
         // uneven ones, none shorter than four tiles.
         auto parts = [](int64_t blocks, int64_t tiles) {
@@ -198,7 +198,7 @@ Params checked(const char* op, const adhip_attention_args& g, const Layout& y, b
     p.splits = y.splits;
     p.part = (float*)(room + y.part);
     p.part_ml = (float*)(room + y.part_ml);
-    p.delta = (float*)(room + y.delta);
+    p.stats = (float*)(room + y.stats);
     p.dq_splits = y.dq_splits;
     p.dk_splits = y.dk_splits;
     p.part_dq = (float*)(room + y.part_dq);

@@ -40,7 +40,7 @@ struct Params {
     int causal, window;
     int tiles, splits;            // row tiles (or key tiles); ranges that the keys (or rows) are split into
     float *part, *part_ml;        // forward, split: [split][b][c][row][D], [..][row][2]
-    float* delta;                 // backward: [b][head][query]
+    float* stats;                 // backward, [2][b][head][query]: lse log2 e (+inf: sees nothing), -delta
     float *part_dq, *part_dk, *part_dv;  // backward, split: [split] of what the gradients are, packed [b][c][row or key][D]
     int dq_splits, dk_splits;
 };
@@ -242,19 +242,24 @@ __device__ __forceinline__ int2 document_range(const int2* ranges, int first, in
 
 // Walks the tiles begin .. stop - 1 that a block needs, 64 candidates at a time: each lane decides on one, all wavefronts
 // alike.  Of those needed, split s of S takes numbers s, s + S, ..: the splits' shares are even whatever the masks leave.
+// needed(tile, documents) also tells the smallest and largest document of the tile (where there are any).
+struct Tile {
+    int t;           // -1: none
+    int2 documents;
+};
 template <class Needed>
 struct Tiles {
     const Needed& needed;
-    int base, end, split, splits, seen = 0;
+    int base, end, split, splits, lane, seen = 0;
     unsigned long long mask = 0;
-    __device__ __forceinline__ Tiles(const Needed& f, int begin, int stop, int split_, int splits_)
-        : needed(f), base(begin - 64), end(stop), split(split_), splits(splits_) {}
-    // the next tile, or -1
-    __device__ __forceinline__ int next(int lane) {
+    int2 documents = {0, 0};
+    __device__ __forceinline__ Tiles(const Needed& f, int begin, int stop, int split_, int splits_, int lane_)
+        : needed(f), base(begin - 64), end(stop), split(split_), splits(splits_), lane(lane_) {}
+    __device__ __forceinline__ Tile next() {
         while (!mask) {
+            if (base + 64 >= end) return {-1, {0, 0}};
             base += 64;
-            if (base >= end) return -1;
-            const bool mine = base + lane < end && needed(base + lane);
+            const bool mine = base + lane < end && needed(base + lane, documents);
             mask = __ballot(mine);
             if (splits > 1) {
                 const int number = seen + __popcll(mask & ((1ull << lane) - 1));
@@ -262,9 +267,60 @@ struct Tiles {
                 mask = __ballot(mine && number % splits == split);
             }
         }
-        const int t = base + __builtin_ctzll(mask);
+        const int i = __builtin_ctzll(mask);
         mask &= mask - 1;
-        return t;
+        return {base + i, {__builtin_amdgcn_readlane(documents.x, i), __builtin_amdgcn_readlane(documents.y, i)}};
+    }
+};
+
+// A ring of BUFS tiles in LDS: the oldest is worked on while the others are under way.  `start(tile, buffer)` begins a
+// tile's loads, of which the last LOADS of each wavefront are its own; `landed(tile, buffer)` runs when it is there and all
+// wavefronts have come.  A load takes one to two microseconds from other memory than the L2, as long as the products of a
+// tile where a compute unit has few wavefronts: then two and three tiles under way are worth their LDS.
+template <int BUFS, int LOADS, class Walk, class Start>
+struct Ring {
+    Walk& walk;
+    const Start& start;
+    Tile queue[BUFS];  // queue[0]: the one worked on
+    int buf = 0;       // its place
+    __device__ __forceinline__ Ring(Walk& w, const Start& s) : walk(w), start(s) {
+        queue[0] = walk.next();
+        if (BUFS > 1 && queue[0].t >= 0) start(queue[0], 0);
+#pragma unroll
+        for (int i = 1; i < BUFS - 1; ++i) {
+            queue[i] = queue[i - 1].t >= 0 ? walk.next() : Tile{-1, {0, 0}};
+            if (queue[i].t >= 0) start(queue[i], i);
+        }
+    }
+    // waits for queue[0], then begins one more
+    __device__ __forceinline__ bool ready() {
+        if (queue[0].t < 0) return false;
+        if (BUFS == 1) {
+            __syncthreads();
+            start(queue[0], 0);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            return true;
+        }
+        if (BUFS > 2 && queue[BUFS > 2 ? BUFS - 2 : 0].t >= 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((BUFS - 2) * LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        return true;
+    }
+    __device__ __forceinline__ void more() {
+        if (BUFS == 1) return;
+        Tile& last = queue[BUFS - 1];
+        last = BUFS == 2 || queue[BUFS > 2 ? BUFS - 2 : 0].t >= 0 ? walk.next() : Tile{-1, {0, 0}};
+        if (last.t >= 0) start(last, buf == 0 ? BUFS - 1 : buf - 1);
+    }
+    __device__ __forceinline__ void pop() {
+        if (BUFS == 1) {
+            queue[0] = walk.next();
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i + 1 < BUFS; ++i) queue[i] = queue[i + 1];
+        buf = buf + 1 == BUFS ? 0 : buf + 1;
     }
 };
 
@@ -285,21 +341,21 @@ struct Place {
     }
 };
 
-// A load of 16 bytes a lane that writes LDS by itself: lane i's go to `to` + 16 i, from `base` (of the whole wavefront) and the
+// A load of 16 (or 4) bytes a lane that writes LDS by itself: lane i's go to `to` + 16 i (4 i), from `base` (of the whole wavefront) and the
 // lane's offset; an offset behind the resource's end gives zeros.  It stands here as the instruction because the compiler
 // orders every later read of LDS behind the one it knows of, and so would wait for a tile that is not needed before the
-// next step; wait_loads() and a barrier stand where it is.  No register is written, so none can be written late.
+// next step; the ring below waits and has a barrier where it is.  No register is written, so none can be written late.
+template <int BYTES>
 __device__ __forceinline__ void load_to_lds(const void* base, unsigned offset, char* to) {
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
     const uintptr_t a = (uintptr_t)base;
     const u32x4 source = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a),
                           (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)) & 0xffffu, 0x7fffffffu, 0x00020000u};
-    const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)to);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(source) : "memory");
+    const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)to);  // an address in LDS ends in its offset
+    static_assert(BYTES == 16 || BYTES == 4, "widths of these loads");
+    if (BYTES == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(source) : "memory");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(source) : "memory");
 }
-// Waits for this wavefront's loads to LDS.
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 // Copies of tiles from an array's rows (a fixed stride apart) into LDS by a workgroup of NT threads: ROWS rows of DP
 // features.  Where rows allow it (VEC) the loads write LDS themselves, 16 bytes a lane, in the order of the tile's places;
 // which piece of which row that is decides each lane's address.  A place without a piece (behind the head's features or
@@ -311,6 +367,7 @@ struct Copy {
     static constexpr int kTotal = ROWS * L::kPlaces, kEach = (kTotal + NT - 1) / NT;
     static constexpr unsigned kNowhere = 0xffffffffu;
     static_assert(kTotal % 64 == 0, "whole wavefronts copy");
+    static constexpr int kLoads = VEC ? kTotal / NT : 0;  // that every wavefront issues at least
     unsigned offset[kEach];
     int wave;
     static __device__ __forceinline__ int row(int c, int tid) { return (tid + c * NT) / L::kPlaces; }
@@ -330,7 +387,7 @@ struct Copy {
             for (int c = 0; c < kEach; ++c) {
                 if (kTotal % NT != 0 && (wave * 64 + c * NT) >= kTotal) break;
                 const unsigned o = whole || row(c, tid) < rows ? offset[c] : kNowhere;
-                load_to_lds(from, o, tile + (wave * 64 + c * NT) * 16);
+                load_to_lds<16>(from, o, tile + (wave * 64 + c * NT) * 16);
             }
         } else {
 #pragma unroll 1
@@ -352,86 +409,54 @@ struct Copy {
     }
 };
 
-// Tiles of keys and values on their way from memory to LDS, one ahead of the products where LDS holds two, with what
-// decides about them: shared by the kernels that own rows.  Keys behind the sequence or of no document are zero, whatever
-// the arrays hold there.
+// ROWS values of 4 bytes, a fixed stride apart, into LDS; zeros behind `count`.  By the first wavefronts; a register is not
+// waited for, so the loads that come after stay under way.
+template <int ROWS>
+__device__ __forceinline__ void copy_words(char* to, const void* from, int64_t stride, int count, int tid, int wave) {
+    static_assert(ROWS % 32 == 0, "half wavefronts");
+    const bool mine = tid < ROWS;
+    if (wave * 64 < ROWS && mine) load_to_lds<4>(from, tid < count ? (unsigned)(tid * stride) * 4u : 0xffffffffu, to + wave * 256);
+}
+
+// Tiles of keys and values on their way from memory to LDS: shared by the kernels that own rows.  Keys behind the sequence
+// or of no document are zero, whatever the arrays hold there.
 template <class T, int DP, class C, bool VEC>
 struct KeyTiles {
     typedef Copy<T, DP, C::BK, C::NT, VEC> S;
     static_assert(C::NT >= C::BK, "one thread a key for the documents");
     static constexpr int kTile = C::BK * Lds<T, DP>::kPitch;
     static constexpr int kBytes = C::kBufs * (2 * kTile + C::BK * 4);
+    static constexpr int kLoads = 2 * S::kLoads;
     const Params& p;
     const T *kb, *vb;
     const int* kd;
-    const int2* kr;
     char* lds;
-    int n, tid, key0;
+    int n, tid;
     S k, v;
-    int doc;
-    int2 range[C::KB];  // documents of the 32 keys of each of the wavefront's products: of the tile that is under way ..
-    int2 now[C::KB];    // .. and of the one in LDS
-    __device__ __forceinline__ KeyTiles(const Params& p_, int b, int c, int n_, int tid_, int key0_, char* lds_)
-        : p(p_), lds(lds_), n(n_), tid(tid_), key0(key0_), k(p_.k.l, p_.D, tid_), v(p_.v.l, p_.D, tid_), doc(0) {
+    __device__ __forceinline__ KeyTiles(const Params& p_, int b, int c, int n_, int tid_, char* lds_)
+        : p(p_), lds(lds_), n(n_), tid(tid_), k(p_.k.l, p_.D, tid_), v(p_.v.l, p_.D, tid_) {
         kb = (const T*)p.k.data + b * p.k.b + c * p.k.h;
         vb = (const T*)p.v.data + b * p.v.b + c * p.v.h;
         kd = p.kdoc ? p.kdoc + b * p.kdoc_b : nullptr;
-        kr = p.krange ? p.krange + (int64_t)b * p.kranges : nullptr;
     }
     __device__ __forceinline__ char* keys(int buf) const { return lds + buf * 2 * kTile; }
     __device__ __forceinline__ char* values(int buf) const { return lds + buf * 2 * kTile + kTile; }
-    __device__ __forceinline__ int* docs(int buf) const { return (int*)(lds + C::kBufs * 2 * kTile) + buf * C::BK; }
-    __device__ __forceinline__ void start(int t, int buf) {
-        const int64_t j0 = (int64_t)t * C::BK;
+    __device__ __forceinline__ char* docs(int buf) const { return lds + C::kBufs * 2 * kTile + buf * C::BK * 4; }
+    __device__ __forceinline__ void operator()(const Tile& tile, int buf) const {
+        const int64_t j0 = (int64_t)tile.t * C::BK;
         const int left = n - (int)j0;
-        if (kd) {  // before the tiles: loads return in order
-            if (tid < C::BK) doc = kd[min((int)j0 + tid, n - 1) * p.kdoc_l];
-#pragma unroll
-            for (int x = 0; x < C::KB; ++x) range[x] = kr[min((int)j0 + key0 + 32 * x, n - 1) / kRange];
-        }
+        if (kd) copy_words<C::BK>(docs(buf), kd + j0 * p.kdoc_l, p.kdoc_l, left, tid, k.wave);
         k.start(keys(buf), kb + j0 * p.k.l, p.k.l, left, p.D, tid);
         v.start(values(buf), vb + j0 * p.v.l, p.v.l, left, p.D, tid);
     }
-    __device__ __forceinline__ void finish(int buf) {
-        wait_loads();
-        if (!kd) {
-            __syncthreads();
-            return;
-        }
-        if (tid < C::BK) docs(buf)[tid] = doc;
-#pragma unroll
-        for (int x = 0; x < C::KB; ++x) now[x] = range[x];
-        if (__syncthreads_or(tid < C::BK && doc < 0)) {
-            const int* of = docs(buf);
-            S::clear(keys(buf), [&](int i) { return of[i] < 0; }, tid);
-            S::clear(values(buf), [&](int i) { return of[i] < 0; }, tid);
-            __syncthreads();
-        }
+    // a tile that has arrived and holds keys of no document
+    __device__ __forceinline__ void clean(const Tile& tile, int buf) const {
+        if (!kd || tile.documents.x >= 0) return;
+        const int* of = (const int*)docs(buf);
+        S::clear(keys(buf), [&](int i) { return of[i] < 0; }, tid);
+        S::clear(values(buf), [&](int i) { return of[i] < 0; }, tid);
+        __syncthreads();
     }
-    __device__ __forceinline__ void begin(int t) {
-        if (C::kBufs == 2 && t >= 0) {
-            start(t, 0);
-            finish(0);
-        }
-    }
-    // before a tile's products: the next one gets under way
-    __device__ __forceinline__ void fetch(int t, int next, int buf) {
-        if (C::kBufs == 2) {
-            if (next >= 0) start(next, buf ^ 1);
-        } else {
-            __syncthreads();
-            start(t, 0);
-            finish(0);
-        }
-    }
-    // behind them: it has arrived
-    __device__ __forceinline__ void advance(int next, int& buf) {
-        if (C::kBufs != 2 || next < 0) return;
-        buf ^= 1;
-        finish(buf);
-    }
-    // all 32 keys of product x are of the document `mine`
-    __device__ __forceinline__ bool one_document(int x, int mine) const { return !kd || (now[x].x == mine && now[x].y == mine); }
 };
 
 // DP: the head's features, rounded up to what the kernels are built for

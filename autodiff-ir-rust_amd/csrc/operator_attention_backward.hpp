@@ -71,7 +71,11 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
         }
     }
     delta = sum_of_halves(delta);
-    if (inside && half == 0 && split == 0) p.delta[((int64_t)b * p.Hk * p.G + head) * p.Lq + token] = delta;
+    if (inside && half == 0 && split == 0) {
+        float* const to = p.stats + ((int64_t)b * p.Hk * p.G + head) * p.Lq + token;
+        to[0] = valid ? lse2 : __builtin_inff();  // p = exp2(z - inf) = 0
+        to[(int64_t)p.B * p.Hk * p.G * p.Lq] = -delta;
+    }
     f32x16 dq[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) dq[d] = zero16();
@@ -81,24 +85,25 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
     const int2* const kr = p.krange ? p.krange + (int64_t)b * p.kranges : nullptr;
     int2 mine = {0, 0};
     if (kr) mine = document_range(p.qrange + (int64_t)b * p.qranges, first, last);
-    auto needed = [&](int t) {
+    auto needed = [&](int t, int2& theirs) {
         const int j0 = t * C::BK, j1 = min(j0 + C::BK, n) - 1;
         if (j0 >= prefix && (j0 > hi_all || j1 < lo_all)) return false;
         if (!kr) return true;
-        const int2 theirs = document_range(kr, j0, j1);
+        theirs = document_range(kr, j0, j1);
         return theirs.x <= mine.y && mine.x <= theirs.y;
     };
-    Tiles<decltype(needed)> tiles(needed, t_first, t_stop, split, p.dq_splits);
-
-    Keys kt(p, b, c, n, tid, 0, lds);
-    int t = tiles.next(lane), buf = 0;
-    kt.begin(t);
-    while (t >= 0) {
-        const int next = tiles.next(lane);
-        kt.fetch(t, next, buf);
+    typedef Tiles<decltype(needed)> Walk;
+    Walk walk(needed, t_first, t_stop, split, p.dq_splits, lane);
+    const Keys kt(p, b, c, n, tid, lds);
+    Ring<C::kBufs, Keys::kLoads, Walk, Keys> ring(walk, kt);
+    for (; ring.ready(); ring.pop()) {
+        const int buf = ring.buf, t = ring.queue[0].t;
+        kt.clean(ring.queue[0], buf);
+        ring.more();
         const char* ks = kt.keys(buf);
         const char* vs = kt.values(buf);
-        const int* docs = kt.docs(buf);
+        const int* docs = (const int*)kt.docs(buf);
+        const bool one_document = !kt.kd || (ring.queue[0].documents.x == doc && ring.queue[0].documents.y == doc);
 #pragma unroll
         for (int x = 0; x < C::KB; ++x) {
             const int key0 = x * 32;
@@ -110,7 +115,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) g = M::mma(rows_frag<T, DP>(vs, key0, k, lane), df[k], g);
             const int j0 = t * C::BK + key0, jl = j0 + 4 * half;
-            const bool masked = !__all(j0 + 31 < n && ((lo <= j0 && j0 + 31 <= hi) || j0 + 31 < pre) && kt.one_document(x, doc));
+            const bool masked = !__all(j0 + 31 < n && ((lo <= j0 && j0 + 31 <= hi) || j0 + 31 < pre) && one_document);
             if (p.cap > 0.f) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -141,8 +146,6 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
                 for (int d = 0; d < DP / 32; ++d) dq[d] = M::mma(cols_frag<DP>((const T*)0, ks, key0 + 16 * h, d * 32, lane), f, dq[d]);
             }
         }
-        kt.advance(next, buf);
-        t = next;
     }
     if (!inside) return;
     float* const part = p.dq_splits > 1 ? p.part_dq + ((((int64_t)split * p.B + b) * p.Hk + c) * p.R + row) * p.D : nullptr;
@@ -167,7 +170,7 @@ struct KeyConfig {
     static constexpr bool K_LDS = K_LDS_, V_LDS = V_LDS_;
     static constexpr int kTile = BR * Lds<T, DP>::kPitch, kOwn = BKEYS * Lds<T, DP>::kPitch;
     static constexpr int kRows = kBufs * 2 * kTile + (K_LDS ? kOwn : 0) + (V_LDS ? kOwn : 0);
-    static constexpr int kLoop = kRows + kBufs * BR * 4 * 4;
+    static constexpr int kLoop = kRows + kBufs * BR * 3 * 4;  // of each row: log-sum, -delta, document
     static constexpr int kMerge = RG > 1 ? (RG - 1) * BKEYS * (DP + 4) * 4 : 0;
     static constexpr int kBytes = kLoop > kMerge ? kLoop : kMerge;
 };
@@ -180,7 +183,6 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
     __shared__ __attribute__((aligned(1024))) char lds[C::kBytes];
     char* const k_own = lds + C::kBufs * 2 * C::kTile;
     char* const v_own = k_own + (C::K_LDS ? C::kOwn : 0);
-    float* const rows = (float*)(lds + C::kRows);  // [bufs][4][BR]: lse, -delta, slope, document
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave % C::KG, rg = wave / C::KG;
 
@@ -231,75 +233,55 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
     const int2* const qr = p.qrange ? p.qrange + (int64_t)b * p.qranges : nullptr;
     int2 mine = {0, 0};
     if (qr && len > 0) mine = document_range(p.krange + (int64_t)b * p.kranges, key_first, key_last);
-    auto needed = [&](int u) {
+    auto needed = [&](int u, int2& theirs) {
         if (!qr) return true;
         const int i0 = (t_first + u % len) * C::BR;
-        const int2 theirs = document_range(qr, i0, min(i0 + C::BR, p.Lq) - 1);
+        theirs = document_range(qr, i0, min(i0 + C::BR, p.Lq) - 1);
         return theirs.x <= mine.y && mine.x <= theirs.y;
     };
-    Tiles<decltype(needed)> tiles(needed, 0, len * p.G, split, p.dk_splits);
+    typedef Tiles<decltype(needed)> Walk;
+    Walk walk(needed, 0, len * p.G, split, p.dk_splits, lane);
 
     typedef Copy<T, DP, C::BR, C::NT, VEC> Rows;
     const Rows copy_q(p.q.l, p.D, tid), copy_g(p.dout.l, p.D, tid);
     static_assert(C::NT >= C::BR, "one thread a row for what rows have beside features");
-    float r_lse = 0.f, r_delta = 0.f, r_slope = 0.f;
-    int r_doc = 0;
-    int2 range = {0, 0}, now = {0, 0};
-    auto start = [&](int u, int buf) {
-        const int g = u / len, i0 = (t_first + u - g * len) * C::BR, h = c * p.G + g, left = p.Lq - i0;
-        if (qr) range = qr[min(i0 + rg * 32, p.Lq - 1) / kRange];
-        r_slope = p.slopes ? p.slopes[h * p.slope_stride] * kLog2e : 0.f;
-        if (tid < C::BR) {
-            const int i = min(i0 + tid, p.Lq - 1);
-            r_lse = tid < left ? p.lse[b * p.lse_b + i * p.lse_l + h * p.lse_h] : -__builtin_inff();
-            r_delta = p.delta[((int64_t)b * p.Hk * p.G + h) * p.Lq + i];
-            if (p.qdoc) r_doc = p.qdoc[b * p.qdoc_b + i * p.qdoc_l];
-        }
+    auto start = [&](const Tile& tile, int buf) {
+        const int g = tile.t / len, i0 = (t_first + tile.t - g * len) * C::BR, h = c * p.G + g, left = p.Lq - i0;
         char* const to_q = lds + buf * 2 * C::kTile;
+        char* const of = lds + C::kRows + buf * 3 * C::BR * 4;
+        const float* const stats = p.stats + ((int64_t)b * p.Hk * p.G + h) * p.Lq + i0;
+        copy_words<C::BR>(of, stats, 1, left, tid, wave);
+        copy_words<C::BR>(of + C::BR * 4, stats + (int64_t)p.B * p.Hk * p.G * p.Lq, 1, left, tid, wave);
+        if (p.qdoc) copy_words<C::BR>(of + 2 * C::BR * 4, p.qdoc + b * p.qdoc_b + i0 * p.qdoc_l, p.qdoc_l, left, tid, wave);
         copy_q.start(to_q, (const T*)p.q.data + b * p.q.b + i0 * p.q.l + h * p.q.h, p.q.l, left, p.D, tid);
         copy_g.start(to_q + C::kTile, (const T*)p.dout.data + b * p.dout.b + i0 * p.dout.l + h * p.dout.h, p.dout.l, left, p.D, tid);
     };
-    auto finish = [&](int buf) {
-        wait_loads();
-        now = range;
-        float* const of = rows + buf * 4 * C::BR;
-        // A row that sees nothing (its log-sum is -inf) is zero, whatever the arrays hold there.
-        const bool none = tid < C::BR && r_lse == -__builtin_inff();
-        if (tid < C::BR) {
-            of[tid] = none ? __builtin_inff() : r_lse * kLog2e;  // p = exp2(z - inf) = 0
-            of[C::BR + tid] = none ? 0.f : -r_delta;
-            of[2 * C::BR + tid] = r_slope;
-            of[3 * C::BR + tid] = __int_as_float(none ? -1 : r_doc);
-        }
-        if (__syncthreads_or(none)) {
-            char* const q = lds + buf * 2 * C::kTile;
-            Rows::clear(q, [&](int i) { return of[i] == __builtin_inff(); }, tid);
-            Rows::clear(q + C::kTile, [&](int i) { return of[i] == __builtin_inff(); }, tid);
-            __syncthreads();
-        }
+    // A row that sees nothing is zero, whatever the arrays hold there.  (Rows behind the last one came as zeros: their
+    // probabilities, of whatever size, meet nothing but zeros.)
+    auto clean = [&](int buf) {
+        const float* const of = (const float*)(lds + C::kRows + buf * 3 * C::BR * 4);
+        if (!__any(of[lane % C::BR] == __builtin_inff())) return;
+        char* const q = lds + buf * 2 * C::kTile;
+        Rows::clear(q, [&](int i) { return of[i] == __builtin_inff(); }, tid);
+        Rows::clear(q + C::kTile, [&](int i) { return of[i] == __builtin_inff(); }, tid);
+        __syncthreads();
     };
+    static_assert(C::BR <= 64, "a wavefront looks over a tile's rows at once");
 
-    int t = tiles.next(lane), buf = 0;
-    if (C::kBufs == 2 && t >= 0) {
-        start(t, 0);
-        finish(0);
-    }
-    while (t >= 0) {
-        const int next = tiles.next(lane);
-        if (C::kBufs == 2) {
-            if (next >= 0) start(next, buf ^ 1);
-        } else {
-            __syncthreads();
-            start(t, 0);
-            finish(0);
-        }
+    Ring<C::kBufs, 2 * Rows::kLoads, Walk, decltype(start)> ring(walk, start);
+    for (; ring.ready(); ring.pop()) {
+        const int buf = ring.buf, t = ring.queue[0].t;
+        clean(buf);
+        ring.more();
         const char* qt = lds + buf * 2 * C::kTile;
         const char* gt = qt + C::kTile;
         const int q0 = rg * 32;
-        const float* of = rows + buf * 4 * C::BR + q0 + 4 * half;  // what the rows of registers 4 g .. have: of[array BR + 8 g + e]
+        // what the rows of registers 4 g .. have, array BR + 8 g + e: the log-sum, -delta, the document
+        const float* of = (const float*)(lds + C::kRows + buf * 3 * C::BR * 4) + q0 + 4 * half;
         {
-            const int first_at = (t_first + t % len) * C::BR + q0 + offset;
-            const bool masked = !__all(from <= first_at && first_at + 31 <= to && (!p.qdoc || (now.x == doc && now.y == doc)));
+            const int g_of = t / len, first_at = (t_first + t - g_of * len) * C::BR + q0 + offset;
+            const int2 theirs = ring.queue[0].documents;
+            const bool masked = !__all(from <= first_at && first_at + 31 <= to && (!p.qdoc || (theirs.x == doc && theirs.y == doc)));
             f32x16 s = zero16();
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
@@ -322,7 +304,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
                 }
             }
             if (p.slopes) {
-                const float slope = of[2 * C::BR];
+                const float slope = p.slopes[(c * p.G + g_of) * p.slope_stride] * kLog2e;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = s[i] * sc.unit - slope * fabsf((float)(first_at + 4 * half + c_row(i) - key));
             }
@@ -337,7 +319,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
                 for (int i = 0; i < 16; ++i) {
                     const int at = first_at + 4 * half + c_row(i);
                     bool sees = from <= at && at <= to;
-                    if (p.qdoc) sees = sees && __float_as_int(of[3 * C::BR + c_row(i)]) == doc;
+                    if (p.qdoc) sees = sees && __float_as_int(of[2 * C::BR + c_row(i)]) == doc;
                     s[i] = sees ? s[i] : 0.f;
                     g[i] = sees ? g[i] : 0.f;
                 }
@@ -359,11 +341,6 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
                 for (int d = 0; d < DP / 32; ++d) dk[d] = M::mma(cols_frag<DP>((const T*)0, qt, q0 + 16 * h, d * 32, lane), f, dk[d]);
             }
         }
-        if (C::kBufs == 2 && next >= 0) {
-            buf ^= 1;
-            finish(buf);
-        }
-        t = next;
     }
     if (C::RG > 1) {
         // the wavefronts that share keys add up, one sum after the other
@@ -437,7 +414,8 @@ template <class T, int DP>
 struct BackwardConfig {
     static constexpr int kRowBytes = DP * (int)sizeof(T);
     // dq: rows and their gradients stay in registers; two workgroups a compute unit up to 128 features in bf16
-    typedef QueryConfig<T, DP, kRowBytes <= 256 ? 64 : 32, kRowBytes <= 768 ? 2 : 1, kRowBytes <= 256 && sizeof(T) == 2 ? 2 : 1> Q;
+    typedef QueryConfig<T, DP, kRowBytes <= 256 ? 64 : 32, kRowBytes <= 128 ? 3 : kRowBytes <= 256 ? 2 : kRowBytes <= 512 ? 4 : kRowBytes <= 768 ? 2 : 1,
+                        kRowBytes <= 256 && sizeof(T) == 2 ? 2 : 1> Q;
 };
 // keys and values in registers where the sums leave room for them, sums of 256 features and more with one wavefront a SIMD
 template <class T, int DP>

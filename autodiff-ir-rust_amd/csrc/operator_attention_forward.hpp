@@ -78,24 +78,25 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
     const int2* const kr = p.krange ? p.krange + (int64_t)b * p.kranges : nullptr;
     int2 mine = {0, 0};
     if (kr) mine = document_range(p.qrange + (int64_t)b * p.qranges, first, last);
-    auto needed = [&](int t) {
+    auto needed = [&](int t, int2& theirs) {
         const int j0 = t * C::BK, j1 = min(j0 + C::BK, n) - 1;
         if (j0 >= prefix && (j0 > hi_all || j1 < lo_all)) return false;
         if (!kr) return true;
-        const int2 theirs = document_range(kr, j0, j1);
+        theirs = document_range(kr, j0, j1);
         return theirs.x <= mine.y && mine.x <= theirs.y;
     };
-    Tiles<decltype(needed)> tiles(needed, t_first, t_stop, split, p.splits);
-
-    Keys kt(p, b, c, n, tid, wk * C::KB * 32, lds);
-    int t = tiles.next(lane), buf = 0;
-    kt.begin(t);
-    while (t >= 0) {
-        const int next = tiles.next(lane);
-        kt.fetch(t, next, buf);
+    typedef Tiles<decltype(needed)> Walk;
+    Walk walk(needed, t_first, t_stop, split, p.splits, lane);
+    const Keys kt(p, b, c, n, tid, lds);
+    Ring<C::kBufs, Keys::kLoads, Walk, Keys> ring(walk, kt);
+    for (; ring.ready(); ring.pop()) {
+        const int buf = ring.buf, t = ring.queue[0].t;
+        kt.clean(ring.queue[0], buf);
+        ring.more();
         const char* ks = kt.keys(buf);
         const char* vs = kt.values(buf);
-        const int* docs = kt.docs(buf);
+        const int* docs = (const int*)kt.docs(buf);
+        const bool one_document = !kt.kd || (ring.queue[0].documents.x == doc && ring.queue[0].documents.y == doc);
         f32x16 s[C::KB];
 #pragma unroll
         for (int x = 0; x < C::KB; ++x) {
@@ -118,10 +119,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
                 for (int i = 0; i < 16; ++i) s[x][i] = s[x][i] * inner - slope * fabsf((float)(at - jl - 32 * x - c_row(i)));
         }
         // masks only where some row of the wavefront does not see all its keys of the tile
-        bool all = j0 + 32 * C::KB <= n && ((lo <= j0 && j0 + 32 * C::KB - 1 <= hi) || j0 + 32 * C::KB <= pre);
-#pragma unroll
-        for (int x = 0; x < C::KB; ++x) all = all && kt.one_document(x, doc);
-        if (!__all(all)) {
+        if (!__all(one_document && j0 + 32 * C::KB <= n && ((lo <= j0 && j0 + 32 * C::KB - 1 <= hi) || j0 + 32 * C::KB <= pre))) {
 #pragma unroll
             for (int x = 0; x < C::KB; ++x)
 #pragma unroll
@@ -165,8 +163,6 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
                 for (int d = 0; d < DP / 32; ++d) o[d] = M::mma(cols_frag<DP>((const T*)0, vs, (wk * C::KB + x) * 32 + 16 * h, d * 32, lane), f, o[d]);
             }
         }
-        kt.advance(next, buf);
-        t = next;
     }
     l = sum_of_halves(l);
     m *= unit;
@@ -280,10 +276,11 @@ __global__ __launch_bounds__(256) void join_kernel(const Params p) {
 
 template <class T, int DP>
 struct ForwardMany {
-    // 64 keys a tile; 32 where two tiles of 64 would not leave room for a second workgroup or, at 512 bytes a feature row and
-    // more, not fit
+    // 64 keys a tile; 32 where tiles of 64 would not leave room for a second workgroup or not fit; as many tiles as LDS has room
+    // for beside the workgroups that registers allow
     static constexpr int kRowBytes = DP * (int)sizeof(T);
-    typedef ForwardConfig<T, DP, 4, 1, kRowBytes <= 256 ? 64 : 32, 2, kRowBytes <= 128 ? 3 : kRowBytes <= 256 ? 2 : 1> C;
+    typedef ForwardConfig<T, DP, 4, 1, kRowBytes <= 256 ? 64 : 32, kRowBytes <= 128 ? 3 : kRowBytes <= 256 ? 2 : kRowBytes <= 512 ? 4 : 2,
+                          kRowBytes <= 128 ? 3 : kRowBytes <= 256 ? 2 : 1> C;
 };
 template <class T, int DP>
 struct ForwardFew {
