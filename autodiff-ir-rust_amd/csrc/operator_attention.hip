@@ -21,14 +21,15 @@ __global__ __launch_bounds__(256) void document_ranges_kernel(const int* q, int6
     if (of_keys && e >= kn) return;
     const int i = e * attn::kRange + lane;
     const bool there = i < (of_keys ? Lk : Lq);
-    const int d = !there ? 0 : max(of_keys ? k[b * kb + i * kl] : q[b * qb + i * ql], -1);
-    int lo = there ? d : 0x7fffffff, hi = there ? d : -2;
+    const int d = !there ? -1 : max(of_keys ? k[b * kb + i * kl] : q[b * qb + i * ql], -1);
+    int lo = d >= 0 ? d : 0x7fffffff, hi = d, none = there && d < 0;
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) {
         lo = min(lo, __shfl_xor(lo, s));
         hi = max(hi, __shfl_xor(hi, s));
+        none |= __shfl_xor(none, s);
     }
-    if (lane == 0) (of_keys ? kr + (int64_t)b * kn : qr + (int64_t)b * qn)[e] = int2{lo, hi};
+    if (lane == 0) (of_keys ? kr + (int64_t)b * kn : qr + (int64_t)b * qn)[e] = int2{none ? ~lo : lo, hi};
 }
 
 attn::Tensor tensor_of(const adhip_array& a) {

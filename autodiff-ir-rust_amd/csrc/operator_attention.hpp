@@ -33,7 +33,7 @@ struct Params {
     int64_t slope_stride;
     const int *lengths, *prefix, *qdoc, *kdoc;
     int64_t lengths_s, prefix_s, qdoc_b, qdoc_l, kdoc_b, kdoc_l;
-    const int2 *qrange, *krange;  // smallest and largest document of every kRange positions, those below 0 as -1
+    const int2 *qrange, *krange;  // the range of documents of every kRange positions (document_range)
     int qranges, kranges;         // entries of a sequence
     int B, Lq, Lk, Hk, G, D, R;   // R = Lq G rows
     float scale, cap;
@@ -224,20 +224,42 @@ struct Band {
     }
 };
 
+// What a lane's row sees of a run of keys, by the run's ends: a wavefront whose rows all see everything skips the masks, one
+// whose rows each see all or nothing takes one choice a row.  Rows that matter to nobody (`idle`: behind the last one, of no
+// document) see everything, so that they keep no wavefront from that; their results are replaced at the end.
+struct Sight {
+    int lo, hi, pre, doc;  // hi below the sequence's end
+    bool idle;
+    __device__ __forceinline__ bool all(int first, int last, bool documents, int2 theirs) const {
+        return idle || (((lo <= first && last <= hi) || last < pre) && (!documents || (theirs.x == doc && theirs.y == doc)));
+    }
+    __device__ __forceinline__ bool none(int first, int last, bool documents, int2 theirs) const {
+        return ((last < lo || first > hi) && first >= pre) || (documents && (doc < (theirs.x < 0 ? ~theirs.x : theirs.x) || doc > theirs.y));
+    }
+    __device__ __forceinline__ bool sees(int j) const { return (unsigned)(j - lo) <= (unsigned)(hi - lo) || j < pre; }
+};
+
 __device__ __forceinline__ int sequence_length(const Params& p, int b) {
     const int n = p.lengths ? p.lengths[b * p.lengths_s] : p.Lk;
     return min(max(n, 0), p.Lk);
 }
 
-// smallest and largest document of positions first .. last from the table of ranges (-1: some belong to none)
+// Smallest and largest document (of those from 0 on) of some positions: x, y; x is its complement, and so negative, where
+// some of the positions belong to none.
 __device__ __forceinline__ int2 document_range(const int2* ranges, int first, int last) {
-    int2 r = {0x7fffffff, -2};
+    int2 r = {0x7fffffff, -1};
+    int none = 0;
     for (int i = first / kRange; i <= last / kRange; ++i) {
         const int2 x = ranges[i];
-        r.x = min(r.x, x.x);
+        none |= x.x;
+        r.x = min(r.x, x.x < 0 ? ~x.x : x.x);
         r.y = max(r.y, x.y);
     }
+    if (none < 0) r.x = ~r.x;
     return r;
+}
+__device__ __forceinline__ bool documents_meet(int2 a, int2 b) {
+    return (a.x < 0 ? ~a.x : a.x) <= b.y && (b.x < 0 ? ~b.x : b.x) <= a.y;
 }
 
 // Walks the tiles begin .. stop - 1 that a block needs, 64 candidates at a time: each lane decides on one, all wavefronts

@@ -45,14 +45,13 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
     bool valid = row < p.R;
     const int token = valid ? row / p.G : 0, head = c * p.G + (valid ? row - token * p.G : 0);
     const int at = token + offset;
-    int lo = at - band.below, hi = at + band.above, pre = prefix;
     const int doc = p.qdoc && valid ? p.qdoc[b * p.qdoc_b + token * p.qdoc_l] : 0;
     const float slope = p.slopes && valid ? p.slopes[head * p.slope_stride] * kLog2e : 0.f;
     const float lse = valid ? p.lse[b * p.lse_b + token * p.lse_l + head * p.lse_h] : -__builtin_inff();
     const bool inside = valid;
     // a row that sees nothing has no gradient, whatever dout holds there
     if (lse == -__builtin_inff()) valid = false;
-    if (!valid || doc < 0) lo = 1, hi = 0, pre = 0;
+    const Sight sight = {at - band.below, min(at + band.above, n - 1), prefix, doc, !valid};
     const float lse2 = lse * kLog2e;
 
     Frag qf[DP / 16], df[DP / 16];
@@ -90,7 +89,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
         if (j0 >= prefix && (j0 > hi_all || j1 < lo_all)) return false;
         if (!kr) return true;
         theirs = document_range(kr, j0, j1);
-        return theirs.x <= mine.y && mine.x <= theirs.y;
+        return documents_meet(mine, theirs);
     };
     typedef Tiles<decltype(needed)> Walk;
     Walk walk(needed, t_first, t_stop, split, p.dq_splits, lane);
@@ -103,7 +102,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
         const char* ks = kt.keys(buf);
         const char* vs = kt.values(buf);
         const int* docs = (const int*)kt.docs(buf);
-        const bool one_document = !kt.kd || (ring.queue[0].documents.x == doc && ring.queue[0].documents.y == doc);
+        const int2 theirs = ring.queue[0].documents;
 #pragma unroll
         for (int x = 0; x < C::KB; ++x) {
             const int key0 = x * 32;
@@ -115,7 +114,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) g = M::mma(rows_frag<T, DP>(vs, key0, k, lane), df[k], g);
             const int j0 = t * C::BK + key0, jl = j0 + 4 * half;
-            const bool masked = !__all(j0 + 31 < n && ((lo <= j0 && j0 + 31 <= hi) || j0 + 31 < pre) && one_document);
+            const bool all = sight.all(j0, j0 + 31, kt.kd, theirs);
             if (p.cap > 0.f) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -129,13 +128,23 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], unit, -lse2)) * g[i];
-            if (masked) {
+            if (!__all(all)) {
+                if (__all(all || sight.none(j0, j0 + 31, kt.kd, theirs))) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = jl + c_row(i);
-                    bool sees = j < n && (j < pre || (lo <= j && j <= hi));
-                    if (kt.kd) sees = sees && docs[key0 + 4 * half + c_row(i)] == doc;
-                    s[i] = sees ? s[i] : 0.f;
+                    for (int i = 0; i < 16; ++i) s[i] = all ? s[i] : 0.f;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = sight.sees(jl + c_row(i)) ? s[i] : 0.f;
+                    if (kt.kd) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const int4 of = *(const int4*)(docs + key0 + 4 * half + c_row(i));
+                            s[i] = of.x == doc ? s[i] : 0.f;
+                            s[i + 1] = of.y == doc ? s[i + 1] : 0.f;
+                            s[i + 2] = of.z == doc ? s[i + 2] : 0.f;
+                            s[i + 3] = of.w == doc ? s[i + 3] : 0.f;
+                        }
+                    }
                 }
             }
 #pragma unroll
@@ -148,6 +157,12 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
         }
     }
     if (!inside) return;
+    if (__any(!valid)) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dq[d][i] = valid ? dq[d][i] : 0.f;
+    }
     float* const part = p.dq_splits > 1 ? p.part_dq + ((((int64_t)split * p.B + b) * p.Hk + c) * p.R + row) * p.D : nullptr;
     T* const out = (T*)p.dq.data + b * p.dq.b + token * p.dq.l + head * p.dq.h;
 #pragma unroll
@@ -199,9 +214,10 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
     const int doc = p.kdoc && key < n ? p.kdoc[b * p.kdoc_b + key * p.kdoc_l] : 0;
     const bool valid = key < n && doc >= 0;
     // rows at positions from .. to see this key (limits of the sequence aside), all rows where it is in the prefix
-    int from = key - band.above, to = key + band.below;
-    if (key < prefix) from = -0x7fffffff, to = 0x7fffffff;
-    if (!valid) from = 1, to = 0;
+    // (a key that no row may see sees everything here, so that it keeps no wavefront from the short way; its gradients are
+    // replaced at the end)
+    const bool free = !valid || key < prefix;
+    const int from = free ? -(1 << 30) : key - band.above, to = free ? 1 << 30 : key + band.below;
 
     Frag kf[C::K_LDS ? 1 : DP / 16], vf[C::V_LDS ? 1 : DP / 16];
     {
@@ -237,7 +253,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         if (!qr) return true;
         const int i0 = (t_first + u % len) * C::BR;
         theirs = document_range(qr, i0, min(i0 + C::BR, p.Lq) - 1);
-        return theirs.x <= mine.y && mine.x <= theirs.y;
+        return documents_meet(mine, theirs);
     };
     typedef Tiles<decltype(needed)> Walk;
     Walk walk(needed, 0, len * p.G, split, p.dk_splits, lane);
@@ -281,7 +297,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         {
             const int g_of = t / len, first_at = (t_first + t - g_of * len) * C::BR + q0 + offset;
             const int2 theirs = ring.queue[0].documents;
-            const bool masked = !__all(from <= first_at && first_at + 31 <= to && (!p.qdoc || (theirs.x == doc && theirs.y == doc)));
+            const bool all = from <= first_at && first_at + 31 <= to && (!p.qdoc || !valid || (theirs.x == doc && theirs.y == doc));
             f32x16 s = zero16();
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
@@ -314,14 +330,30 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + e], unit, -lse[e]));
             }
-            if (masked) {
+            if (!__all(all)) {
+                const bool none = first_at > to || first_at + 31 < from ||
+                                  (p.qdoc && (doc < (theirs.x < 0 ? ~theirs.x : theirs.x) || doc > theirs.y));
+                if (__all(all || none)) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int at = first_at + 4 * half + c_row(i);
-                    bool sees = from <= at && at <= to;
-                    if (p.qdoc) sees = sees && __float_as_int(of[2 * C::BR + c_row(i)]) == doc;
-                    s[i] = sees ? s[i] : 0.f;
-                    g[i] = sees ? g[i] : 0.f;
+                    for (int i = 0; i < 16; ++i) s[i] = all ? s[i] : 0.f, g[i] = all ? g[i] : 0.f;
+                } else {
+                    const int rel = first_at + 4 * half - from;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const bool sees = (unsigned)(rel + c_row(i)) <= (unsigned)(to - from);
+                        s[i] = sees ? s[i] : 0.f;
+                        g[i] = sees ? g[i] : 0.f;
+                    }
+                    if (p.qdoc) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const int4 x = *(const int4*)(of + 2 * C::BR + c_row(i));
+                            s[i] = x.x == doc ? s[i] : 0.f, g[i] = x.x == doc ? g[i] : 0.f;
+                            s[i + 1] = x.y == doc ? s[i + 1] : 0.f, g[i + 1] = x.y == doc ? g[i + 1] : 0.f;
+                            s[i + 2] = x.z == doc ? s[i + 2] : 0.f, g[i + 2] = x.z == doc ? g[i + 2] : 0.f;
+                            s[i + 3] = x.w == doc ? s[i + 3] : 0.f, g[i + 3] = x.w == doc ? g[i + 3] : 0.f;
+                        }
+                    }
                 }
             }
 #pragma unroll
@@ -376,6 +408,12 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         if (rg > 0) return;
     }
     if (key >= p.Lk) return;
+    if (__any(!valid)) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dk[d][i] = valid ? dk[d][i] : 0.f, dv[d][i] = valid ? dv[d][i] : 0.f;
+    }
     const int64_t part_at = ((((int64_t)split * p.B + b) * p.Hk + c) * p.Lk + key) * p.D;
     T* ko = (T*)p.dk.data + b * p.dk.b + key * p.dk.l + c * p.dk.h;
     T* vo = (T*)p.dv.data + b * p.dv.b + key * p.dv.l + c * p.dv.h;

@@ -51,9 +51,9 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
     const bool valid = row < p.R;
     const int token = valid ? row / p.G : 0, head = c * p.G + (valid ? row - token * p.G : 0);
     const int at = token + offset;
-    int lo = at - band.below, hi = at + band.above, pre = prefix;
     const int doc = p.qdoc && valid ? p.qdoc[b * p.qdoc_b + token * p.qdoc_l] : 0;
-    if (!valid || doc < 0) lo = 1, hi = 0, pre = 0;
+    const bool blind = doc < 0;  // of no document
+    const Sight sight = {at - band.below, min(at + band.above, n - 1), prefix, doc, !valid || blind};
     const float slope = p.slopes && valid ? p.slopes[head * p.slope_stride] * kLog2e : 0.f;
 
     Frag qf[DP / 16];
@@ -83,7 +83,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         if (j0 >= prefix && (j0 > hi_all || j1 < lo_all)) return false;
         if (!kr) return true;
         theirs = document_range(kr, j0, j1);
-        return theirs.x <= mine.y && mine.x <= theirs.y;
+        return documents_meet(mine, theirs);
     };
     typedef Tiles<decltype(needed)> Walk;
     Walk walk(needed, t_first, t_stop, split, p.splits, lane);
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         const char* ks = kt.keys(buf);
         const char* vs = kt.values(buf);
         const int* docs = (const int*)kt.docs(buf);
-        const bool one_document = !kt.kd || (ring.queue[0].documents.x == doc && ring.queue[0].documents.y == doc);
+        const int2 theirs = ring.queue[0].documents;
         f32x16 s[C::KB];
 #pragma unroll
         for (int x = 0; x < C::KB; ++x) {
@@ -118,17 +118,32 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[x][i] = s[x][i] * inner - slope * fabsf((float)(at - jl - 32 * x - c_row(i)));
         }
-        // masks only where some row of the wavefront does not see all its keys of the tile
-        if (!__all(one_document && j0 + 32 * C::KB <= n && ((lo <= j0 && j0 + 32 * C::KB - 1 <= hi) || j0 + 32 * C::KB <= pre))) {
+        const int j1 = j0 + 32 * C::KB - 1;
+        const bool all = sight.all(j0, j1, kt.kd, theirs);
+        if (!__all(all)) {
+            if (__all(all || sight.none(j0, j1, kt.kd, theirs))) {
 #pragma unroll
-            for (int x = 0; x < C::KB; ++x)
+                for (int x = 0; x < C::KB; ++x)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = jl + 32 * x + c_row(i);
-                    bool sees = j < n && (j < pre || (lo <= j && j <= hi));
-                    if (kt.kd) sees = sees && docs[(wk * C::KB + x) * 32 + 4 * half + c_row(i)] == doc;
-                    s[x][i] = sees ? s[x][i] : -__builtin_inff();
+                    for (int i = 0; i < 16; ++i) s[x][i] = all ? s[x][i] : -__builtin_inff();
+            } else {
+#pragma unroll
+                for (int x = 0; x < C::KB; ++x)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[x][i] = sight.sees(jl + 32 * x + c_row(i)) ? s[x][i] : -__builtin_inff();
+                if (kt.kd) {
+#pragma unroll
+                    for (int x = 0; x < C::KB; ++x)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const int4 of = *(const int4*)(docs + (wk * C::KB + x) * 32 + 4 * half + c_row(i));
+                            s[x][i] = of.x == doc ? s[x][i] : -__builtin_inff();
+                            s[x][i + 1] = of.y == doc ? s[x][i + 1] : -__builtin_inff();
+                            s[x][i + 2] = of.z == doc ? s[x][i + 2] : -__builtin_inff();
+                            s[x][i + 3] = of.w == doc ? s[x][i + 3] : -__builtin_inff();
+                        }
                 }
+            }
         }
         float top = s[0][0];
 #pragma unroll
@@ -166,6 +181,14 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
     }
     l = sum_of_halves(l);
     m *= unit;
+    if (__any(blind)) {
+        l = blind ? 0.f : l;
+        m = blind ? -__builtin_inff() : m;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = blind ? 0.f : o[d][i];
+    }
 
     const int64_t rows_before = (((int64_t)split * p.B + b) * p.Hk + c) * p.R;
     if (C::WK == 1) {
