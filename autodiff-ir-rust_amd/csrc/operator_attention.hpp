@@ -81,13 +81,33 @@ struct Lds {
     static constexpr int kPieces = DP * (int)sizeof(T) / 16;
     static constexpr int kPlaces = kPieces == 12 ? 16 : kPieces;  // the exchange wants a power of two in each row
     static constexpr int kPitch = kPlaces * 16;                   // bytes
-    static __device__ __forceinline__ int swap(int row) {
+    static __device__ __forceinline__ constexpr int swap(int row) {
         if (kPlaces % 16 == 0) return (row & 3) << 2 | (row >> 2 & 3);
         if (kPlaces % 8 == 0) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
         return row >> 2 & 3;
     }
-    static __device__ __forceinline__ int at(int row, int piece) { return row * kPitch + (piece ^ swap(row)) * 16; }
+    static constexpr int kSwapped = kPlaces % 16 == 0 ? 15 : kPlaces % 8 == 0 ? 7 : 3;  // bits of a piece's number that are
+    static __device__ __forceinline__ constexpr int at(int row, int piece) { return row * kPitch + (piece ^ swap(row)) * 16; }
+    // From the address of (row, piece) to that of (row + rows, piece + pieces), where neither addition carries: the exchange is
+    // linear in the bits.
+    static __device__ __forceinline__ constexpr unsigned step(unsigned from, int rows, int pieces) {
+        return (from ^ (unsigned)((swap(rows) ^ pieces) & kSwapped) * 16u) + (unsigned)((pieces & ~kSwapped) * 16 + rows * kPitch);
+    }
 };
+
+// Addresses in LDS as numbers
+template <class V>
+__device__ __forceinline__ V lds_read(unsigned at) {
+    return *(__attribute__((address_space(3))) const V*)(uintptr_t)at;
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)p; }  // (it ends in the offset)
+
+// Where a lane's part of an operand begins in a tile: the operand's other parts are an exclusive or and a fixed offset away.
+// `here` keeps the compiler from computing all of them ahead of a loop, where they would fill registers.
+__device__ __forceinline__ unsigned here(unsigned x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 
 __device__ __forceinline__ f32x16 zero16() {
     f32x16 z;
@@ -96,40 +116,45 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
-// A (or B) operand whose rows are rows of the tile: rows row0 .. + 31 (row0 a multiple of 16), features 16 step .. + 15
+// A (or B) operand whose rows are rows of the tile: rows row0 .. + 31 (row0 a multiple of 16), features 16 step .. + 15;
+// `from`: the tile's address + rows_lane()
 template <class T, int DP>
-__device__ __forceinline__ typename Matrix<T>::Frag rows_frag(const char* tile, int row0, int step, int lane) {
+__device__ __forceinline__ unsigned rows_lane(int lane) {
+    return (unsigned)Lds<T, DP>::at(lane & 31, (lane >> 5) * (int)(sizeof(typename Matrix<T>::Frag) / 16));
+}
+template <class T, int DP>
+__device__ __forceinline__ typename Matrix<T>::Frag rows_frag(unsigned from, int row0, int step) {
     typedef typename Matrix<T>::Frag Frag;
     constexpr int N = sizeof(Frag) / 16;
     Frag f;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        ((uint4*)&f)[i] = *(const uint4*)(tile + row0 * Lds<T, DP>::kPitch + Lds<T, DP>::at(lane & 31, (2 * step + (lane >> 5)) * N + i));
+    for (int i = 0; i < N; ++i) ((f32x4*)&f)[i] = lds_read<f32x4>(Lds<T, DP>::step(from, row0, 2 * N * step + i));
     return f;
 }
 
 // A operand whose rows are features d0 .. + 31 of the tile and whose k are its rows k0 .. + 15 (a multiple of 16), in the order
-// of C's registers
-template <int DP>
-__device__ __forceinline__ bf16x8 cols_frag(const bf16*, const char* tile, int k0, int d0, int lane) {
-    typedef __attribute__((address_space(3))) s16x4* Ptr;
-    typedef Lds<bf16, DP> L;
-    const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), piece = d0 / 8 + (lane >> 4 & 1) * 2 + (lane >> 1 & 1);
-    const char* base = tile + k0 * L::kPitch + 8 * (lane & 1);
-    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(base + L::at(row, piece)));
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(base + L::at(row + 8, piece)));
-    const s16x8 r = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-    return __builtin_bit_cast(bf16x8, r);
+// of C's registers; `from`: the tile's address + cols_lane()
+template <class T, int DP>
+__device__ __forceinline__ unsigned cols_lane(int lane) {
+    if (sizeof(T) == 2)
+        return (unsigned)Lds<T, DP>::at(4 * (lane >> 5) + ((lane & 15) >> 2), (lane >> 4 & 1) * 2 + (lane >> 1 & 1)) + 8 * (lane & 1);
+    return (unsigned)Lds<T, DP>::at(4 * (lane >> 5), (lane & 31) >> 2) + 4 * (lane & 3);
 }
-template <int DP>
-__device__ __forceinline__ f32x8 cols_frag(const float*, const char* tile, int k0, int d0, int lane) {
-    typedef Lds<float, DP> L;
-    const int piece = d0 / 4 + ((lane & 31) >> 2);
-    const char* base = tile + k0 * L::kPitch + 4 * (lane & 3);
-    f32x8 r;
+template <class T, int DP>
+__device__ __forceinline__ typename Matrix<T>::Frag cols_frag(unsigned from, int k0, int d0) {
+    typedef Lds<T, DP> L;
+    if constexpr (sizeof(T) == 2) {
+        typedef __attribute__((address_space(3))) s16x4* Ptr;
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(uintptr_t)L::step(from, k0, d0 / 8));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(uintptr_t)L::step(from, k0 + 8, d0 / 8));
+        const s16x8 r = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_bit_cast(bf16x8, r);
+    } else {
+        f32x8 r;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = *(const float*)(base + L::at(4 * (lane >> 5) + (e & 3) + 2 * (e & 4), piece));
-    return r;
+        for (int e = 0; e < 8; ++e) r[e] = lds_read<float>(L::step(from, k0 + (e & 3) + 2 * (e & 4), d0 / 4));
+        return r;
+    }
 }
 
 // registers 8 s .. + 7 of a C tile as a B operand.  Probabilities and score gradients are rounded to the operands' type

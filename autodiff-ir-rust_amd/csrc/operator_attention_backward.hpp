@@ -91,6 +91,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
         theirs = document_range(kr, j0, j1);
         return documents_meet(mine, theirs);
     };
+    const unsigned r_lane = rows_lane<T, DP>(lane), c_lane = cols_lane<T, DP>(lane);
     typedef Tiles<decltype(needed)> Walk;
     Walk walk(needed, t_first, t_stop, split, p.dq_splits, lane);
     const Keys kt(p, b, c, n, tid, lds);
@@ -99,8 +100,8 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
         const int buf = ring.buf, t = ring.queue[0].t;
         kt.clean(ring.queue[0], buf);
         ring.more();
-        const char* ks = kt.keys(buf);
-        const char* vs = kt.values(buf);
+        const unsigned kr_at = here(lds_address(kt.keys(buf)) + r_lane), vr_at = here(lds_address(kt.values(buf)) + r_lane);
+        const unsigned kc_at = here(lds_address(kt.keys(buf)) + c_lane);
         const int* docs = (const int*)kt.docs(buf);
         const int2 theirs = ring.queue[0].documents;
 #pragma unroll
@@ -110,9 +111,9 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
 #pragma unroll
             for (int i = 0; i < 16; ++i) g[i] = -delta;
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) s = M::mma(rows_frag<T, DP>(ks, key0, k, lane), qf[k], s);
+            for (int k = 0; k < DP / 16; ++k) s = M::mma(rows_frag<T, DP>(kr_at, key0, k), qf[k], s);
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) g = M::mma(rows_frag<T, DP>(vs, key0, k, lane), df[k], g);
+            for (int k = 0; k < DP / 16; ++k) g = M::mma(rows_frag<T, DP>(vr_at, key0, k), df[k], g);
             const int j0 = t * C::BK + key0, jl = j0 + 4 * half;
             const bool all = sight.all(j0, j0 + 31, kt.kd, theirs);
             if (p.cap > 0.f) {
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
                 Frag f;
                 to_frag(s, h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dq[d] = M::mma(cols_frag<DP>((const T*)0, ks, key0 + 16 * h, d * 32, lane), f, dq[d]);
+                for (int d = 0; d < DP / 32; ++d) dq[d] = M::mma(cols_frag<T, DP>(kc_at, key0 + 16 * h, d * 32), f, dq[d]);
             }
         }
     }
@@ -255,6 +256,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         theirs = document_range(qr, i0, min(i0 + C::BR, p.Lq) - 1);
         return documents_meet(mine, theirs);
     };
+    const unsigned r_lane = rows_lane<T, DP>(lane), c_lane = cols_lane<T, DP>(lane);
     typedef Tiles<decltype(needed)> Walk;
     Walk walk(needed, 0, len * p.G, split, p.dk_splits, lane);
 
@@ -289,9 +291,10 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         const int buf = ring.buf, t = ring.queue[0].t;
         clean(buf);
         ring.more();
-        const char* qt = lds + buf * 2 * C::kTile;
-        const char* gt = qt + C::kTile;
         const int q0 = rg * 32;
+        const unsigned tile_at = lds_address(lds) + buf * 2 * C::kTile + q0 * L::kPitch;
+        const unsigned rows_at = here(tile_at + r_lane), cols_at = here(tile_at + c_lane);  // of q; of dout kTile behind
+        const unsigned own_at = here(lds_address(k_own) + kg * 32 * L::kPitch + r_lane);
         // what the rows of registers 4 g .. have, array BR + 8 g + e: the log-sum, -delta, the document
         const float* of = (const float*)(lds + C::kRows + buf * 3 * C::BR * 4) + q0 + 4 * half;
         {
@@ -301,7 +304,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
             f32x16 s = zero16();
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
-                s = M::mma(rows_frag<T, DP>(qt, q0, k, lane), C::K_LDS ? rows_frag<T, DP>(k_own, kg * 32, k, lane) : kf[C::K_LDS ? 0 : k], s);
+                s = M::mma(rows_frag<T, DP>(rows_at, 0, k), C::K_LDS ? rows_frag<T, DP>(own_at, 0, k) : kf[C::K_LDS ? 0 : k], s);
             f32x16 g;
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
@@ -311,7 +314,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
             }
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
-                g = M::mma(rows_frag<T, DP>(gt, q0, k, lane), C::V_LDS ? rows_frag<T, DP>(v_own, kg * 32, k, lane) : vf[C::V_LDS ? 0 : k], g);
+                g = M::mma(rows_frag<T, DP>(rows_at, C::BR, k), C::V_LDS ? rows_frag<T, DP>(own_at, C::K_LDS ? C::BKEYS : 0, k) : vf[C::V_LDS ? 0 : k], g);
             if (p.cap > 0.f) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -361,7 +364,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
                 Frag f;
                 to_frag(s, h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dv[d] = M::mma(cols_frag<DP>((const T*)0, gt, q0 + 16 * h, d * 32, lane), f, dv[d]);
+                for (int d = 0; d < DP / 32; ++d) dv[d] = M::mma(cols_frag<T, DP>(cols_at, C::BR + 16 * h, d * 32), f, dv[d]);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] *= g[i];
@@ -370,7 +373,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
                 Frag f;
                 to_frag(s, h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dk[d] = M::mma(cols_frag<DP>((const T*)0, qt, q0 + 16 * h, d * 32, lane), f, dk[d]);
+                for (int d = 0; d < DP / 32; ++d) dk[d] = M::mma(cols_frag<T, DP>(cols_at, 16 * h, d * 32), f, dk[d]);
             }
         }
     }

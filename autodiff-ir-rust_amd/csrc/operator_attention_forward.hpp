@@ -85,6 +85,9 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         theirs = document_range(kr, j0, j1);
         return documents_meet(mine, theirs);
     };
+    // the lane's place in the wavefront's keys of a tile
+    const unsigned k_lane = rows_lane<T, DP>(lane) + wk * C::KB * 32 * Lds<T, DP>::kPitch;
+    const unsigned v_lane = cols_lane<T, DP>(lane) + wk * C::KB * 32 * Lds<T, DP>::kPitch;
     typedef Tiles<decltype(needed)> Walk;
     Walk walk(needed, t_first, t_stop, split, p.splits, lane);
     const Keys kt(p, b, c, n, tid, lds);
@@ -93,8 +96,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         const int buf = ring.buf, t = ring.queue[0].t;
         kt.clean(ring.queue[0], buf);
         ring.more();
-        const char* ks = kt.keys(buf);
-        const char* vs = kt.values(buf);
+        const unsigned ks = here(lds_address(kt.keys(buf)) + k_lane), vs = here(lds_address(kt.values(buf)) + v_lane);
         const int* docs = (const int*)kt.docs(buf);
         const int2 theirs = ring.queue[0].documents;
         f32x16 s[C::KB];
@@ -102,7 +104,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         for (int x = 0; x < C::KB; ++x) {
             s[x] = zero16();
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) s[x] = M::mma(rows_frag<T, DP>(ks, (wk * C::KB + x) * 32, k, lane), qf[k], s[x]);
+            for (int k = 0; k < DP / 16; ++k) s[x] = M::mma(rows_frag<T, DP>(ks, x * 32, k), qf[k], s[x]);
         }
         const int j0 = t * C::BK + wk * C::KB * 32, jl = j0 + 4 * half;  // register i of s[x] has key jl + 32 x + c_row(i)
         if (p.cap > 0.f) {
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
                 Frag f;
                 to_frag(s[x], h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) o[d] = M::mma(cols_frag<DP>((const T*)0, vs, (wk * C::KB + x) * 32 + 16 * h, d * 32, lane), f, o[d]);
+                for (int d = 0; d < DP / 32; ++d) o[d] = M::mma(cols_frag<T, DP>(vs, x * 32 + 16 * h, d * 32), f, o[d]);
             }
         }
     }
