@@ -32,6 +32,37 @@ __global__ __launch_bounds__(256) void document_ranges_kernel(const int* q, int6
     if (lane == 0) (of_keys ? kr + (int64_t)b * kn : qr + (int64_t)b * qn)[e] = int2{none ? ~lo : lo, hi};
 }
 
+// Arrays [B, L, H, D] of f32 as three bf16 parts: planes [B, L, H, D3], the features behind D zeros.  A thread a piece of 8.
+struct PartsJob {
+    attn::Tensor in;
+    bf16* out;
+    int64_t rows;  // B L H
+    int L, H;
+};
+struct PartsJobs {
+    PartsJob job[4];
+};
+__global__ __launch_bounds__(256) void parts_kernel(const PartsJobs jobs, int D, int D3) {
+    const PartsJob j = jobs.job[blockIdx.y];
+    const int pieces = D3 / 8;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / pieces, plane = j.rows * D3;
+    if (row >= j.rows) return;
+    const int d = (int)(at - row * pieces) * 8, h = (int)(row % j.H);
+    const int64_t bl = row / j.H, b = bl / j.L;
+    const float* x = (const float*)j.in.data + b * j.in.b + (bl - b * j.L) * j.in.l + h * j.in.h;
+    attn::f32x8 f;
+    if (j.in.vec && d + 8 <= D) {
+        ((float4*)&f)[0] = *(const float4*)(x + d);
+        ((float4*)&f)[1] = *(const float4*)(x + d + 4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = d + e < D ? x[d + e] : 0.f;
+    }
+    const attn::Frag3 p = attn::MatrixInParts::operand(f);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *(attn::bf16x8*)(j.out + i * plane + row * D3 + d) = p.p[i];
+}
+
 attn::Tensor tensor_of(const adhip_array& a) {
     const int chunk = 16 / type_bytes(a.type);
     attn::Tensor t = {a.data, a.strides[0], a.strides[1], a.strides[2], 0};
@@ -46,7 +77,8 @@ size_t rounded(size_t n) { return (n + 255) & ~size_t(255); }
 struct Layout {
     bool few_rows;
     int row_tile, tiles, splits, dq_splits, dk_splits;
-    size_t qrange, krange, part, part_ml, stats, part_dq, part_dk, part_dv, bytes;
+    size_t qrange, krange, part, part_ml, stats, part_dq, part_dk, part_dv, q3, k3, v3, dout3, bytes;
+    bool parts;
 };
 
 Layout layout_of(const adhip_attention_args& g, bool backward) {
@@ -70,6 +102,18 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
     at += rounded((size_t)(B * ((Lq + attn::kRange - 1) / attn::kRange)) * sizeof(int2));
     y.krange = at;
     at += rounded((size_t)(B * ((Lk + attn::kRange - 1) / attn::kRange)) * sizeof(int2));
+    y.parts = attn::in_parts(g.q.type, (int)D, backward ? false : y.few_rows);
+    if (y.parts) {
+        const size_t keys = rounded((size_t)(B * Lk * Hk * attn::parts_size((int)D)) * 6), rows = rounded((size_t)(B * Lq * H * attn::parts_size((int)D)) * 6);
+        y.k3 = at;
+        y.v3 = at + keys;
+        at += 2 * keys;
+        if (backward) {
+            y.q3 = at;
+            y.dout3 = at + rows;
+            at += 2 * rows;
+        }
+    }
     size_t forward = at, back = at;
     if (y.splits > 1) {
         y.part = forward;
@@ -195,6 +239,16 @@ Params checked(const char* op, const adhip_attention_args& g, const Layout& y, b
     p.cap = g.cap;
     p.causal = g.causal != 0;
     p.window = (int)std::min<int64_t>(g.window, int64_t(1) << 30);
+    if (y.parts) {
+        const int D3 = attn::parts_size((int)D);
+        p.D3 = D3;
+        p.k_plane = B * Lk * Hk * D3;
+        p.q_plane = B * Lq * H * D3;
+        p.k3 = {room + y.k3, Lk * Hk * D3, Hk * D3, D3, 1};
+        p.v3 = {room + y.v3, Lk * Hk * D3, Hk * D3, D3, 1};
+        p.q3 = {room + y.q3, Lq * H * D3, H * D3, D3, 1};
+        p.dout3 = {room + y.dout3, Lq * H * D3, H * D3, D3, 1};
+    }
     p.tiles = y.tiles;
     p.splits = y.splits;
     p.part = (float*)(room + y.part);
@@ -213,6 +267,20 @@ void document_ranges(const Params& p, hipStream_t stream) {
     if (!p.qdoc || entries == 0 || p.B == 0) return;
     document_ranges_kernel<<<(unsigned)((entries + 7) / 8 * p.B), 256, 0, stream>>>(
         p.qdoc, p.qdoc_b, p.qdoc_l, p.Lq, (int2*)p.qrange, p.qranges, p.kdoc, p.kdoc_b, p.kdoc_l, p.Lk, (int2*)p.krange, p.kranges);
+    check_launch("adhip_attention");
+}
+
+// Keys and values, with `rows` queries and out's gradient too, in parts
+void split_into_parts(const Params& p, bool rows, hipStream_t stream) {
+    PartsJobs jobs = {};
+    const int64_t keys = (int64_t)p.B * p.Lk * p.Hk, queries = (int64_t)p.B * p.Lq * p.Hk * p.G;
+    jobs.job[0] = {p.k, (bf16*)p.k3.data, keys, p.Lk, p.Hk};
+    jobs.job[1] = {p.v, (bf16*)p.v3.data, keys, p.Lk, p.Hk};
+    jobs.job[2] = {p.q, (bf16*)p.q3.data, queries, p.Lq, p.Hk * p.G};
+    jobs.job[3] = {p.dout, (bf16*)p.dout3.data, queries, p.Lq, p.Hk * p.G};
+    const int64_t most = (rows ? std::max(keys, queries) : keys) * (p.D3 / 8);
+    if (most == 0) return;
+    parts_kernel<<<dim3((unsigned)((most + 255) / 256), rows ? 4 : 2), 256, 0, stream>>>(jobs, p.D, p.D3);
     check_launch("adhip_attention");
 }
 
@@ -241,6 +309,7 @@ int adhip_attention(adhip_ctx* ctx, const adhip_attention_args* args, void* stre
         const Params p = checked(op, *args, y, false);
         if (p.R == 0 || p.B == 0) return;
         document_ranges(p, (hipStream_t)stream);
+        if (y.parts) split_into_parts(p, false, (hipStream_t)stream);
         if (args->q.type == ADHIP_BF16) attn::forward_bf16(p, y.few_rows, (hipStream_t)stream);
         else attn::forward_f32(p, y.few_rows, (hipStream_t)stream);
     });
@@ -255,6 +324,7 @@ int adhip_attention_backward(adhip_ctx* ctx, const adhip_attention_args* args, v
         const Params p = checked(op, *args, y, true);
         if (p.B == 0) return;
         document_ranges(p, (hipStream_t)stream);
+        if (y.parts) split_into_parts(p, true, (hipStream_t)stream);
         if (args->q.type == ADHIP_BF16) attn::backward_bf16(p, (hipStream_t)stream);
         else attn::backward_f32(p, (hipStream_t)stream);
     });

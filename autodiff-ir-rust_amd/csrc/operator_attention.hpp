@@ -9,7 +9,7 @@
 // k is free as long as A and B agree, so registers 8 s .. 8 s + 7 of a C tile are, as they stand, the B operand of a product
 // over its rows 16 s .. + 15: scores become the operand of the next product without leaving their lanes.  Its A operand
 // takes rows 16 s + 4 (lane / 32) + {0..3, 8..11} of the column lane % 32: the transposing reads of LDS for 16-bit
-// types, single words for 32-bit ones.  bf16 takes one instruction (32x32x16), f32 eight (32x32x2), with the same layouts.
+// types, single words for 32-bit ones.
 #pragma once
 #include "operators.hpp"
 
@@ -27,6 +27,9 @@ struct Tensor {
 
 struct Params {
     Tensor q, k, v, out, dout, dq, dk, dv;  // out: written by the forward kernels, read by the backward ones
+    Tensor q3, k3, v3, dout3;               // f32 in parts: three planes of bf16, q_plane or k_plane elements apart,
+    int64_t q_plane, k_plane;               // rows of D3 features, the last of them zeros
+    int D3;
     float* lse;
     int64_t lse_b, lse_l, lse_h;
     const float* slopes;
@@ -52,23 +55,81 @@ typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
-template <class T>
+// Ways to multiply: the type of arrays (IO) and of elements in LDS (E), the operand as loaded (Raw) and as multiplied.
+//   bf16   one instruction for 16 of k
+//   float  FP32 matrix cores, eight instructions of 64 cycles each
+//   Parts  f32 as the sum of three bf16 parts (24 bits: exactly), six products of parts on the bf16 matrix cores, what is
+//          left out being 2^-24 of the product: 192 cycles instead of 512.  Tiles hold three planes of parts, which a kernel
+//          of its own has made of the arrays, once for all workgroups.
+//   Split  the same with f32 in LDS, split where an operand is read: for keys that are read by one wavefront only.
+// Infinities lose their sign in the parts' products: where one is seen, the result is NaN.
+struct Parts {};
+struct Split {};
+struct Frag3 {
+    bf16x8 p[3];
+};
+template <class X>
 struct Matrix;
 template <>
 struct Matrix<bf16> {
+    typedef bf16 IO;
+    typedef bf16 E;
+    typedef bf16x8 Raw;
     typedef bf16x8 Frag;
-    static constexpr int kChunk = 8;  // elements of 16 bytes
-    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static constexpr int kChunk = 8, kPlanes = 1;  // elements of 16 bytes; tiles that make one
+    static __device__ __forceinline__ Frag operand(const Raw& x) { return x; }
+    static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Matrix<float> {
+    typedef float IO;
+    typedef float E;
+    typedef f32x8 Raw;
     typedef f32x8 Frag;
-    static constexpr int kChunk = 4;
-    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+    static constexpr int kChunk = 4, kPlanes = 1;
+    static __device__ __forceinline__ Frag operand(const Raw& x) { return x; }
+    static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
         return c;
     }
+};
+struct MatrixInParts {
+    typedef float IO;
+    typedef f32x8 Raw;
+    typedef Frag3 Frag;
+    static __device__ __forceinline__ Frag operand(const Raw& x) {
+        Frag f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bf16 hi = (bf16)x[e];
+            const float r = x[e] - (float)hi;
+            const bf16 mid = (bf16)r;
+            f.p[0][e] = hi;
+            f.p[1][e] = mid;
+            f.p[2][e] = (bf16)(r - (float)mid);
+        }
+        return f;
+    }
+    // the smallest products first
+    static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[2], b.p[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[2], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+    }
+};
+template <>
+struct Matrix<Parts> : MatrixInParts {
+    typedef bf16 E;
+    static constexpr int kChunk = 8, kPlanes = 3;
+};
+template <>
+struct Matrix<Split> : MatrixInParts {
+    typedef float E;
+    static constexpr int kChunk = 4, kPlanes = 1;
 };
 
 // Tiles in LDS: rows of DP features in pieces of 16 bytes, whose places within a row are exchanged by an exclusive or
@@ -76,9 +137,9 @@ struct Matrix<float> {
 // banks, and so do 4 rows at four pieces (the transposing reads): 230 and 200 bytes a clock, where rows padded by 16 bytes
 // give the first 230 and the second 62, unpadded ones 16 and less.  The exchange costs one instruction an address, and
 // pieces keep places of 16 bytes, so that loads can go to LDS without passing through registers.
-template <class T, int DP>
+template <class E, int DP>
 struct Lds {
-    static constexpr int kPieces = DP * (int)sizeof(T) / 16;
+    static constexpr int kPieces = DP * (int)sizeof(E) / 16;
     static constexpr int kPlaces = kPieces == 12 ? 16 : kPieces;  // the exchange wants a power of two in each row
     static constexpr int kPitch = kPlaces * 16;                   // bytes
     static __device__ __forceinline__ constexpr int swap(int row) {
@@ -116,44 +177,58 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
-// A (or B) operand whose rows are rows of the tile: rows row0 .. + 31 (row0 a multiple of 16), features 16 step .. + 15;
-// `from`: the tile's address + rows_lane()
-template <class T, int DP>
+// A (or B) operand whose rows are rows of a tile of ROWS rows: rows row0 .. + 31 (row0 a multiple of 16), features 16 step ..
+// + 15; `from`: the tile's address + rows_lane()
+template <class X, int DP>
 __device__ __forceinline__ unsigned rows_lane(int lane) {
-    return (unsigned)Lds<T, DP>::at(lane & 31, (lane >> 5) * (int)(sizeof(typename Matrix<T>::Frag) / 16));
+    typedef typename Matrix<X>::E E;
+    return (unsigned)Lds<E, DP>::at(lane & 31, (lane >> 5) * (int)sizeof(E) / 2);
 }
-template <class T, int DP>
-__device__ __forceinline__ typename Matrix<T>::Frag rows_frag(unsigned from, int row0, int step) {
-    typedef typename Matrix<T>::Frag Frag;
-    constexpr int N = sizeof(Frag) / 16;
-    Frag f;
+template <class X, int DP, int ROWS>
+__device__ __forceinline__ typename Matrix<X>::Frag rows_frag(unsigned from, int row0, int step) {
+    typedef Matrix<X> M;
+    typedef Lds<typename M::E, DP> L;
+    if constexpr (sizeof(typename M::E) == 2) {
+        typename M::Frag f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) ((f32x4*)&f)[i] = lds_read<f32x4>(Lds<T, DP>::step(from, row0, 2 * N * step + i));
-    return f;
+        for (int i = 0; i < M::kPlanes; ++i) ((f32x4*)&f)[i] = lds_read<f32x4>(L::step(from, row0 + i * ROWS, 2 * step));
+        return f;
+    } else {
+        typename M::Raw f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ((f32x4*)&f)[i] = lds_read<f32x4>(L::step(from, row0, 4 * step + i));
+        return M::operand(f);
+    }
 }
 
 // A operand whose rows are features d0 .. + 31 of the tile and whose k are its rows k0 .. + 15 (a multiple of 16), in the order
 // of C's registers; `from`: the tile's address + cols_lane()
-template <class T, int DP>
+template <class X, int DP>
 __device__ __forceinline__ unsigned cols_lane(int lane) {
-    if (sizeof(T) == 2)
-        return (unsigned)Lds<T, DP>::at(4 * (lane >> 5) + ((lane & 15) >> 2), (lane >> 4 & 1) * 2 + (lane >> 1 & 1)) + 8 * (lane & 1);
-    return (unsigned)Lds<T, DP>::at(4 * (lane >> 5), (lane & 31) >> 2) + 4 * (lane & 3);
+    typedef typename Matrix<X>::E E;
+    if (sizeof(E) == 2)
+        return (unsigned)Lds<E, DP>::at(4 * (lane >> 5) + ((lane & 15) >> 2), (lane >> 4 & 1) * 2 + (lane >> 1 & 1)) + 8 * (lane & 1);
+    return (unsigned)Lds<E, DP>::at(4 * (lane >> 5), (lane & 31) >> 2) + 4 * (lane & 3);
 }
-template <class T, int DP>
-__device__ __forceinline__ typename Matrix<T>::Frag cols_frag(unsigned from, int k0, int d0) {
-    typedef Lds<T, DP> L;
-    if constexpr (sizeof(T) == 2) {
+template <class X, int DP, int ROWS>
+__device__ __forceinline__ typename Matrix<X>::Frag cols_frag(unsigned from, int k0, int d0) {
+    typedef Matrix<X> M;
+    typedef Lds<typename M::E, DP> L;
+    if constexpr (sizeof(typename M::E) == 2) {
         typedef __attribute__((address_space(3))) s16x4* Ptr;
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(uintptr_t)L::step(from, k0, d0 / 8));
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(uintptr_t)L::step(from, k0 + 8, d0 / 8));
-        const s16x8 r = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-        return __builtin_bit_cast(bf16x8, r);
+        typename M::Frag f;
+#pragma unroll
+        for (int i = 0; i < M::kPlanes; ++i) {
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(uintptr_t)L::step(from, k0 + i * ROWS, d0 / 8));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(uintptr_t)L::step(from, k0 + 8 + i * ROWS, d0 / 8));
+            ((s16x8*)&f)[i] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return f;
     } else {
-        f32x8 r;
+        typename M::Raw r;
 #pragma unroll
         for (int e = 0; e < 8; ++e) r[e] = lds_read<float>(L::step(from, k0 + (e & 3) + 2 * (e & 4), d0 / 4));
-        return r;
+        return M::operand(r);
     }
 }
 
@@ -166,6 +241,11 @@ __device__ __forceinline__ void to_frag(const f32x16& c, int s, bf16x8& f) {
 __device__ __forceinline__ void to_frag(const f32x16& c, int s, f32x8& f) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = c[8 * s + e];
+}
+__device__ __forceinline__ void to_frag(const f32x16& c, int s, Frag3& f) {
+    f32x8 x;
+    to_frag(c, s, x);
+    f = MatrixInParts::operand(x);
 }
 
 // 16 bytes of a row of D features from d on; what lies behind the row's end is zero.  VEC: rows begin at multiples of 16
@@ -186,8 +266,8 @@ __device__ __forceinline__ uint4 load_chunk(const T* row, int d, int D) {
 
 // the stationary operand of a product: eight features of one row of an array
 template <bool VEC, class T>
-__device__ __forceinline__ typename Matrix<T>::Frag load_frag(const T* row, int d, int D, bool valid) {
-    typename Matrix<T>::Frag f;
+__device__ __forceinline__ typename Matrix<T>::Raw load_frag(const T* row, int d, int D, bool valid) {
+    typename Matrix<T>::Raw f;
     uint4* u = (uint4*)&f;
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(f) / 16); ++i)
@@ -467,23 +547,27 @@ __device__ __forceinline__ void copy_words(char* to, const void* from, int64_t s
 
 // Tiles of keys and values on their way from memory to LDS: shared by the kernels that own rows.  Keys behind the sequence
 // or of no document are zero, whatever the arrays hold there.
-template <class T, int DP, class C, bool VEC>
+template <class X, int DP, class C, bool VEC>
 struct KeyTiles {
-    typedef Copy<T, DP, C::BK, C::NT, VEC> S;
+    typedef Matrix<X> M;
+    typedef typename M::E E;
+    typedef Copy<E, DP, C::BK, C::NT, VEC || M::kPlanes == 3> S;
     static_assert(C::NT >= C::BK, "one thread a key for the documents");
-    static constexpr int kTile = C::BK * Lds<T, DP>::kPitch;
+    static constexpr int kPlane = C::BK * Lds<E, DP>::kPitch, kTile = M::kPlanes * kPlane;
     static constexpr int kBytes = C::kBufs * (2 * kTile + C::BK * 4);
-    static constexpr int kLoads = 2 * S::kLoads;
+    static constexpr int kLoads = 2 * M::kPlanes * S::kLoads;
     const Params& p;
-    const T *kb, *vb;
+    const Tensor &kt, &vt;
+    const E *kb, *vb;
     const int* kd;
     char* lds;
-    int n, tid;
+    int n, tid, D;
     S k, v;
     __device__ __forceinline__ KeyTiles(const Params& p_, int b, int c, int n_, int tid_, char* lds_)
-        : p(p_), lds(lds_), n(n_), tid(tid_), k(p_.k.l, p_.D, tid_), v(p_.v.l, p_.D, tid_) {
-        kb = (const T*)p.k.data + b * p.k.b + c * p.k.h;
-        vb = (const T*)p.v.data + b * p.v.b + c * p.v.h;
+        : p(p_), kt(M::kPlanes == 3 ? p_.k3 : p_.k), vt(M::kPlanes == 3 ? p_.v3 : p_.v), lds(lds_), n(n_), tid(tid_),
+          D(M::kPlanes == 3 ? p_.D3 : p_.D), k(kt.l, D, tid_), v(vt.l, D, tid_) {
+        kb = (const E*)kt.data + b * kt.b + c * kt.h;
+        vb = (const E*)vt.data + b * vt.b + c * vt.h;
         kd = p.kdoc ? p.kdoc + b * p.kdoc_b : nullptr;
     }
     __device__ __forceinline__ char* keys(int buf) const { return lds + buf * 2 * kTile; }
@@ -493,18 +577,24 @@ struct KeyTiles {
         const int64_t j0 = (int64_t)tile.t * C::BK;
         const int left = n - (int)j0;
         if (kd) copy_words<C::BK>(docs(buf), kd + j0 * p.kdoc_l, p.kdoc_l, left, tid, k.wave);
-        k.start(keys(buf), kb + j0 * p.k.l, p.k.l, left, p.D, tid);
-        v.start(values(buf), vb + j0 * p.v.l, p.v.l, left, p.D, tid);
+#pragma unroll
+        for (int i = 0; i < M::kPlanes; ++i) k.start(keys(buf) + i * kPlane, kb + i * p.k_plane + j0 * kt.l, kt.l, left, D, tid);
+#pragma unroll
+        for (int i = 0; i < M::kPlanes; ++i) v.start(values(buf) + i * kPlane, vb + i * p.k_plane + j0 * vt.l, vt.l, left, D, tid);
     }
     // a tile that has arrived and holds keys of no document
     __device__ __forceinline__ void clean(const Tile& tile, int buf) const {
         if (!kd || tile.documents.x >= 0) return;
         const int* of = (const int*)docs(buf);
-        S::clear(keys(buf), [&](int i) { return of[i] < 0; }, tid);
-        S::clear(values(buf), [&](int i) { return of[i] < 0; }, tid);
+#pragma unroll 1
+        for (int i = 0; i < 2 * M::kPlanes; ++i) S::clear(keys(buf) + i * kPlane, [&](int r) { return of[r] < 0; }, tid);
         __syncthreads();
     }
 };
+
+// What is taken in parts (more than a token's worth of rows of f32, at most 128 features), and its features there.
+inline bool in_parts(int type, int D, bool few_rows) { return type == ADHIP_F32 && D <= 128 && !few_rows; }
+inline int parts_size(int D) { return (D + 7) / 8 * 8; }
 
 // DP: the head's features, rounded up to what the kernels are built for
 inline int padded_size(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }

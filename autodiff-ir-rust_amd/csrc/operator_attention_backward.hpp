@@ -16,16 +16,17 @@ namespace attn {
 
 // ---- dq: the forward kernel's walk ------------------------------------------------------------------------------------
 
-template <class T, int DP, int BK_, int BUFS, int WAVES_>
+template <int BK_, int BUFS, int WAVES_>
 struct QueryConfig {
     static constexpr int BK = BK_, kBufs = BUFS, WAVES = WAVES_, NT = 256, BQ = 128, KB = BK / 32;
 };
 
-template <class T, int DP, bool VEC, class C>
+template <class X, int DP, bool VEC, class C>
 __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const Params p) {
-    typedef Matrix<T> M;
+    typedef Matrix<X> M;
+    typedef typename M::IO T;
     typedef typename M::Frag Frag;
-    typedef KeyTiles<T, DP, C, VEC> Keys;
+    typedef KeyTiles<X, DP, C, VEC> Keys;
     __shared__ __attribute__((aligned(1024))) char lds[Keys::kBytes];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -62,11 +63,11 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
         const T* o = (const T*)p.out.data + b * p.out.b + token * p.out.l + head * p.out.h;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
-            qf[s] = load_frag<VEC>(q, s * 16 + half * 8, p.D, valid);
-            df[s] = load_frag<VEC>(d, s * 16 + half * 8, p.D, valid);
-            const Frag of = load_frag<VEC>(o, s * 16 + half * 8, p.D, valid);
+            qf[s] = M::operand(load_frag<VEC>(q, s * 16 + half * 8, p.D, valid));
+            const typename M::Raw x = load_frag<VEC>(d, s * 16 + half * 8, p.D, valid), y = load_frag<VEC>(o, s * 16 + half * 8, p.D, valid);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) delta += (float)df[s][e] * (float)of[e];
+            for (int e = 0; e < 8; ++e) delta += (float)x[e] * (float)y[e];
+            df[s] = M::operand(x);
         }
     }
     delta = sum_of_halves(delta);
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
         theirs = document_range(kr, j0, j1);
         return documents_meet(mine, theirs);
     };
-    const unsigned r_lane = rows_lane<T, DP>(lane), c_lane = cols_lane<T, DP>(lane);
+    const unsigned r_lane = rows_lane<X, DP>(lane), c_lane = cols_lane<X, DP>(lane);
     typedef Tiles<decltype(needed)> Walk;
     Walk walk(needed, t_first, t_stop, split, p.dq_splits, lane);
     const Keys kt(p, b, c, n, tid, lds);
@@ -111,9 +112,9 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
 #pragma unroll
             for (int i = 0; i < 16; ++i) g[i] = -delta;
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) s = M::mma(rows_frag<T, DP>(kr_at, key0, k), qf[k], s);
+            for (int k = 0; k < DP / 16; ++k) s = M::mma(rows_frag<X, DP, C::BK>(kr_at, key0, k), qf[k], s);
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) g = M::mma(rows_frag<T, DP>(vr_at, key0, k), df[k], g);
+            for (int k = 0; k < DP / 16; ++k) g = M::mma(rows_frag<X, DP, C::BK>(vr_at, key0, k), df[k], g);
             const int j0 = t * C::BK + key0, jl = j0 + 4 * half;
             const bool all = sight.all(j0, j0 + 31, kt.kd, theirs);
             if (p.cap > 0.f) {
@@ -153,7 +154,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
                 Frag f;
                 to_frag(s, h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dq[d] = M::mma(cols_frag<T, DP>(kc_at, key0 + 16 * h, d * 32), f, dq[d]);
+                for (int d = 0; d < DP / 32; ++d) dq[d] = M::mma(cols_frag<X, DP, C::BK>(kc_at, key0 + 16 * h, d * 32), f, dq[d]);
             }
         }
     }
@@ -180,22 +181,26 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
 
 // KG wavefronts own 32 keys each, RG of them share the keys and take every RG-th 32 rows of a tile of BR.
 // K_LDS, V_LDS: the keys or values are read from LDS, where the two sums leave no registers for them.
-template <class T, int DP, int KG_, int RG_, int BUFS, bool K_LDS_, bool V_LDS_, int WAVES_>
+template <class X, int DP, int KG_, int RG_, int BUFS, bool K_LDS_, bool V_LDS_, int WAVES_>
 struct KeyConfig {
     static constexpr int KG = KG_, RG = RG_, BR = 32 * RG, kBufs = BUFS, NT = 64 * KG * RG, BKEYS = 32 * KG, WAVES = WAVES_;
     static constexpr bool K_LDS = K_LDS_, V_LDS = V_LDS_;
-    static constexpr int kTile = BR * Lds<T, DP>::kPitch, kOwn = BKEYS * Lds<T, DP>::kPitch;
+    static constexpr int kPlanes = Matrix<X>::kPlanes, kPitch = Lds<typename Matrix<X>::E, DP>::kPitch;
+    static constexpr int kTile = kPlanes * BR * kPitch, kOwn = BKEYS * kPitch;
+    static_assert(kPlanes == 1 || (!K_LDS && !V_LDS), "keys and values in parts stay in registers");
     static constexpr int kRows = kBufs * 2 * kTile + (K_LDS ? kOwn : 0) + (V_LDS ? kOwn : 0);
     static constexpr int kLoop = kRows + kBufs * BR * 3 * 4;  // of each row: log-sum, -delta, document
     static constexpr int kMerge = RG > 1 ? (RG - 1) * BKEYS * (DP + 4) * 4 : 0;
     static constexpr int kBytes = kLoop > kMerge ? kLoop : kMerge;
 };
 
-template <class T, int DP, bool VEC, class C>
+template <class X, int DP, bool VEC, class C>
 __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Params p) {
-    typedef Matrix<T> M;
+    typedef Matrix<X> M;
+    typedef typename M::IO T;
+    typedef typename M::E E;
     typedef typename M::Frag Frag;
-    typedef Lds<T, DP> L;
+    typedef Lds<E, DP> L;
     __shared__ __attribute__((aligned(1024))) char lds[C::kBytes];
     char* const k_own = lds + C::kBufs * 2 * C::kTile;
     char* const v_own = k_own + (C::K_LDS ? C::kOwn : 0);
@@ -224,18 +229,18 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
     {
         const T* k = (const T*)p.k.data + b * p.k.b + key * p.k.l + c * p.k.h;
         const T* v = (const T*)p.v.data + b * p.v.b + key * p.v.l + c * p.v.h;
-        constexpr int N = sizeof(Frag) / 16;
+        constexpr int N = sizeof(typename M::Raw) / 16;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
-            const Frag x = load_frag<VEC>(k, s * 16 + half * 8, p.D, valid), y = load_frag<VEC>(v, s * 16 + half * 8, p.D, valid);
+            const typename M::Raw x = load_frag<VEC>(k, s * 16 + half * 8, p.D, valid), y = load_frag<VEC>(v, s * 16 + half * 8, p.D, valid);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int at = L::at(kg * 32 + (lane & 31), (2 * s + half) * N + i);
                 if (C::K_LDS && rg == 0) *(uint4*)(k_own + at) = ((const uint4*)&x)[i];
                 if (C::V_LDS && rg == 0) *(uint4*)(v_own + at) = ((const uint4*)&y)[i];
             }
-            if (!C::K_LDS) kf[s] = x;
-            if (!C::V_LDS) vf[s] = y;
+            if (!C::K_LDS) kf[s] = M::operand(x);
+            if (!C::V_LDS) vf[s] = M::operand(y);
         }
     }
     f32x16 dk[DP / 32], dv[DP / 32];
@@ -256,12 +261,15 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         theirs = document_range(qr, i0, min(i0 + C::BR, p.Lq) - 1);
         return documents_meet(mine, theirs);
     };
-    const unsigned r_lane = rows_lane<T, DP>(lane), c_lane = cols_lane<T, DP>(lane);
+    const unsigned r_lane = rows_lane<X, DP>(lane), c_lane = cols_lane<X, DP>(lane);
     typedef Tiles<decltype(needed)> Walk;
     Walk walk(needed, 0, len * p.G, split, p.dk_splits, lane);
 
-    typedef Copy<T, DP, C::BR, C::NT, VEC> Rows;
-    const Rows copy_q(p.q.l, p.D, tid), copy_g(p.dout.l, p.D, tid);
+    constexpr bool kParts = M::kPlanes == 3;
+    typedef Copy<E, DP, C::BR, C::NT, VEC || kParts> Rows;
+    const Tensor &tq = kParts ? p.q3 : p.q, &tg = kParts ? p.dout3 : p.dout;
+    const int D = kParts ? p.D3 : p.D;
+    const Rows copy_q(tq.l, D, tid), copy_g(tg.l, D, tid);
     static_assert(C::NT >= C::BR, "one thread a row for what rows have beside features");
     auto start = [&](const Tile& tile, int buf) {
         const int g = tile.t / len, i0 = (t_first + tile.t - g * len) * C::BR, h = c * p.G + g, left = p.Lq - i0;
@@ -271,8 +279,12 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         copy_words<C::BR>(of, stats, 1, left, tid, wave);
         copy_words<C::BR>(of + C::BR * 4, stats + (int64_t)p.B * p.Hk * p.G * p.Lq, 1, left, tid, wave);
         if (p.qdoc) copy_words<C::BR>(of + 2 * C::BR * 4, p.qdoc + b * p.qdoc_b + i0 * p.qdoc_l, p.qdoc_l, left, tid, wave);
-        copy_q.start(to_q, (const T*)p.q.data + b * p.q.b + i0 * p.q.l + h * p.q.h, p.q.l, left, p.D, tid);
-        copy_g.start(to_q + C::kTile, (const T*)p.dout.data + b * p.dout.b + i0 * p.dout.l + h * p.dout.h, p.dout.l, left, p.D, tid);
+#pragma unroll
+        for (int i = 0; i < M::kPlanes; ++i)
+            copy_q.start(to_q + i * C::BR * L::kPitch, (const E*)tq.data + i * p.q_plane + b * tq.b + i0 * tq.l + h * tq.h, tq.l, left, D, tid);
+#pragma unroll
+        for (int i = 0; i < M::kPlanes; ++i)
+            copy_g.start(to_q + C::kTile + i * C::BR * L::kPitch, (const E*)tg.data + i * p.q_plane + b * tg.b + i0 * tg.l + h * tg.h, tg.l, left, D, tid);
     };
     // A row that sees nothing is zero, whatever the arrays hold there.  (Rows behind the last one came as zeros: their
     // probabilities, of whatever size, meet nothing but zeros.)
@@ -280,13 +292,14 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         const float* const of = (const float*)(lds + C::kRows + buf * 3 * C::BR * 4);
         if (!__any(of[lane % C::BR] == __builtin_inff())) return;
         char* const q = lds + buf * 2 * C::kTile;
-        Rows::clear(q, [&](int i) { return of[i] == __builtin_inff(); }, tid);
-        Rows::clear(q + C::kTile, [&](int i) { return of[i] == __builtin_inff(); }, tid);
+#pragma unroll 1
+        for (int i = 0; i < 2 * M::kPlanes; ++i)
+            Rows::clear(q + i * C::BR * L::kPitch, [&](int r) { return of[r] == __builtin_inff(); }, tid);
         __syncthreads();
     };
     static_assert(C::BR <= 64, "a wavefront looks over a tile's rows at once");
 
-    Ring<C::kBufs, 2 * Rows::kLoads, Walk, decltype(start)> ring(walk, start);
+    Ring<C::kBufs, 2 * M::kPlanes * Rows::kLoads, Walk, decltype(start)> ring(walk, start);
     for (; ring.ready(); ring.pop()) {
         const int buf = ring.buf, t = ring.queue[0].t;
         clean(buf);
@@ -304,7 +317,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
             f32x16 s = zero16();
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
-                s = M::mma(rows_frag<T, DP>(rows_at, 0, k), C::K_LDS ? rows_frag<T, DP>(own_at, 0, k) : kf[C::K_LDS ? 0 : k], s);
+                s = M::mma(rows_frag<X, DP, C::BR>(rows_at, 0, k), C::K_LDS ? rows_frag<X, DP, C::BKEYS>(own_at, 0, k) : kf[C::K_LDS ? 0 : k], s);
             f32x16 g;
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
@@ -314,7 +327,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
             }
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
-                g = M::mma(rows_frag<T, DP>(rows_at, C::BR, k), C::V_LDS ? rows_frag<T, DP>(own_at, C::K_LDS ? C::BKEYS : 0, k) : vf[C::V_LDS ? 0 : k], g);
+                g = M::mma(rows_frag<X, DP, C::BR>(rows_at, M::kPlanes * C::BR, k), C::V_LDS ? rows_frag<X, DP, C::BKEYS>(own_at, C::K_LDS ? C::BKEYS : 0, k) : vf[C::V_LDS ? 0 : k], g);
             if (p.cap > 0.f) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -364,7 +377,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
                 Frag f;
                 to_frag(s, h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dv[d] = M::mma(cols_frag<T, DP>(cols_at, C::BR + 16 * h, d * 32), f, dv[d]);
+                for (int d = 0; d < DP / 32; ++d) dv[d] = M::mma(cols_frag<X, DP, C::BR>(cols_at, M::kPlanes * C::BR + 16 * h, d * 32), f, dv[d]);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] *= g[i];
@@ -373,7 +386,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
                 Frag f;
                 to_frag(s, h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dk[d] = M::mma(cols_frag<T, DP>(cols_at, 16 * h, d * 32), f, dk[d]);
+                for (int d = 0; d < DP / 32; ++d) dk[d] = M::mma(cols_frag<X, DP, C::BR>(cols_at, 16 * h, d * 32), f, dk[d]);
             }
         }
     }
@@ -451,32 +464,34 @@ __global__ __launch_bounds__(256) void add_parts_kernel(const float* part, int s
     }
 }
 
-template <class T, int DP>
-struct BackwardConfig {
-    static constexpr int kRowBytes = DP * (int)sizeof(T);
-    // dq: rows and their gradients stay in registers; two workgroups a compute unit up to 128 features in bf16
-    typedef QueryConfig<T, DP, kRowBytes <= 256 ? 64 : 32, kRowBytes <= 128 ? 3 : kRowBytes <= 256 ? 2 : kRowBytes <= 512 ? 4 : kRowBytes <= 768 ? 2 : 1,
-                        kRowBytes <= 256 && sizeof(T) == 2 ? 2 : 1> Q;
+// Rows and their gradients stay in registers; two workgroups a compute unit up to 128 features in bf16.
+template <class X, int DP>
+struct QueryChoice {
+    static constexpr int kRow = DP * (int)sizeof(typename Matrix<X>::E);
+    typedef QueryConfig<kRow <= 256 ? 64 : 32, kRow <= 128 ? 3 : kRow <= 256 ? 2 : kRow <= 512 ? 4 : kRow <= 768 ? 2 : 1,
+                        kRow <= 256 && sizeof(typename Matrix<X>::E) == 2 ? 2 : 1> C;
 };
-// keys and values in registers where the sums leave room for them, sums of 256 features and more with one wavefront a SIMD
-template <class T, int DP>
-struct KeyChoice { typedef KeyConfig<T, DP, 4, 1, 2, false, false, 1> K; };
+template <int DP>
+struct QueryChoice<Parts, DP> { typedef QueryConfig<32, 3, DP <= 64 ? 2 : 1> C; };
+// Keys and values in registers where the sums leave room for them, one wavefront a SIMD where they do not leave room for two.
+template <class X, int DP>
+struct KeyChoice { typedef KeyConfig<X, DP, 4, 1, 2, false, false, 1> C; };
+template <int DP>
+struct KeyChoice<Parts, DP> { typedef KeyConfig<Parts, DP, 4, 1, 3, false, false, DP <= 32 ? 2 : 1> C; };
 template <>
-struct KeyChoice<bf16, 32> { typedef KeyConfig<bf16, 32, 4, 2, 2, false, false, 2> K; };
+struct KeyChoice<bf16, 32> { typedef KeyConfig<bf16, 32, 4, 2, 2, false, false, 2> C; };
 template <>
-struct KeyChoice<bf16, 64> { typedef KeyConfig<bf16, 64, 4, 2, 2, false, false, 2> K; };
+struct KeyChoice<bf16, 64> { typedef KeyConfig<bf16, 64, 4, 2, 2, false, false, 2> C; };
 template <>
-struct KeyChoice<bf16, 96> { typedef KeyConfig<bf16, 96, 4, 2, 2, false, true, 2> K; };
+struct KeyChoice<bf16, 96> { typedef KeyConfig<bf16, 96, 4, 2, 2, false, true, 2> C; };
 template <>
-struct KeyChoice<bf16, 128> { typedef KeyConfig<bf16, 128, 4, 2, 2, true, true, 2> K; };
+struct KeyChoice<bf16, 128> { typedef KeyConfig<bf16, 128, 4, 2, 2, true, true, 2> C; };
 template <>
-struct KeyChoice<bf16, 256> { typedef KeyConfig<bf16, 256, 4, 1, 2, false, true, 1> K; };
+struct KeyChoice<bf16, 256> { typedef KeyConfig<bf16, 256, 4, 1, 2, false, true, 1> C; };
 template <>
-struct KeyChoice<float, 128> { typedef KeyConfig<float, 128, 4, 1, 2, false, false, 1> K; };
+struct KeyChoice<float, 192> { typedef KeyConfig<float, 192, 2, 1, 1, false, true, 1> C; };
 template <>
-struct KeyChoice<float, 192> { typedef KeyConfig<float, 192, 2, 1, 1, false, true, 1> K; };
-template <>
-struct KeyChoice<float, 256> { typedef KeyConfig<float, 256, 2, 1, 1, false, true, 1> K; };
+struct KeyChoice<float, 256> { typedef KeyConfig<float, 256, 2, 1, 1, false, true, 1> C; };
 
 template <class T>
 void add_parts(const float* part, int splits, const Tensor& out, int B, int Hk, int L, int G, int D, hipStream_t stream) {
@@ -486,38 +501,27 @@ void add_parts(const float* part, int splits, const Tensor& out, int B, int Hk, 
     check_launch("adhip_attention_backward");
 }
 
-template <class T, int DP>
+template <class X, int DP>
 void launch_backward(const Params& p, hipStream_t stream) {
-    typedef typename BackwardConfig<T, DP>::Q Q;
-    typedef typename KeyChoice<T, DP>::K K;
+    typedef typename Matrix<X>::IO T;
+    typedef typename QueryChoice<X, DP>::C Q;
+    typedef typename KeyChoice<X, DP>::C K;
     Params x = p;
     const bool vec = p.q.vec && p.k.vec && p.v.vec && p.out.vec && p.dout.vec;
     x.tiles = (p.R + Q::BQ - 1) / Q::BQ;
     unsigned grid = (unsigned)((int64_t)x.tiles * p.dq_splits * p.Hk * p.B);
-    if (grid > 0 && vec) query_gradient_kernel<T, DP, true, Q><<<grid, Q::NT, 0, stream>>>(x);
-    else if (grid > 0) query_gradient_kernel<T, DP, false, Q><<<grid, Q::NT, 0, stream>>>(x);
+    if (grid > 0 && vec) query_gradient_kernel<X, DP, true, Q><<<grid, Q::NT, 0, stream>>>(x);
+    else if (grid > 0) query_gradient_kernel<X, DP, false, Q><<<grid, Q::NT, 0, stream>>>(x);
     check_launch("adhip_attention_backward");
     if (p.dq_splits > 1) add_parts<T>(p.part_dq, p.dq_splits, p.dq, p.B, p.Hk, p.Lq, p.G, p.D, stream);
     x.tiles = (p.Lk + K::BKEYS - 1) / K::BKEYS;
     grid = (unsigned)((int64_t)x.tiles * p.dk_splits * p.Hk * p.B);
-    if (grid > 0 && vec) key_gradient_kernel<T, DP, true, K><<<grid, K::NT, 0, stream>>>(x);
-    else if (grid > 0) key_gradient_kernel<T, DP, false, K><<<grid, K::NT, 0, stream>>>(x);
+    if (grid > 0 && vec) key_gradient_kernel<X, DP, true, K><<<grid, K::NT, 0, stream>>>(x);
+    else if (grid > 0) key_gradient_kernel<X, DP, false, K><<<grid, K::NT, 0, stream>>>(x);
     check_launch("adhip_attention_backward");
     if (p.dk_splits > 1) {
         add_parts<T>(p.part_dk, p.dk_splits, p.dk, p.B, p.Hk, p.Lk, 1, p.D, stream);
         add_parts<T>(p.part_dv, p.dk_splits, p.dv, p.B, p.Hk, p.Lk, 1, p.D, stream);
-    }
-}
-
-template <class T>
-void backward(const Params& p, hipStream_t stream) {
-    switch (padded_size(p.D)) {
-        case 32: return launch_backward<T, 32>(p, stream);
-        case 64: return launch_backward<T, 64>(p, stream);
-        case 96: return launch_backward<T, 96>(p, stream);
-        case 128: return launch_backward<T, 128>(p, stream);
-        case 192: return launch_backward<T, 192>(p, stream);
-        case 256: return launch_backward<T, 256>(p, stream);
     }
 }
 

@@ -16,18 +16,19 @@ namespace attn {
 
 // BUFS: tiles of keys in LDS; with two, one is under way while the other is worked on.
 // WAVES: wavefronts of a SIMD that registers must leave room for.
-template <class T, int DP, int WQ_, int WK_, int BK_, int BUFS, int WAVES_>
+template <int DP, int WQ_, int WK_, int BK_, int BUFS, int WAVES_>
 struct ForwardConfig {
     static constexpr int WQ = WQ_, WK = WK_, BK = BK_, kBufs = BUFS, WAVES = WAVES_;
     static constexpr int NT = 64 * WQ * WK, BQ = 32 * WQ, KB = BK / (32 * WK);
     static constexpr int kMerge = WK > 1 ? WK * 32 * (DP + 4) * 4 + WK * 64 * 4 : 0;
 };
 
-template <class T, int DP, bool VEC, class C>
+template <class X, int DP, bool VEC, class C>
 __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p) {
-    typedef Matrix<T> M;
+    typedef Matrix<X> M;
+    typedef typename M::IO T;
     typedef typename M::Frag Frag;
-    typedef KeyTiles<T, DP, C, VEC> Keys;
+    typedef KeyTiles<X, DP, C, VEC> Keys;
     __shared__ __attribute__((aligned(1024))) char lds[Keys::kBytes > C::kMerge ? Keys::kBytes : C::kMerge];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wq = wave % C::WQ, wk = wave / C::WQ;
@@ -61,10 +62,11 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         const T* q = (const T*)p.q.data + b * p.q.b + token * p.q.l + head * p.q.h;
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
-            qf[s] = load_frag<VEC>(q, s * 16 + half * 8, p.D, valid && p.scale != 0.f);
+            typename M::Raw x = load_frag<VEC>(q, s * 16 + half * 8, p.D, valid && p.scale != 0.f);
             if (sign < 0.f)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) qf[s][e] = -qf[s][e];
+                for (int e = 0; e < 8; ++e) x[e] = -x[e];
+            qf[s] = M::operand(x);
         }
     }
     f32x16 o[DP / 32];
@@ -86,8 +88,8 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         return documents_meet(mine, theirs);
     };
     // the lane's place in the wavefront's keys of a tile
-    const unsigned k_lane = rows_lane<T, DP>(lane) + wk * C::KB * 32 * Lds<T, DP>::kPitch;
-    const unsigned v_lane = cols_lane<T, DP>(lane) + wk * C::KB * 32 * Lds<T, DP>::kPitch;
+    const unsigned k_lane = rows_lane<X, DP>(lane) + wk * C::KB * 32 * Lds<typename M::E, DP>::kPitch;
+    const unsigned v_lane = cols_lane<X, DP>(lane) + wk * C::KB * 32 * Lds<typename M::E, DP>::kPitch;
     typedef Tiles<decltype(needed)> Walk;
     Walk walk(needed, t_first, t_stop, split, p.splits, lane);
     const Keys kt(p, b, c, n, tid, lds);
@@ -104,7 +106,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
         for (int x = 0; x < C::KB; ++x) {
             s[x] = zero16();
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) s[x] = M::mma(rows_frag<T, DP>(ks, x * 32, k), qf[k], s[x]);
+            for (int k = 0; k < DP / 16; ++k) s[x] = M::mma(rows_frag<X, DP, C::BK>(ks, x * 32, k), qf[k], s[x]);
         }
         const int j0 = t * C::BK + wk * C::KB * 32, jl = j0 + 4 * half;  // register i of s[x] has key jl + 32 x + c_row(i)
         if (p.cap > 0.f) {
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
                 Frag f;
                 to_frag(s[x], h, f);
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) o[d] = M::mma(cols_frag<T, DP>(vs, x * 32 + 16 * h, d * 32), f, o[d]);
+                for (int d = 0; d < DP / 32; ++d) o[d] = M::mma(cols_frag<X, DP, C::BK>(vs, x * 32 + 16 * h, d * 32), f, o[d]);
             }
         }
     }
@@ -299,45 +301,42 @@ __global__ __launch_bounds__(256) void join_kernel(const Params p) {
     if (lane == 0) p.lse[b * p.lse_b + token * p.lse_l + head * p.lse_h] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-template <class T, int DP>
+// Bytes of a row of a tile decide how many keys a tile has and how many tiles LDS holds: 64 keys where tiles leave room for
+// the workgroups that registers allow, 32 else, and as many tiles as then fit.
+template <class X, int DP>
 struct ForwardMany {
-    // 64 keys a tile; 32 where tiles of 64 would not leave room for a second workgroup or not fit; as many tiles as LDS has room
-    // for beside the workgroups that registers allow
-    static constexpr int kRowBytes = DP * (int)sizeof(T);
-    typedef ForwardConfig<T, DP, 4, 1, kRowBytes <= 256 ? 64 : 32, kRowBytes <= 128 ? 3 : kRowBytes <= 256 ? 2 : kRowBytes <= 512 ? 4 : 2,
-                          kRowBytes <= 128 ? 3 : kRowBytes <= 256 ? 2 : 1> C;
+    static constexpr int kRow = DP * (int)sizeof(typename Matrix<X>::E);
+    typedef ForwardConfig<DP, 4, 1, kRow <= 256 ? 64 : 32, kRow <= 128 ? 3 : kRow <= 256 ? 2 : kRow <= 512 ? 4 : 2, kRow <= 128 ? 3 : kRow <= 256 ? 2 : 1> C;
 };
-template <class T, int DP>
+template <int DP>
+struct ForwardMany<Parts, DP> {
+    typedef ForwardConfig<DP, 4, 1, 32, 3, DP <= 64 ? 2 : 1> C;
+};
+template <class X, int DP>
 struct ForwardFew {
-    static constexpr int kRowBytes = DP * (int)sizeof(T);
+    static constexpr int kRow = DP * (int)sizeof(typename Matrix<X>::E);
     // as many wavefronts along the keys as LDS holds tiles for twice
-    static constexpr int WK = kRowBytes <= 256 ? 4 : kRowBytes <= 512 ? 2 : 1;
-    typedef ForwardConfig<T, DP, 1, WK, 32 * WK, 2, 1> C;
+    static constexpr int WK = kRow <= 256 ? 4 : kRow <= 512 ? 2 : 1;
+    typedef ForwardConfig<DP, 1, WK, 32 * WK, 2, 1> C;
 };
 
-template <class T, int DP, class C>
+template <class X, int DP, class C>
 void launch_forward(const Params& p, hipStream_t stream) {
     const unsigned grid = (unsigned)((int64_t)p.tiles * p.splits * p.Hk * p.B);
-    if (p.q.vec && p.k.vec && p.v.vec) forward_kernel<T, DP, true, C><<<grid, C::NT, 0, stream>>>(p);
-    else forward_kernel<T, DP, false, C><<<grid, C::NT, 0, stream>>>(p);
+    if (p.q.vec && p.k.vec && p.v.vec) forward_kernel<X, DP, true, C><<<grid, C::NT, 0, stream>>>(p);
+    else forward_kernel<X, DP, false, C><<<grid, C::NT, 0, stream>>>(p);
     check_launch("adhip_attention");
     if (p.splits > 1) {
-        join_kernel<T><<<(unsigned)(((int64_t)p.B * p.Hk * p.R + 3) / 4), 256, 0, stream>>>(p);
+        join_kernel<typename Matrix<X>::IO><<<(unsigned)(((int64_t)p.B * p.Hk * p.R + 3) / 4), 256, 0, stream>>>(p);
         check_launch("adhip_attention");
     }
 }
 
-template <class T>
-void forward(const Params& p, bool few_rows, hipStream_t stream) {
-    switch (padded_size(p.D)) {
-#define ADHIP_CASE(DP)                                                                                   \
-    case DP:                                                                                             \
-        if (few_rows) launch_forward<T, DP, typename ForwardFew<T, DP>::C>(p, stream);                   \
-        else launch_forward<T, DP, typename ForwardMany<T, DP>::C>(p, stream);                           \
-        break;
-        ADHIP_CASE(32) ADHIP_CASE(64) ADHIP_CASE(96) ADHIP_CASE(128) ADHIP_CASE(192) ADHIP_CASE(256)
-#undef ADHIP_CASE
-    }
+// Many: what multiplies where rows fill workgroups; Few: where they do not
+template <class Many, class Few, int DP>
+void launch_forward(const Params& p, bool few_rows, hipStream_t stream) {
+    if (few_rows) launch_forward<Few, DP, typename ForwardFew<Few, DP>::C>(p, stream);
+    else launch_forward<Many, DP, typename ForwardMany<Many, DP>::C>(p, stream);
 }
 
 }  // namespace attn
