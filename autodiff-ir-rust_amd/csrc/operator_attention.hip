@@ -87,7 +87,7 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
     const int64_t R = Hk > 0 ? Lq * (H / Hk) : 0;
     // One wavefront's 32 columns hold all rows of a key head: the wavefronts of a workgroup go along the keys.
     y.few_rows = R <= 32;
-    y.row_tile = y.few_rows ? 32 : 128;
+    y.row_tile = attn::forward_rows(g.q.type, attn::padded_size((int)D), y.few_rows);
     y.tiles = (int)((R + y.row_tile - 1) / y.row_tile);
     // Ranges of keys: as many as give every compute unit two workgroups, none shorter than two tiles of keys.
     const int64_t blocks = (int64_t)y.tiles * Hk * B, keys = y.few_rows ? 128 : 64;
@@ -125,11 +125,13 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
     if (backward) {
         y.stats = back;
         back += rounded((size_t)(B * Hk * R) * 2 * 4);
-        // Parts of the backward walks: as many as give every compute unit four workgroups, which evens out a causal mask's
-        // uneven ones, none shorter than four tiles.
+        // Parts of the backward walks: as many as give every compute unit two workgroups, which evens out a causal mask's
+        // uneven ones, none shorter than four tiles.  More parts cost more memory to add up than they even out: 2048 x 8 heads of
+        // 128 in f32 448 us with two a compute unit, 498 with one, 518 with four.
+        constexpr int64_t kTarget = 512;
         auto parts = [](int64_t blocks, int64_t tiles) {
-            if (blocks <= 0 || blocks >= 1024) return 1;
-            return (int)std::max<int64_t>(1, std::min<int64_t>((1024 + blocks - 1) / blocks, tiles / 4));
+            if (blocks <= 0 || blocks >= kTarget) return 1;
+            return (int)std::max<int64_t>(1, std::min<int64_t>((kTarget + blocks - 1) / blocks, tiles / 4));
         };
         const int64_t rows = (R + 127) / 128 * Hk * B, keys = (Lk + 127) / 128 * Hk * B;
         y.dq_splits = parts(rows, (Lk + 63) / 64);

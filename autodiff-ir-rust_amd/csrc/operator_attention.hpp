@@ -594,6 +594,8 @@ struct KeyTiles {
 
 // What is taken in parts (more than a token's worth of rows of f32, at most 128 features), and its features there.
 inline bool in_parts(int type, int D, bool few_rows) { return type == ADHIP_F32 && D <= 128 && !few_rows; }
+// Rows of a workgroup of the forward kernels
+constexpr int forward_rows(int type, int D, bool few_rows) { return few_rows ? 32 : type == ADHIP_F32 && D > 64 && D <= 128 ? 256 : 128; }
 inline int parts_size(int D) { return (D + 7) / 8 * 8; }
 
 // DP: the head's features, rounded up to what the kernels are built for

@@ -306,11 +306,14 @@ __global__ __launch_bounds__(256) void join_kernel(const Params p) {
 template <class X, int DP>
 struct ForwardMany {
     static constexpr int kRow = DP * (int)sizeof(typename Matrix<X>::E);
-    typedef ForwardConfig<DP, 4, 1, kRow <= 256 ? 64 : 32, kRow <= 128 ? 3 : kRow <= 256 ? 2 : kRow <= 512 ? 4 : 2, kRow <= 128 ? 3 : kRow <= 256 ? 2 : 1> C;
+    typedef ForwardConfig<DP, 4, 1, kRow <= 256 ? 64 : 32, kRow <= 128 ? 3 : kRow <= 384 ? 2 : kRow <= 512 ? 4 : 2,
+                          kRow <= 128 ? 3 : kRow <= 384 ? 2 : 1> C;
 };
+// In parts: two workgroups of four wavefronts up to 64 features, one of eight above, so that a SIMD always has two and one's
+// matrix instructions run beside the other's splitting and exponentials.
 template <int DP>
 struct ForwardMany<Parts, DP> {
-    typedef ForwardConfig<DP, 4, 1, 32, 3, DP <= 64 ? 2 : 1> C;
+    typedef ForwardConfig<DP, forward_rows(ADHIP_F32, DP, false) / 32, 1, 32, 3, 2> C;
 };
 template <class X, int DP>
 struct ForwardFew {
