@@ -2,9 +2,11 @@
 // the pair give.  Cosines and sines come from tables, so a scaled table serves longer contexts and the angles have the
 // precision that the table was made with.
 //
-// One read and one write of the heads' features bounds it; the arithmetic is nothing.  A lane owns V pairs of a token and
-// turns them in up to U heads: their cosines and sines are loaded once, and 2 U loads are under way before the first is
-// used.  V is as large as 16 bytes, the number of pairs and the arrays' alignment allow.
+// One read and one write of the heads' features bounds it; the arithmetic is nothing.  A lane turns V pairs of one head (or
+// copies V features); V is as large as 16 bytes, the number of pairs and the arrays' alignment allow.  Four heads a lane,
+// with the cosines and sines loaded once for all, were no faster on long sequences (16384 tokens of 32 + 8 heads of 128 in
+// bf16: 61 us, 5.5 TB/s, either way) and slower on short ones, where lanes in number hide the way to memory: 3003 tokens of
+// 8 + 8 heads of 80, half of them turned, in f32, 20 us with four heads and 8 with one.
 #include "operators.hpp"
 
 namespace adhip {
@@ -14,7 +16,7 @@ struct RotaryArray {
     const void* x;
     void* out;
     int64_t xb, xl, xh, ob, ol, oh;  // strides of batch, length and heads
-    int heads, groups;               // groups of U heads
+    int heads;
 };
 
 struct RotaryParams {
@@ -25,13 +27,13 @@ struct RotaryParams {
     int64_t rows;     // of the tables
     unsigned tokens, length;
     int size, pairs;
-    unsigned chunks, turned;  // chunks of V pairs or V copied features of a head; the first `turned` are pairs
-    unsigned items;           // lanes that a token takes: chunks * groups of both arrays
+    unsigned turned, copied;  // chunks of V pairs and of V copied features of a head
+    unsigned turns, items;    // lanes that a token takes: `turns` for its pairs, the others for copies
     unsigned per_block;       // tokens of a block (1 where a token takes several)
     float sign;
 };
 
-template <class T, int V, int U, bool INTERLEAVED>
+template <class T, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
     unsigned item = blockIdx.y * 256 + threadIdx.x, token = blockIdx.x;
     if (p.per_block > 1) {
@@ -41,35 +43,29 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
         token = token * p.per_block + t;
     }
     if (item >= p.items || token >= p.tokens) return;
-    const unsigned group = item / p.chunks, chunk = item - group * p.chunks;
-    const bool second = group >= (unsigned)p.a[0].groups;
-    const RotaryArray& a = second ? p.a[1] : p.a[0];
-    const int h0 = (int)(second ? group - p.a[0].groups : group) * U;
+    // (pairs first, of all heads: a wavefront has one of the two to do)
+    const bool copies = item >= p.turns;
+    const unsigned of = copies ? p.copied : p.turned, at_item = copies ? item - p.turns : item;
+    const unsigned number = at_item / of, chunk = at_item - number * of;
+    const bool second = number >= (unsigned)p.a[0].heads;
+    // field by field: an index by lane would send every lane to the kernel's arguments in memory
+    const RotaryArray &one = p.a[0], &two = p.a[1];
+    const RotaryArray a = {second ? two.x : one.x,   second ? two.out : one.out, second ? two.xb : one.xb, second ? two.xl : one.xl,
+                           second ? two.xh : one.xh, second ? two.ob : one.ob,   second ? two.ol : one.ol, second ? two.oh : one.oh,
+                           0};
+    const int64_t h = second ? number - one.heads : number;
     const unsigned b = token / p.length, l = token - b * p.length;
-    const T* x = (const T*)a.x + b * a.xb + l * a.xl + h0 * a.xh;
-    T* o = (T*)a.out + b * a.ob + l * a.ol + h0 * a.oh;
-    const int n = min(U, a.heads - h0);
+    const T* x = (const T*)a.x + b * a.xb + l * a.xl + h * a.xh;
+    T* o = (T*)a.out + b * a.ob + l * a.ol + h * a.oh;
     typedef Pack<T, V> P;
-    if (chunk >= p.turned) {
-        const int at = 2 * p.pairs + (int)(chunk - p.turned) * V;
-        P r[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (u < n) r[u] = *(const P*)(x + u * a.xh + at);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (u < n) *(P*)(o + u * a.oh + at) = r[u];
+    if (copies) {
+        const int at = 2 * p.pairs + (int)chunk * V;
+        *(P*)(o + at) = *(const P*)(x + at);
         return;
     }
     const int pair = (int)chunk * V;
     const int i0 = INTERLEAVED ? 2 * pair : pair, i1 = INTERLEAVED ? 2 * pair + V : pair + p.pairs;
-    P r0[U], r1[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (u < n) {
-            r0[u] = *(const P*)(x + u * a.xh + i0);
-            r1[u] = *(const P*)(x + u * a.xh + i1);
-        }
+    P r0 = *(const P*)(x + i0), r1 = *(const P*)(x + i1);
     const int64_t row = p.positions[b * p.pb + l * p.pl];
     constexpr int W = V < 4 ? V : 4;
     float c[V], s[V];
@@ -85,44 +81,34 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) s[i] *= p.sign;
+    if (INTERLEAVED) {
+        T f[2 * V];
+        *(P*)f = r0;
+        *(P*)(f + V) = r1;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (u >= n) break;
-        if (INTERLEAVED) {
-            T f[2 * V];
-            *(P*)f = r0[u];
-            *(P*)(f + V) = r1[u];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float x0 = (float)f[2 * i], x1 = (float)f[2 * i + 1];
-                f[2 * i] = (T)(x0 * c[i] - x1 * s[i]);
-                f[2 * i + 1] = (T)(x0 * s[i] + x1 * c[i]);
-            }
-            r0[u] = *(P*)f;
-            r1[u] = *(P*)(f + V);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float x0 = (float)r0[u].v[i], x1 = (float)r1[u].v[i];
-                r0[u].v[i] = (T)(x0 * c[i] - x1 * s[i]);
-                r1[u].v[i] = (T)(x0 * s[i] + x1 * c[i]);
-            }
+        for (int i = 0; i < V; ++i) {
+            const float x0 = (float)f[2 * i], x1 = (float)f[2 * i + 1];
+            f[2 * i] = (T)(x0 * c[i] - x1 * s[i]);
+            f[2 * i + 1] = (T)(x0 * s[i] + x1 * c[i]);
         }
-        *(P*)(o + u * a.oh + i0) = r0[u];
-        *(P*)(o + u * a.oh + i1) = r1[u];
+        r0 = *(P*)f;
+        r1 = *(P*)(f + V);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float x0 = (float)r0.v[i], x1 = (float)r1.v[i];
+            r0.v[i] = (T)(x0 * c[i] - x1 * s[i]);
+            r1.v[i] = (T)(x0 * s[i] + x1 * c[i]);
+        }
     }
-}
-
-template <class T, int V, int U>
-void launch_rotary(const RotaryParams& p, bool interleaved, dim3 grid, hipStream_t stream) {
-    if (interleaved) rotary_kernel<T, V, U, true><<<grid, 256, 0, stream>>>(p);
-    else rotary_kernel<T, V, U, false><<<grid, 256, 0, stream>>>(p);
+    *(P*)(o + i0) = r0;
+    *(P*)(o + i1) = r1;
 }
 
 template <class T, int V>
-void launch_rotary(const RotaryParams& p, int u, bool interleaved, dim3 grid, hipStream_t stream) {
-    if (u == 4) launch_rotary<T, V, 4>(p, interleaved, grid, stream);
-    else launch_rotary<T, V, 1>(p, interleaved, grid, stream);
+void launch_rotary(const RotaryParams& p, bool interleaved, dim3 grid, hipStream_t stream) {
+    if (interleaved) rotary_kernel<T, V, true><<<grid, 256, 0, stream>>>(p);
+    else rotary_kernel<T, V, false><<<grid, 256, 0, stream>>>(p);
 }
 
 void rotary(const adhip_rotary_args& g, hipStream_t stream) {
@@ -172,10 +158,7 @@ void rotary(const adhip_rotary_args& g, hipStream_t stream) {
     const adhip_array* in[2] = {&g.x, &g.second};
     const adhip_array* to[2] = {&g.out, &g.second_out};
     p.turned = (unsigned)(pairs / v);
-    p.chunks = p.turned + (unsigned)((size - 2 * pairs) / v);
-    // Four heads a lane once that still leaves every compute unit eight wavefronts of lanes; below, one head a lane is
-    // the shorter way (a token of 8 + 8 heads: one wavefront's trip to memory instead of four in a row).
-    const int u = tokens * heads * p.chunks >= int64_t(4) * 256 * 8 * 64 ? 4 : 1;
+    p.copied = (unsigned)((size - 2 * pairs) / v);
     for (int i = 0; i < (two ? 2 : 1); ++i) {
         RotaryArray& a = p.a[i];
         a.x = in[i]->data;
@@ -183,7 +166,6 @@ void rotary(const adhip_rotary_args& g, hipStream_t stream) {
         a.xb = in[i]->strides[0], a.xl = in[i]->strides[1], a.xh = in[i]->strides[2];
         a.ob = to[i]->strides[0], a.ol = to[i]->strides[1], a.oh = to[i]->strides[2];
         a.heads = (int)in[i]->dims[2];
-        a.groups = (a.heads + u - 1) / u;
     }
     p.cos = (const float*)g.cos.data;
     p.sin = (const float*)g.sin.data;
@@ -194,21 +176,22 @@ void rotary(const adhip_rotary_args& g, hipStream_t stream) {
     p.length = (unsigned)length;
     p.size = (int)size;
     p.pairs = (int)pairs;
-    p.items = p.chunks * (unsigned)(p.a[0].groups + p.a[1].groups);
+    p.turns = p.turned * (unsigned)(p.a[0].heads + p.a[1].heads);
+    p.items = p.turns + p.copied * (unsigned)(p.a[0].heads + p.a[1].heads);
     p.per_block = p.items < 256 ? 256 / p.items : 1;
     p.sign = g.inverse ? -1.f : 1.f;
     const dim3 grid((unsigned)((tokens + p.per_block - 1) / p.per_block), (p.items + 255) / 256);
     ADHIP_CHECK(grid.y < 65536, "%s: heads of %lld x %lld features are too many for one call", op, (long long)heads, (long long)size);
     const bool il = g.interleaved != 0;
     if (type == ADHIP_BF16) {
-        if (v == 8) launch_rotary<bf16, 8>(p, u, il, grid, stream);
-        else if (v == 4) launch_rotary<bf16, 4>(p, u, il, grid, stream);
-        else if (v == 2) launch_rotary<bf16, 2>(p, u, il, grid, stream);
-        else launch_rotary<bf16, 1>(p, u, il, grid, stream);
+        if (v == 8) launch_rotary<bf16, 8>(p, il, grid, stream);
+        else if (v == 4) launch_rotary<bf16, 4>(p, il, grid, stream);
+        else if (v == 2) launch_rotary<bf16, 2>(p, il, grid, stream);
+        else launch_rotary<bf16, 1>(p, il, grid, stream);
     } else {
-        if (v == 4) launch_rotary<float, 4>(p, u, il, grid, stream);
-        else if (v == 2) launch_rotary<float, 2>(p, u, il, grid, stream);
-        else launch_rotary<float, 1>(p, u, il, grid, stream);
+        if (v == 4) launch_rotary<float, 4>(p, il, grid, stream);
+        else if (v == 2) launch_rotary<float, 2>(p, il, grid, stream);
+        else launch_rotary<float, 1>(p, il, grid, stream);
     }
     check_launch(op);
 }
