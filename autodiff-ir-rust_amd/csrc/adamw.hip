@@ -72,24 +72,50 @@ __device__ __forceinline__ unsigned encode4(const float (&f)[4]) {
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], c, true);
 }
 
+// The largest of a wavefront's values, in all lanes: within 16 lanes by rotations, then by exchanges of rows.
+template <int CTRL>
+__device__ __forceinline__ unsigned max_with(unsigned x) {
+    return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+    x = max_with<0xb1>(x);   // the other of a pair
+    x = max_with<0x4e>(x);   // the other pair of four
+    x = max_with<0x124>(x);  // four and eight lanes round
+    x = max_with<0x128>(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(r[0], r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max(h[0], h[1]);
+}
+
 // The scale of a block from its values: their largest magnitude, by the bits, so that a NaN is the largest of all.
 __device__ __forceinline__ float block_scale(const float (&f)[4]) {
     unsigned most = __float_as_uint(0x1p-100f);
 #pragma unroll
     for (int k = 0; k < 4; ++k) most = max(most, __float_as_uint(f[k]) & 0x7fffffffu);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) most = max(most, (unsigned)__shfl_xor((int)most, d));
-    return __uint_as_float(most) * (1.f / 448.f);
+    return __uint_as_float(wave_max(most)) * (1.f / 448.f);
 }
 
-template <class PT, class GT, bool EIGHT>
-__global__ __launch_bounds__(256) void adamw_kernel(const AdamwLaunch a) {
-    int i = 0;
-    while (i + 1 < a.n && blockIdx.x >= a.first[i + 1]) ++i;
-    const adhip_adamw_tensor t = a.t[i];
-    const bool aligned = a.aligned >> i & 1;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t unit0 = (int64_t)(blockIdx.x - a.first[i]) * (kChunk / kBlock) + wave * kUnits;
+// x / scale for the four values of a lane, rounded correctly: from the scale's reciprocal, with one correction by the exact
+// remainder (Markstein 1990); a scale that is not finite takes the divisions.
+__device__ __forceinline__ void over_scale(const float (&x)[4], float scale, float (&q)[4]) {
+    if (scale < __builtin_inff()) {
+        const float r = 1.f / scale;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float y = x[k] * r;
+            q[k] = __builtin_fmaf(__builtin_fmaf(-y, scale, x[k]), r, y);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = x[k] / scale;
+    }
+}
+
+// A wavefront's blocks of a tensor.  WHOLE: all of them are there and can be read four elements at once; then no load waits
+// for a choice, and all are under way together.
+template <class PT, class GT, bool EIGHT, bool WHOLE>
+__device__ __forceinline__ void adamw_blocks(const AdamwLaunch& a, const adhip_adamw_tensor& t, bool aligned, int64_t unit0, int lane) {
     const int64_t n = t.count;
     float p[kUnits][4], g[kUnits][4], m[kUnits][4], v[kUnits][4];
     unsigned mc[kUnits], vc[kUnits];
@@ -97,8 +123,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwLaunch a) {
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
         const int64_t at = (unit0 + u) * kBlock + lane * 4;
-        if ((unit0 + u) * kBlock >= n) continue;
-        const bool whole = aligned && at + 4 <= n;
+        if (!WHOLE && (unit0 + u) * kBlock >= n) break;
+        const bool whole = WHOLE || (aligned && at + 4 <= n);
         load4((const PT*)t.p, at, n, whole, p[u]);
         load4((const GT*)t.g, at, n, whole, g[u]);
         if (EIGHT) {
@@ -114,8 +140,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwLaunch a) {
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
         const int64_t at = (unit0 + u) * kBlock + lane * 4;
-        if ((unit0 + u) * kBlock >= n) return;
-        const bool whole = aligned && at + 4 <= n;
+        if (!WHOLE && (unit0 + u) * kBlock >= n) return;
+        const bool whole = WHOLE || (aligned && at + 4 <= n);
         float root[4];
         if (EIGHT) {
             decode4(mc[u], m[u]);
@@ -143,14 +169,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwLaunch a) {
                 if (at + k >= n) m[u][k] = root[k] = 0.f;
             const float m_scale = block_scale(m[u]), v_scale = block_scale(root);
             float c[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) c[k] = m[u][k] / m_scale;
+            over_scale(m[u], m_scale, c);
             ((unsigned*)t.m_out)[(unit0 + u) * 64 + lane] = encode4(c);
+            over_scale(root, v_scale, c);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float r = root[k] / v_scale;
-                c[k] = root[k] > 0.f ? (r < 0x1p-9f ? 0x1p-9f : r) : root[k];
-            }
+            for (int k = 0; k < 4; ++k) c[k] = root[k] > 0.f ? (c[k] < 0x1p-9f ? 0x1p-9f : c[k]) : root[k];
             ((unsigned*)t.v_out)[(unit0 + u) * 64 + lane] = encode4(c);
             if (lane == 0) {
                 t.m_scale_out[unit0 + u] = m_scale;
@@ -161,6 +184,18 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwLaunch a) {
             store4((float*)t.v_out, at, n, whole, v[u]);
         }
     }
+}
+
+template <class PT, class GT, bool EIGHT>
+__global__ __launch_bounds__(256) void adamw_kernel(const AdamwLaunch a) {
+    int i = 0;
+    while (i + 1 < a.n && blockIdx.x >= a.first[i + 1]) ++i;
+    const adhip_adamw_tensor t = a.t[i];
+    const bool aligned = a.aligned >> i & 1;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t unit0 = (int64_t)(blockIdx.x - a.first[i]) * (kChunk / kBlock) + wave * kUnits;
+    if (aligned && (unit0 + kUnits) * kBlock <= t.count) adamw_blocks<PT, GT, EIGHT, true>(a, t, aligned, unit0, lane);
+    else adamw_blocks<PT, GT, EIGHT, false>(a, t, aligned, unit0, lane);
 }
 
 template <bool EIGHT>
