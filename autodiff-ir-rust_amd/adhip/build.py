@@ -12,6 +12,11 @@ import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
+# Matrix instructions add up in the registers that vector instructions reach too: by default a kernel that has all of a SIMD's
+# registers carries its sums to the other half and back in every step.
+KERNEL_FLAGS = ["-O3", "-mllvm", "-amdgpu-mfma-vgpr-form"]
+# Sums that fill one half are better off in the other.
+WIDE_SUMS = {"operator_attention_backward_f32_wide.hip"}
 CSRC = os.path.join(os.path.dirname(_PKG_DIR), "csrc")
 
 
@@ -25,7 +30,7 @@ def build_library(verbose: bool = False) -> str:
         # kernels first: their files take longest
         for src in sorted(glob.glob(os.path.join(CSRC, "*.hip"))) + sorted(glob.glob(os.path.join(CSRC, "*.cpp"))):
             objects.append(os.path.join(work, os.path.basename(src) + ".o"))
-            steps.append([hipcc, *flags, "-O3" if src.endswith(".hip") else "-O2", "-c", src, "-o", objects[-1]])
+            steps.append([hipcc, *flags, *(["-O2"] if src.endswith(".cpp") else ["-O3"] if os.path.basename(src) in WIDE_SUMS else KERNEL_FLAGS), "-c", src, "-o", objects[-1]])
         steps_at_once = int(os.environ.get("MAX_JOBS", min(16, os.cpu_count() or 1)))
         with ThreadPoolExecutor(max(1, steps_at_once)) as pool:
             def compile_one(cmd):

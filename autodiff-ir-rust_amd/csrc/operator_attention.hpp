@@ -77,6 +77,7 @@ struct Matrix<bf16> {
     typedef bf16x8 Raw;
     typedef bf16x8 Frag;
     static constexpr int kChunk = 8, kPlanes = 1;  // elements of 16 bytes; tiles that make one
+    static constexpr bool kAside = true;           // (keep_aside)
     static __device__ __forceinline__ Frag operand(const Raw& x) { return x; }
     static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -87,6 +88,7 @@ struct Matrix<float> {
     typedef f32x8 Raw;
     typedef f32x8 Frag;
     static constexpr int kChunk = 4, kPlanes = 1;
+    static constexpr bool kAside = false;  // used where sums fill that half
     static __device__ __forceinline__ Frag operand(const Raw& x) { return x; }
     static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
 #pragma unroll
@@ -98,6 +100,7 @@ struct MatrixInParts {
     typedef float IO;
     typedef f32x8 Raw;
     typedef Frag3 Frag;
+    static constexpr bool kAside = true;
     static __device__ __forceinline__ Frag operand(const Raw& x) {
         Frag f;
 #pragma unroll
@@ -175,6 +178,19 @@ __device__ __forceinline__ f32x16 zero16() {
 #pragma unroll
     for (int i = 0; i < 16; ++i) z[i] = 0.f;
     return z;
+}
+
+// Holds an operand that stays in the half of the registers that only matrix instructions reach, where one wavefront has all
+// of a SIMD's: the other half is left to sums and scores, which vector instructions work on.
+__device__ __forceinline__ void keep_aside(bf16x8& f) {
+    f32x4 x = __builtin_bit_cast(f32x4, f);
+    asm volatile("" : "+a"(x));
+    f = __builtin_bit_cast(bf16x8, x);
+}
+__device__ __forceinline__ void keep_aside(f32x8& f) { asm volatile("" : "+a"(f)); }
+__device__ __forceinline__ void keep_aside(Frag3& f) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) keep_aside(f.p[i]);
 }
 
 // A (or B) operand whose rows are rows of a tile of ROWS rows: rows row0 .. + 31 (row0 a multiple of 16), features 16 step ..
@@ -606,6 +622,7 @@ void forward_bf16(const Params& p, bool few_rows, hipStream_t stream);
 void forward_f32(const Params& p, bool few_rows, hipStream_t stream);
 void backward_bf16(const Params& p, hipStream_t stream);
 void backward_f32(const Params& p, hipStream_t stream);
+void backward_f32_wide(const Params& p, hipStream_t stream);
 
 }  // namespace attn
 }  // namespace adhip

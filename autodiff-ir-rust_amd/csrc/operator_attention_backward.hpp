@@ -68,6 +68,10 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta += (float)x[e] * (float)y[e];
             df[s] = M::operand(x);
+            if (C::WAVES == 1 && M::kAside) {
+                keep_aside(qf[s]);
+                keep_aside(df[s]);
+            }
         }
     }
     delta = sum_of_halves(delta);
@@ -239,8 +243,14 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
                 if (C::K_LDS && rg == 0) *(uint4*)(k_own + at) = ((const uint4*)&x)[i];
                 if (C::V_LDS && rg == 0) *(uint4*)(v_own + at) = ((const uint4*)&y)[i];
             }
-            if (!C::K_LDS) kf[s] = M::operand(x);
-            if (!C::V_LDS) vf[s] = M::operand(y);
+            if (!C::K_LDS) {
+                kf[s] = M::operand(x);
+                if (C::WAVES == 1 && M::kAside) keep_aside(kf[s]);
+            }
+            if (!C::V_LDS) {
+                vf[s] = M::operand(y);
+                if (C::WAVES == 1 && M::kAside) keep_aside(vf[s]);
+            }
         }
     }
     f32x16 dk[DP / 32], dv[DP / 32];

@@ -9,6 +9,8 @@
 // tile of keys.  Few rows (one token a sequence): four wavefronts share 32 rows and split each tile of keys, the keys are
 // split over workgroups beside that, and the parts are joined, with their maxima and sums, in LDS and by a second kernel.
 #pragma once
+#include <algorithm>
+
 #include "operator_attention.hpp"
 
 namespace adhip {
@@ -67,6 +69,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = -x[e];
             qf[s] = M::operand(x);
+            if (C::WAVES == 1 && M::kAside) keep_aside(qf[s]);
         }
     }
     f32x16 o[DP / 32];
@@ -273,32 +276,78 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
     }
 }
 
-// Joins the ranges of keys: a wavefront a row.
+// Joins the ranges of keys.  A row takes `pieces` threads of four features for each of `groups` runs of ranges, which are
+// added up in LDS: with one wavefront a row that walked its ranges one after the other, the join of 64 ranges took longer
+// than the attention before it.
 template <class T>
-__global__ __launch_bounds__(256) void join_kernel(const Params p) {
-    const int64_t rows = (int64_t)p.B * p.Hk * p.R, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (at >= rows) return;
-    float m = -__builtin_inff();
-    for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, p.part_ml[(s * rows + at) * 2]);
+__global__ __launch_bounds__(256) void join_kernel(const Params p, int pieces, int groups, int rows_each) {
+    __shared__ float ml[2 * 2048];
+    __shared__ f32x4 sums[256];
+    const int64_t rows = (int64_t)p.B * p.Hk * p.R, row0 = (int64_t)blockIdx.x * rows_each;
+    const int tid = threadIdx.x, here_rows = (int)min((int64_t)rows_each, rows - row0);
+    for (int i = tid; i < here_rows * p.splits; i += 256) {
+        const int r = i / p.splits, s = i - r * p.splits;
+        const float2 x = *(const float2*)(p.part_ml + (s * rows + row0 + r) * 2);
+        ml[2 * i] = x.x;
+        ml[2 * i + 1] = x.y;
+    }
+    __syncthreads();
+    const int r = tid / (pieces * groups), in_row = tid - r * pieces * groups, g = in_row / pieces, d = (in_row - g * pieces) * 4;
+    const bool mine = r < here_rows;
+    const int64_t at = row0 + r;
+    float m = -__builtin_inff(), sum = 0.f;
+    f32x4 f = {0.f, 0.f, 0.f, 0.f};
+    if (mine) {
+        const float* of = ml + 2 * r * p.splits;
+#pragma unroll 4
+        for (int s = 0; s < p.splits; ++s) m = fmaxf(m, of[2 * s]);
+        const float base = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll 4
+        for (int s = 0; s < p.splits; ++s) sum += of[2 * s + 1] * __builtin_amdgcn_exp2f(of[2 * s] - base);
+        const bool vec = (p.D & 3) == 0;
+#pragma unroll 4
+        for (int s = g; s < p.splits; s += groups) {
+            const float w = __builtin_amdgcn_exp2f(of[2 * s] - base);
+            const float* x = p.part + (s * rows + at) * p.D + d;
+            if (vec) {
+                const f32x4 y = *(const f32x4*)x;
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    const float base = m == -__builtin_inff() ? 0.f : m;
-    float sum = 0.f;
-    for (int s = lane; s < p.splits; s += 64) sum += p.part_ml[(s * rows + at) * 2 + 1] * __builtin_amdgcn_exp2f(p.part_ml[(s * rows + at) * 2] - base);
+                for (int e = 0; e < 4; ++e) f[e] += y[e] * w;
+            } else {
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+                for (int e = 0; e < 4; ++e) f[e] += d + e < p.D ? x[e] * w : 0.f;
+            }
+        }
+    }
+    if (groups > 1) {
+        sums[tid] = f;
+        __syncthreads();
+        if (g > 0) return;
+        for (int i = 1; i < groups; ++i) {
+            const f32x4 y = sums[tid + i * pieces];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] += y[e];
+        }
+    }
+    if (!mine) return;
     const int64_t bc = at / p.R;
     const int row = (int)(at - bc * p.R), c = (int)(bc % p.Hk), token = row / p.G, head = c * p.G + row - token * p.G;
     const int64_t b = bc / p.Hk;
-    const float r = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    T* out = (T*)p.out.data + b * p.out.b + token * p.out.l + head * p.out.h;
-    for (int d = lane; d < p.D; d += 64) {
-        float f = 0.f;
-        for (int s = 0; s < p.splits; ++s) f += p.part[(s * rows + at) * p.D + d] * __builtin_amdgcn_exp2f(p.part_ml[(s * rows + at) * 2] - base);
-        out[d] = (T)(f * r);
-    }
-    if (lane == 0) p.lse[b * p.lse_b + token * p.lse_l + head * p.lse_h] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+    const float over = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const float y[4] = {f[0] * over, f[1] * over, f[2] * over, f[3] * over};
+    store4((T*)p.out.data + b * p.out.b + token * p.out.l + head * p.out.h, d, p.D, p.out.vec, y);
+    if (d == 0) p.lse[b * p.lse_b + token * p.lse_l + head * p.lse_h] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+template <class T>
+void launch_join(const Params& p, hipStream_t stream) {
+    const int pieces = (p.D + 3) / 4;
+    // as many runs as ranges leave four each for, and threads allow
+    int groups = 1;
+    while (groups * 8 <= p.splits && pieces * groups * 2 <= 256) groups *= 2;
+    const int rows_each = std::min(256 / (pieces * groups), 2048 / p.splits);
+    join_kernel<T><<<(unsigned)(((int64_t)p.B * p.Hk * p.R + rows_each - 1) / rows_each), 256, 0, stream>>>(p, pieces, groups, rows_each);
+    check_launch("adhip_attention");
 }
 
 // Bytes of a row of a tile decide how many keys a tile has and how many tiles LDS holds: 64 keys where tiles leave room for
@@ -329,10 +378,7 @@ void launch_forward(const Params& p, hipStream_t stream) {
     if (p.q.vec && p.k.vec && p.v.vec) forward_kernel<X, DP, true, C><<<grid, C::NT, 0, stream>>>(p);
     else forward_kernel<X, DP, false, C><<<grid, C::NT, 0, stream>>>(p);
     check_launch("adhip_attention");
-    if (p.splits > 1) {
-        join_kernel<typename Matrix<X>::IO><<<(unsigned)(((int64_t)p.B * p.Hk * p.R + 3) / 4), 256, 0, stream>>>(p);
-        check_launch("adhip_attention");
-    }
+    if (p.splits > 1) launch_join<typename Matrix<X>::IO>(p, stream);
 }
 
 // Many: what multiplies where rows fill workgroups; Few: where they do not
