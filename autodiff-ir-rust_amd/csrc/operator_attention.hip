@@ -89,14 +89,14 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
     y.few_rows = R <= 32;
     y.row_tile = attn::forward_rows(g.q.type, attn::padded_size((int)D), y.few_rows);
     y.tiles = (int)((R + y.row_tile - 1) / y.row_tile);
-    // Ranges of keys: as many as give every compute unit two workgroups, or one where rows are few (a workgroup fills LDS then
-    // and keeps 64 KB under way: 8 sequences of 16384 keys, 105 us with one, 113 with four), none shorter than two tiles.
-    const int64_t blocks = (int64_t)y.tiles * Hk * B, keys = y.few_rows ? 128 : 64;
+    // Ranges of keys, none shorter than two tiles.  Many rows: as many as give every compute unit the workgroups that it can
+    // hold, which also evens out a causal mask (2 x 2048 x 8 heads of 64 in f32: 122 us unsplit, 82 with two a compute unit, 73
+    // with three; of 128, 157, 131 and 148).  Few rows: one, as a workgroup fills LDS then and keeps 64 KB under way (8
+    // sequences of 16384 keys: 105 us with one, 113 with four).
+    const int64_t blocks = (int64_t)y.tiles * Hk * B, keys = y.few_rows ? 128 : 64, target = y.few_rows ? 256 : D <= 64 ? 768 : 512;
     y.splits = 1;
-    if (blocks > 0 && blocks < 256) {
-        const int64_t want = ((y.few_rows ? 256 : 512) + blocks - 1) / blocks, most = (Lk + 2 * keys - 1) / (2 * keys);
-        y.splits = (int)std::max<int64_t>(1, std::min(std::min(want, most), (int64_t)256));
-    }
+    if (blocks > 0 && blocks < target)
+        y.splits = (int)std::max<int64_t>(1, std::min({(target + blocks - 1) / blocks, (Lk + 2 * keys - 1) / (2 * keys), (int64_t)256}));
     size_t at = 0;
     // (whether documents are given or not: what a call needs goes by shapes alone)
     y.qrange = at;
@@ -219,6 +219,9 @@ Params checked(const char* op, const adhip_attention_args& g, const Layout& y, b
         check_array(op, "key_documents", g.key_documents, ADHIP_I32, 2);
         check_dims(op, "query_documents", g.query_documents, {B, Lq});
         check_dims(op, "key_documents", g.key_documents, {B, Lk});
+        for (const adhip_array* a : {&g.query_documents, &g.key_documents})  // a tile's offsets are to fit 31 bits
+            ADHIP_CHECK(a->dims[1] <= 1 || a->strides[1] <= (1 << 20), "%s: documents lie %lld elements apart, at most %d are supported", op,
+                        (long long)a->strides[1], 1 << 20);
         p.qdoc = (const int*)g.query_documents.data;
         p.kdoc = (const int*)g.key_documents.data;
         p.qdoc_b = g.query_documents.strides[0], p.qdoc_l = g.query_documents.strides[1];

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
     // the running maximum wants a positive unit: the scale's sign goes to the queries
     const float sign = p.scale < 0.f ? -1.f : 1.f;
     const Scoring sc(p);
-    const float unit = p.slopes ? 1.f : p.scale == 0.f ? 1.f : sign * sc.unit;
+    const float unit = p.slopes || p.scale == 0.f ? 1.f : p.cap > 0.f ? sc.unit : sign * sc.unit;
     const int row0 = tile * C::BQ, row1 = min(row0 + C::BQ, p.R) - 1;
     const int first = row0 / p.G, last = row1 / p.G;  // tokens of the tile
 

@@ -55,6 +55,12 @@ ATTENTION = {
 }
 
 
+# the same with scales that are given: below zero the largest product is the smallest score
+SCALES = [("causal over several tiles", dict(scale=-0.11)), ("33 rows", dict(scale=-0.2)), ("prefix", dict(scale=-0.1, cap=2.0)),
+          ("prefix and window, shorter", dict(scale=-0.3)), ("tokens against a cache", dict(scale=-0.09, cap=1.5)), ("one token", dict(scale=0.0)),
+          ("full, odd", dict(scale=0.0, cap=3.0)), ("several tokens against a cache", dict(scale=3.0, cap=0.5))]
+
+
 def attention_inputs(name, dtype, layout="plain", seed=0):
     B, Lq, Lk, H, Hk, D, how = ATTENTION[name]
     how = dict(how)
@@ -113,8 +119,8 @@ def run_attention(dev, a, how, backward, strided_out=False):
 
 def check_attention(dev, name, dtype, layout="plain", strided_out=False):
     a, how = attention_inputs(name, dtype, layout)
-    scale = how.get("scale", 1.0 / math.sqrt(a["q"].shape[-1]))
-    want, bound = oracle.attention(a["q"], a["k"], a["v"], out_grad=a["out_grad"], rounding=W[dtype], **{**how, "scale": scale})
+    scale = 1.0 / math.sqrt(a["q"].shape[-1])
+    want, bound = oracle.attention(a["q"], a["k"], a["v"], out_grad=a["out_grad"], rounding=W[dtype], scale=scale, **how)
     got = run_attention(dev, a, how, True, strided_out)
     for n in want:
         assert_within(got[n], want[n], bound[n], f"{name}, {dtype}, {layout}: {n}")
@@ -131,6 +137,33 @@ def test_attention_and_its_gradients(hip_device, name, dtype):
 @pytest.mark.parametrize("name", ["tokens against a cache", "causal over several tiles", "shared by 5, odd", "wide heads, not whole"])
 def test_attention_on_other_layouts(hip_device, name, layout, dtype):
     check_attention(hip_device, name, dtype, layout, strided_out=layout == "heads first")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name,change", SCALES)
+def test_attention_with_scales_of_either_sign(hip_device, name, change, dtype):
+    a, how = attention_inputs(name, dtype)
+    how |= change
+    want, bound = oracle.attention(a["q"], a["k"], a["v"], out_grad=a["out_grad"], rounding=W[dtype], **how)
+    got = run_attention(hip_device, a, how, True)
+    for n in want:
+        assert_within(got[n], want[n], bound[n], f"{name}, {change}, {dtype}: {n}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_in_split_walks(hip_device, dtype):
+    """Few heads and many positions: forward and both backward walks in parts, the keys' documents and lengths uneven."""
+    g = torch.Generator().manual_seed(2)
+    B, L, H, Hk, D = 1, 1900, 2, 1, 48
+    a = {n: torch.randn(B, L, h, D, generator=g).to(TYPES[dtype]) for n, h in (("q", H), ("k", Hk), ("v", Hk), ("out_grad", H))}
+    d = torch.cumsum(torch.rand((B, L), generator=g) < 0.002, 1).to(torch.int32)
+    d[:, 1700:] = -1
+    for how in (dict(causal=True), dict(causal=True, window=300, prefix=torch.tensor([100], dtype=torch.int32)),
+                dict(causal=True, query_documents=d, key_documents=d), dict(lengths=torch.tensor([1234], dtype=torch.int32), cap=4.0)):
+        want, bound = oracle.attention(a["q"], a["k"], a["v"], out_grad=a["out_grad"], rounding=W[dtype], scale=D ** -0.5, **how)
+        got = run_attention(hip_device, a, how, True)
+        for n in want:
+            assert_within(got[n], want[n], bound[n], f"{list(how)}, {dtype}: {n}")
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -486,6 +519,7 @@ def test_refusals_of_attention(hip_device):
     refused("slopes", slopes=f(2))
     refused("key_documents", query_documents=i(2, 8))
     refused("query_documents", query_documents=i(2, 9), key_documents=i(2, 9))
+    refused("elements apart", query_documents=i(2, 8), key_documents=torch.as_strided(i(9 << 21), (2, 9), (1, 1 << 21)))
     refused("cap", cap=-1.0)
     refused("cap", cap=math.nan)
     refused("scale", scale=math.inf)
