@@ -78,6 +78,7 @@ struct Matrix<bf16> {
     typedef bf16x8 Frag;
     static constexpr int kChunk = 8, kPlanes = 1;  // elements of 16 bytes; tiles that make one
     static constexpr bool kAside = true;           // (keep_aside)
+    static constexpr bool kFine = false;           // (tanh_of)
     static __device__ __forceinline__ Frag operand(const Raw& x) { return x; }
     static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -89,6 +90,7 @@ struct Matrix<float> {
     typedef f32x8 Frag;
     static constexpr int kChunk = 4, kPlanes = 1;
     static constexpr bool kAside = false;  // used where sums fill that half
+    static constexpr bool kFine = true;
     static __device__ __forceinline__ Frag operand(const Raw& x) { return x; }
     static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
 #pragma unroll
@@ -100,7 +102,7 @@ struct MatrixInParts {
     typedef float IO;
     typedef f32x8 Raw;
     typedef Frag3 Frag;
-    static constexpr bool kAside = true;
+    static constexpr bool kAside = true, kFine = true;
     static __device__ __forceinline__ Frag operand(const Raw& x) {
         Frag f;
 #pragma unroll
@@ -308,10 +310,16 @@ __device__ __forceinline__ void store4(T* row, int d, int D, int vec, const floa
     }
 }
 
-// tanh(x) from y = 2 x log2 e, to about 2e-7: what a capped score takes, in units of the cap
+// tanh(x) from y = 2 x log2 e: what a capped score takes, in units of the cap.  To about 1.5e-7; FINE, for f32, also in
+// relation to small values, where scores mostly lie: by the series below 0.3, 5e-8 of the value.
+template <bool FINE>
 __device__ __forceinline__ float tanh_of(float y) {
-    const float e = __builtin_amdgcn_exp2f(y);
-    return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
+    const float e = __builtin_amdgcn_exp2f(y), far = __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
+    if (!FINE) return far;
+    const float x = y * (0.5f * kLn2), t = x * x;
+    const float near = __builtin_fmaf(
+        x * t, __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), x);
+    return t < 0.09f ? near : far;
 }
 
 // The larger (the sum) of a lane's value and that of the lane 32 away, in both.

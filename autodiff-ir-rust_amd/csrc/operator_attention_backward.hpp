@@ -124,7 +124,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
             if (p.cap > 0.f) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[i] = tanh_of(s[i] * sc.bend);
+                    s[i] = tanh_of<M::kFine>(s[i] * sc.bend);
                     g[i] *= 1.f - s[i] * s[i];
                 }
             }
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
             if (p.cap > 0.f) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[i] = tanh_of(s[i] * sc.bend);
+                    s[i] = tanh_of<M::kFine>(s[i] * sc.bend);
                     g[i] *= 1.f - s[i] * s[i];
                 }
             }

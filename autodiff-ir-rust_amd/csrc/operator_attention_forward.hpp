@@ -116,7 +116,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
 #pragma unroll
             for (int x = 0; x < C::KB; ++x)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[x][i] = tanh_of(s[x][i] * (sign * sc.bend));
+                for (int i = 0; i < 16; ++i) s[x][i] = tanh_of<M::kFine>(s[x][i] * (sign * sc.bend));
         }
         if (p.slopes) {
             const float inner = p.cap > 0.f ? sc.unit : sign * sc.unit;
