@@ -88,6 +88,11 @@ class DeviceArray:
             raise ValueError(f"{values.size} values for {list(self.shape)}")
         _check(self._dev, _lib(self._dev).adhip_copy_in(self._dev._ctx, self._data, values.ctypes.data, values.nbytes), "adhip_copy_in")
 
+    def clear(self) -> None:
+        """Zeros in every byte (waits)."""
+        zeros = np.zeros(self.nbytes, np.uint8)
+        _check(self._dev, _lib(self._dev).adhip_copy_in(self._dev._ctx, self._data, zeros.ctypes.data, zeros.nbytes), "adhip_copy_in")
+
     def numpy(self) -> np.ndarray:
         """A copy on the host (waits); bfloat16 as float32, 8-bit codes as uint8."""
         kind = {F32: np.float32, BF16: np.uint16, I32: np.int32, E4M3: np.uint8}[_TYPES[self.dtype]]
