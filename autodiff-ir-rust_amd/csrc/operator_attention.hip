@@ -81,6 +81,47 @@ struct Layout {
     bool parts;
 };
 
+constexpr int kUnits = 256;  // compute units
+
+// How many ranges (at most `most`) the keys are split into where rows fill workgroups: the smallest sum of two times, in us.
+//   walk  a workgroup's tiles, and one more for its beginning and end, at `pair` ps for a row and a key, as measured with one
+//         workgroup a compute unit (bf16 64 features 140, 128 180, 192 350, 256 380; f32 464, 464 with eight wavefronts, -,
+//         1760).  Workgroups that share a compute unit finish 1.4 (two) and 1.8 (three) times as much.  Where all walks are
+//         equally long, the compute unit with the most workgroups decides; where a causal mask makes them uneven, given out
+//         from the longest, it is the longest walk or the average load, whichever is more, and a part of the other.
+//   join  0.36 us a MB of parts, written and read again, and 6 us for the launch and the parts' ends
+// Over 32 shapes (300 to 8192 positions, bf16 64 to 256 features, f32 64 to 256) the choice is within 3 % of the best number in
+// the mean; as many ranges as fill the card alone was 17 % off (2 x 8 x 300 positions of 16 heads: 18 us, 37 with two ranges that
+// the card had room for).
+int ranges_of_many(const adhip_attention_args& g, int64_t blocks, int row_tile, bool causal, int64_t window, int most) {
+    const int64_t B = g.q.dims[0], Lq = g.q.dims[1], H = g.q.dims[2], D = g.q.dims[3], Lk = g.k.dims[1], Hk = g.k.dims[2];
+    const bool f32 = g.q.type == ADHIP_F32;
+    const int DP = attn::padded_size((int)D), keys = f32 || DP > 128 ? 32 : 64, room = f32 ? (DP <= 64 ? 2 : 1) : DP <= 64 ? 3 : DP <= 192 ? 2 : 1;
+    const double pair = !f32 ? 70 + 1.15 * DP : DP > 128 ? 7. * DP : (100 + 5. * DP) / (row_tile == 256 ? 1.5 : 1.);
+    const double tile = pair * row_tile * keys * 1e-6;
+    double longest = (double)Lk, mean = causal ? std::max((double)Lk - Lq / 2., Lk / 2.) : (double)Lk;
+    if (window > 0) {
+        longest = std::min(longest, (causal ? 1. : 2.) * (double)window + (double)(row_tile / (H / Hk)));
+        mean = std::min(mean, longest);
+    }
+    const bool even = mean > 0.75 * longest;
+    const double part_bytes = (double)B * (double)Lq * (double)H * (double)D * 4;
+    double best = 0;
+    int choice = 1;
+    for (int s = 1; s <= most && (s == 1 || ((int64_t)s * keys * 2 <= Lk + keys && s * blocks <= 4 * kUnits)); s += 1 + s / 8) {
+        const double walk = (std::ceil(longest / keys / s) + 1) * tile, workgroups = (double)(blocks * s);
+        const double each = std::ceil(workgroups / kUnits), faster = 1 + 0.4 * (std::min<double>(each, room) - 1);
+        double time = each * walk / faster;
+        if (!even) {
+            const double load = workgroups / kUnits * (mean / keys / s + 1) * tile / faster, more = std::max(walk, load), less = std::min(walk, load);
+            time = more + less * less * less / (3 * more * more);
+        }
+        if (s > 1) time += 6 + 0.36e-6 * s * part_bytes;
+        if (s == 1 || time < best) best = time, choice = s;
+    }
+    return choice;
+}
+
 Layout layout_of(const adhip_attention_args& g, bool backward) {
     Layout y = {};
     const int64_t B = g.q.dims[0], Lq = g.q.dims[1], H = g.q.dims[2], D = g.q.dims[3], Lk = g.k.dims[1], Hk = g.k.dims[2];
@@ -89,14 +130,18 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
     y.few_rows = R <= 32;
     y.row_tile = attn::forward_rows(g.q.type, attn::padded_size((int)D), y.few_rows);
     y.tiles = (int)((R + y.row_tile - 1) / y.row_tile);
-    // Ranges of keys, none shorter than two tiles.  Many rows: as many as give every compute unit the workgroups that it can
-    // hold, which also evens out a causal mask (2 x 2048 x 8 heads of 64 in f32: 122 us unsplit, 82 with two a compute unit, 73
-    // with three; of 128, 157, 131 and 148).  Few rows: one, as a workgroup fills LDS then and keeps 64 KB under way (8
-    // sequences of 16384 keys: 105 us with one, 113 with four).
-    const int64_t blocks = (int64_t)y.tiles * Hk * B, keys = y.few_rows ? 128 : 64, target = y.few_rows ? 256 : D <= 64 ? 768 : 512;
+    // Ranges of keys, none shorter than two tiles.  Few rows: one workgroup a compute unit, as it fills LDS then and keeps 64 KB
+    // under way (8 sequences of 16384 keys: 105 us with one, 113 with four).  Many rows: ranges_of_many.
+    const int64_t blocks = (int64_t)y.tiles * Hk * B;
+    int most = 1;
     y.splits = 1;
-    if (blocks > 0 && blocks < target)
-        y.splits = (int)std::max<int64_t>(1, std::min({(target + blocks - 1) / blocks, (Lk + 2 * keys - 1) / (2 * keys), (int64_t)256}));
+    if (y.few_rows && blocks > 0 && blocks < kUnits)
+        most = y.splits = (int)std::max<int64_t>(1, std::min({(kUnits + blocks - 1) / blocks, (Lk + 255) / 256, (int64_t)256}));
+    if (!y.few_rows && blocks > 0) {
+        // (what a call needs goes by shapes alone, how it is cut up by its masks too)
+        most = std::max(ranges_of_many(g, blocks, y.row_tile, false, 0, 256), ranges_of_many(g, blocks, y.row_tile, true, 0, 256));
+        y.splits = ranges_of_many(g, blocks, y.row_tile, g.causal != 0, g.window, most);
+    }
     size_t at = 0;
     // (whether documents are given or not: what a call needs goes by shapes alone)
     y.qrange = at;
@@ -116,11 +161,11 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
         }
     }
     size_t forward = at, back = at;
-    if (y.splits > 1) {
+    if (most > 1) {
         y.part = forward;
-        forward += rounded((size_t)(y.splits * B * Hk * R * D) * 4);
+        forward += rounded((size_t)(most * B * Hk * R * D) * 4);
         y.part_ml = forward;
-        forward += rounded((size_t)(y.splits * B * Hk * R * 2) * 4);
+        forward += rounded((size_t)(most * B * Hk * R * 2) * 4);
     }
     y.dq_splits = y.dk_splits = 1;
     if (backward) {
