@@ -9,6 +9,8 @@
 // Where there are too few workgroups for the card, or too few for the uneven work of a causal mask to even out, each walk
 // is split and the parts are added, in order, by a third kernel.
 #pragma once
+#include <algorithm>
+
 #include "operator_attention.hpp"
 
 namespace adhip {
@@ -460,18 +462,41 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         }
 }
 
-// Adds the parts of split walks: [splits][B][Hk][L G][D] to an array [B, L, Hk G, D], an element a thread at a time.
+// Adds the parts of split walks, in their order: [splits][B][Hk][rows][D] to arrays [B, rows / G, Hk G, D].  A thread four
+// features of a row, all gradients in one launch.  (Walks are split where there are fewer than 65536 rows: 32 bits hold all
+// numbers.)
+struct PartsToAdd {
+    const float* part;
+    Tensor out;
+    unsigned splits, rows, G;
+};
+struct AllPartsToAdd {
+    PartsToAdd of[3];
+};
 template <class T>
-__global__ __launch_bounds__(256) void add_parts_kernel(const float* part, int splits, Tensor out, int B, int Hk, int L, int G, int D) {
-    const int64_t count = (int64_t)B * Hk * L * G * D;
-    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < count; at += (int64_t)gridDim.x * 256) {
-        float f = 0.f;
-        for (int s = 0; s < splits; ++s) f += part[s * count + at];
-        const int64_t row = at / D;
-        const int d = (int)(at - row * D), r = (int)(row % ((int64_t)L * G)), i = r / G;
-        const int64_t bc = row / ((int64_t)L * G), b = bc / Hk;
-        ((T*)out.data)[b * out.b + i * out.l + ((bc - b * Hk) * G + r - i * G) * out.h + d] = (T)f;
+__global__ __launch_bounds__(256) void add_parts_kernel(const AllPartsToAdd all, unsigned B, unsigned Hk, int D) {
+    const PartsToAdd& j = all.of[blockIdx.y];
+    const unsigned pieces = (D + 3) / 4, total = B * Hk * j.rows, at = blockIdx.x * 256 + threadIdx.x, row = at / pieces;
+    if (row >= total) return;
+    const int d = (int)(at - row * pieces) * 4;
+    const float* from = j.part + (int64_t)row * D + d;
+    const int64_t step = (int64_t)total * D;
+    f32x4 f = {0.f, 0.f, 0.f, 0.f};
+    if (D % 4 == 0) {
+#pragma unroll 4
+        for (unsigned s = 0; s < j.splits; ++s) {
+            const f32x4 x = *(const f32x4*)(from + s * step);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] += x[e];
+        }
+    } else {
+        for (unsigned s = 0; s < j.splits; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] += d + e < D ? from[s * step + e] : 0.f;
     }
+    const unsigned bc = row / j.rows, r = row - bc * j.rows, i = r / j.G, b = bc / Hk, head = (bc - b * Hk) * j.G + r - i * j.G;
+    const float y[4] = {f[0], f[1], f[2], f[3]};
+    store4((T*)j.out.data + b * j.out.b + i * j.out.l + head * j.out.h, d, D, j.out.vec, y);
 }
 
 // Rows and their gradients stay in registers; two workgroups a compute unit up to 128 features in bf16.
@@ -504,10 +529,21 @@ template <>
 struct KeyChoice<float, 256> { typedef KeyConfig<float, 256, 2, 1, 1, false, true, 1> C; };
 
 template <class T>
-void add_parts(const float* part, int splits, const Tensor& out, int B, int Hk, int L, int G, int D, hipStream_t stream) {
-    const int64_t count = (int64_t)B * Hk * L * G * D;
-    const unsigned blocks = (unsigned)std::min<int64_t>((count + 255) / 256, 4096);
-    if (blocks) add_parts_kernel<T><<<blocks, 256, 0, stream>>>(part, splits, out, B, Hk, L, G, D);
+void add_parts(const Params& p, hipStream_t stream) {
+    AllPartsToAdd all;
+    unsigned n = 0, most = 0;
+    auto add = [&](const float* part, const Tensor& out, int splits, int rows, int G) {
+        all.of[n++] = {part, out, (unsigned)splits, (unsigned)rows, (unsigned)G};
+        most = std::max(most, (unsigned)rows);
+    };
+    if (p.dq_splits > 1) add(p.part_dq, p.dq, p.dq_splits, p.R, p.G);
+    if (p.dk_splits > 1) {
+        add(p.part_dk, p.dk, p.dk_splits, p.Lk, 1);
+        add(p.part_dv, p.dv, p.dk_splits, p.Lk, 1);
+    }
+    if (n == 0) return;
+    const unsigned items = p.B * p.Hk * most * ((p.D + 3) / 4);
+    add_parts_kernel<T><<<dim3((items + 255) / 256, n), 256, 0, stream>>>(all, p.B, p.Hk, p.D);
     check_launch("adhip_attention_backward");
 }
 
@@ -523,16 +559,12 @@ void launch_backward(const Params& p, hipStream_t stream) {
     if (grid > 0 && vec) query_gradient_kernel<X, DP, true, Q><<<grid, Q::NT, 0, stream>>>(x);
     else if (grid > 0) query_gradient_kernel<X, DP, false, Q><<<grid, Q::NT, 0, stream>>>(x);
     check_launch("adhip_attention_backward");
-    if (p.dq_splits > 1) add_parts<T>(p.part_dq, p.dq_splits, p.dq, p.B, p.Hk, p.Lq, p.G, p.D, stream);
     x.tiles = (p.Lk + K::BKEYS - 1) / K::BKEYS;
     grid = (unsigned)((int64_t)x.tiles * p.dk_splits * p.Hk * p.B);
     if (grid > 0 && vec) key_gradient_kernel<X, DP, true, K><<<grid, K::NT, 0, stream>>>(x);
     else if (grid > 0) key_gradient_kernel<X, DP, false, K><<<grid, K::NT, 0, stream>>>(x);
     check_launch("adhip_attention_backward");
-    if (p.dk_splits > 1) {
-        add_parts<T>(p.part_dk, p.dk_splits, p.dk, p.B, p.Hk, p.Lk, 1, p.D, stream);
-        add_parts<T>(p.part_dv, p.dk_splits, p.dv, p.B, p.Hk, p.Lk, 1, p.D, stream);
-    }
+    add_parts<T>(p, stream);
 }
 
 }  // namespace attn

@@ -26,7 +26,7 @@ struct RotaryParams {
     int64_t pb, pl;   // strides of positions
     int64_t rows;     // of the tables
     unsigned tokens, length;
-    int size, pairs;
+    int pairs;
     unsigned turned, copied;  // chunks of V pairs and of V copied features of a head
     unsigned turns, items;    // lanes that a token takes: `turns` for its pairs, the others for copies
     unsigned per_block;       // tokens of a block (1 where a token takes several)
@@ -174,7 +174,6 @@ void rotary(const adhip_rotary_args& g, hipStream_t stream) {
     p.rows = g.cos.dims[0];
     p.tokens = (unsigned)tokens;
     p.length = (unsigned)length;
-    p.size = (int)size;
     p.pairs = (int)pairs;
     p.turns = p.turned * (unsigned)(p.a[0].heads + p.a[1].heads);
     p.items = p.turns + p.copied * (unsigned)(p.a[0].heads + p.a[1].heads);

@@ -54,6 +54,17 @@ ATTENTION = {
     "256 features, few rows": (2, 1, 300, 4, 2, 256, dict(causal=True, lengths=[300, 31])),
 }
 
+# few tiles of rows and long keys, or the other way round: walks in ranges (two to eight, and more), joined and added up
+LONG = {
+    "ranges, 100 features": (1, 40, 1500, 2, 1, 100, dict(causal=True, cap=20.0)),
+    "ranges, 61 features": (2, 50, 1100, 2, 2, 61, dict(lengths=[1100, 301])),
+    "ranges, 256 features": (1, 35, 900, 4, 2, 256, dict(causal=True, window=800)),
+    "ranges, 33 features, many": (1, 64, 9001, 1, 1, 33, dict(causal=True, prefix=[4000])),
+    "ranges, 128 features, many": (1, 40, 9003, 2, 1, 128, dict(slopes=True)),
+    "ranges, documents": (1, 2000, 2000, 2, 2, 64, dict(causal=True, documents=True)),
+    "ranges of rows": (1, 1501, 70, 4, 2, 90, {}),
+}
+
 
 # the same with scales that are given: below zero the largest product is the smallest score
 SCALES = [("causal over several tiles", dict(scale=-0.11)), ("33 rows", dict(scale=-0.2)), ("prefix", dict(scale=-0.1, cap=2.0)),
@@ -62,7 +73,7 @@ SCALES = [("causal over several tiles", dict(scale=-0.11)), ("33 rows", dict(sca
 
 
 def attention_inputs(name, dtype, layout="plain", seed=0):
-    B, Lq, Lk, H, Hk, D, how = ATTENTION[name]
+    B, Lq, Lk, H, Hk, D, how = {**ATTENTION, **LONG}[name]
     how = dict(how)
     g = torch.Generator().manual_seed(seed + len(name))
 
@@ -130,6 +141,13 @@ def check_attention(dev, name, dtype, layout="plain", strided_out=False):
 @pytest.mark.parametrize("name", ATTENTION)
 def test_attention_and_its_gradients(hip_device, name, dtype):
     check_attention(hip_device, name, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["plain", "unaligned"])
+@pytest.mark.parametrize("name", LONG)
+def test_attention_in_ranges(hip_device, name, layout, dtype):
+    check_attention(hip_device, name, dtype, layout)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
