@@ -427,7 +427,8 @@ struct Tiles {
 // A ring of BUFS tiles in LDS: the oldest is worked on while the others are under way.  `start(tile, buffer)` begins a
 // tile's loads, of which the last LOADS of each wavefront are its own; `landed(tile, buffer)` runs when it is there and all
 // wavefronts have come.  A load takes one to two microseconds from other memory than the L2, as long as the products of a
-// tile where a compute unit has few wavefronts: then two and three tiles under way are worth their LDS.
+// tile where a compute unit has few wavefronts: then two and three tiles under way are worth their LDS (causal, 2 x 4096 x 16
+// heads of 128, one under way and waited for as a whole: 175 us forward, 676 backward; so: 166, 559).
 template <int BUFS, int LOADS, class Walk, class Start>
 struct Ring {
     Walk& walk;
@@ -495,7 +496,7 @@ struct Place {
 // A load of 16 (or 4) bytes a lane that writes LDS by itself: lane i's go to `to` + 16 i (4 i), from `base` (of the whole wavefront) and the
 // lane's offset; an offset behind the resource's end gives zeros.  It stands here as the instruction because the compiler
 // orders every later read of LDS behind the one it knows of, and so would wait for a tile that is not needed before the
-// next step; the ring below waits and has a barrier where it is.  No register is written, so none can be written late.
+// next step; the ring above waits and has a barrier where it is.  No register is written, so none can be written late.
 template <int BYTES>
 __device__ __forceinline__ void load_to_lds(const void* base, unsigned offset, char* to) {
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));

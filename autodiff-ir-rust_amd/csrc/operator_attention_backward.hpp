@@ -513,6 +513,8 @@ struct QueryChoice {
 template <int DP>
 struct QueryChoice<Parts, DP> { typedef QueryConfig<32, 3, DP <= 64 ? 2 : 1> C; };
 // Keys and values in registers where the sums leave room for them, one wavefront a SIMD where they do not leave room for two.
+// Two take 8 wavefronts that share a tile of rows: causal training of 2 x 4096 x 16 heads on 4 of 128, capped, took 893 us in
+// all with two a SIMD, 1037 with one.
 template <class X, int DP>
 struct KeyChoice { typedef KeyConfig<X, DP, 4, 1, 2, false, false, 1> C; };
 template <int DP>

@@ -406,7 +406,8 @@ void launch_join(const Params& p, hipStream_t stream) {
 }
 
 // Bytes of a row of a tile decide how many keys a tile has and how many tiles LDS holds: 64 keys where tiles leave room for
-// the workgroups that registers allow, 32 else, and as many tiles as then fit.
+// the workgroups that registers allow, 32 else, and as many tiles as then fit.  (Heads of 256, one workgroup a compute unit: 2 x
+// 4096 x 8 heads 220 us with four tiles of 32.)
 template <class X, int DP>
 struct ForwardMany {
     static constexpr int kRow = DP * (int)sizeof(typename Matrix<X>::E);
@@ -414,7 +415,8 @@ struct ForwardMany {
                           kRow <= 128 ? 3 : kRow <= 384 ? 2 : 1> C;
 };
 // In parts: two workgroups of four wavefronts up to 64 features, one of eight above, so that a SIMD always has two and one's
-// matrix instructions run beside the other's splitting and exponentials.
+// matrix instructions run beside the other's splitting and exponentials.  (2048 x 8 heads of 128, forward and backward: 415 us, with
+// four wavefronts above 64 as well 537.)
 template <int DP>
 struct ForwardMany<Parts, DP> {
     typedef ForwardConfig<DP, forward_rows(ADHIP_F32, DP, false) / 32, 1, 32, 3, 2> C;
