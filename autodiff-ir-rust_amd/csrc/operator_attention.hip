@@ -84,44 +84,66 @@ struct Layout {
 
 constexpr int kUnits = 256;  // compute units
 
-// How many ranges (at most `most`) the keys are split into where rows fill workgroups: the smallest sum of two times, in us.
-//   walk  a workgroup's tiles, and one more for its beginning and end, at `pair` ps for a row and a key, as measured with one
-//         workgroup a compute unit (bf16 64 features 140, 128 180, 192 350, 256 380; f32 464, 464 with eight wavefronts, -,
-//         1760).  Workgroups that share a compute unit finish 1.4 (two) and 1.8 (three) times as much.  Where all walks are
-//         equally long, the compute unit with the most workgroups decides; where a causal mask makes them uneven, given out
-//         from the longest, it is the longest walk or the average load, whichever is more, and a part of the other.
+// A kind of walk: workgroups of `own` rows (or keys), each of which goes over keys (or rows) in tiles of `step`.
+struct Walks {
+    int64_t blocks;     // workgroups with one range each
+    int own, step;
+    int room;           // workgroups that registers and LDS of a compute unit hold
+    double across;      // keys (rows) in all, and what it counts for each key: 1, or G where rows are walked
+    int times;
+    double part_bytes;  // what a range more takes of memory
+};
+
+// How many ranges (at most `most`) such walks are split into where rows fill workgroups: the smallest sum of two times, in us.
+//   walk  a workgroup's tiles, and one more for its beginning and end, at `pair` ps for a row and a key, as measured for the
+//         forward kernels with one workgroup a compute unit (bf16 64 features 140, 128 180, 192 350, 256 380; f32 464, 464 with
+//         eight wavefronts, -, 1760).  Workgroups that share a compute unit finish 1.4 (two) and 1.8 (three) times as much.
+//         Where all walks are equally long, the compute unit with the most workgroups decides; where a causal mask makes them
+//         uneven, given out from the longest, it is the longest walk or the average load, whichever is more, and a little of
+//         the other.  With documents they are taken for a quarter as long, and all alike (8191 positions in documents of
+//         1200, forward and backward, 8 heads of 64: 195 us, 210 with the ranges that the causal mask alone would take).
 //   join  0.36 us a MB of parts, written and read again, and 6 us for the launch and the parts' ends
-// Over 32 shapes (300 to 8192 positions, bf16 64 to 256 features, f32 64 to 256) the choice is within 3 % of the best number in
-// the mean; as many ranges as fill the card alone was 17 % off (2 x 8 x 300 positions of 16 heads: 18 us, 37 with two ranges that
-// the card had room for).
-int ranges_of_many(const adhip_attention_args& g, int64_t blocks, int row_tile, bool causal, int64_t window, int most) {
-    const int64_t B = g.q.dims[0], Lq = g.q.dims[1], H = g.q.dims[2], D = g.q.dims[3], Lk = g.k.dims[1], Hk = g.k.dims[2];
-    const bool f32 = g.q.type == ADHIP_F32;
-    const int DP = attn::padded_size((int)D), keys = f32 || DP > 128 ? 32 : 64, room = f32 ? (DP <= 64 ? 2 : 1) : DP <= 64 ? 3 : DP <= 192 ? 2 : 1;
-    const double pair = !f32 ? 70 + 1.15 * DP : DP > 128 ? 7. * DP : (100 + 5. * DP) / (row_tile == 256 ? 1.5 : 1.);
-    const double tile = pair * row_tile * keys * 1e-6;
-    double longest = (double)Lk, mean = causal ? std::max((double)Lk - Lq / 2., Lk / 2.) : (double)Lk;
+// Over 32 shapes (300 to 8192 positions, bf16 64 to 256 features, f32 64 to 256) the choice is within 1 % of the best number in
+// the mean, for the backward walks within 2 % over 34; as many ranges as fill the card alone were 17 and 9 % off (8 x 300
+// positions of 16 heads of 128 forward: 18 us, 37 with the two ranges that the card had room for).
+int ranges(const adhip_attention_args& g, const Walks& w, bool causal, int64_t window, bool documents, int most) {
+    const int64_t Lq = g.q.dims[1], D = g.q.dims[3], Lk = g.k.dims[1];
+    const int DP = attn::padded_size((int)D);
+    const double pair = g.q.type != ADHIP_F32 ? 70 + 1.15 * DP : DP > 128 ? 7. * DP : (100 + 5. * DP) / (w.own == 256 ? 1.5 : 1.);
+    const double tile = pair * w.own * w.step * 1e-6;
+    // what the longest walk and the mean one go over
+    double longest = w.across, mean = causal ? std::max(1. - Lq / (2. * std::max<double>((double)Lk, 1)), 0.5) * w.across : w.across;
     if (window > 0) {
-        longest = std::min(longest, (causal ? 1. : 2.) * (double)window + (double)(row_tile / (H / Hk)));
+        longest = std::min(longest, ((causal ? 1. : 2.) * (double)window + (double)w.own * w.times / (double)(g.q.dims[2] / g.k.dims[2])) * w.times);
         mean = std::min(mean, longest);
     }
+    if (documents) longest = mean = std::min(mean, w.across / 4);
     const bool even = mean > 0.75 * longest;
-    const double part_bytes = (double)B * (double)Lq * (double)H * (double)D * 4;
     double best = 0;
     int choice = 1;
-    for (int s = 1; s <= most && (s == 1 || ((int64_t)s * keys * 2 <= Lk + keys && s * blocks <= 4 * kUnits)); s += 1 + s / 8) {
-        const double walk = (std::ceil(longest / keys / s) + 1) * tile, workgroups = (double)(blocks * s);
-        const double each = std::ceil(workgroups / kUnits), faster = 1 + 0.4 * (std::min<double>(each, room) - 1);
+    for (int s = 1; s <= most && (s == 1 || ((double)s * w.step * 2 <= w.across + w.step && s * w.blocks <= 4 * kUnits)); s += 1 + s / 8) {
+        const double walk = (std::ceil(longest / w.step / s) + 1) * tile, workgroups = (double)(w.blocks * s);
+        const double each = std::ceil(workgroups / kUnits), faster = 1 + 0.4 * (std::min<double>(each, w.room) - 1);
         double time = each * walk / faster;
         if (!even) {
-            const double load = workgroups / kUnits * (mean / keys / s + 1) * tile / faster, more = std::max(walk, load), less = std::min(walk, load);
-            time = more + less * less * less / (3 * more * more);
+            const double load = workgroups / kUnits * (mean / w.step / s + 1) * tile / faster;
+            time = std::max(walk, load) + 0.05 * std::min(walk, load);
         }
-        if (s > 1) time += 6 + 0.36e-6 * s * part_bytes;
+        if (s > 1) time += 6 + 0.36e-6 * s * w.part_bytes;
         if (s == 1 || time < best) best = time, choice = s;
     }
     return choice;
 }
+// for a call, and the most that a call on arrays of these shapes takes, whatever its masks
+struct Ranges {
+    int now = 1, most = 1;
+    Ranges() {}
+    Ranges(const adhip_attention_args& g, const Walks& w) {
+        if (w.blocks <= 0) return;
+        most = std::max(ranges(g, w, false, 0, false, 256), ranges(g, w, true, 0, false, 256));
+        now = ranges(g, w, g.causal != 0, g.window, g.key_documents.data != nullptr, most);
+    }
+};
 
 Layout layout_of(const adhip_attention_args& g, bool backward) {
     Layout y = {};
@@ -132,17 +154,16 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
     y.row_tile = attn::forward_rows(g.q.type, attn::padded_size((int)D), y.few_rows);
     y.tiles = (int)((R + y.row_tile - 1) / y.row_tile);
     // Ranges of keys, none shorter than two tiles.  Few rows: one workgroup a compute unit, as it fills LDS then and keeps 64 KB
-    // under way (8 sequences of 16384 keys: 105 us with one, 113 with four).  Many rows: ranges_of_many.
+    // under way (8 sequences of 16384 keys: 105 us with one, 113 with four).
     const int64_t blocks = (int64_t)y.tiles * Hk * B;
-    int most = 1;
-    y.splits = 1;
-    if (y.few_rows && blocks > 0 && blocks < kUnits)
-        most = y.splits = (int)std::max<int64_t>(1, std::min({(kUnits + blocks - 1) / blocks, (Lk + 255) / 256, (int64_t)256}));
-    if (!y.few_rows && blocks > 0) {
-        // (what a call needs goes by shapes alone, how it is cut up by its masks too)
-        most = std::max(ranges_of_many(g, blocks, y.row_tile, false, 0, 256), ranges_of_many(g, blocks, y.row_tile, true, 0, 256));
-        y.splits = ranges_of_many(g, blocks, y.row_tile, g.causal != 0, g.window, most);
-    }
+    const bool f32 = g.q.type == ADHIP_F32;
+    const int DP = attn::padded_size((int)D), step = f32 || DP > 128 ? 32 : 64;
+    const double row_bytes = 4. * (double)B * (double)Lq * (double)H * (double)D, key_bytes = 4. * (double)B * (double)Lk * (double)Hk * (double)D;
+    Ranges forward_ranges;
+    if (!y.few_rows) forward_ranges = Ranges(g, {blocks, y.row_tile, step, f32 ? (DP <= 64 ? 2 : 1) : DP <= 64 ? 3 : DP <= 192 ? 2 : 1, (double)Lk, 1, row_bytes});
+    else if (blocks > 0 && blocks < kUnits)
+        forward_ranges.most = forward_ranges.now = (int)std::max<int64_t>(1, std::min({(kUnits + blocks - 1) / blocks, (Lk + 255) / 256, (int64_t)256}));
+    y.splits = forward_ranges.now;
     size_t at = 0;
     // (whether documents are given or not: what a call needs goes by shapes alone)
     y.qrange = at;
@@ -162,6 +183,8 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
         }
     }
     size_t forward = at, back = at;
+    // (what a call needs goes by shapes alone, how it is cut up by its masks too)
+    const int64_t most = forward_ranges.most;
     if (most > 1) {
         y.part = forward;
         forward += rounded((size_t)(most * B * Hk * R * D) * 4);
@@ -172,26 +195,20 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
     if (backward) {
         y.stats = back;
         back += rounded((size_t)(B * Hk * R) * 2 * 4);
-        // Parts of the backward walks: as many as give every compute unit two workgroups, which evens out a causal mask's
-        // uneven ones, none shorter than four tiles.  More parts cost more memory to add up than they even out: 2048 x 8 heads of
-        // 128 in f32 448 us with two a compute unit, 498 with one, 518 with four.
-        constexpr int64_t kTarget = 512;
-        auto parts = [](int64_t blocks, int64_t tiles) {
-            if (blocks <= 0 || blocks >= kTarget) return 1;
-            return (int)std::max<int64_t>(1, std::min<int64_t>((kTarget + blocks - 1) / blocks, tiles / 4));
-        };
-        const int64_t rows = (R + 127) / 128 * Hk * B, keys = (Lk + 127) / 128 * Hk * B;
-        y.dq_splits = parts(rows, (Lk + 63) / 64);
-        y.dk_splits = parts(keys, (R + 63) / 64);
-        if (y.dq_splits > 1) {
+        // the walks of 128 rows over keys and of 128 keys over the rows of all their heads
+        const Ranges of_rows(g, {(R + 127) / 128 * Hk * B, 128, step, DP <= (f32 ? 64 : 128) ? 2 : 1, (double)Lk, 1, row_bytes});
+        const Ranges of_keys(g, {(Lk + 127) / 128 * Hk * B, 128, step, 1, (double)R, (int)(H / Hk), 2 * key_bytes});
+        y.dq_splits = of_rows.now;
+        y.dk_splits = of_keys.now;
+        if (of_rows.most > 1) {
             y.part_dq = back;
-            back += rounded((size_t)(y.dq_splits * B * Hk * R * D) * 4);
+            back += rounded((size_t)(of_rows.most * B * Hk * R * D) * 4);
         }
-        if (y.dk_splits > 1) {
+        if (of_keys.most > 1) {
             y.part_dk = back;
-            back += rounded((size_t)(y.dk_splits * B * Hk * Lk * D) * 4);
+            back += rounded((size_t)(of_keys.most * B * Hk * Lk * D) * 4);
             y.part_dv = back;
-            back += rounded((size_t)(y.dk_splits * B * Hk * Lk * D) * 4);
+            back += rounded((size_t)(of_keys.most * B * Hk * Lk * D) * 4);
         }
     }
     y.bytes = std::max(forward, back);

@@ -41,7 +41,7 @@ def reference(weights, x, target, heads, key_heads, size, steps, *, rate, cap, w
         optimizer.zero_grad()
         loss.backward()
         optimizer.step()
-        losses.append(float(loss))
+        losses.append(float(loss.detach()))
     return losses, {n: t.detach().numpy() for n, t in w.items()}
 
 
