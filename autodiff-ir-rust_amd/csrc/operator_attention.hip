@@ -100,13 +100,14 @@ struct Walks {
 //         eight wavefronts, -, 1760).  Workgroups that share a compute unit finish 1.4 (two) and 1.8 (three) times as much.
 //         Where all walks are equally long, the compute unit with the most workgroups decides; where a causal mask makes them
 //         uneven, given out from the longest, it is the longest walk or the average load, whichever is more, and a little of
-//         the other.  With documents they are taken for a quarter as long, and all alike (8191 positions in documents of
-//         1200, forward and backward, 8 heads of 64: 195 us, 210 with the ranges that the causal mask alone would take).
+//         the other.  Documents, which end walks where they fall, are not looked at: the more ranges of the mask alone even them out too
+//         (8191 positions, 8 heads of 64, eight draws of documents of 1200 on average, forward and backward: 192 to 350 us;
+//         with the ranges of short walks, mostly one, 197 to 422).
 //   join  0.36 us a MB of parts, written and read again, and 6 us for the launch and the parts' ends
 // Over 32 shapes (300 to 8192 positions, bf16 64 to 256 features, f32 64 to 256) the choice is within 1 % of the best number in
 // the mean, for the backward walks within 2 % over 34; as many ranges as fill the card alone were 17 and 9 % off (8 x 300
 // positions of 16 heads of 128 forward: 18 us, 37 with the two ranges that the card had room for).
-int ranges(const adhip_attention_args& g, const Walks& w, bool causal, int64_t window, bool documents, int most) {
+int ranges(const adhip_attention_args& g, const Walks& w, bool causal, int64_t window, int most) {
     const int64_t Lq = g.q.dims[1], D = g.q.dims[3], Lk = g.k.dims[1];
     const int DP = attn::padded_size((int)D);
     const double pair = g.q.type != ADHIP_F32 ? 70 + 1.15 * DP : DP > 128 ? 7. * DP : (100 + 5. * DP) / (w.own == 256 ? 1.5 : 1.);
@@ -117,7 +118,6 @@ int ranges(const adhip_attention_args& g, const Walks& w, bool causal, int64_t w
         longest = std::min(longest, ((causal ? 1. : 2.) * (double)window + (double)w.own * w.times / (double)(g.q.dims[2] / g.k.dims[2])) * w.times);
         mean = std::min(mean, longest);
     }
-    if (documents) longest = mean = std::min(mean, w.across / 4);
     const bool even = mean > 0.75 * longest;
     double best = 0;
     int choice = 1;
@@ -140,8 +140,8 @@ struct Ranges {
     Ranges() {}
     Ranges(const adhip_attention_args& g, const Walks& w) {
         if (w.blocks <= 0) return;
-        most = std::max(ranges(g, w, false, 0, false, 256), ranges(g, w, true, 0, false, 256));
-        now = ranges(g, w, g.causal != 0, g.window, g.key_documents.data != nullptr, most);
+        most = std::max(ranges(g, w, false, 0, 256), ranges(g, w, true, 0, 256));
+        now = ranges(g, w, g.causal != 0, g.window, most);
     }
 };
 
