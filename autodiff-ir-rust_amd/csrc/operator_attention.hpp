@@ -496,7 +496,10 @@ struct Place {
 // A load of 16 (or 4) bytes a lane that writes LDS by itself: lane i's go to `to` + 16 i (4 i), from `base` (of the whole wavefront) and the
 // lane's offset; an offset behind the resource's end gives zeros.  It stands here as the instruction because the compiler
 // orders every later read of LDS behind the one it knows of, and so would wait for a tile that is not needed before the
-// next step; the ring above waits and has a barrier where it is.  No register is written, so none can be written late.
+// next step; the ring above waits and has a barrier where it is.  No vector register is written, so none can be written late.
+// A descriptor's word may come straight from v_readfirstlane, whose result a memory instruction may read five wait states later:
+// the compiler sees to that between its own instructions, here s_nop 4 does.  m0, where the instruction finds its place in LDS, is
+// an operand, so that the compiler knows it to be in use.
 template <int BYTES>
 __device__ __forceinline__ void load_to_lds(const void* base, unsigned offset, char* to) {
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -505,8 +508,8 @@ __device__ __forceinline__ void load_to_lds(const void* base, unsigned offset, c
                           (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)) & 0xffffu, 0x7fffffffu, 0x00020000u};
     const unsigned lds = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)to);  // an address in LDS ends in its offset
     static_assert(BYTES == 16 || BYTES == 4, "widths of these loads");
-    if (BYTES == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(source) : "memory");
-    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(source) : "memory");
+    if (BYTES == 16) asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(lds), "v"(offset), "s"(source) : "memory");
+    else asm volatile("s_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"{m0}"(lds), "v"(offset), "s"(source) : "memory");
 }
 // Copies of tiles from an array's rows (a fixed stride apart) into LDS by a workgroup of NT threads: ROWS rows of DP
 // features.  Where rows allow it (VEC) the loads write LDS themselves, 16 bytes a lane, in the order of the tile's places;
