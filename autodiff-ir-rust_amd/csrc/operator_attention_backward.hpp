@@ -229,11 +229,13 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
     const int key = key_first + kg * 32 + (lane & 31);
     const int doc = p.kdoc && key < n ? p.kdoc[b * p.kdoc_b + key * p.kdoc_l] : 0;
     const bool valid = key < n && doc >= 0;
-    // rows at positions from .. to see this key (limits of the sequence aside), all rows where it is in the prefix
+    // rows at positions from .. to see this key, all up to the last one, at n - 1, where it is in the prefix: rows behind the last
+    // one fill up a tile, and a slope below zero would make infinite probabilities of their distances
     // (a key that no row may see sees everything here, so that it keeps no wavefront from the short way; its gradients are
     // replaced at the end)
+    constexpr int kFar = 1 << 29;  // more than any position
     const bool free = !valid || key < prefix;
-    const int from = free ? -(1 << 30) : key - band.above, to = free ? 1 << 30 : key + band.below;
+    const int from = free ? -kFar : key - band.above, to = !valid ? kFar : min(free ? kFar : key + band.below, n - 1);
 
     Frag kf[C::K_LDS ? 1 : DP / 16], vf[C::V_LDS ? 1 : DP / 16];
     {
@@ -302,8 +304,8 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void key_gradient_kernel(const Par
         for (int i = 0; i < M::kPlanes; ++i)
             copy_g.start(to_q + C::kTile + i * C::BR * L::kPitch, (const E*)tg.data + i * p.q_plane + b * tg.b + i0 * tg.l + h * tg.h, tg.l, left, D, tid);
     };
-    // A row that sees nothing is zero, whatever the arrays hold there.  (Rows behind the last one came as zeros: their
-    // probabilities, of whatever size, meet nothing but zeros.)
+    // A row that sees nothing is zero, whatever the arrays hold there.  (Rows behind the last one came as zeros, and no key sees
+    // them.)
     auto clean = [&](int buf) {
         const float* const of = (const float*)(lds + C::kRows + buf * 3 * C::BR * 4);
         if (!__any(of[lane % C::BR] == __builtin_inff())) return;

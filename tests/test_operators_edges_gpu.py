@@ -1,0 +1,62 @@
+"""Inputs at the edges of what the operators on device arrays promise, against the 64-bit restatements of operator_oracle.py
+with its bounds: distances that score upwards, values that nothing may use, widths between the tested ones, numbers that fill a
+launch."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import operator_oracle as oracle
+from adhip import operators as ops
+from test_operators_gpu import TYPES, W, assert_within, here, run_attention, to_gpu
+
+pytestmark = pytest.mark.gpu
+
+
+def inputs(dtype, B, Lq, Lk, H, Hk, D, seed=0, unaligned=False):
+    g = torch.Generator().manual_seed(seed)
+
+    def array(length, heads):
+        x = torch.randn((B, length, heads, D), generator=g).to(TYPES[dtype])
+        if not unaligned:
+            return x
+        wide = torch.zeros((B, length, heads, D + 3), dtype=x.dtype)
+        wide[..., 1:-2] = x
+        return wide[..., 1:-2]
+
+    return {n: array(length, heads) for n, length, heads in (("q", Lq, H), ("k", Lk, Hk), ("v", Lk, Hk), ("out_grad", Lq, H))}
+
+
+def documents(B, L, rate, none, seed=0):
+    """Rising numbers of documents, the last `none` positions of no document."""
+    d = torch.cumsum(torch.rand((B, L), generator=torch.Generator().manual_seed(seed)) < rate, 1).to(torch.int32)
+    d[:, L - none:] = -1
+    return d
+
+
+def check(dev, a, dtype, what, **how):
+    how.setdefault("scale", 1.0 / math.sqrt(a["q"].shape[-1]))
+    want, bound = oracle.attention(a["q"], a["k"], a["v"], out_grad=a["out_grad"], rounding=W[dtype], **how)
+    got = run_attention(dev, a, how, True)
+    for n in want:
+        assert_within(got[n], want[n], bound[n], f"{what}, {dtype}: {n}")
+
+
+# ---- attention: scores that rise with distance --------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries,size,how", [
+    (181, 64, dict(causal=True)),
+    (181, 64, dict(causal=True, prefix=[130, 0])),
+    (215, 128, dict(causal=True, cap=5.0, lengths=[215, 200])),
+    (203, 40, dict()),
+    (183, 192, dict(causal=True)),
+    (181, 256, dict(causal=True)),
+])
+def test_attention_with_slopes_below_zero(hip_device, queries, size, how, dtype):
+    """exp(0.5 x 180) passes what 32 bits hold: a row that is not there must not meet the products with it."""
+    a = inputs(dtype, 2, queries, queries, 4, 2, size, seed=queries)
+    how = {n: torch.tensor(x, dtype=torch.int32) if isinstance(x, list) else x for n, x in how.items()}
+    check(hip_device, a, dtype, f"{queries} x {size}, {list(how)}", slopes=torch.tensor([-0.5, 0.25, -0.75, -0.6]), **how)
