@@ -573,8 +573,8 @@ __device__ __forceinline__ void copy_words(char* to, const void* from, int64_t s
     if (wave * 64 < ROWS && mine) load_to_lds<4>(from, tid < count ? (unsigned)(tid * stride) * 4u : 0xffffffffu, to + wave * 256);
 }
 
-// Tiles of keys and values on their way from memory to LDS: shared by the kernels that own rows.  Keys behind the sequence
-// or of no document are zero, whatever the arrays hold there.
+// Tiles of keys and values on their way from memory to LDS: shared by the kernels that own rows.  Keys behind the sequence, of
+// no document, or between the prefix and the first query's window are zero, whatever the arrays hold there.
 template <class X, int DP, class C, bool VEC>
 struct KeyTiles {
     typedef Matrix<X> M;
@@ -589,11 +589,11 @@ struct KeyTiles {
     const E *kb, *vb;
     const int* kd;
     char* lds;
-    int n, tid, D;
+    int n, prefix, window, tid, D;  // window: where the first query's begins
     S k, v;
-    __device__ __forceinline__ KeyTiles(const Params& p_, int b, int c, int n_, int tid_, char* lds_)
-        : p(p_), kt(M::kPlanes == 3 ? p_.k3 : p_.k), vt(M::kPlanes == 3 ? p_.v3 : p_.v), lds(lds_), n(n_), tid(tid_),
-          D(M::kPlanes == 3 ? p_.D3 : p_.D), k(kt.l, D, tid_), v(vt.l, D, tid_) {
+    __device__ __forceinline__ KeyTiles(const Params& p_, int b, int c, int n_, int prefix_, const Band& band, int tid_, char* lds_)
+        : p(p_), kt(M::kPlanes == 3 ? p_.k3 : p_.k), vt(M::kPlanes == 3 ? p_.v3 : p_.v), lds(lds_), n(n_), prefix(prefix_),
+          window(n_ - p_.Lq - band.below), tid(tid_), D(M::kPlanes == 3 ? p_.D3 : p_.D), k(kt.l, D, tid_), v(vt.l, D, tid_) {
         kb = (const E*)kt.data + b * kt.b + c * kt.h;
         vb = (const E*)vt.data + b * vt.b + c * vt.h;
         kd = p.kdoc ? p.kdoc + b * p.kdoc_b : nullptr;
@@ -610,12 +610,15 @@ struct KeyTiles {
 #pragma unroll
         for (int i = 0; i < M::kPlanes; ++i) v.start(values(buf) + i * kPlane, vb + i * p.k_plane + j0 * vt.l, vt.l, left, D, tid);
     }
-    // a tile that has arrived and holds keys of no document
+    // a tile that has arrived and holds keys of no document or in front of every window
     __device__ __forceinline__ void clean(const Tile& tile, int buf) const {
-        if (!kd || tile.documents.x >= 0) return;
+        const int j0 = tile.t * C::BK;
+        const bool strays = kd && tile.documents.x < 0, early = j0 < window && j0 + C::BK > prefix;
+        if (!strays && !early) return;
         const int* of = (const int*)docs(buf);
 #pragma unroll 1
-        for (int i = 0; i < 2 * M::kPlanes; ++i) S::clear(keys(buf) + i * kPlane, [&](int r) { return of[r] < 0; }, tid);
+        for (int i = 0; i < 2 * M::kPlanes; ++i)
+            S::clear(keys(buf) + i * kPlane, [&](int r) { return (strays && of[r] < 0) || (j0 + r >= prefix && j0 + r < window); }, tid);
         __syncthreads();
     }
 };

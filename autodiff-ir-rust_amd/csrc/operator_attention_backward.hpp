@@ -105,7 +105,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void query_gradient_kernel(const P
     const unsigned r_lane = rows_lane<X, DP>(lane), c_lane = cols_lane<X, DP>(lane);
     typedef Tiles<decltype(needed)> Walk;
     Walk walk(needed, t_first, t_stop, split, p.dq_splits, lane);
-    const Keys kt(p, b, c, n, tid, lds);
+    const Keys kt(p, b, c, n, prefix, band, tid, lds);
     Ring<C::kBufs, Keys::kLoads, Walk, Keys> ring(walk, kt);
     for (; ring.ready(); ring.pop()) {
         const int buf = ring.buf, t = ring.queue[0].t;

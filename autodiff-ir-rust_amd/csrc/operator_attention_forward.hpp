@@ -100,7 +100,7 @@ __global__ __launch_bounds__(C::NT, C::WAVES) void forward_kernel(const Params p
     const unsigned v_lane = cols_lane<X, DP>(lane) + wk * C::KB * 32 * Lds<typename M::E, DP>::kPitch;
     typedef Tiles<decltype(needed)> Walk;
     Walk walk(needed, t_first, t_stop, split, p.splits, lane);
-    const Keys kt(p, b, c, n, tid, lds);
+    const Keys kt(p, b, c, n, prefix, band, tid, lds);
     Ring<C::kBufs, Keys::kLoads, Walk, Keys> ring(walk, kt);
     for (; ring.ready(); ring.pop()) {
         const int buf = ring.buf, t = ring.queue[0].t;

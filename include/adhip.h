@@ -204,10 +204,11 @@ int adhip_adamw(adhip_ctx* ctx, const adhip_adamw_args* args, void* stream);
  * and scores it with
  *     z = cap tanh(scale q.k / cap) - slopes[h] |at - j|      (cap 0: scale q.k uncapped; no slopes: no second term).
  * out = softmax(z) v over what it sees, lse = log(sum(exp(z))) (f32, [batch, queries, heads]).  A query that sees nothing
- * gives out = 0 and lse = -infinity; keys and values that no query may see (behind lengths, documents below 0) are not
- * used, whatever they hold.  lengths (int32 [batch]; default: keys) is clamped to 0 .. keys.  A key that some query of the
- * call may see must be finite, its value too: a tile is multiplied as a whole, and a probability of zero times an infinity
- * is NaN.  (In f32 an infinity that is seen gives NaN as well.)  documents may lie at most 2^20 elements apart.
+ * gives out = 0 and lse = -infinity.  Keys and values behind lengths, of documents below 0, or between the prefix and the
+ * beginning of the first query's window (keys up to its position - window) are not used, whatever they hold.  All others must be finite, also
+ * those that no query sees for another reason (the documents of a call's queries, for instance): a tile is multiplied as a
+ * whole, and a probability of zero times an infinity is NaN.  (In f32 an infinity that is seen gives NaN as well.)
+ * lengths (int32 [batch]; default: keys) is clamped to 0 .. keys.  documents may lie at most 2^20 elements apart.
  * workspace: device memory of at least adhip_attention_workspace() bytes, aligned to 256, used until the call's kernels
  * are done. */
 typedef struct adhip_attention_args {

@@ -60,3 +60,38 @@ def test_attention_with_slopes_below_zero(hip_device, queries, size, how, dtype)
     a = inputs(dtype, 2, queries, queries, 4, 2, size, seed=queries)
     how = {n: torch.tensor(x, dtype=torch.int32) if isinstance(x, list) else x for n, x in how.items()}
     check(hip_device, a, dtype, f"{queries} x {size}, {list(how)}", slopes=torch.tensor([-0.5, 0.25, -0.75, -0.6]), **how)
+
+
+# ---- attention: values that nothing may use --------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries,heads,size,how", [
+    (1, 8, 128, dict(causal=True, window=40)),
+    (1, 4, 64, dict(window=1)),
+    (5, 6, 80, dict(causal=True, window=100, prefix=[0, 70, 150], cap=4.0)),
+    (2, 2, 192, dict(causal=True, window=33, prefix=[3, 0, 0])),
+    (70, 4, 64, dict(causal=True, window=50, lengths=[300, 91, 40])),
+    (40, 2, 256, dict(window=64, prefix=[33, 0, 64])),
+    (130, 2, 128, dict(causal=True, window=129, documents=True)),
+])
+def test_attention_reads_nothing_in_front_of_every_window(hip_device, queries, heads, size, how, dtype):
+    """A cache of 300 positions whose windows have moved on: what lies between the prefix and the first query's window is NaN and
+    infinite."""
+    B, Lk = 3, 300
+    how = dict(how)
+    a = inputs(dtype, B, queries, Lk, heads, 2, size, seed=queries + size)
+    n = how.get("lengths", [Lk] * B)
+    first = [n[b] - queries - how["window"] + 1 for b in range(B)]
+    prefix = how.get("prefix", [0] * B)
+    hidden = 0
+    for b in range(B):
+        a["k"][b, prefix[b]:max(first[b], prefix[b])] = math.nan
+        a["v"][b, prefix[b]:max(first[b], prefix[b])] = math.inf
+        hidden += max(first[b] - prefix[b], 0)
+    assert hidden > 50
+    if how.pop("documents", False):
+        d = documents(B, Lk, 0.01, 20)
+        how |= dict(key_documents=d, query_documents=d[:, Lk - queries:].contiguous())
+    how = {x: torch.tensor(y, dtype=torch.int32) if isinstance(y, list) else y for x, y in how.items()}
+    check(hip_device, a, dtype, f"{queries} x {size}, {list(how)}", **how)
