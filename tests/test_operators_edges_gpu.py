@@ -95,3 +95,30 @@ def test_attention_reads_nothing_in_front_of_every_window(hip_device, queries, h
         how |= dict(key_documents=d, query_documents=d[:, Lk - queries:].contiguous())
     how = {x: torch.tensor(y, dtype=torch.int32) if isinstance(y, list) else y for x, y in how.items()}
     check(hip_device, a, dtype, f"{queries} x {size}, {list(how)}", **how)
+
+
+# ---- attention: widths and walks between the tested ones -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("unaligned", [False, True])
+@pytest.mark.parametrize("batch,queries,keys,heads,shared,size,how", [
+    (1, 300, 300, 4, 2, 192, dict(causal=True, cap=20.0)),
+    (2, 170, 231, 2, 1, 150, dict(causal=True, window=60)),
+    (1, 210, 210, 3, 3, 129, dict(slopes=True)),
+    (1, 70, 1900, 1, 1, 192, dict(causal=True)),           # walks in ranges
+    (1, 1300, 90, 2, 2, 176, dict()),                      # ranges of rows
+    (2, 260, 260, 2, 2, 192, dict(causal=True, documents=True, lengths=[260, 133])),
+    (2, 150, 150, 2, 1, 256, dict(documents=True, lengths=[90, 150])),
+    (1, 1100, 1100, 1, 1, 240, dict(causal=True, documents=True)),
+])
+def test_attention_of_129_features_and_more(hip_device, batch, queries, keys, heads, shared, size, how, unaligned, dtype):
+    how = dict(how)
+    a = inputs(dtype, batch, queries, keys, heads, shared, size, seed=queries + size, unaligned=unaligned)
+    if how.pop("slopes", False):
+        how["slopes"] = torch.tensor([2.0 ** -(h + 1) for h in range(heads)])
+    if how.pop("documents", False):
+        how["query_documents"] = how["key_documents"] = documents(batch, keys, 0.02, 20)
+    if "lengths" in how:
+        how["lengths"] = torch.tensor(how["lengths"], dtype=torch.int32)
+    check(hip_device, a, dtype, f"{queries} x {keys} x {size}, {list(how)}, unaligned {unaligned}", **how)
