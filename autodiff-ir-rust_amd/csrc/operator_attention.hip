@@ -215,11 +215,12 @@ Layout layout_of(const adhip_attention_args& g, bool backward) {
     return y;
 }
 
+// Shapes and types of q, k and v: what the workspace goes by
 void check_sizes(const char* op, const adhip_attention_args& g) {
     ADHIP_CHECK(g.q.type == ADHIP_F32 || g.q.type == ADHIP_BF16, "%s: q is %s, f32 or bf16 is wanted", op, type_name(g.q.type));
-    check_array(op, "q", g.q, g.q.type, 4);
-    check_array(op, "k", g.k, g.q.type, 4);
-    check_array(op, "v", g.v, g.q.type, 4);
+    check_shape(op, "q", g.q, g.q.type, 4);
+    check_shape(op, "k", g.k, g.q.type, 4);
+    check_shape(op, "v", g.v, g.q.type, 4);
     const int64_t B = g.q.dims[0], Lq = g.q.dims[1], H = g.q.dims[2], D = g.q.dims[3], Lk = g.k.dims[1], Hk = g.k.dims[2];
     check_dims(op, "k", g.k, {B, Lk, Hk, D});
     check_dims(op, "v", g.v, {B, Lk, Hk, D});

@@ -28,16 +28,25 @@ inline std::string array_str(const adhip_array& a) {
     return s + "]";
 }
 
-// `a` is given, has this type (-1: any) and rank, extents that are not negative and a memory extent that fits 2^62 bytes.
-inline void check_array(const char* op, const char* name, const adhip_array& a, int type, int rank) {
+// `a` has this type (-1: any) and rank, and extents that are not negative.  Returns how many elements it has.
+inline int64_t check_shape(const char* op, const char* name, const adhip_array& a, int type, int rank) {
     ADHIP_CHECK(a.rank == rank, "%s: %s has %d dims, %d are wanted", op, name, (int)a.rank, rank);
     ADHIP_CHECK(type < 0 || a.type == type, "%s: %s is %s, %s is wanted", op, name, type_name(a.type), type_name(type));
-    int64_t span = 0, count = 1;
+    int64_t count = 1;
     for (int i = 0; i < rank; ++i) {
         ADHIP_CHECK(a.dims[i] >= 0, "%s: %s has a negative extent: %s", op, name, array_str(a).c_str());
-        ADHIP_CHECK(a.strides[i] >= 0, "%s: %s has a negative stride", op, name);
         ADHIP_CHECK(!__builtin_mul_overflow(count, a.dims[i], &count) && count < (int64_t(1) << 60), "%s: %s is too large: %s", op, name,
                     array_str(a).c_str());
+    }
+    return count;
+}
+
+// The same, and it is given, with a memory extent that fits 2^62 bytes.
+inline void check_array(const char* op, const char* name, const adhip_array& a, int type, int rank) {
+    const int64_t count = check_shape(op, name, a, type, rank);
+    int64_t span = 0;
+    for (int i = 0; i < rank; ++i) {
+        ADHIP_CHECK(a.strides[i] >= 0, "%s: %s has a negative stride", op, name);
         int64_t far = 0;
         ADHIP_CHECK(!__builtin_mul_overflow(a.dims[i] > 0 ? a.dims[i] - 1 : 0, a.strides[i], &far) && !__builtin_add_overflow(span, far, &span) &&
                         span < (int64_t(1) << 60),

@@ -122,3 +122,28 @@ def test_attention_of_129_features_and_more(hip_device, batch, queries, keys, he
     if "lengths" in how:
         how["lengths"] = torch.tensor(how["lengths"], dtype=torch.int32)
     check(hip_device, a, dtype, f"{queries} x {keys} x {size}, {list(how)}, unaligned {unaligned}", **how)
+
+
+# ---- what the host decides ---------------------------------------------------------------------------------------------------
+
+
+class Shape:
+    """An array that has a shape and a type, and memory nowhere."""
+
+    def __init__(self, *shape, dtype="float32"):
+        self.shape, self.dtype = shape, dtype
+
+    def stride(self):
+        return tuple(math.prod(self.shape[i + 1:]) for i in range(len(self.shape)))
+
+    def data_ptr(self):
+        return 0
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_attention_workspace_goes_by_shapes_alone(hip_device, backward):
+    for dtype in TYPES:
+        q, k = torch.empty((2, 50, 4, 64), dtype=TYPES[dtype], device="cuda"), torch.empty((2, 900, 2, 64), dtype=TYPES[dtype], device="cuda")
+        need = ops.attention_workspace(hip_device, q, k, k, backward=backward)
+        q, k = Shape(*q.shape, dtype=q.dtype), Shape(*k.shape, dtype=k.dtype)
+        assert ops.attention_workspace(hip_device, q, k, k, backward=backward) == need > 0
