@@ -201,11 +201,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwLaunch a) {
 }
 
 template <bool EIGHT>
-void launch_adamw(const AdamwLaunch& a, int p_type, int g_type, unsigned blocks, hipStream_t stream) {
-    if (p_type == ADHIP_F32 && g_type == ADHIP_F32) adamw_kernel<float, float, EIGHT><<<blocks, 256, 0, stream>>>(a);
-    else if (p_type == ADHIP_F32) adamw_kernel<float, bf16, EIGHT><<<blocks, 256, 0, stream>>>(a);
-    else if (g_type == ADHIP_F32) adamw_kernel<bf16, float, EIGHT><<<blocks, 256, 0, stream>>>(a);
-    else adamw_kernel<bf16, bf16, EIGHT><<<blocks, 256, 0, stream>>>(a);
+void launch_adamw(const char* op, const AdamwLaunch& a, int p_type, int g_type, unsigned blocks, hipStream_t stream) {
+    if (p_type == ADHIP_F32 && g_type == ADHIP_F32) launch(op, adamw_kernel<float, float, EIGHT>, blocks, 256, stream, a);
+    else if (p_type == ADHIP_F32) launch(op, adamw_kernel<float, bf16, EIGHT>, blocks, 256, stream, a);
+    else if (g_type == ADHIP_F32) launch(op, adamw_kernel<bf16, float, EIGHT>, blocks, 256, stream, a);
+    else launch(op, adamw_kernel<bf16, bf16, EIGHT>, blocks, 256, stream, a);
 }
 
 bool aligned_to(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
@@ -248,9 +248,8 @@ void adamw(const adhip_adamw_args& g, hipStream_t stream) {
     uint64_t blocks = 0;
     auto flush = [&] {
         if (a.n == 0) return;
-        if (eight) launch_adamw<true>(a, g.p_type, g.g_type, (unsigned)blocks, stream);
-        else launch_adamw<false>(a, g.p_type, g.g_type, (unsigned)blocks, stream);
-        check_launch(op);
+        if (eight) launch_adamw<true>(op, a, g.p_type, g.g_type, (unsigned)blocks, stream);
+        else launch_adamw<false>(op, a, g.p_type, g.g_type, (unsigned)blocks, stream);
         a.n = 0;
         a.aligned = 0;
         blocks = 0;

@@ -335,9 +335,8 @@ Params checked(const char* op, const adhip_attention_args& g, const Layout& y, b
 void document_ranges(const Params& p, hipStream_t stream) {
     const int entries = p.qranges + p.kranges;
     if (!p.qdoc || entries == 0 || p.B == 0) return;
-    document_ranges_kernel<<<(unsigned)((entries + 7) / 8 * p.B), 256, 0, stream>>>(
-        p.qdoc, p.qdoc_b, p.qdoc_l, p.Lq, (int2*)p.qrange, p.qranges, p.kdoc, p.kdoc_b, p.kdoc_l, p.Lk, (int2*)p.krange, p.kranges);
-    check_launch("adhip_attention");
+    launch("adhip_attention", document_ranges_kernel, (unsigned)((entries + 7) / 8 * p.B), 256, stream, p.qdoc, p.qdoc_b, p.qdoc_l, p.Lq,
+           (int2*)p.qrange, p.qranges, p.kdoc, p.kdoc_b, p.kdoc_l, p.Lk, (int2*)p.krange, p.kranges);
 }
 
 // Keys and values, with `rows` queries and out's gradient too, in parts
@@ -350,8 +349,7 @@ void split_into_parts(const Params& p, bool rows, hipStream_t stream) {
     jobs.job[3] = {p.dout, (bf16*)p.dout3.data, queries, p.Lq, p.Hk * p.G};
     const int64_t most = (rows ? std::max(keys, queries) : keys) * (p.D3 / 8);
     if (most == 0) return;
-    parts_kernel<<<dim3((unsigned)((most + 255) / 256), rows ? 4 : 2), 256, 0, stream>>>(jobs, p.D, p.D3);
-    check_launch("adhip_attention");
+    launch("adhip_attention", parts_kernel, dim3((unsigned)((most + 255) / 256), rows ? 4 : 2), 256, stream, jobs, p.D, p.D3);
 }
 
 }  // namespace

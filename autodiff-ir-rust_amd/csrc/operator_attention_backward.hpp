@@ -551,8 +551,7 @@ void add_parts(const Params& p, hipStream_t stream) {
     }
     if (n == 0) return;
     const unsigned items = p.B * p.Hk * most * ((p.D + 3) / 4);
-    add_parts_kernel<T><<<dim3((items + 255) / 256, n), 256, 0, stream>>>(all, p.B, p.Hk, p.D);
-    check_launch("adhip_attention_backward");
+    launch("adhip_attention_backward", add_parts_kernel<T>, dim3((items + 255) / 256, n), 256, stream, all, (unsigned)p.B, (unsigned)p.Hk, p.D);
 }
 
 template <class X, int DP>
@@ -564,14 +563,11 @@ void launch_backward(const Params& p, hipStream_t stream) {
     const bool vec = p.q.vec && p.k.vec && p.v.vec && p.out.vec && p.dout.vec;
     x.tiles = (p.R + Q::BQ - 1) / Q::BQ;
     unsigned grid = (unsigned)((int64_t)x.tiles * p.dq_splits * p.Hk * p.B);
-    if (grid > 0 && vec) query_gradient_kernel<X, DP, true, Q><<<grid, Q::NT, 0, stream>>>(x);
-    else if (grid > 0) query_gradient_kernel<X, DP, false, Q><<<grid, Q::NT, 0, stream>>>(x);
-    check_launch("adhip_attention_backward");
+    const char* const op = "adhip_attention_backward";
+    if (grid > 0) launch(op, vec ? query_gradient_kernel<X, DP, true, Q> : query_gradient_kernel<X, DP, false, Q>, grid, Q::NT, stream, x);
     x.tiles = (p.Lk + K::BKEYS - 1) / K::BKEYS;
     grid = (unsigned)((int64_t)x.tiles * p.dk_splits * p.Hk * p.B);
-    if (grid > 0 && vec) key_gradient_kernel<X, DP, true, K><<<grid, K::NT, 0, stream>>>(x);
-    else if (grid > 0) key_gradient_kernel<X, DP, false, K><<<grid, K::NT, 0, stream>>>(x);
-    check_launch("adhip_attention_backward");
+    if (grid > 0) launch(op, vec ? key_gradient_kernel<X, DP, true, K> : key_gradient_kernel<X, DP, false, K>, grid, K::NT, stream, x);
     add_parts<T>(p, stream);
 }
 

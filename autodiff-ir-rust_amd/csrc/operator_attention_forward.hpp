@@ -393,16 +393,15 @@ void launch_join(const Params& p, hipStream_t stream) {
     const int pieces = (p.D + 3) / 4;
     // (keys are split where there are at most 1024 workgroups: 32 bits hold all numbers)
     if (p.splits <= kFewRanges) {
-        join_few_kernel<T><<<(unsigned)(((int64_t)p.B * p.Hk * p.R * pieces + 255) / 256), 256, 0, stream>>>(p);
-        check_launch("adhip_attention");
+        launch("adhip_attention", join_few_kernel<T>, (unsigned)(((int64_t)p.B * p.Hk * p.R * pieces + 255) / 256), 256, stream, p);
         return;
     }
     // as many runs as ranges leave four each for, and threads allow
     int groups = 1;
     while (groups * 8 <= p.splits && pieces * groups * 2 <= 256) groups *= 2;
     const int rows_each = std::min(256 / (pieces * groups), 2048 / p.splits);
-    join_kernel<T><<<(unsigned)(((int64_t)p.B * p.Hk * p.R + rows_each - 1) / rows_each), 256, 0, stream>>>(p, pieces, groups, rows_each);
-    check_launch("adhip_attention");
+    launch("adhip_attention", join_kernel<T>, (unsigned)(((int64_t)p.B * p.Hk * p.R + rows_each - 1) / rows_each), 256, stream, p, pieces, groups,
+           rows_each);
 }
 
 // Bytes of a row of a tile decide how many keys a tile has and how many tiles LDS holds: 64 keys where tiles leave room for
@@ -432,9 +431,8 @@ struct ForwardFew {
 template <class X, int DP, class C>
 void launch_forward(const Params& p, hipStream_t stream) {
     const unsigned grid = (unsigned)((int64_t)p.tiles * p.splits * p.Hk * p.B);
-    if (p.q.vec && p.k.vec && p.v.vec) forward_kernel<X, DP, true, C><<<grid, C::NT, 0, stream>>>(p);
-    else forward_kernel<X, DP, false, C><<<grid, C::NT, 0, stream>>>(p);
-    check_launch("adhip_attention");
+    const bool vec = p.q.vec && p.k.vec && p.v.vec;
+    launch("adhip_attention", vec ? forward_kernel<X, DP, true, C> : forward_kernel<X, DP, false, C>, grid, C::NT, stream, p);
     if (p.splits > 1) launch_join<typename Matrix<X>::IO>(p, stream);
 }
 

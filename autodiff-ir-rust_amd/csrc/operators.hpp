@@ -4,16 +4,19 @@
 
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "common.hpp"
 #include "runtime.hpp"
 
 namespace adhip {
 
-// After a launch: its error, if it could not be queued.
-inline void check_launch(const char* what) {
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) throw Error(strf("%s: the launch failed: %s", what, hipGetErrorString(e)));
+// Queues a kernel; an error is the launch's own, not one that another call of the process has left behind.
+template <class... P>
+void launch(const char* op, void (*kernel)(P...), dim3 grid, unsigned threads, hipStream_t stream, const std::common_type_t<P>&... args) {
+    void* at[] = {(void*)&args...};
+    const hipError_t e = hipLaunchKernel((const void*)kernel, grid, dim3(threads), at, 0, stream);
+    if (e != hipSuccess) throw Error(strf("%s: the launch failed: %s", op, hipGetErrorString(e)));
 }
 
 inline int type_bytes(int type) { return type == ADHIP_BF16 ? 2 : type == ADHIP_E4M3 ? 1 : 4; }

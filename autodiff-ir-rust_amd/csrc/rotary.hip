@@ -106,9 +106,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
 }
 
 template <class T, int V>
-void launch_rotary(const RotaryParams& p, bool interleaved, dim3 grid, hipStream_t stream) {
-    if (interleaved) rotary_kernel<T, V, true><<<grid, 256, 0, stream>>>(p);
-    else rotary_kernel<T, V, false><<<grid, 256, 0, stream>>>(p);
+void launch_rotary(const char* op, const RotaryParams& p, bool interleaved, dim3 grid, hipStream_t stream) {
+    launch(op, interleaved ? rotary_kernel<T, V, true> : rotary_kernel<T, V, false>, grid, 256, stream, p);
 }
 
 void rotary(const adhip_rotary_args& g, hipStream_t stream) {
@@ -183,16 +182,15 @@ void rotary(const adhip_rotary_args& g, hipStream_t stream) {
     ADHIP_CHECK(grid.y < 65536, "%s: heads of %lld x %lld features are too many for one call", op, (long long)heads, (long long)size);
     const bool il = g.interleaved != 0;
     if (type == ADHIP_BF16) {
-        if (v == 8) launch_rotary<bf16, 8>(p, il, grid, stream);
-        else if (v == 4) launch_rotary<bf16, 4>(p, il, grid, stream);
-        else if (v == 2) launch_rotary<bf16, 2>(p, il, grid, stream);
-        else launch_rotary<bf16, 1>(p, il, grid, stream);
+        if (v == 8) launch_rotary<bf16, 8>(op, p, il, grid, stream);
+        else if (v == 4) launch_rotary<bf16, 4>(op, p, il, grid, stream);
+        else if (v == 2) launch_rotary<bf16, 2>(op, p, il, grid, stream);
+        else launch_rotary<bf16, 1>(op, p, il, grid, stream);
     } else {
-        if (v == 4) launch_rotary<float, 4>(p, il, grid, stream);
-        else if (v == 2) launch_rotary<float, 2>(p, il, grid, stream);
-        else launch_rotary<float, 1>(p, il, grid, stream);
+        if (v == 4) launch_rotary<float, 4>(op, p, il, grid, stream);
+        else if (v == 2) launch_rotary<float, 2>(op, p, il, grid, stream);
+        else launch_rotary<float, 1>(op, p, il, grid, stream);
     }
-    check_launch(op);
 }
 
 }  // namespace

@@ -147,3 +147,24 @@ def test_attention_workspace_goes_by_shapes_alone(hip_device, backward):
         need = ops.attention_workspace(hip_device, q, k, k, backward=backward)
         q, k = Shape(*q.shape, dtype=q.dtype), Shape(*k.shape, dtype=k.dtype)
         assert ops.attention_workspace(hip_device, q, k, k, backward=backward) == need > 0
+
+
+def test_an_error_that_another_call_left_is_not_the_operators(hip_device):
+    """A failed call of the HIP runtime stands as its last error until it is asked for: the operators neither report nor take it."""
+    x = torch.randn((1, 3, 2, 8), device="cuda")
+    out, at = torch.empty_like(x), torch.zeros((1, 3), dtype=torch.int32, device="cuda")
+    cos, sin = (torch.from_numpy(t).cuda() for t in ops.rotary_table(8, 8))
+    lse, room = torch.empty((1, 3, 2), device="cuda"), torch.empty(ops.attention_workspace(hip_device, x, x, x, backward=True), dtype=torch.uint8, device="cuda")
+    grads, moments = [torch.empty_like(x) for _ in range(3)], [torch.zeros_like(x) for _ in range(2)]
+    torch.cuda.synchronize()
+    stream, runtime = here(), hip_device._lib
+    refused = runtime.hipSetDevice(1000)
+    try:
+        ops.rotary(hip_device, x, out, cos, sin, at, stream=stream)
+        ops.attention(hip_device, x, x, x, out, lse, workspace=room, stream=stream)
+        ops.attention_backward(hip_device, x, x, x, out, lse, out, *grads, workspace=room, stream=stream)
+        ops.adamw(hip_device, [x], [out], moments[:1], moments[1:], step=1, rate=0.1, stream=stream)
+    finally:
+        left = runtime.hipGetLastError()
+    assert refused != 0 and left == refused
+    torch.cuda.synchronize()
