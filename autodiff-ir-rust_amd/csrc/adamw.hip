@@ -27,6 +27,7 @@ constexpr int kTensors = 32;           // of a launch: their descriptors stay wi
 constexpr int kBlock = ADHIP_ADAMW_BLOCK;
 constexpr int kUnits = 4;              // blocks of 256 that a wavefront has under way
 constexpr int kChunk = 4 * kUnits * kBlock;  // elements of a workgroup (four wavefronts)
+constexpr uint64_t kBlocks = 0xffffffffu / 256;  // workgroups of a launch: it holds fewer than 2^32 threads
 
 struct AdamwLaunch {
     adhip_adamw_tensor t[kTensors];
@@ -225,7 +226,7 @@ void adamw(const adhip_adamw_args& g, hipStream_t stream) {
     for (int64_t i = 0; i < g.n_tensors; ++i) {
         const adhip_adamw_tensor& t = g.tensors[i];
         const long long at = (long long)i;
-        ADHIP_CHECK(t.count >= 0 && t.count < (int64_t(1) << 42), "%s: tensor %lld has %lld elements", op, at, (long long)t.count);
+        ADHIP_CHECK(t.count >= 0 && t.count <= (int64_t)kBlocks * kChunk, "%s: tensor %lld has %lld elements", op, at, (long long)t.count);
         if (t.count == 0) continue;
         ADHIP_CHECK(t.p && t.g && t.m && t.v && t.p_out && t.m_out && t.v_out, "%s: an array of tensor %lld is missing", op, at);
         ADHIP_CHECK(!eight || (t.m_scale && t.v_scale && t.m_scale_out && t.v_scale_out), "%s: a scale array of tensor %lld is missing", op, at);
@@ -258,7 +259,7 @@ void adamw(const adhip_adamw_args& g, hipStream_t stream) {
         const adhip_adamw_tensor& t = g.tensors[i];
         if (t.count == 0) continue;
         const uint64_t own = (uint64_t)((t.count + kChunk - 1) / kChunk);
-        if (a.n == kTensors || blocks + own > 0x7fffffffu) flush();
+        if (a.n == kTensors || blocks + own > kBlocks) flush();
         a.t[a.n] = t;
         a.first[a.n] = (unsigned)blocks;
         bool whole = aligned_to(t.p, 4 * pw) && aligned_to(t.p_out, 4 * pw) && aligned_to(t.g, 4 * gw);

@@ -228,10 +228,21 @@ void check_sizes(const char* op, const adhip_attention_args& g) {
     ADHIP_CHECK(Hk >= 1 && H >= 1 && H % Hk == 0, "%s: %lld heads cannot share %lld key heads", op, (long long)H, (long long)Hk);
     // positions and rows in 32 bits, with room for a window on either side
     constexpr int64_t kMost = int64_t(1) << 28;
-    ADHIP_CHECK(Lq <= kMost && Lk <= kMost && Lq * (H / Hk) <= kMost && B * H <= kMost, "%s: q %s and k %s are too large", op, array_str(g.q).c_str(),
+    ADHIP_CHECK(Lq <= kMost && Lk <= kMost && B <= kMost && H <= kMost && Lq * (H / Hk) <= kMost && B * H <= kMost, "%s: q %s and k %s are too large", op, array_str(g.q).c_str(),
                 array_str(g.k).c_str());
     ADHIP_CHECK(B * Hk * ((Lq * (H / Hk) + 31) / 32 + (Lk + 31) / 32) <= kMost, "%s: q %s and k %s are too large", op, array_str(g.q).c_str(),
                 array_str(g.k).c_str());
+}
+
+// Every kernel of a call fits a launch.
+void check_launches(const char* op, const adhip_attention_args& g, const Layout& y, bool backward) {
+    const int64_t B = g.q.dims[0], Lq = g.q.dims[1], H = g.q.dims[2], D = g.q.dims[3], Lk = g.k.dims[1], Hk = g.k.dims[2], R = Lq * (H / Hk);
+    bool fit;
+    if (!backward) fit = fits_launch(y.tiles * Hk * B * y.splits, y.row_tile == 256 ? 512 : 256);
+    else fit = fits_launch((R + 127) / 128 * Hk * B * y.dq_splits, 256) && fits_launch((Lk + 127) / 128 * Hk * B * y.dk_splits, 512);
+    if (y.parts) fit = fit && fits_launch(((backward ? std::max(Lq * H, Lk * Hk) : Lk * Hk) * B * (attn::parts_size((int)D) / 8) + 255) / 256, 256);
+    fit = fit && fits_launch(((Lq + 31) / 32 + (Lk + 31) / 32 + 7) / 8 * B, 256);  // documents
+    ADHIP_CHECK(fit, "%s: q %s and k %s are too large for one call", op, array_str(g.q).c_str(), array_str(g.k).c_str());
 }
 
 Params checked(const char* op, const adhip_attention_args& g, const Layout& y, bool backward) {
@@ -364,7 +375,9 @@ int adhip_attention_workspace(adhip_ctx* ctx, const adhip_attention_args* args, 
         const char* op = "adhip_attention_workspace";
         ADHIP_CHECK(args && bytes, "%s: no arguments", op);
         check_sizes(op, *args);
-        *bytes = layout_of(*args, backward != 0).bytes;
+        const Layout y = layout_of(*args, backward != 0);
+        check_launches(op, *args, y, backward != 0);
+        *bytes = y.bytes;
     });
 }
 
@@ -374,6 +387,7 @@ int adhip_attention(adhip_ctx* ctx, const adhip_attention_args* args, void* stre
         ADHIP_CHECK(args, "%s: no arguments", op);
         check_sizes(op, *args);
         const Layout y = layout_of(*args, false);
+        check_launches(op, *args, y, false);
         const Params p = checked(op, *args, y, false);
         if (p.R == 0 || p.B == 0) return;
         document_ranges(p, (hipStream_t)stream);
@@ -389,6 +403,7 @@ int adhip_attention_backward(adhip_ctx* ctx, const adhip_attention_args* args, v
         ADHIP_CHECK(args, "%s: no arguments", op);
         check_sizes(op, *args);
         const Layout y = layout_of(*args, true);
+        check_launches(op, *args, y, true);
         const Params p = checked(op, *args, y, true);
         if (p.B == 0) return;
         document_ranges(p, (hipStream_t)stream);

@@ -11,10 +11,15 @@
 
 namespace adhip {
 
+// What a launch holds: fewer than 2^32 threads in each dimension.  Of more, the runtime says nothing and the hardware sees the
+// remainder.
+inline bool fits_launch(int64_t blocks, unsigned threads) { return blocks <= (int64_t)(0xffffffffu / threads); }
+
 // Queues a kernel; an error is the launch's own, not one that another call of the process has left behind.
 template <class... P>
 void launch(const char* op, void (*kernel)(P...), dim3 grid, unsigned threads, hipStream_t stream, const std::common_type_t<P>&... args) {
     void* at[] = {(void*)&args...};
+    ADHIP_CHECK(fits_launch(grid.x, threads), "%s: %u blocks are too many for a launch", op, grid.x);
     const hipError_t e = hipLaunchKernel((const void*)kernel, grid, dim3(threads), at, 0, stream);
     if (e != hipSuccess) throw Error(strf("%s: the launch failed: %s", op, hipGetErrorString(e)));
 }

@@ -9,6 +9,8 @@
 // 8 + 8 heads of 80, half of them turned, in f32, 20 us with four heads and 8 with one.
 #include "operators.hpp"
 
+#include <algorithm>
+
 namespace adhip {
 namespace {
 
@@ -35,7 +37,7 @@ struct RotaryParams {
 
 template <class T, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
-    unsigned item = blockIdx.y * 256 + threadIdx.x, token = blockIdx.x;
+    unsigned item = blockIdx.y * 256 + threadIdx.x, token = blockIdx.z * gridDim.x + blockIdx.x;
     if (p.per_block > 1) {
         const unsigned t = item / p.items;
         if (t >= p.per_block) return;
@@ -178,7 +180,9 @@ void rotary(const adhip_rotary_args& g, hipStream_t stream) {
     p.items = p.turns + p.copied * (unsigned)(p.a[0].heads + p.a[1].heads);
     p.per_block = p.items < 256 ? 256 / p.items : 1;
     p.sign = g.inverse ? -1.f : 1.f;
-    const dim3 grid((unsigned)((tokens + p.per_block - 1) / p.per_block), (p.items + 255) / 256);
+    // 2^23 blocks in a row of the grid, so that it holds fewer than 2^32 threads
+    const int64_t across = (tokens + p.per_block - 1) / p.per_block;
+    const dim3 grid((unsigned)std::min<int64_t>(across, 1 << 23), (p.items + 255) / 256, (unsigned)((across + (1 << 23) - 1) >> 23));
     ADHIP_CHECK(grid.y < 65536, "%s: heads of %lld x %lld features are too many for one call", op, (long long)heads, (long long)size);
     const bool il = g.interleaved != 0;
     if (type == ADHIP_BF16) {

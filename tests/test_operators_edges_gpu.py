@@ -168,3 +168,31 @@ def test_an_error_that_another_call_left_is_not_the_operators(hip_device):
         left = runtime.hipGetLastError()
     assert refused != 0 and left == refused
     torch.cuda.synchronize()
+
+
+def test_attention_of_more_workgroups_than_a_launch_holds_is_refused(hip_device):
+    """2^24 workgroups of 256 threads: the number of threads would begin anew at 2^32."""
+    for sequences, queries, keys, backward, fits in [(2 ** 21 - 1, 1, 3, False, True), (2 ** 21, 1, 3, False, False), (2 ** 20 - 1, 1, 3, True, True),
+                                                     (2 ** 20, 1, 3, True, False), (2 ** 20, 1, 3, False, True)]:
+        q, k = Shape(sequences, queries, 8, 8, dtype="bfloat16"), Shape(sequences, keys, 8, 8, dtype="bfloat16")
+        if fits:
+            assert ops.attention_workspace(hip_device, q, k, k, backward=backward) > 0
+        else:
+            with pytest.raises(RuntimeError, match="too large for one call"):
+                ops.attention_workspace(hip_device, q, k, k, backward=backward)
+
+
+def test_rotary_of_more_tokens_than_a_row_of_a_launch_holds(hip_device):
+    """2^24 tokens of a block each, 129 heads of one pair: every one of them is turned."""
+    tokens = 2 ** 24 + 5
+    x = torch.randn((1, 1, 129, 2), device="cuda").to(torch.bfloat16).expand(1, tokens, 129, 2)
+    out = torch.zeros((1, tokens, 129, 2), dtype=torch.bfloat16, device="cuda")
+    cos, sin = (torch.from_numpy(t) for t in ops.rotary_table(8, 2))
+    at = torch.tensor([[3]], dtype=torch.int32)
+    ops.rotary(hip_device, x, out, cos.cuda(), sin.cuda(), at.cuda().expand(1, tokens), stream=here())
+    want, bound = oracle.rotary(x[:, :1].cpu(), cos, sin, at, False, False)
+    assert_within(out[:, :1], want, bound + W["bf16"] * want.abs(), "the first token")
+    for i in range(0, tokens, 2 ** 20):
+        assert (out[:, i:i + 2 ** 20] == out[:, :1]).all(), f"from token {i}"
+    del out
+    torch.cuda.empty_cache()
