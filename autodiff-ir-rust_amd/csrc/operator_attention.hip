@@ -242,6 +242,8 @@ void check_launches(const char* op, const adhip_attention_args& g, const Layout&
     else fit = fits_launch((R + 127) / 128 * Hk * B * y.dq_splits, 256) && fits_launch((Lk + 127) / 128 * Hk * B * y.dk_splits, 512);
     if (y.parts) fit = fit && fits_launch(((backward ? std::max(Lq * H, Lk * Hk) : Lk * Hk) * B * (attn::parts_size((int)D) / 8) + 255) / 256, 256);
     fit = fit && fits_launch(((Lq + 31) / 32 + (Lk + 31) / 32 + 7) / 8 * B, 256);  // documents
+    // (a tile of planes has 32 rows, whose offsets are to fit 31 bits, as those of the arrays' own tiles do)
+    if (y.parts) fit = fit && (backward ? H : Hk) * attn::parts_size((int)D) <= (int64_t(1) << 25);
     ADHIP_CHECK(fit, "%s: q %s and k %s are too large for one call", op, array_str(g.q).c_str(), array_str(g.k).c_str());
 }
 

@@ -196,3 +196,17 @@ def test_rotary_of_more_tokens_than_a_row_of_a_launch_holds(hip_device):
         assert (out[:, i:i + 2 ** 20] == out[:, :1]).all(), f"from token {i}"
     del out
     torch.cuda.empty_cache()
+
+
+def test_attention_in_f32_of_heads_that_pass_the_offsets_of_a_tile_is_refused(hip_device):
+    """f32 in parts: 32 rows of 2^25 features and more reach 2^31 bytes from a tile's first, where its loads end."""
+    for heads, shared, backward, fits in [(2 ** 18, 2 ** 18, False, True), (300_000, 300_000, False, False), (300_000, 300_000, True, False),
+                                          (300_000, 100_000, False, True), (300_000, 100_000, True, False)]:
+        q, k = Shape(1, 40, heads, 128), Shape(1, 3, shared, 128)
+        if fits:
+            assert ops.attention_workspace(hip_device, q, k, k, backward=backward) > 0
+        else:
+            with pytest.raises(RuntimeError, match="too large for one call"):
+                ops.attention_workspace(hip_device, q, k, k, backward=backward)
+    q, k = (Shape(1, n, 300_000, 128, dtype="bfloat16") for n in (40, 3))
+    assert ops.attention_workspace(hip_device, q, k, k) > 0
