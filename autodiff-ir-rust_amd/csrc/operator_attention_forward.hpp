@@ -328,12 +328,28 @@ __global__ __launch_bounds__(256) void join_few_kernel(const Params p) {
 // Joins more of them.  A row takes `pieces` threads of four features for each of `groups` runs of ranges, which are
 // added up in LDS: with one wavefront a row that walked its ranges one after the other, the join of 64 ranges took longer
 // than the attention before it.
+struct JoinShape {
+    int pieces, groups, rows;  // rows of a workgroup
+    JoinShape(int D, int splits) : pieces((D + 3) / 4), groups(1) {
+        // as many runs as ranges leave four each for, and threads allow
+        while (groups * 8 <= splits && pieces * groups * 2 <= 256) groups *= 2;
+        rows = std::min(256 / (pieces * groups), 2048 / splits);
+    }
+};
+struct JoinPlace {
+    int row, group, d;
+    bool mine;  // (some threads behind the last row are left over)
+    __host__ __device__ JoinPlace(const JoinShape& j, int rows, int tid)
+        : row(tid / (j.pieces * j.groups)), group(tid / j.pieces - row * j.groups), d((tid % j.pieces) * 4), mine(row < rows) {}
+    // the thread that adds up its own sum and those of the groups behind it, every `pieces` threads
+    __host__ __device__ bool adds() const { return mine && group == 0; }
+};
 template <class T>
-__global__ __launch_bounds__(256) void join_kernel(const Params p, int pieces, int groups, int rows_each) {
+__global__ __launch_bounds__(256) void join_kernel(const Params p, const JoinShape j) {
     __shared__ float ml[2 * 2048];
     __shared__ f32x4 sums[256];
-    const int64_t rows = (int64_t)p.B * p.Hk * p.R, row0 = (int64_t)blockIdx.x * rows_each;
-    const int tid = threadIdx.x, here_rows = (int)min((int64_t)rows_each, rows - row0);
+    const int64_t rows = (int64_t)p.B * p.Hk * p.R, row0 = (int64_t)blockIdx.x * j.rows;
+    const int tid = threadIdx.x, here_rows = (int)min((int64_t)j.rows, rows - row0);
     for (int i = tid; i < here_rows * p.splits; i += 256) {
         const int r = i / p.splits, s = i - r * p.splits;
         const float2 x = *(const float2*)(p.part_ml + (s * rows + row0 + r) * 2);
@@ -341,12 +357,12 @@ __global__ __launch_bounds__(256) void join_kernel(const Params p, int pieces, i
         ml[2 * i + 1] = x.y;
     }
     __syncthreads();
-    const int r = tid / (pieces * groups), in_row = tid - r * pieces * groups, g = in_row / pieces, d = (in_row - g * pieces) * 4;
-    const bool mine = r < here_rows;
+    const JoinPlace place(j, here_rows, tid);
+    const int r = place.row, d = place.d;
     const int64_t at = row0 + r;
     float m = -__builtin_inff(), sum = 0.f;
     f32x4 f = {0.f, 0.f, 0.f, 0.f};
-    if (mine) {
+    if (place.mine) {
         const float* of = ml + 2 * r * p.splits;
 #pragma unroll 4
         for (int s = 0; s < p.splits; ++s) m = fmaxf(m, of[2 * s]);
@@ -355,7 +371,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Params p, int pieces, i
         for (int s = 0; s < p.splits; ++s) sum += of[2 * s + 1] * __builtin_amdgcn_exp2f(of[2 * s] - base);
         const bool vec = (p.D & 3) == 0;
 #pragma unroll 4
-        for (int s = g; s < p.splits; s += groups) {
+        for (int s = place.group; s < p.splits; s += j.groups) {
             const float w = __builtin_amdgcn_exp2f(of[2 * s] - base);
             const float* x = p.part + (s * rows + at) * p.D + d;
             if (vec) {
@@ -368,17 +384,17 @@ __global__ __launch_bounds__(256) void join_kernel(const Params p, int pieces, i
             }
         }
     }
-    if (groups > 1) {
+    if (j.groups > 1) {
         sums[tid] = f;
         __syncthreads();
-        if (g > 0) return;
-        for (int i = 1; i < groups; ++i) {
-            const f32x4 y = sums[tid + i * pieces];
+        if (!place.adds()) return;
+        for (int i = 1; i < j.groups; ++i) {
+            const f32x4 y = sums[tid + i * j.pieces];
 #pragma unroll
             for (int e = 0; e < 4; ++e) f[e] += y[e];
         }
     }
-    if (!mine) return;
+    if (!place.mine) return;
     const int64_t bc = at / p.R;
     const int row = (int)(at - bc * p.R), c = (int)(bc % p.Hk), token = row / p.G, head = c * p.G + row - token * p.G;
     const int64_t b = bc / p.Hk;
@@ -396,12 +412,8 @@ void launch_join(const Params& p, hipStream_t stream) {
         launch("adhip_attention", join_few_kernel<T>, (unsigned)(((int64_t)p.B * p.Hk * p.R * pieces + 255) / 256), 256, stream, p);
         return;
     }
-    // as many runs as ranges leave four each for, and threads allow
-    int groups = 1;
-    while (groups * 8 <= p.splits && pieces * groups * 2 <= 256) groups *= 2;
-    const int rows_each = std::min(256 / (pieces * groups), 2048 / p.splits);
-    launch("adhip_attention", join_kernel<T>, (unsigned)(((int64_t)p.B * p.Hk * p.R + rows_each - 1) / rows_each), 256, stream, p, pieces, groups,
-           rows_each);
+    const JoinShape j(p.D, p.splits);
+    launch("adhip_attention", join_kernel<T>, (unsigned)(((int64_t)p.B * p.Hk * p.R + j.rows - 1) / j.rows), 256, stream, p, j);
 }
 
 // Bytes of a row of a tile decide how many keys a tile has and how many tiles LDS holds: 64 keys where tiles leave room for

@@ -70,3 +70,42 @@ def test_loads_to_lds_wait_for_their_descriptors(instructions):
                 at -= 1
     assert loads > 1000, "the kernels of attention bring their tiles to LDS this way"
     assert not early, f"{len(early)} loads of {loads} read a descriptor too early, the first: {early[0]}"
+
+
+def test_the_join_of_ranges_stays_within_its_sums(tmp_path):
+    """Every thread of the joining kernel that adds up reads sums of its own row, and none behind the last thread's, for every
+    width and number of ranges.  The kernel's own indices, run on the host."""
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    if not os.path.exists(hipcc):
+        pytest.skip("no hipcc to build the indices with")
+    src = tmp_path / "join.hip"
+    src.write_text('''#include <cstdio>
+#include "operator_attention_forward.hpp"
+using namespace adhip::attn;
+int main() {
+    long outside = 0, foreign = 0, left_over = 0;
+    for (int D = 1; D <= 256; ++D)
+        for (int splits = kFewRanges + 1; splits <= 256; ++splits) {
+            const JoinShape j(D, splits);
+            if (j.rows < 1 || j.rows * splits > 2048 || j.rows * j.pieces * j.groups > 256) return 1;
+            for (int rows = 1; rows <= j.rows; rows += j.rows > 1 ? j.rows - 1 : 1)
+                for (int tid = 0; tid < 256; ++tid) {
+                    const JoinPlace place(j, rows, tid);
+                    left_over += place.row >= j.rows;
+                    if (!place.adds()) continue;
+                    for (int i = 1; i < j.groups; ++i) {
+                        const JoinPlace other(j, rows, tid + i * j.pieces);
+                        outside += tid + i * j.pieces >= 256;
+                        foreign += other.row != place.row || other.group != i || other.d != place.d;
+                    }
+                }
+        }
+    printf("%ld %ld %d\\n", outside, foreign, left_over > 0);
+    return 0;
+}''')
+    csrc = os.path.dirname(library_path())
+    exe = tmp_path / "join"
+    subprocess.run([hipcc, "--offload-arch=gfx950", "-std=c++17", "-O1", "--cuda-host-only", "-I", csrc, str(src), "-o", str(exe)], check=True,
+                   capture_output=True)
+    done = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert (done.returncode, done.stdout.split()) == (0, ["0", "0", "1"])
