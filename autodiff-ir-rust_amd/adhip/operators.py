@@ -4,7 +4,8 @@ are behind the C ABI (`adhip_rotary`, `adhip_attention`, `adhip_attention_backwa
 where the formulas stand); they have no counterpart in the reference.
 
 An array is a `DeviceArray` (`DeviceArray.empty`, `DeviceArray.of`, `program_array`) or anything on the device's memory with
-`data_ptr()`, `shape`, `stride()` and `dtype` (for AdamW also `numel()` and `is_contiguous()`), such as a torch tensor.  Every call queues its kernels on `stream`
+`data_ptr()`, `shape`, `stride()` and `dtype` (for AdamW also `numel()` and `is_contiguous()`), such as a torch tensor; one that says by
+`is_cuda` that it is elsewhere is refused.  Every call queues its kernels on `stream`
 (a hipStream_t as an integer, for instance `torch.cuda.current_stream().cuda_stream`; the device's own stream where it is
 not given) and returns: results are there when the stream has got to them, and arrays and workspaces must live and keep
 still until then.  Nothing is allocated and nothing is kept between calls.
@@ -14,6 +15,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+from array import array
 from typing import List, Optional, Sequence
 
 import numpy as np
@@ -27,6 +29,8 @@ ADAMW_BLOCK = 256  # elements that share a scale where states are held in 8 bits
 
 class DeviceArray:
     """Packed device memory of a `HipDevice`; freed with the object where the object allocated it."""
+
+    is_cuda = True  # what torch calls memory of a GPU
 
     def __init__(self, dev, shape: Sequence[int], dtype: str = "float32", data: Optional[int] = None, owner=None):
         if dtype not in _TYPES:
@@ -139,6 +143,8 @@ _PADS = [(0,) * (4 - n) for n in range(5)]
 _ROTARY_TAIL = struct.Struct("=ii")
 _ATTENTION_TAIL = struct.Struct("=ffiiqQQ")
 _ADAMW = struct.Struct("=Qqiiii6d")
+_SIZE = struct.Struct("=q").unpack_from
+_NO_GRADIENTS = _NONE * 4
 _NO_MORE = _NONE * 11 + bytes(_ATTENTION_TAIL.size)
 
 
@@ -155,9 +161,14 @@ def _kind(dtype) -> int:
     return kind
 
 
-def _array(a) -> bytes:
+def _array(a, shape_alone: bool = False) -> bytes:
     if a is None:
         return _NONE
+    try:
+        if not (a.is_cuda or shape_alone):
+            raise ValueError(f"an array of shape {list(a.shape)} is not in device memory")
+    except AttributeError:  # an array that does not say
+        pass
     shape = a.shape
     n = len(shape)
     kind = _kinds.get(a.dtype)
@@ -247,34 +258,35 @@ def rotary(dev, x, out, cos, sin, positions, *, second=None, second_out=None, in
     """Turns the feature pairs of x [batch, length, heads, size] by the angles of `positions` [batch, length] into out
     (x itself is allowed); `second` [batch, length, other heads, size] by the same angles in the same launch.  cos and sin
     are tables [rows, pairs]; features behind 2 pairs are copied.  `inverse` is the gradient's rule."""
-    args = (_array(x) + _array(out) + _array(second) + _array(second_out) + _array(cos) + _array(sin) + _array(positions)
-            + _ROTARY_TAIL.pack(bool(interleaved), bool(inverse)))
+    args = b"".join((_array(x), _array(out), _array(second), _array(second_out), _array(cos), _array(sin), _array(positions),
+                     _ROTARY_TAIL.pack(bool(interleaved), bool(inverse))))
     _check(dev, _lib(dev).adhip_rotary(dev._ctx, args, _stream(dev, stream)), "adhip_rotary")
 
 
 # ---- attention ------------------------------------------------------------------------------------------------------
 
 
-def _attention_args(q, k, v, out=None, lse=None, out_grad=None, q_grad=None, k_grad=None, v_grad=None, scale=None, causal=False,
-                    window=0, cap=0.0, slopes=None, lengths=None, prefix=None, query_documents=None, key_documents=None,
-                    workspace=None) -> bytes:
+def _attention_tail(q: bytes, scale, causal, window, cap, workspace) -> bytes:
     if scale is None:
-        scale = 1.0 / math.sqrt(max(1, q.shape[-1]))
+        scale = 1.0 / math.sqrt(max(1, _SIZE(q, 40)[0]))  # (the last extent of four)
     room, room_bytes = 0, 0
     if workspace is not None:
+        if not getattr(workspace, "is_cuda", True):
+            raise ValueError("the workspace is not in device memory")
         room, room_bytes = workspace.data_ptr(), workspace.nbytes
-    return (_array(q) + _array(k) + _array(v) + _array(out) + _array(lse)
-            + (_NONE * 5 if slopes is lengths is prefix is query_documents is key_documents is None else
-               b"".join([_array(a) for a in (slopes, lengths, prefix, query_documents, key_documents)]))
-            + (_NONE * 4 if out_grad is q_grad is k_grad is v_grad is None else
-               b"".join([_array(a) for a in (out_grad, q_grad, k_grad, v_grad)]))
-            + _ATTENTION_TAIL.pack(scale, cap, bool(causal), 0, window, room, room_bytes))
+    return _ATTENTION_TAIL.pack(scale, cap, bool(causal), 0, window, room, room_bytes)
+
+
+def _masks(slopes, lengths, prefix, query_documents, key_documents) -> bytes:
+    if slopes is lengths is prefix is query_documents is key_documents is None:
+        return _NONE * 5
+    return b"".join([_array(a) for a in (slopes, lengths, prefix, query_documents, key_documents)])
 
 
 def attention_workspace(dev, q, k, v, *, backward: bool = False) -> int:
     """Bytes of workspace that `attention`, and with `backward` also `attention_backward`, take on arrays of these shapes."""
     need = ctypes.c_size_t()
-    args = _array(q) + _array(k) + _array(v) + _NO_MORE
+    args = _array(q, True) + _array(k, True) + _array(v, True) + _NO_MORE
     _check(dev, _lib(dev).adhip_attention_workspace(dev._ctx, args, bool(backward), ctypes.byref(need)), "adhip_attention_workspace")
     return need.value
 
@@ -287,8 +299,9 @@ def attention(dev, q, k, v, out, lse, *, scale: Optional[float] = None, causal: 
     q, out [batch, queries, heads, size]; k, v [batch, keys, key heads, size]; lse f32 [batch, queries, heads].  Scores are
     cap tanh(scale q.k / cap) - slopes[head] |distance|; what a query sees is said by causal, window, lengths [batch],
     prefix [batch] and documents [batch, queries] / [batch, keys].  scale is 1 / sqrt(size) where it is not given."""
-    args = _attention_args(q, k, v, out, lse, None, None, None, None, scale, causal, window, cap, slopes, lengths, prefix,
-                           query_documents, key_documents, workspace)
+    first = _array(q)
+    args = b"".join((first, _array(k), _array(v), _array(out), _array(lse), _masks(slopes, lengths, prefix, query_documents, key_documents),
+                     _NO_GRADIENTS, _attention_tail(first, scale, causal, window, cap, workspace)))
     _check(dev, _lib(dev).adhip_attention(dev._ctx, args, _stream(dev, stream)), "adhip_attention")
 
 
@@ -296,8 +309,10 @@ def attention_backward(dev, q, k, v, out, lse, out_grad, q_grad, k_grad, v_grad,
                        causal: bool = False, window: int = 0, cap: float = 0.0, slopes=None, lengths=None, prefix=None,
                        query_documents=None, key_documents=None, workspace=None, stream: Optional[int] = None) -> None:
     """Gradients of q, k and v from `attention`'s out and lse and the gradient of out; the other arguments as there."""
-    args = _attention_args(q, k, v, out, lse, out_grad, q_grad, k_grad, v_grad, scale, causal, window, cap, slopes, lengths, prefix,
-                           query_documents, key_documents, workspace)
+    first = _array(q)
+    args = b"".join((first, _array(k), _array(v), _array(out), _array(lse), _masks(slopes, lengths, prefix, query_documents, key_documents),
+                     _array(out_grad), _array(q_grad), _array(k_grad), _array(v_grad),
+                     _attention_tail(first, scale, causal, window, cap, workspace)))
     _check(dev, _lib(dev).adhip_attention_backward(dev._ctx, args, _stream(dev, stream)), "adhip_attention_backward")
 
 
@@ -305,7 +320,10 @@ def attention_backward(dev, q, k, v, out, lse, out_grad, q_grad, k_grad, v_grad,
 
 
 def _one_kind(name, arrays, allowed) -> int:
-    kinds = {_kind(t) for t in {a.dtype for a in arrays}}
+    kinds = {a.dtype for a in arrays}
+    if len(kinds) == 1 and _kinds.get(*kinds) in allowed:
+        return _kinds[kinds.pop()]
+    kinds = {_kind(t) for t in kinds}
     if len(kinds) != 1 or not kinds <= allowed:
         raise ValueError(f"{name} must all have one supported type, not {sorted({str(a.dtype) for a in arrays})}")
     return kinds.pop()
@@ -313,11 +331,18 @@ def _one_kind(name, arrays, allowed) -> int:
 
 def _addresses(name, arrays, counts) -> List[int]:
     """Where the packed arrays begin, of these numbers of elements."""
-    if [a.numel() for a in arrays] != counts or not all([a.is_contiguous() for a in arrays]):
-        if len(arrays) != len(counts):
-            raise ValueError(f"{len(arrays)} {name} for {len(counts)} parameters")
-        i = next(i for i, (a, n) in enumerate(zip(arrays, counts)) if a.numel() != n or not a.is_contiguous())
-        raise ValueError(f"{name}[{i}] is {list(arrays[i].shape)}: {counts[i]} packed elements are wanted")
+    if len(arrays) != len(counts):
+        raise ValueError(f"{len(arrays)} {name} for {len(counts)} parameters")
+    try:
+        if all([a.is_cuda and a.is_contiguous() and a.numel() == n for a, n in zip(arrays, counts)]):
+            return [a.data_ptr() for a in arrays]
+    except AttributeError:  # arrays that do not say where they are
+        pass
+    for i, (a, n) in enumerate(zip(arrays, counts)):
+        if a.numel() != n or not a.is_contiguous():
+            raise ValueError(f"{name}[{i}] is {list(a.shape)}: {n} packed elements are wanted")
+        if not getattr(a, "is_cuda", True):
+            raise ValueError(f"{name}[{i}] is not in device memory")
     return [a.data_ptr() for a in arrays]
 
 
@@ -357,9 +382,8 @@ def adamw(dev, parameters: List, gradients: List, first: List, second: List, *, 
             own = _addresses(name, arrays, size)
         outs.append(own)
     flat = [x for row in zip(*columns, *scales, *outs, counts) for x in row]
-    tensors = struct.pack(f"={12 * n}q", *flat)
-    held_bytes = ctypes.c_char_p(tensors)
-    args = _ADAMW.pack(ctypes.cast(held_bytes, ctypes.c_void_p).value, n, p_type, g_type, state, step, rate, beta1, beta2, eps, decay, grad_scale)
+    tensors = array("q", flat)  # n of the C struct; read before the call returns
+    args = _ADAMW.pack(tensors.buffer_info()[0], n, p_type, g_type, state, step, rate, beta1, beta2, eps, decay, grad_scale)
     _check(dev, _lib(dev).adhip_adamw(dev._ctx, args, _stream(dev, stream)), "adhip_adamw")
 
 
