@@ -27,6 +27,15 @@ _WIDTH = {F32: 4, BF16: 2, I32: 4, E4M3: 1}
 ADAMW_BLOCK = 256  # elements that share a scale where states are held in 8 bits
 
 
+def _host_values(values, dtype: str) -> np.ndarray:
+    """Packed float32 or int32; whole numbers are not cut off to 32 bits."""
+    values = np.ascontiguousarray(values)
+    out = values.astype(dtype, copy=False)
+    if dtype == "int32" and not np.array_equal(out, values):
+        raise ValueError("values that are no whole numbers of 32 bits")
+    return out
+
+
 class DeviceArray:
     """Packed device memory of a `HipDevice`; freed with the object where the object allocated it."""
 
@@ -50,8 +59,8 @@ class DeviceArray:
     @classmethod
     def of(cls, dev, values) -> "DeviceArray":
         """A copy of host values: float32 or int32."""
-        values = np.ascontiguousarray(values)
-        values = values.astype(np.int32 if values.dtype.kind in "iub" else np.float32, copy=False)
+        values = np.asarray(values)
+        values = _host_values(values, "int32" if values.dtype.kind in "iub" else "float32")
         a = cls(dev, values.shape, str(values.dtype))
         a.set(values)
         return a
@@ -87,7 +96,7 @@ class DeviceArray:
         """Copies host values in (waits)."""
         if self.dtype not in ("float32", "int32"):
             raise ValueError(f"host values of type {self.dtype} are not supported")
-        values = np.ascontiguousarray(values, dtype=self.dtype)
+        values = _host_values(values, self.dtype)
         if values.size != math.prod(self.shape):
             raise ValueError(f"{values.size} values for {list(self.shape)}")
         _check(self._dev, _lib(self._dev).adhip_copy_in(self._dev._ctx, self._data, values.ctypes.data, values.nbytes), "adhip_copy_in")

@@ -1,4 +1,5 @@
 """What the Python side of the operators on device arrays decides before it calls the library (no GPU)."""
+import numpy as np
 import pytest
 import torch
 
@@ -65,3 +66,18 @@ def test_host_tensors_are_refused():
         scales = [[one] if i == bad else [Elsewhere(1)] for i in range(4)]
         refused(ops.adamw, [Elsewhere(1)], [Elsewhere(1)], states, states, first_scales=scales[0], second_scales=scales[1],
                 first_scales_out=scales[2], second_scales_out=scales[3], **how)
+
+
+def test_whole_numbers_keep_their_value():
+    """Numbers of documents are often hashes of 64 bits: cut off to 32 they would meet others, or belong to none."""
+    for values in ([2 ** 31], [-2 ** 31 - 1], [0, 2 ** 40]):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.DeviceArray.of(None, np.array(values))
+    ends = [-2 ** 31, 0, 2 ** 31 - 1]
+    kept = ops._host_values(np.array([ends, ends]).T, "int32")
+    assert kept.dtype == np.int32 and kept.flags.c_contiguous and kept.tolist() == np.array([ends, ends]).T.tolist()
+    assert ops._host_values(np.array([True, False]), "int32").tolist() == [1, 0]
+    assert ops._host_values(7, "int32").tolist() == [7]
+    for values in ([0.5], [2 ** 40]):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops._host_values(values, "int32")
