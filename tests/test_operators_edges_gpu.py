@@ -210,3 +210,25 @@ def test_attention_in_f32_of_heads_that_pass_the_offsets_of_a_tile_is_refused(hi
                 ops.attention_workspace(hip_device, q, k, k, backward=backward)
     q, k = (Shape(1, n, 300_000, 128, dtype="bfloat16") for n in (40, 3))
     assert ops.attention_workspace(hip_device, q, k, k) > 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,queries,keys,heads,shared,size,how", [
+    (1, 1, 9000, 2, 1, 33, dict(causal=True)),
+    (2, 1, 7001, 3, 1, 61, dict(causal=True, lengths=[7001, 12])),
+    (3, 2, 6000, 4, 2, 128, dict(causal=True, cap=8.0, lengths=[0, 6000, 3111])),
+    (1, 4, 5003, 8, 1, 256, dict(causal=True, slopes=True)),
+    (1, 3, 8000, 2, 2, 200, dict(causal=True, window=5000, prefix=[100])),
+    (2, 1, 12000, 1, 1, 64, dict(causal=True, documents=True)),
+])
+def test_attention_of_tokens_over_many_ranges(hip_device, batch, queries, keys, heads, shared, size, how, dtype):
+    """Caches long enough that the keys of a token are split into more ranges than one thread joins."""
+    how = dict(how)
+    a = inputs(dtype, batch, queries, keys, heads, shared, size, seed=keys)
+    if how.pop("slopes", False):
+        how["slopes"] = torch.tensor([2.0 ** -(h + 5) for h in range(heads)])
+    if how.pop("documents", False):
+        d = documents(batch, keys, 0.0003, 0)
+        how |= dict(key_documents=d, query_documents=d[:, keys - queries:].contiguous())
+    how = {x: torch.tensor(y, dtype=torch.int32) if isinstance(y, list) else y for x, y in how.items()}
+    check(hip_device, a, dtype, f"{queries} x {keys} x {size}, {list(how)}", **how)
