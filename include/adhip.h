@@ -125,8 +125,8 @@ int adhip_compile_check(const uint8_t* program, size_t program_len, const char* 
  * program (adhip_program_buffer), arrays from adhip_alloc, or any other HIP allocation on the context's device -- and
  * queue their kernels on `stream` (a hipStream_t; NULL is HIP's default stream, adhip_stream(ctx) the context's own):
  * they allocate nothing, keep nothing and do not wait, so they may be captured into a graph.  Arguments are checked
- * before anything is queued; what a kernel cannot check (addresses) is the caller's.  Outputs must not overlap inputs
- * except where it is said. */
+ * before anything is queued, sizes that a launch does not hold (2^32 threads) among them; what a kernel cannot check
+ * (addresses) is the caller's.  Outputs must not overlap inputs except where it is said. */
 
 enum { ADHIP_F32 = 0, ADHIP_BF16 = 1, ADHIP_I32 = 2, ADHIP_E4M3 = 3 };
 
@@ -208,12 +208,13 @@ int adhip_adamw(adhip_ctx* ctx, const adhip_adamw_args* args, void* stream);
  * beginning of the first query's window (keys up to its position - window) are not used, whatever they hold.  All others must be finite, also
  * those that no query sees for another reason (the documents of a call's queries, for instance): a tile is multiplied as a
  * whole, and a probability of zero times an infinity is NaN.  (In f32 an infinity that is seen gives NaN as well.)
- * lengths (int32 [batch]; default: keys) is clamped to 0 .. keys.  documents may lie at most 2^20 elements apart.
+ * lengths (int32 [batch]; default: keys) is clamped to 0 .. keys.  documents may lie at most 2^20 elements apart, and in f32
+ * a position has at most 2^25 features over all heads.
  * workspace: device memory of at least adhip_attention_workspace() bytes, aligned to 256, used until the call's kernels
  * are done. */
 typedef struct adhip_attention_args {
     adhip_array q, k, v, out, lse;
-    adhip_array slopes, lengths, prefix, query_documents, key_documents; /* slopes f32 [heads], the others int32 */
+    adhip_array slopes, lengths, prefix, query_documents, key_documents; /* slopes f32 [heads], of either sign, the others int32 */
     /* backward only: gradient of out, gradients of q, k and v (of the arrays' own shapes and type) */
     adhip_array out_grad, q_grad, k_grad, v_grad;
     float scale, cap;
@@ -222,7 +223,8 @@ typedef struct adhip_attention_args {
     void* workspace;
     size_t workspace_bytes;
 } adhip_attention_args;
-/* What a call on arrays of these shapes needs: only the shapes and types of q, k and v are looked at. */
+/* What a call on arrays of these shapes needs: only the shapes and types of q, k and v are looked at, which need not be
+ * there yet. */
 int adhip_attention_workspace(adhip_ctx* ctx, const adhip_attention_args* args, int backward, size_t* bytes);
 int adhip_attention(adhip_ctx* ctx, const adhip_attention_args* args, void* stream);
 /* Gradients of q, k and v from what adhip_attention gave (out, lse) and the gradient of out.  The order of additions
