@@ -1,10 +1,12 @@
 """Operators on device arrays: rotary positions, attention with masks, capped scores, distance bias and shared heads
-(forward, backward, single tokens against a cache), and AdamW over many tensors.  The kernels and the checks of arguments
-are behind the C ABI (`adhip_rotary`, `adhip_attention`, `adhip_attention_backward`, `adhip_adamw` in include/adhip.h,
-where the formulas stand); they have no counterpart in the reference.
+(forward, backward, single tokens against a cache), layer norm with its residual and its weights' gradients, a gated linear
+recurrence over positions (forward, backward, single tokens), the norm over all gradients with clipping, and AdamW over many
+tensors.  The kernels and the checks of arguments are behind the C ABI (`adhip_rotary`, `adhip_attention`, `adhip_layer_norm`,
+`adhip_recurrence`, `adhip_clip_gradients`, `adhip_adamw` and their companions in include/adhip.h, where the formulas stand);
+they have no counterpart in the reference.
 
 An array is a `DeviceArray` (`DeviceArray.empty`, `DeviceArray.of`, `program_array`) or anything on the device's memory with
-`data_ptr()`, `shape`, `stride()` and `dtype` (for AdamW also `numel()` and `is_contiguous()`), such as a torch tensor; one that says by
+`data_ptr()`, `shape`, `stride()` and `dtype` (for AdamW and gradients also `numel()` and `is_contiguous()`), such as a torch tensor; one that says by
 `is_cuda` that it is elsewhere is refused.  Every call queues its kernels on `stream`
 (a hipStream_t as an integer, for instance `torch.cuda.current_stream().cuda_stream`; the device's own stream where it is
 not given) and returns: results are there when the stream has got to them, and arrays and workspaces must live and keep
@@ -25,6 +27,7 @@ _TYPES = {"float32": F32, "torch.float32": F32, "bfloat16": BF16, "torch.bfloat1
           "float8_e4m3fn": E4M3, "torch.float8_e4m3fn": E4M3}
 _WIDTH = {F32: 4, BF16: 2, I32: 4, E4M3: 1}
 ADAMW_BLOCK = 256  # elements that share a scale where states are held in 8 bits
+RECURRENCE_BLOCK = 256  # positions between the states that a recurrence keeps for its backward pass
 
 
 def _host_values(values, dtype: str) -> np.ndarray:
@@ -152,9 +155,14 @@ _PADS = [(0,) * (4 - n) for n in range(5)]
 _ROTARY_TAIL = struct.Struct("=ii")
 _ATTENTION_TAIL = struct.Struct("=ffiiqQQ")
 _ADAMW = struct.Struct("=Qqiiii6d")
+_NORM_TAIL = struct.Struct("=dqQQ")
+_RECURRENCE_TAIL = struct.Struct("=qQQ")
+_GRADIENTS = struct.Struct("=QqddQQQQ")
 _SIZE = struct.Struct("=q").unpack_from
 _NO_GRADIENTS = _NONE * 4
 _NO_MORE = _NONE * 11 + bytes(_ATTENTION_TAIL.size)
+_NORM_X = _NONE * 11 + bytes(_NORM_TAIL.size)
+_RECURRENCE_X = _NONE * 12 + bytes(_RECURRENCE_TAIL.size)
 
 
 _kinds = {}  # type objects met so far -> our number of the type
@@ -202,11 +210,18 @@ def _declared(lib):
     lib.adhip_copy_out.argtypes = [vp, vp, vp, sz]
     lib.adhip_sync.argtypes = [vp]
     lib.adhip_program_buffer.argtypes = [vp, c.c_char_p, c.POINTER(vp), c.POINTER(c.POINTER(c.c_uint64)), c.POINTER(sz)]
-    lib.adhip_attention_workspace.argtypes = [vp, c.c_char_p, i32, c.POINTER(sz)]
-    for name in ("adhip_rotary", "adhip_attention", "adhip_attention_backward", "adhip_adamw"):
+    calls = ("adhip_rotary", "adhip_attention", "adhip_attention_backward", "adhip_adamw", "adhip_layer_norm", "adhip_layer_norm_backward",
+             "adhip_recurrence", "adhip_recurrence_backward", "adhip_gradient_norm", "adhip_clip_gradients")
+    for name in ("adhip_attention_workspace", "adhip_recurrence_workspace"):
+        getattr(lib, name).argtypes = [vp, c.c_char_p, i32, c.POINTER(sz)]
+    for name in ("adhip_layer_norm_workspace", "adhip_gradient_norm_workspace"):
+        getattr(lib, name).argtypes = [vp, c.c_char_p, c.POINTER(sz)]
+    for name in calls:
         getattr(lib, name).argtypes = [vp, c.c_char_p, vp]
-    for name in ("adhip_alloc", "adhip_free", "adhip_copy_in", "adhip_copy_out", "adhip_sync", "adhip_program_buffer",
-                 "adhip_attention_workspace", "adhip_rotary", "adhip_attention", "adhip_attention_backward", "adhip_adamw"):
+    lib.adhip_adamw_scaled.argtypes = [vp, c.c_char_p, vp, vp]
+    for name in (*calls, "adhip_alloc", "adhip_free", "adhip_copy_in", "adhip_copy_out", "adhip_sync", "adhip_program_buffer",
+                 "adhip_attention_workspace", "adhip_recurrence_workspace", "adhip_layer_norm_workspace", "adhip_gradient_norm_workspace",
+                 "adhip_adamw_scaled"):
         getattr(lib, name).restype = i32
     lib.adhip_stream.argtypes = [vp]
     lib.adhip_stream.restype = vp
@@ -226,6 +241,26 @@ def _check(dev, rc: int, what: str) -> None:
 
 def _stream(dev, stream: Optional[int]) -> int:
     return _lib(dev).adhip_stream(dev._ctx) if stream is None else stream
+
+
+def _room(workspace):
+    """Address and bytes of a workspace."""
+    if workspace is None:
+        return 0, 0
+    if not getattr(workspace, "is_cuda", True):
+        raise ValueError("the workspace is not in device memory")
+    return workspace.data_ptr(), workspace.nbytes
+
+
+def _number(name, a) -> int:
+    """Where the one f32 number of an array is."""
+    if a is None:
+        return 0
+    if not getattr(a, "is_cuda", True):
+        raise ValueError(f"{name} is not in device memory")
+    if _kind(a.dtype) != F32 or math.prod(a.shape) != 1:
+        raise ValueError(f"{name} is {a.dtype} {list(a.shape)}: one f32 number is wanted")
+    return a.data_ptr()
 
 
 # ---- rotary positions -----------------------------------------------------------------------------------------------
@@ -278,12 +313,7 @@ def rotary(dev, x, out, cos, sin, positions, *, second=None, second_out=None, in
 def _attention_tail(q: bytes, scale, causal, window, cap, workspace) -> bytes:
     if scale is None:
         scale = 1.0 / math.sqrt(max(1, _SIZE(q, 40)[0]))  # (the last extent of four)
-    room, room_bytes = 0, 0
-    if workspace is not None:
-        if not getattr(workspace, "is_cuda", True):
-            raise ValueError("the workspace is not in device memory")
-        room, room_bytes = workspace.data_ptr(), workspace.nbytes
-    return _ATTENTION_TAIL.pack(scale, cap, bool(causal), 0, window, room, room_bytes)
+    return _ATTENTION_TAIL.pack(scale, cap, bool(causal), 0, window, *_room(workspace))
 
 
 def _masks(slopes, lengths, prefix, query_documents, key_documents) -> bytes:
@@ -359,13 +389,15 @@ def adamw(dev, parameters: List, gradients: List, first: List, second: List, *, 
           beta2: float = 0.999, eps: float = 1e-8, decay: float = 0.01, grad_scale: float = 1.0, first_scales: Optional[List] = None,
           second_scales: Optional[List] = None, parameters_out: Optional[List] = None, first_out: Optional[List] = None,
           second_out: Optional[List] = None, first_scales_out: Optional[List] = None, second_scales_out: Optional[List] = None,
-          stream: Optional[int] = None) -> None:
+          factor=None, stream: Optional[int] = None) -> None:
     """One AdamW step on every tensor of the list: parameters and gradients f32 or bf16, moments `first` and `second` f32 of
     the parameters' sizes, or float8_e4m3fn codes [blocks, 256] with f32 scales [blocks] (`adamw_blocks`).  In place where
-    no *_out list is given.  Arrays are packed."""
+    no *_out list is given.  Arrays are packed.  `factor` is one f32 number on the device that gradients are multiplied by beside
+    grad_scale, for instance where `gradient_norm` leaves it."""
     n = len(parameters)
     if n == 0:
         return
+    factor = _number("factor", factor)
     counts = [p.numel() for p in parameters]
     p_type = _one_kind("parameters", parameters, {F32, BF16})
     g_type = _one_kind("gradients", gradients, {F32, BF16})
@@ -393,9 +425,121 @@ def adamw(dev, parameters: List, gradients: List, first: List, second: List, *, 
     flat = [x for row in zip(*columns, *scales, *outs, counts) for x in row]
     tensors = array("q", flat)  # n of the C struct; read before the call returns
     args = _ADAMW.pack(tensors.buffer_info()[0], n, p_type, g_type, state, step, rate, beta1, beta2, eps, decay, grad_scale)
-    _check(dev, _lib(dev).adhip_adamw(dev._ctx, args, _stream(dev, stream)), "adhip_adamw")
+    if factor:
+        _check(dev, _lib(dev).adhip_adamw_scaled(dev._ctx, args, factor, _stream(dev, stream)), "adhip_adamw_scaled")
+    else:
+        _check(dev, _lib(dev).adhip_adamw(dev._ctx, args, _stream(dev, stream)), "adhip_adamw")
 
 
 def adamw_blocks(count: int) -> int:
     """Blocks of 256 elements, one scale each, that a tensor of `count` elements has where its states are held in 8 bits."""
     return -(-count // ADAMW_BLOCK)
+
+
+# ---- the norm over all gradients ------------------------------------------------------------------------------------
+
+
+def _gradients(gradients, outs, limit, grad_scale, norm, factor, room):
+    """The C struct, and the list that it points to (read before the call returns)."""
+    counts = [g.numel() for g in gradients]
+    at = _addresses("gradients", gradients, counts)
+    kinds = [_kind(g.dtype) for g in gradients]
+    if outs is None or outs is gradients:
+        to = at
+    else:
+        to = _addresses("gradients_out", outs, counts)
+        for i, (o, kind) in enumerate(zip(outs, kinds)):
+            if _kind(o.dtype) != kind:
+                raise ValueError(f"gradients_out[{i}] is {o.dtype}, the gradient's own type is wanted")
+    flat = array("q", [x for row in zip(at, to, counts, kinds) for x in row])
+    return _GRADIENTS.pack(flat.buffer_info()[0], len(at), limit, grad_scale, norm, factor, *room), flat
+
+
+def gradient_norm_workspace(dev, gradients: List) -> int:
+    """Bytes of workspace that `gradient_norm` and `clip_gradients` take on gradients of these sizes."""
+    need = ctypes.c_size_t()
+    flat = array("q", [x for g in gradients for x in (0, 0, g.numel(), _kind(g.dtype))])
+    args = _GRADIENTS.pack(flat.buffer_info()[0], len(gradients), 0.0, 0.0, 0, 0, 0, 0)
+    _check(dev, _lib(dev).adhip_gradient_norm_workspace(dev._ctx, args, ctypes.byref(need)), "adhip_gradient_norm_workspace")
+    return need.value
+
+
+def gradient_norm(dev, gradients: List, norm, *, limit: float = math.inf, factor=None, grad_scale: float = 1.0, workspace=None,
+                  stream: Optional[int] = None) -> None:
+    """norm = |grad_scale| sqrt(sum of all squares) over a list of packed f32 and bf16 gradients; factor = 1 where norm <= limit,
+    limit / norm otherwise (`adamw` takes it from there).  norm and factor are one f32 number each, on the device."""
+    args, keep = _gradients(gradients, None, limit, grad_scale, _number("norm", norm), _number("factor", factor), _room(workspace))
+    _check(dev, _lib(dev).adhip_gradient_norm(dev._ctx, args, _stream(dev, stream)), "adhip_gradient_norm")
+
+
+def clip_gradients(dev, gradients: List, norm, *, limit: float, gradients_out: Optional[List] = None, factor=None, grad_scale: float = 1.0,
+                   workspace=None, stream: Optional[int] = None) -> None:
+    """`gradient_norm`, and each gradient times grad_scale and the factor, in place where no gradients_out is given."""
+    args, keep = _gradients(gradients, gradients_out, limit, grad_scale, _number("norm", norm), _number("factor", factor), _room(workspace))
+    _check(dev, _lib(dev).adhip_clip_gradients(dev._ctx, args, _stream(dev, stream)), "adhip_clip_gradients")
+
+
+# ---- layer norm -----------------------------------------------------------------------------------------------------
+
+
+def layer_norm_workspace(dev, x) -> int:
+    """Bytes of workspace that `layer_norm_backward` takes for the weights' gradients on arrays of x's shape."""
+    need = ctypes.c_size_t()
+    _check(dev, _lib(dev).adhip_layer_norm_workspace(dev._ctx, _array(x, True) + _NORM_X, ctypes.byref(need)), "adhip_layer_norm_workspace")
+    return need.value
+
+
+def layer_norm(dev, x, out, *, weight=None, bias=None, eps: float = 1e-5, centered: bool = True, added=None, total=None, stats=None,
+               stream: Optional[int] = None) -> None:
+    """out = (t - mean) / sqrt(variance + eps) weight + bias along the last of x's 2 to 4 dims, with t = x, or total = x + added where
+    both are given; `stats` [..., 2] receives mean and 1 / sqrt(variance + eps) for the backward pass.  Without the mean
+    (centered = False) and a bias it is RMS norm."""
+    args = b"".join((_array(x), _array(added), _array(total), _array(out), _array(weight), _array(bias), _array(stats), _NONE * 5,
+                     _NORM_TAIL.pack(eps, bool(centered), 0, 0)))
+    _check(dev, _lib(dev).adhip_layer_norm(dev._ctx, args, _stream(dev, stream)), "adhip_layer_norm")
+
+
+def layer_norm_backward(dev, x, stats, out_grad, x_grad, *, weight=None, weight_grad=None, bias_grad=None, centered: bool = True,
+                        total_grad=None, workspace=None, stream: Optional[int] = None) -> None:
+    """Gradients from what `layer_norm` normed (x, or total where something was added) and its stats.  total_grad, the gradient that
+    reaches the sum by another way, is added to x_grad; weight_grad and bias_grad, where they are given, take a workspace."""
+    args = b"".join((_array(x), _NONE * 3, _array(weight), _NONE, _array(stats), _array(out_grad), _array(total_grad), _array(x_grad),
+                     _array(weight_grad), _array(bias_grad), _NORM_TAIL.pack(1.0, bool(centered), *_room(workspace))))
+    _check(dev, _lib(dev).adhip_layer_norm_backward(dev._ctx, args, _stream(dev, stream)), "adhip_layer_norm_backward")
+
+
+# ---- gated recurrence -----------------------------------------------------------------------------------------------
+
+
+def recurrence_blocks(length: int) -> int:
+    """States that a recurrence over `length` positions keeps for its backward pass: one before every 256th position."""
+    return -(-length // RECURRENCE_BLOCK)
+
+
+def recurrence_workspace(dev, x, *, backward: bool = False) -> int:
+    """Bytes of workspace that `recurrence`, and with `backward` also `recurrence_backward`, take on arrays of x's shape."""
+    need = ctypes.c_size_t()
+    args = _array(x, True) + _RECURRENCE_X
+    _check(dev, _lib(dev).adhip_recurrence_workspace(dev._ctx, args, bool(backward), ctypes.byref(need)), "adhip_recurrence_workspace")
+    return need.value
+
+
+def recurrence(dev, x, gates, out, *, factors: bool = False, initial=None, final=None, states=None, lengths=None, documents=None,
+               workspace=None, stream: Optional[int] = None) -> None:
+    """h = a h + (1 - a) x with a = sigmoid(gates) over the positions of x [batch, length, channels], each channel by itself, or with
+    `factors` h = gates h + x.  initial and final [batch, channels] (f32; one array where a state is carried on) are the states before and
+    after, states [batch, recurrence_blocks(length), channels] (f32) what `recurrence_backward` wants; lengths [batch] and documents
+    [batch, length] say which positions count and where the state begins anew."""
+    args = b"".join((_array(x), _array(gates), _array(out), _array(initial), _array(final), _array(states), _array(lengths), _array(documents),
+                     _NONE * 5, _RECURRENCE_TAIL.pack(bool(factors), *_room(workspace))))
+    _check(dev, _lib(dev).adhip_recurrence(dev._ctx, args, _stream(dev, stream)), "adhip_recurrence")
+
+
+def recurrence_backward(dev, x, gates, states, out_grad, x_grad, gates_grad, *, factors: bool = False, final_grad=None, initial_grad=None,
+                        lengths=None, documents=None, workspace=None, stream: Optional[int] = None) -> None:
+    """Gradients of x, gates and, where it is given, initial from `recurrence`'s states and the gradients of out and, where it is
+    given, final; the other arguments as there."""
+    args = b"".join((_array(x), _array(gates), _NONE * 3, _array(states), _array(lengths), _array(documents), _array(out_grad),
+                     _array(final_grad), _array(x_grad), _array(gates_grad), _array(initial_grad),
+                     _RECURRENCE_TAIL.pack(bool(factors), *_room(workspace))))
+    _check(dev, _lib(dev).adhip_recurrence_backward(dev._ctx, args, _stream(dev, stream)), "adhip_recurrence_backward")

@@ -35,6 +35,7 @@ struct AdamwLaunch {
     int n;
     unsigned aligned;              // bit i: every array of tensor i can be read four elements at once
     float grad_scale, beta1, grow1, beta2, grow2, root_scale, eps, keep, rate;
+    const float* factor;           // a number in device memory that grad_scale is multiplied by, where it is given
 };
 
 template <class T>
@@ -118,7 +119,7 @@ __device__ __forceinline__ void over_scale(const float (&x)[4], float scale, flo
 // A wavefront's blocks of a tensor.  WHOLE: all of them are there and can be read four elements at once; then no load waits
 // for a choice, and all are under way together.
 template <class PT, class GT, bool EIGHT, bool WHOLE>
-__device__ __forceinline__ void adamw_blocks(const AdamwLaunch& a, const adhip_adamw_tensor& t, bool aligned, int64_t unit0, int lane) {
+__device__ __forceinline__ void adamw_blocks(const AdamwLaunch& a, const adhip_adamw_tensor& t, float grad_scale, bool aligned, int64_t unit0, int lane) {
     const int64_t n = t.count;
     float p[kUnits][4], g[kUnits][4], m[kUnits][4], v[kUnits][4];
     unsigned mc[kUnits], vc[kUnits];
@@ -157,7 +158,7 @@ __device__ __forceinline__ void adamw_blocks(const AdamwLaunch& a, const adhip_a
                 const float r = v[u][k] * vs[u];
                 v[u][k] = r * r;
             }
-            const float x = g[u][k] * a.grad_scale;
+            const float x = g[u][k] * grad_scale;
             m[u][k] = m[u][k] * a.beta1 + x * a.grow1;
             v[u][k] = v[u][k] * a.beta2 + x * x * a.grow2;
             root[k] = sqrtf(v[u][k]);
@@ -197,8 +198,9 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AdamwLaunch a) {
     const bool aligned = a.aligned >> i & 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int64_t unit0 = (int64_t)(blockIdx.x - a.first[i]) * (kChunk / kBlock) + wave * kUnits;
-    if (aligned && (unit0 + kUnits) * kBlock <= t.count) adamw_blocks<PT, GT, EIGHT, true>(a, t, aligned, unit0, lane);
-    else adamw_blocks<PT, GT, EIGHT, false>(a, t, aligned, unit0, lane);
+    const float grad_scale = a.factor ? a.grad_scale * *a.factor : a.grad_scale;
+    if (aligned && (unit0 + kUnits) * kBlock <= t.count) adamw_blocks<PT, GT, EIGHT, true>(a, t, grad_scale, aligned, unit0, lane);
+    else adamw_blocks<PT, GT, EIGHT, false>(a, t, grad_scale, aligned, unit0, lane);
 }
 
 template <bool EIGHT>
@@ -211,8 +213,7 @@ void launch_adamw(const char* op, const AdamwLaunch& a, int p_type, int g_type, 
 
 bool aligned_to(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
 
-void adamw(const adhip_adamw_args& g, hipStream_t stream) {
-    const char* op = "adhip_adamw";
+void adamw(const char* op, const adhip_adamw_args& g, const float* factor, hipStream_t stream) {
     ADHIP_CHECK(g.p_type == ADHIP_F32 || g.p_type == ADHIP_BF16, "%s: parameters are %s, f32 or bf16 is wanted", op, type_name(g.p_type));
     ADHIP_CHECK(g.g_type == ADHIP_F32 || g.g_type == ADHIP_BF16, "%s: gradients are %s, f32 or bf16 is wanted", op, type_name(g.g_type));
     ADHIP_CHECK(g.state_type == ADHIP_F32 || g.state_type == ADHIP_E4M3, "%s: states are %s, f32 or e4m3 is wanted", op, type_name(g.state_type));
@@ -236,7 +237,9 @@ void adamw(const adhip_adamw_args& g, hipStream_t stream) {
                               (const void*)t.m_scale_out, (const void*)t.v_scale_out})
             ADHIP_CHECK(aligned_to(s, 4), "%s: a state array of tensor %lld is not aligned to 4 bytes", op, at);
     }
+    ADHIP_CHECK(aligned_to(factor, 4), "%s: factor is not aligned to its type", op);
     AdamwLaunch a = {};
+    a.factor = factor;
     a.grad_scale = (float)g.grad_scale;
     a.beta1 = (float)g.beta1;
     a.grow1 = (float)(1.0 - g.beta1);
@@ -276,9 +279,19 @@ void adamw(const adhip_adamw_args& g, hipStream_t stream) {
 }  // namespace
 }  // namespace adhip
 
-extern "C" int adhip_adamw(adhip_ctx* ctx, const adhip_adamw_args* args, void* stream) {
+extern "C" {
+
+int adhip_adamw(adhip_ctx* ctx, const adhip_adamw_args* args, void* stream) {
     return adhip::context_guarded(ctx, [&] {
         ADHIP_CHECK(args, "adhip_adamw: no arguments");
-        adhip::adamw(*args, (hipStream_t)stream);
+        adhip::adamw("adhip_adamw", *args, nullptr, (hipStream_t)stream);
     });
+}
+
+int adhip_adamw_scaled(adhip_ctx* ctx, const adhip_adamw_args* args, const float* factor, void* stream) {
+    return adhip::context_guarded(ctx, [&] {
+        ADHIP_CHECK(args, "adhip_adamw_scaled: no arguments");
+        adhip::adamw("adhip_adamw_scaled", *args, factor, (hipStream_t)stream);
+    });
+}
 }

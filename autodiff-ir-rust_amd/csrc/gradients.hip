@@ -1,0 +1,261 @@
+// The norm over all gradients of a step and clipping by it (Pascanu et al. 2013): norm = |grad_scale| sqrt(sum g^2), factor =
+// norm <= limit ? 1 : limit / norm, clipped gradients g grad_scale factor.  The norm and the factor stay on the device: the
+// clipping pass, or AdamW, reads the factor from there, and no stream waits for the host.
+//
+// Memory bounds it: one read of every gradient for the norm, and one more read and a write to clip, which cannot begin before
+// the norm is known.  Squares are added in 64 bits, whose exponents hold the squares of all f32 numbers and whose sums lose
+// nothing that counts; the vector units have the time (three instructions an element).  Each workgroup leaves one partial sum
+// and a last workgroup adds them in the order of their numbers, so the same gradients give the same bits.
+#include "operators.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+#pragma clang fp contract(off)
+
+namespace adhip {
+namespace {
+
+constexpr int kTensors = 128;    // of a launch: their descriptors stay within 4 KiB of kernel arguments
+constexpr int kThreads = 256;
+constexpr int kChunk = 16384;    // elements of a workgroup
+constexpr uint64_t kBlocks = 0xffffffffu / kThreads;  // workgroups of a launch: it holds fewer than 2^32 threads
+
+struct GradientLaunch {
+    const void* g[kTensors];
+    void* out[kTensors];
+    int64_t count[kTensors];
+    unsigned first[kTensors + 1];                            // the workgroup that begins each tensor
+    unsigned bf16s[kTensors / 32], aligned[kTensors / 32];   // bit i: tensor i is bf16; it can be read 16 bytes at once
+    int n;
+    float grad_scale;
+    const float* factor;
+    double* partial;  // of the launch's first workgroup
+};
+
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+    for (int off = 32; off; off >>= 1) x += __shfl_xor(x, off);
+    return x;
+}
+
+// The sum over a workgroup's threads, in the same order every time; thread 0 has it.
+template <int THREADS>
+__device__ __forceinline__ double block_sum(double x) {
+    __shared__ double part[THREADS / 64];
+    x = wave_sum(x);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = 0;
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i) x += part[i];
+    return x;
+}
+
+// The tensor that a workgroup belongs to.
+__device__ __forceinline__ int tensor_of(const GradientLaunch& a, unsigned block) {
+    int lo = 0, hi = a.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (a.first[mid] <= block) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <class T, int V>
+__device__ __forceinline__ double square_chunk(const T* g, int64_t begin, int64_t end) {
+    double s[2] = {0, 0};
+    int64_t i = begin + (int64_t)threadIdx.x * V;
+    if (V > 1) {
+        // whole packs, eight of them under way
+        constexpr int U = 8;
+        for (; i + (U - 1) * kThreads * V + V <= end; i += U * kThreads * V) {
+            Pack<T, V> r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) r[u] = *(const Pack<T, V>*)(g + i + u * kThreads * V);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const double x = (float)r[u].v[k];
+                    s[k & 1] = __builtin_fma(x, x, s[k & 1]);
+                }
+        }
+    }
+    for (; i < end; i += kThreads * V)
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (i + k < end) {
+                const double x = (float)g[i + k];
+                s[0] = __builtin_fma(x, x, s[0]);
+            }
+    return s[0] + s[1];
+}
+
+template <class T>
+__device__ __forceinline__ double squares(const void* g, int64_t begin, int64_t end, bool aligned) {
+    return aligned ? square_chunk<T, 16 / sizeof(T)>((const T*)g, begin, end) : square_chunk<T, 1>((const T*)g, begin, end);
+}
+
+__global__ __launch_bounds__(kThreads) void gradient_squares_kernel(const GradientLaunch a) {
+    const int t = tensor_of(a, blockIdx.x);
+    const int64_t begin = (int64_t)(blockIdx.x - a.first[t]) * kChunk, end = min(begin + kChunk, a.count[t]);
+    const bool aligned = a.aligned[t >> 5] >> (t & 31) & 1;
+    const double s = a.bf16s[t >> 5] >> (t & 31) & 1 ? squares<bf16>(a.g[t], begin, end, aligned) : squares<float>(a.g[t], begin, end, aligned);
+    const double sum = block_sum<kThreads>(s);
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = sum;
+}
+
+__device__ __forceinline__ float clip_factor(double norm, double limit) { return norm <= limit ? 1.f : (float)(limit / norm); }
+
+constexpr int kFinish = 1024;
+
+__global__ __launch_bounds__(kFinish) void gradient_norm_kernel(const double* partial, int64_t n, double grad_scale, double limit, float* norm,
+                                                                float* factor) {
+    double s = 0;
+    for (int64_t i = threadIdx.x; i < n; i += kFinish) s += partial[i];
+    const double length = sqrt(block_sum<kFinish>(s)) * fabs(grad_scale);
+    if (threadIdx.x == 0) {
+        *norm = (float)length;
+        if (factor) *factor = clip_factor(length, limit);
+    }
+}
+
+template <class T, int V>
+__device__ __forceinline__ void scale_chunk(const T* g, T* out, int64_t begin, int64_t end, float scale) {
+    int64_t i = begin + (int64_t)threadIdx.x * V;
+    if (V > 1) {
+        constexpr int U = 8;
+        for (; i + (U - 1) * kThreads * V + V <= end; i += U * kThreads * V) {
+            Pack<T, V> r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) r[u] = *(const Pack<T, V>*)(g + i + u * kThreads * V);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) r[u].v[k] = (T)((float)r[u].v[k] * scale);
+                *(Pack<T, V>*)(out + i + u * kThreads * V) = r[u];
+            }
+        }
+    }
+    for (; i < end; i += kThreads * V)
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (i + k < end) out[i + k] = (T)((float)g[i + k] * scale);
+}
+
+template <class T>
+__device__ __forceinline__ void scaled(const void* g, void* out, int64_t begin, int64_t end, bool aligned, float scale) {
+    if (aligned) scale_chunk<T, 16 / sizeof(T)>((const T*)g, (T*)out, begin, end, scale);
+    else scale_chunk<T, 1>((const T*)g, (T*)out, begin, end, scale);
+}
+
+__global__ __launch_bounds__(kThreads) void gradient_scale_kernel(const GradientLaunch a) {
+    const int t = tensor_of(a, blockIdx.x);
+    const float scale = a.grad_scale * *a.factor;
+    // in place, a factor of one leaves every number as it is (a NaN too)
+    if (scale == 1.f && a.out[t] == a.g[t]) return;
+    const int64_t begin = (int64_t)(blockIdx.x - a.first[t]) * kChunk, end = min(begin + kChunk, a.count[t]);
+    const bool aligned = a.aligned[t >> 5] >> (t & 31) & 1;
+    if (a.bf16s[t >> 5] >> (t & 31) & 1) scaled<bf16>(a.g[t], a.out[t], begin, end, aligned, scale);
+    else scaled<float>(a.g[t], a.out[t], begin, end, aligned, scale);
+}
+
+int64_t blocks_of(int64_t count) { return (count + kChunk - 1) / kChunk; }
+
+// Workgroups of all tensors: one partial sum each.
+int64_t check_tensors(const char* op, const adhip_gradients_args& g) {
+    ADHIP_CHECK(g.n_tensors >= 0 && (g.tensors || g.n_tensors == 0), "%s: no tensors", op);
+    int64_t blocks = 0;
+    for (int64_t i = 0; i < g.n_tensors; ++i) {
+        const adhip_gradient& t = g.tensors[i];
+        ADHIP_CHECK(t.type == ADHIP_F32 || t.type == ADHIP_BF16, "%s: gradient %lld is %s, f32 or bf16 is wanted", op, (long long)i, type_name((int)std::min<int64_t>(std::max<int64_t>(t.type, -1), 4)));
+        ADHIP_CHECK(t.count >= 0 && t.count <= (int64_t)kBlocks * kChunk, "%s: gradient %lld has %lld elements", op, (long long)i, (long long)t.count);
+        blocks += blocks_of(t.count);
+        ADHIP_CHECK(blocks < (int64_t(1) << 40), "%s: too many elements", op);
+    }
+    return blocks;
+}
+
+// (a factor that nobody asked for has its place behind the partial sums)
+size_t workspace_of(int64_t blocks) { return (size_t)(blocks + 1) * sizeof(double); }
+
+void gradients(const char* op, const adhip_gradients_args& g, bool clip, hipStream_t stream) {
+    const int64_t blocks = check_tensors(op, g);
+    ADHIP_CHECK(g.limit > 0, "%s: limit %g is not above zero", op, g.limit);
+    ADHIP_CHECK(std::isfinite((float)g.grad_scale), "%s: grad_scale must be finite", op);
+    ADHIP_CHECK(g.norm && (uintptr_t)g.norm % 4 == 0 && (uintptr_t)g.factor % 4 == 0, "%s: norm is missing, or norm or factor is not aligned to its type", op);
+    ADHIP_CHECK(g.workspace && (uintptr_t)g.workspace % 8 == 0 && g.workspace_bytes >= workspace_of(blocks),
+                "%s: the workspace has %zu bytes, %zu are wanted, aligned to 8", op, g.workspace ? g.workspace_bytes : (size_t)0, workspace_of(blocks));
+    for (int64_t i = 0; i < g.n_tensors; ++i) {
+        const adhip_gradient& t = g.tensors[i];
+        const size_t w = (size_t)type_bytes((int)t.type);
+        ADHIP_CHECK(t.count == 0 || (t.g && (t.out || !clip)), "%s: an array of gradient %lld is missing", op, (long long)i);
+        ADHIP_CHECK((uintptr_t)t.g % w == 0 && (!clip || (uintptr_t)t.out % w == 0), "%s: an array of gradient %lld is not aligned to its type", op,
+                    (long long)i);
+    }
+    double* const partial = (double*)g.workspace;
+    float* const factor = g.factor || !clip ? g.factor : (float*)(partial + blocks);
+    auto each_launch = [&](bool scales) {
+        GradientLaunch a = {};
+        a.grad_scale = (float)g.grad_scale;
+        a.factor = factor;
+        a.partial = partial;
+        uint64_t of_launch = 0;
+        auto flush = [&] {
+            if (a.n == 0) return;
+            launch(op, scales ? gradient_scale_kernel : gradient_squares_kernel, (unsigned)of_launch, kThreads, stream, a);
+            a.partial += of_launch;
+            of_launch = 0;
+            a.n = 0;
+            for (int k = 0; k < kTensors / 32; ++k) a.bf16s[k] = a.aligned[k] = 0;
+        };
+        for (int64_t i = 0; i < g.n_tensors; ++i) {
+            const adhip_gradient& t = g.tensors[i];
+            if (t.count == 0) continue;
+            const uint64_t own = (uint64_t)blocks_of(t.count);
+            if (a.n == kTensors || of_launch + own > kBlocks) flush();
+            a.g[a.n] = t.g;
+            a.out[a.n] = t.out;
+            a.count[a.n] = t.count;
+            a.first[a.n] = (unsigned)of_launch;
+            if (t.type == ADHIP_BF16) a.bf16s[a.n >> 5] |= 1u << (a.n & 31);
+            if ((uintptr_t)t.g % 16 == 0 && (!scales || (uintptr_t)t.out % 16 == 0)) a.aligned[a.n >> 5] |= 1u << (a.n & 31);
+            ++a.n;
+            of_launch += own;
+            a.first[a.n] = (unsigned)of_launch;
+        }
+        flush();
+    };
+    each_launch(false);
+    launch(op, gradient_norm_kernel, 1, kFinish, stream, partial, blocks, g.grad_scale, g.limit, g.norm, factor);
+    if (clip) each_launch(true);
+}
+
+}  // namespace
+}  // namespace adhip
+
+extern "C" {
+
+int adhip_gradient_norm_workspace(adhip_ctx* ctx, const adhip_gradients_args* args, size_t* bytes) {
+    return adhip::context_guarded(ctx, [&] {
+        ADHIP_CHECK(args && bytes, "adhip_gradient_norm_workspace: no arguments");
+        *bytes = adhip::workspace_of(adhip::check_tensors("adhip_gradient_norm_workspace", *args));
+    });
+}
+
+int adhip_gradient_norm(adhip_ctx* ctx, const adhip_gradients_args* args, void* stream) {
+    return adhip::context_guarded(ctx, [&] {
+        ADHIP_CHECK(args, "adhip_gradient_norm: no arguments");
+        adhip::gradients("adhip_gradient_norm", *args, false, (hipStream_t)stream);
+    });
+}
+
+int adhip_clip_gradients(adhip_ctx* ctx, const adhip_gradients_args* args, void* stream) {
+    return adhip::context_guarded(ctx, [&] {
+        ADHIP_CHECK(args, "adhip_clip_gradients: no arguments");
+        adhip::gradients("adhip_clip_gradients", *args, true, (hipStream_t)stream);
+    });
+}
+}

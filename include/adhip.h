@@ -194,6 +194,35 @@ typedef struct adhip_adamw_args {
     double rate, beta1, beta2, eps, decay, grad_scale;
 } adhip_adamw_args;
 int adhip_adamw(adhip_ctx* ctx, const adhip_adamw_args* args, void* stream);
+/* The same with grad_scale times the f32 number that `factor` points to in device memory when the kernels run, for instance
+ * where adhip_gradient_norm left it (NULL: adhip_adamw). */
+int adhip_adamw_scaled(adhip_ctx* ctx, const adhip_adamw_args* args, const float* factor, void* stream);
+
+/* The norm over all gradients of a step, and clipping by it.
+ *     norm = |grad_scale| sqrt(sum over all tensors of g g),    factor = 1 where norm <= limit, limit / norm otherwise
+ * with the sum in 64 bits, added in an order that only the tensors' sizes, types and alignment decide.  norm and factor are f32 numbers in device memory
+ * (factor may be NULL).  adhip_clip_gradients also writes  out = g (grad_scale factor)  of each tensor, rounded once; `out`
+ * may be `g` itself.  A gradient that is not finite shows: a NaN makes norm, factor and every clipped gradient NaN; an infinity
+ * makes the norm infinite and, under a finite limit, the factor 0 (and itself NaN).  Gradients are ADHIP_F32 or ADHIP_BF16,
+ * each of its own type, packed; no gradients at all have norm 0.
+ * limit is above zero, and may be infinite.  workspace: adhip_gradient_norm_workspace() bytes, aligned to 8, used until the
+ * call's kernels are done (only sizes and types are looked at for it). */
+typedef struct adhip_gradient {
+    const void* g;
+    void* out; /* adhip_clip_gradients only */
+    int64_t count, type;
+} adhip_gradient;
+typedef struct adhip_gradients_args {
+    const adhip_gradient* tensors; /* host memory, read before the call returns */
+    int64_t n_tensors;
+    double limit, grad_scale;
+    float *norm, *factor;
+    void* workspace;
+    size_t workspace_bytes;
+} adhip_gradients_args;
+int adhip_gradient_norm_workspace(adhip_ctx* ctx, const adhip_gradients_args* args, size_t* bytes);
+int adhip_gradient_norm(adhip_ctx* ctx, const adhip_gradients_args* args, void* stream);
+int adhip_clip_gradients(adhip_ctx* ctx, const adhip_gradients_args* args, void* stream);
 
 /* Attention.  q and out are [batch, queries, heads, size], k and v [batch, keys, key heads, size] (f32 or bf16, one type),
  * heads a multiple of the key heads (head h reads key head h / (heads / key heads)), size at most 256.  Query i of
@@ -230,6 +259,65 @@ int adhip_attention(adhip_ctx* ctx, const adhip_attention_args* args, void* stre
 /* Gradients of q, k and v from what adhip_attention gave (out, lse) and the gradient of out.  The order of additions
  * is fixed: the same inputs give the same bits. */
 int adhip_attention_backward(adhip_ctx* ctx, const adhip_attention_args* args, void* stream);
+
+/* Layer norm of rows.  x, added, total and out have one shape of 2 to 4 dims and one type (f32 or bf16); the last dim is the
+ * row, of 1 to 16384 elements.
+ *     t = x, or  total = x + added  (a sum in 32 bits, rounded as it is written) where `added` and `total` are given
+ *     mean = sum(t) / size  (0 unless `centered`),  root = 1 / sqrt(sum((t - mean)^2) / size + eps)
+ *     out = (t - mean) root weight + bias
+ * weight and bias [size] are f32 or of x's type, both alike; no weight is a weight of 1, no bias a bias of 0.  Not centered and
+ * without a bias it is RMS norm.  stats (f32, x's leading dims and 2, packed, aligned to 8 bytes; may be left out) receives mean and root.  total and out
+ * may be x or added themselves, under the same strides (out not beside a total that is the same array). */
+typedef struct adhip_layer_norm_args {
+    adhip_array x, added, total, out, weight, bias, stats;
+    /* backward only */
+    adhip_array out_grad, total_grad, x_grad, weight_grad, bias_grad;
+    double eps;
+    int64_t centered;
+    void* workspace; /* backward only */
+    size_t workspace_bytes;
+} adhip_layer_norm_args;
+/* What the backward call's sums over rows need: only the shape and type of x are looked at. */
+int adhip_layer_norm_workspace(adhip_ctx* ctx, const adhip_layer_norm_args* args, size_t* bytes);
+int adhip_layer_norm(adhip_ctx* ctx, const adhip_layer_norm_args* args, void* stream);
+/* Gradients, from x (what was normed: `total` where something was added), stats, weight and the gradient of out.  x_grad is that of t;
+ * total_grad (may be left out), a gradient that reaches t by another way, is added to it.  Where something was added x_grad is the gradient of both x and
+ * added.  x_grad may be out_grad, total_grad or x itself, under the same strides.  weight_grad and bias_grad ([size], f32 or bf16, each may be left out)
+ * are sums over all rows in 32 bits, added in an order that only the shape decides; with either a workspace of
+ * adhip_layer_norm_workspace() bytes, aligned to 16, is used until the call's kernels are done.  added, total, out and bias are
+ * not looked at. */
+int adhip_layer_norm_backward(adhip_ctx* ctx, const adhip_layer_norm_args* args, void* stream);
+
+/* A gated linear recurrence over positions, each channel by itself.  x, gates and out are [batch, length, channels] (f32 or
+ * bf16, one type):
+ *     h[t] = a[t] h[t-1] + b[t],  out[t] = h[t],    a = sigmoid(gates), b = (1 - a) x,    or  a = gates, b = x  with `factors`
+ * States are f32.  h[-1] is initial ([batch, channels]; 0 where it is not given), final receives the last state and may be
+ * initial itself (a state that is carried from call to call; one position a call is a decoder's step).  lengths (int32 [batch], clamped
+ * to 0 .. length): positions behind a sequence's length leave the state as it is.  documents (int32 [batch, length]): the state
+ * begins at 0 at every position whose document is not that of the position before (the first position goes on from initial), and is 0 behind a
+ * position of a document below 0.  Positions behind lengths or of documents below 0 give out = 0 and gradients 0, whatever x,
+ * gates and out_grad hold there; everything else must be finite (gates may be infinite).  A factor of 0 drops the state before it, whatever
+ * that is.  Factors are multiplied over runs of positions: where such a product passes 2^128, results may be infinite or NaN up to the next factor of 0
+ * or document.
+ * states (f32 [batch, ceil(length / 256), channels]; may be left out) receives the state before every 256th position, for the
+ * backward pass.  out may be x or gates themselves, under the same strides.
+ * workspace: adhip_recurrence_workspace() bytes, aligned to 16, used until the call's kernels are done; needs no more where it is 0. */
+#define ADHIP_RECURRENCE_BLOCK 256
+typedef struct adhip_recurrence_args {
+    adhip_array x, gates, out, initial, final, states, lengths, documents;
+    /* backward only */
+    adhip_array out_grad, final_grad, x_grad, gates_grad, initial_grad;
+    int64_t factors;
+    void* workspace;
+    size_t workspace_bytes;
+} adhip_recurrence_args;
+/* Only the shape and type of x are looked at. */
+int adhip_recurrence_workspace(adhip_ctx* ctx, const adhip_recurrence_args* args, int backward, size_t* bytes);
+int adhip_recurrence(adhip_ctx* ctx, const adhip_recurrence_args* args, void* stream);
+/* Gradients of x, gates and, where asked for, initial, from x, gates, the forward call's states, the gradient of out and, where it
+ * is given, that of final ([batch, channels]); lengths, documents and factors as there.  x_grad and gates_grad may be x, gates or out_grad
+ * themselves, under the same strides.  out, initial and final are not looked at.  The order of additions is fixed. */
+int adhip_recurrence_backward(adhip_ctx* ctx, const adhip_recurrence_args* args, void* stream);
 
 #ifdef __cplusplus
 }
