@@ -19,12 +19,16 @@ namespace adhip {
 namespace {
 
 constexpr int kBlock = ADHIP_RECURRENCE_BLOCK;  // positions between states that are kept
-constexpr int kWaves = 8, kThreads = kWaves * 64;
-constexpr int kLanes = 16;                      // of a row of channels: four positions' threads a wavefront
+constexpr int kTile = kBlock;                   // positions that a workgroup takes at once: a tile begins at a state that is kept
 constexpr int kSteps = 8;                       // consecutive positions of a thread
-constexpr int kTile = kThreads / kLanes * kSteps;
-static_assert(kTile == kBlock, "a tile of the backward pass begins at a state that is kept");
+// A workgroup takes rows of LANES times 4 bytes of channels; as many threads of each lane share the positions of a tile.
+template <int LANES>
+struct Team {
+    static constexpr int kThreads = kTile / kSteps * LANES, kWaves = kThreads / 64, kSpread = 64 / LANES;
+};
 constexpr unsigned kAll = (1u << kSteps) - 1;
+constexpr int kNarrow = 16, kWide = 32;         // lanes of a row of channels
+constexpr int kFull = 256;                      // workgroups that give every compute unit one
 
 struct Rows {
     int64_t b, t;  // strides of batch and positions
@@ -36,35 +40,65 @@ struct RecurrenceParams {
     const float *initial, *final_grad;
     float *states, *final, *initial_grad;
     const int *lengths, *documents;
+    float2* carry;  // [ranges, batch, channels]: what a range does to a state
     Rows x_at, gates_at, out_at, out_grad_at, x_grad_at, gates_grad_at, states_at, documents_at;
     int64_t initial_b, final_b, final_grad_b, initial_grad_b, lengths_b;
     int length, channels, groups;  // groups: of channels that a workgroup takes
+    int batch, ranges, tiles;      // of positions, and tiles of a range
 };
 
-// Elements that begin at any of their own addresses: global memory takes such accesses.
-template <class T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) Loose {
-    T v[N];
+// Operand of a wait for all memory operations of a wavefront, and of nothing else.
+constexpr int kNoneUnderWay = 0x0f70;
+
+// 4 bytes of channels, beginning at any element: global memory takes such accesses.
+template <class T>
+constexpr int kPack = 4 / sizeof(T);
+template <class T>
+struct __attribute__((packed, aligned(sizeof(T)))) Word {
+    unsigned w;
 };
 
-// 1 / (1 + exp(-g)) and 1 / (1 + exp(g)), each to its own last bits.
+template <class T>
+__device__ __forceinline__ void unpack(unsigned w, float (&f)[kPack<T>]) {
+    if constexpr (sizeof(T) == 4) {
+        f[0] = __uint_as_float(w);
+    } else {
+        f[0] = __uint_as_float(w << 16);
+        f[1] = __uint_as_float(w & 0xffff0000u);
+    }
+}
+template <class T>
+__device__ __forceinline__ unsigned pack(const float (&f)[kPack<T>]) {
+    union {
+        T v[kPack<T>];
+        unsigned w;
+    } u;
+#pragma unroll
+    for (int v = 0; v < kPack<T>; ++v) u.v[v] = (T)f[v];
+    return u.w;
+}
+
+// a = 1 / (1 + exp(-g)) and rest = 1 / (1 + exp(g)), each to its own last bits.
 template <class T>
 __device__ __forceinline__ void sigmoids(float g, float& a, float& rest) {
     constexpr float kLog2 = 1.44269504f;
-    float y = -fabsf(g);
-    float e;
-    if (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4) {
+        float y = -fabsf(g);
         y = y < -150.f ? -150.f : y;  // (infinities have no remainder; a NaN stays one)
         const float t = y * kLog2;
         const float low = __builtin_fmaf(y, 1.92596299e-8f, __builtin_fmaf(y, kLog2, -t));
-        e = __builtin_amdgcn_exp2f(t);
+        float e = __builtin_amdgcn_exp2f(t);
         e = __builtin_fmaf(e, low * 0.693147181f, e);
+        const float r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
+        a = g < 0.f ? s : r;
+        rest = g < 0.f ? r : s;
     } else {
-        e = __builtin_amdgcn_exp2f(y * kLog2);  // (|g| 2^-24 off, far below what is kept of a result)
+        // The exponent is |g| 2^-24 off, far below what is kept of a result.  Below -83 a gate counts as -83 (a = 2^-120), whose
+        // exponential still has a reciprocal.
+        const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -kLog2, 120.f));
+        a = __builtin_amdgcn_rcpf(1.f + e);
+        rest = e * a;
     }
-    const float r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
-    a = g < 0.f ? s : r;
-    rest = g < 0.f ? r : s;
 }
 
 // The map h -> a h + b of a state, and the factor of two maps one after the other.  A factor of zero drops what was there and a
@@ -84,54 +118,124 @@ __device__ __forceinline__ float together(float a, float b) {
 struct Marks {
     unsigned live, cut;
     int count;
-    __device__ __forceinline__ Marks(const RecurrenceParams& p, int64_t b, int t, int length) {
-        count = min(max(length - t, 0), kSteps);
-        live = (1u << count) - 1;
-        cut = 0;
-        if (p.documents && count > 0) {
-            const int* d = p.documents + b * p.documents_at.b;
-            int before = d[(int64_t)(t > 0 ? t - 1 : t) * p.documents_at.t];
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k)
-                if (k < count) {
-                    const int here = d[(int64_t)(t + k) * p.documents_at.t];
-                    if (here < 0) live &= ~(1u << k);
-                    if (here < 0 || here != before) cut |= 1u << k;
-                    before = here;
-                }
-        }
-    }
     __device__ __forceinline__ bool plain() const { return live == kAll && cut == 0; }
 };
 
-// K positions of V channels; zeros where there are none.
-template <class T, int V>
-struct Steps {
-    Loose<T, V> r[kSteps];
-    __device__ __forceinline__ void load(const void* from, const Rows& at, int64_t b, int t, int c, int length, int channels) {
-        const T* x = (const T*)from + b * at.b + (int64_t)t * at.t + c;
-        if (t + kSteps <= length && c + V <= channels) {
+// Documents of K positions and of the one before them.
+struct Documents {
+    int d[kSteps + 1];
+    __device__ __forceinline__ void load(const RecurrenceParams& p, int64_t b, int t) {
+        const int* from = p.documents + b * p.documents_at.b;
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) r[k] = *(const Loose<T, V>*)(x + k * at.t);
+        for (int k = 0; k <= kSteps; ++k) d[k] = from[(int64_t)min(max(t - 1 + k, 0), p.length - 1) * p.documents_at.t];
+    }
+    __device__ __forceinline__ Marks marks(int count) const {
+        Marks m = {(1u << count) - 1, 0, count};
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            const bool none = d[k + 1] < 0;
+            if (k < count) {
+                m.live &= ~((unsigned)none << k);
+                m.cut |= (unsigned)(none || d[k + 1] != d[k]) << k;
+            }
+        }
+        return m;
+    }
+};
+
+// An address that all lanes share stays in scalar registers; folded into the lanes' own it would take two registers of each.
+template <class P>
+__device__ __forceinline__ P* row_of(P* p) {
+    asm("" : "+s"(p));
+    return p;
+}
+
+// K positions of a pack of channels.
+template <class T>
+struct Steps {
+    unsigned w[kSteps];
+};
+
+// Where a workgroup and a thread of it are.
+template <class T, int LANES>
+struct Seat {
+    static constexpr int V = kPack<T>;
+    int lane, wave, slot, base, c, own, range, first, tiles, length;
+    int64_t batch, state;  // state: of the channels in [batch, channels]
+    bool lone;
+    __device__ __forceinline__ Seat(const RecurrenceParams& p) {
+        lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), slot = (lane & (LANES - 1)) * V;
+        // Workgroups go to the eight dies in turn: neighbours of a row, whose channels share cache lines, go to one die.
+        unsigned at = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+        const unsigned group = at % (unsigned)p.groups;
+        at /= (unsigned)p.groups;
+        batch = at % (unsigned)p.batch;
+        range = (int)(at / (unsigned)p.batch);
+        // Packs that would pass the row's end begin before it: their lanes compute what a neighbour in their wavefront computes too, bit
+        // for bit.  A lone last channel has no neighbour here, but in another workgroup, which may already have written there.
+        base = (int)group * LANES * V;
+        lone = base + V > p.channels;
+        c = lone ? base : min(base + slot, p.channels - V);
+        own = (wave * Team<LANES>::kSpread + lane / LANES) * kSteps;
+        first = range * p.tiles * kTile;
+        tiles = min(p.tiles, (p.length - first + kTile - 1) / kTile);
+        length = p.lengths ? min(max(p.lengths[batch * p.lengths_b], 0), p.length) : p.length;
+        state = batch * p.channels + c;
+    }
+    // (a launch has a multiple of eight workgroups)
+    __device__ __forceinline__ bool there(int ranges) const { return range < ranges; }
+    // Tiles of this range that have positions of the sequence.
+    __device__ __forceinline__ int used() const { return min((max(length - first, 0) + kTile - 1) / kTile, tiles); }
+};
+
+// An array's tiles as seen by a thread: uniform addresses of positions, and this thread's own bytes from there.  Whole tiles, tiles
+// that end within and lone channels make the same number of loads, without a branch between them, so that the compiler knows
+// how many are under way and waits for those that it needs alone.
+template <class T>
+struct Side {
+    char* tile;
+    int64_t step;
+    unsigned off, lane;
+    template <int LANES>
+    __device__ __forceinline__ Side(const void* p, const Rows& at, const Seat<T, LANES>& seat)
+        : tile((char*)p + (seat.batch * at.b + (int64_t)seat.first * at.t + seat.base) * (int64_t)sizeof(T)), step(at.t * (int64_t)sizeof(T)),
+          off((unsigned)seat.own * (unsigned)step), lane((unsigned)(seat.c - seat.base) * (unsigned)sizeof(T)) {}
+    // Tile i, of which `rows` positions are there (those behind are read as the last one), or where `there` says that there is none,
+    // bytes of its beginning that cost next to nothing.
+    template <int LANES>
+    __device__ __forceinline__ void load(Steps<T>& s, const Seat<T, LANES>& seat, int i, int rows, bool there) const {
+        const char* from = tile + (int64_t)i * kTile * step;
+        if (rows >= kTile && !seat.lone) {
+            const unsigned at = there ? off + lane : 0;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) s.w[k] = ((const Word<T>*)(row_of(from + k * step) + at))->w;
+        } else if (!seat.lone) {
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+                s.w[k] = ((const Word<T>*)(from + ((unsigned)min(seat.own + k, rows - 1) * (unsigned)step + lane)))->w;
         } else {
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                for (int v = 0; v < V; ++v) r[k].v[v] = t + k < length && c + v < channels ? x[k * at.t + v] : (T)0.f;
+                s.w[k] = *(const unsigned short*)(from + (unsigned)min(seat.own + k, rows - 1) * (unsigned)step);
         }
     }
-    __device__ __forceinline__ void store(void* to, const Rows& at, int64_t b, int t, int c, int length, int channels) const {
-        T* x = (T*)to + b * at.b + (int64_t)t * at.t + c;
-        if (t + kSteps <= length && c + V <= channels) {
+    template <int LANES>
+    __device__ __forceinline__ void store(const Steps<T>& s, const Seat<T, LANES>& seat, int i, int rows) const {
+        char* to = tile + (int64_t)i * kTile * step;
+        if (rows >= kTile && !seat.lone) {
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) *(Loose<T, V>*)(x + k * at.t) = r[k];
-        } else {
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (t + k < length && c + v < channels) x[k * at.t + v] = r[k].v[v];
+            for (int k = 0; k < kSteps; ++k) ((Word<T>*)(row_of(to + k * step) + (off + lane)))->w = s.w[k];
+            return;
         }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+            if (seat.own + k < rows) {
+                char* at = to + ((unsigned)(seat.own + k) * (unsigned)step + lane);
+                if (seat.lone) *(unsigned short*)at = (unsigned short)s.w[k];
+                else ((Word<T>*)at)->w = s.w[k];
+            }
+        // Stores that only some ways make would have the compiler wait for those of whole tiles too: it sees here that none is left.
+        __builtin_amdgcn_s_waitcnt(kNoneUnderWay);
     }
 };
 
@@ -147,40 +251,52 @@ __device__ __forceinline__ void store_state(float* to, int64_t at, int c, int ch
         if (c + v < channels) to[at + c + v] = h[v];
 }
 
-// The maps of a thread's positions.
-template <class T, int V, bool FACTORS>
-__device__ __forceinline__ void maps(const Steps<T, V>& x, const Steps<T, V>& g, const Marks& m, float (&a)[kSteps][V], float (&b)[kSteps][V]) {
+// The maps of a thread's positions as they are, and with marks.
+template <class T, bool FACTORS>
+__device__ __forceinline__ void maps(const Steps<T>& x, const Steps<T>& g, float (&a)[kSteps][kPack<T>], float (&b)[kSteps][kPack<T>]) {
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+        float in[kPack<T>], gate[kPack<T>];
+        unpack<T>(x.w[k], in);
+        unpack<T>(g.w[k], gate);
+#pragma unroll
+        for (int v = 0; v < kPack<T>; ++v) {
+            if (FACTORS) {
+                a[k][v] = gate[v];
+                b[k][v] = in[v];
+            } else {
+                float rest;
+                sigmoids<T>(gate[v], a[k][v], rest);
+                b[k][v] = rest * in[v];
+            }
+        }
+    }
+}
+template <int V>
+__device__ __forceinline__ void mark(const Marks& m, float (&a)[kSteps][V], float (&b)[kSteps][V]) {
+    if (m.plain()) return;
 #pragma unroll
     for (int k = 0; k < kSteps; ++k)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const float in = (float)x.r[k].v[v];
-            if (FACTORS) {
-                a[k][v] = (float)g.r[k].v[v];
-                b[k][v] = in;
-            } else {
-                float rest;
-                sigmoids<T>((float)g.r[k].v[v], a[k][v], rest);
-                b[k][v] = rest * in;
-            }
+            a[k][v] = m.cut >> k & 1 ? 0.f : k < m.count ? a[k][v] : 1.f;
+            b[k][v] = m.live >> k & 1 ? b[k][v] : 0.f;
         }
-    if (!m.plain())
+}
+template <class T>
+__device__ __forceinline__ void hide(const Marks& m, Steps<T>& s) {
+    if (m.live == kAll) return;
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                a[k][v] = m.cut >> k & 1 ? 0.f : k < m.count ? a[k][v] : 1.f;
-                b[k][v] = m.live >> k & 1 ? b[k][v] : 0.f;
-            }
+    for (int k = 0; k < kSteps; ++k) s.w[k] = m.live >> k & 1 ? s.w[k] : 0;
 }
 
-// The exchange between the four threads of a wavefront that have the same channels: composes A h + B of the threads before this
-// one (behind it where BACK), and of all four.
-template <bool FACTORS, bool BACK>
+// The exchange between the threads of a wavefront that have the same channels: composes A h + B of the threads before this
+// one (behind it where BACK), and of all of them.
+template <int LANES, bool FACTORS, bool BACK>
 __device__ __forceinline__ void across(int lane, float& A, float& B, float& preA, float& preB) {
     preA = 1, preB = 0;
 #pragma unroll
-    for (int off = kLanes; off < 64; off *= 2) {
+    for (int off = LANES; off < 64; off *= 2) {
         const float otherA = __shfl_xor(A, off), otherB = __shfl_xor(B, off);
         if (((lane & off) != 0) != BACK) {
             preB = onward<FACTORS>(preA, otherB, preB);
@@ -193,39 +309,36 @@ __device__ __forceinline__ void across(int lane, float& A, float& B, float& preA
     }
 }
 
-template <class T, int V, bool FACTORS>
-__global__ __launch_bounds__(kThreads) void recurrence_kernel(const RecurrenceParams p) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), slot = (lane & (kLanes - 1)) * V;
-    const int64_t batch = blockIdx.x / (unsigned)p.groups;
-    const int c = (int)(blockIdx.x % (unsigned)p.groups) * kLanes * V + slot;
-    const int length = p.lengths ? min(max(p.lengths[batch * p.lengths_b], 0), p.length) : p.length;
-    const int own = (wave * 4 + lane / kLanes) * kSteps;  // this thread's positions in a tile
-    __shared__ float2 parts[2][kWaves][kLanes * V];       // (by turns: the other one's barrier stands between readers and writers)
+template <class T, int LANES, bool FACTORS, bool DOCS>
+__global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const RecurrenceParams p) {
+    constexpr int V = kPack<T>, kWaves = Team<LANES>::kWaves;
+    const Seat<T, LANES> seat(p);
+    if (!seat.there(p.ranges)) return;
+    const int lane = seat.lane, wave = seat.wave, slot = seat.slot;
+    __shared__ float2 parts[2][kWaves][LANES * V];  // (by turns: the other one's barrier stands between readers and writers)
     float carry[V];
-    load_state<V>(p.initial, batch * p.initial_b, c, p.channels, carry);
-    Steps<T, V> x, g, next_x, next_g;
-    x.load(p.x, p.x_at, batch, own, c, length, p.channels);
-    g.load(p.gates, p.gates_at, batch, own, c, length, p.channels);
+    load_state<V>(p.initial, seat.batch * p.initial_b, seat.c, p.channels, carry);
+    for (int r = 0; r < seat.range; ++r)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (seat.c + v < p.channels) {
+                const float2 m = p.carry[(int64_t)r * p.batch * p.channels + seat.state + v];
+                carry[v] = onward<FACTORS>(m.x, carry[v], m.y);
+            }
     int turn = 0;
-    for (int begin = 0; begin < p.length; begin += kTile, turn ^= 1) {
-        const int t = begin + own;
-        if (begin + kTile < p.length) {
-            next_x.load(p.x, p.x_at, batch, t + kTile, c, length, p.channels);
-            next_g.load(p.gates, p.gates_at, batch, t + kTile, c, length, p.channels);
-        }
-        const Marks m(p, batch, t, length);
-        float a[kSteps][V], b[kSteps][V], A[V], B[V], preA[V], preB[V], h[V];
-        maps<T, V, FACTORS>(x, g, m, a, b);
+    // From the maps of a tile to its states, and the state behind it.
+    auto states = [&](const float (&a)[kSteps][V], const float (&b)[kSteps][V], int begin, Steps<T>& o) {
+        float A[V], B[V], preA[V], preB[V], h[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            A[v] = 1, B[v] = 0;
+            A[v] = a[0][v], B[v] = b[0][v];
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
+            for (int k = 1; k < kSteps; ++k) {
                 A[v] = together<FACTORS>(A[v], a[k][v]);
                 B[v] = onward<FACTORS>(a[k][v], B[v], b[k][v]);
             }
-            across<FACTORS, false>(lane, A[v], B[v], preA[v], preB[v]);
-            if (lane < kLanes) parts[turn][wave][slot + v] = make_float2(A[v], B[v]);
+            across<LANES, FACTORS, false>(lane, A[v], B[v], preA[v], preB[v]);
+            if (lane < LANES) parts[turn][wave][slot + v] = make_float2(A[v], B[v]);
         }
         __syncthreads();
 #pragma unroll
@@ -238,123 +351,363 @@ __global__ __launch_bounds__(kThreads) void recurrence_kernel(const RecurrencePa
             }
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = onward<FACTORS>(preA[v], h[v], preB[v]);
-        if (p.states && own == 0) store_state<V>(p.states, batch * p.states_at.b + (int64_t)(t / kBlock) * p.states_at.t, c, p.channels, h);
-        Steps<T, V> o;
+        turn ^= 1;
+        if (p.states && seat.own == 0) store_state<V>(p.states, seat.batch * p.states_at.b + (int64_t)(begin / kBlock) * p.states_at.t, seat.c, p.channels, h);
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k)
+        for (int k = 0; k < kSteps; ++k) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                h[v] = onward<FACTORS>(a[k][v], h[v], b[k][v]);
-                o.r[k].v[v] = (T)(m.live >> k & 1 ? h[v] : 0.f);
-            }
-        o.store(p.out, p.out_at, batch, t, c, p.length, p.channels);
-        x = next_x;
-        g = next_g;
+            for (int v = 0; v < V; ++v) h[v] = onward<FACTORS>(a[k][v], h[v], b[k][v]);
+            o.w[k] = pack<T>(h);
+        }
+    };
+    const Side<T> x_side(p.x, p.x_at, seat), g_side(p.gates, p.gates_at, seat), o_side(p.out, p.out_at, seat);
+    struct Tile {
+        Steps<T> x, g;
+        Documents documents;
+    };
+    const int used = seat.used();
+    auto load = [&](Tile& s, int i) {
+        const bool there = i < used;
+        i = min(i, used - 1);
+        const int begin = seat.first + i * kTile;
+        x_side.load(s.x, seat, i, p.length - begin, there);
+        g_side.load(s.g, seat, i, p.length - begin, there);
+        if (DOCS) s.documents.load(p, seat.batch, begin + seat.own);
+    };
+    Tile one;
+    if (used > 0) load(one, 0);
+    for (int i = 0; i < used; ++i) {
+        const int begin = seat.first + i * kTile, count = min(max(seat.length - begin - seat.own, 0), kSteps);
+        float a[kSteps][V], b[kSteps][V];
+        maps<T, FACTORS>(one.x, one.g, a, b);
+        Marks m = {(1u << count) - 1, 0, count};
+        if (DOCS) m = one.documents.marks(count);
+        mark<V>(m, a, b);
+        load(one, i + 1);
+        Steps<T> o;
+        states(a, b, begin, o);
+        hide(m, o);
+        o_side.store(o, seat, i, p.length - begin);
     }
-    if (p.final && own == 0) store_state<V>(p.final, batch * p.final_b, c, p.channels, carry);
+    for (int i = used; i < seat.tiles; ++i) {  // behind the sequence
+        const int begin = seat.first + i * kTile;
+        if (p.states && seat.own == 0)
+            store_state<V>(p.states, seat.batch * p.states_at.b + (int64_t)(begin / kBlock) * p.states_at.t, seat.c, p.channels, carry);
+        Steps<T> o = {};
+        o_side.store(o, seat, i, p.length - begin);
+    }
+    if (p.final && seat.own == 0 && seat.range == p.ranges - 1) store_state<V>(p.final, seat.batch * p.final_b, seat.c, p.channels, carry);
 }
 
-template <class T, int V, bool FACTORS>
-__global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(const RecurrenceParams p) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), slot = (lane & (kLanes - 1)) * V;
-    const int64_t batch = blockIdx.x / (unsigned)p.groups;
-    const int c = (int)(blockIdx.x % (unsigned)p.groups) * kLanes * V + slot;
-    const int length = p.lengths ? min(max(p.lengths[batch * p.lengths_b], 0), p.length) : p.length;
-    const int own = (wave * 4 + lane / kLanes) * kSteps;
-    __shared__ float2 parts[2][kWaves][kLanes * V];
-    __shared__ float back_parts[2][kWaves][kLanes * V];
-    float carry[V];  // the gradient of the state behind the tile
-    load_state<V>(p.final_grad, batch * p.final_grad_b, c, p.channels, carry);
+template <class T, int LANES, bool FACTORS, bool DOCS>
+__global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_kernel(const RecurrenceParams p) {
+    constexpr int V = kPack<T>, kWaves = Team<LANES>::kWaves;
+    const Seat<T, LANES> seat(p);
+    if (!seat.there(p.ranges)) return;
+    const int lane = seat.lane, wave = seat.wave, slot = seat.slot;
+    __shared__ float2 parts[2][kWaves][LANES * V];
+    __shared__ float back_parts[2][kWaves][LANES * V];
+    float carry[V];  // the gradient of the state behind a tile
+    load_state<V>(p.final_grad, seat.batch * p.final_grad_b, seat.c, p.channels, carry);
+    for (int r = p.ranges - 1; r > seat.range; --r)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (seat.c + v < p.channels) {
+                const float2 m = p.carry[(int64_t)r * p.batch * p.channels + seat.state + v];
+                carry[v] = onward<FACTORS>(m.x, carry[v], m.y);
+            }
     int turn = 0;
-    for (int begin = (p.length - 1) / kTile * kTile; begin >= 0 && p.length > 0; begin -= kTile, turn ^= 1) {
-        const int t = begin + own;
-        Steps<T, V> x, g, d;
-        x.load(p.x, p.x_at, batch, t, c, length, p.channels);
-        g.load(p.gates, p.gates_at, batch, t, c, length, p.channels);
-        d.load(p.out_grad, p.out_grad_at, batch, t, c, length, p.channels);
-        float state[V];
-        load_state<V>(p.states, batch * p.states_at.b + (int64_t)(begin / kBlock) * p.states_at.t, c, p.channels, state);
-        const Marks m(p, batch, t, length);
-        float a[kSteps][V], b[kSteps][V], A[V], B[V], preA[V], preB[V], back[V], behindA[V], behindB[V], h[V], l[V];
-        maps<T, V, FACTORS>(x, g, m, a, b);
-        if (m.live != kAll)
+    // From a tile's inputs to the gradients of x and gates, in their places.  `more` is called as soon as the inputs are in
+    // other registers.  What one instruction makes of them again (the halves of a pack, b = rest x) is not kept from the first walk to
+    // the second: registers decide how many wavefronts there are.
+    auto gradients = [&](Steps<T>& x, Steps<T>& g, Steps<T>& d, const float (&state)[V], const Marks& m, auto&& more) {
+        float a[kSteps][V], rest[kSteps][V], A[V], B[V], preA[V], preB[V], back[V], behindA[V], behindB[V], h[V], l[V];
+        hide(m, x);
+        hide(m, d);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            float f[V];
+            unpack<T>(g.w[k], f);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (FACTORS) a[k][v] = f[v];
+                else sigmoids<T>(f[v], a[k][v], rest[k][v]);
+            }
+        }
+        if (!m.plain())
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-                for (int v = 0; v < V; ++v) d.r[k].v[v] = m.live >> k & 1 ? d.r[k].v[v] : (T)0.f;
+                for (int v = 0; v < V; ++v) {
+                    a[k][v] = m.cut >> k & 1 ? 0.f : k < m.count ? a[k][v] : 1.f;
+                    if (!FACTORS) rest[k][v] = m.live >> k & 1 ? rest[k][v] : 0.f;
+                }
+        Steps<T> in = x, gate = g, out_grad = d;
+        more();
+        auto put_in = [&](int k, float (&b)[V]) {
+            unpack<T>(in.w[k], b);
+#pragma unroll
+            for (int v = 0; v < V; ++v) b[v] = FACTORS ? b[v] : rest[k][v] * b[v];
+        };
+#pragma unroll
+        for (int v = 0; v < V; ++v) A[v] = 1, B[v] = 0, back[v] = 0;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            float b[V];
+            put_in(k, b);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                A[v] = together<FACTORS>(A[v], a[k][v]);
+                B[v] = onward<FACTORS>(a[k][v], B[v], b[v]);
+            }
+        }
+#pragma unroll
+        for (int k = kSteps - 1; k >= 0; --k) {
+            float f[V];
+            unpack<T>(out_grad.w[k], f);
+#pragma unroll
+            for (int v = 0; v < V; ++v) back[v] = onward<FACTORS>(a[k][v], back[v] + f[v], 0.f);
+        }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            A[v] = 1, B[v] = 0, back[v] = 0;
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                A[v] = together<FACTORS>(A[v], a[k][v]);
-                B[v] = onward<FACTORS>(a[k][v], B[v], b[k][v]);
-            }
-#pragma unroll
-            for (int k = kSteps - 1; k >= 0; --k) back[v] = onward<FACTORS>(a[k][v], back[v] + (float)d.r[k].v[v], 0.f);
             float again = A[v];
-            across<FACTORS, false>(lane, A[v], B[v], preA[v], preB[v]);
-            across<FACTORS, true>(lane, again, back[v], behindA[v], behindB[v]);
-            if (lane < kLanes) {
+            across<LANES, FACTORS, false>(lane, A[v], B[v], preA[v], preB[v]);
+            across<LANES, FACTORS, true>(lane, again, back[v], behindA[v], behindB[v]);
+            if (lane < LANES) {
                 parts[turn][wave][slot + v] = make_float2(A[v], B[v]);
                 back_parts[turn][wave][slot + v] = back[v];
             }
         }
         __syncthreads();
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            h[v] = state[v];
+        for (int v = 0; v < V; ++v) h[v] = state[v];
+        for (int w = 0; w < wave; ++w)
 #pragma unroll
-            for (int w = 0; w < kWaves - 1; ++w) {
+            for (int v = 0; v < V; ++v) {
                 const float2 part = parts[turn][w][slot + v];
-                if (w < wave) h[v] = onward<FACTORS>(part.x, h[v], part.y);
+                h[v] = onward<FACTORS>(part.x, h[v], part.y);
             }
+#pragma unroll 4
+        for (int w = kWaves - 1; w >= 0; --w)
 #pragma unroll
-            for (int w = kWaves - 1; w >= 0; --w) {
+            for (int v = 0; v < V; ++v) {
                 if (w == wave) l[v] = carry[v];
                 carry[v] = onward<FACTORS>(parts[turn][w][slot + v].x, carry[v], back_parts[turn][w][slot + v]);
             }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
             h[v] = onward<FACTORS>(preA[v], h[v], preB[v]);
             l[v] = onward<FACTORS>(behindA[v], l[v], behindB[v]);
         }
-        // forwards: b becomes the state before each position (what the factor is multiplied with)
+        turn ^= 1;
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k)
+        for (int k = 0; k < kSteps; ++k) asm volatile("" : "+v"(in.w[k]), "+v"(out_grad.w[k]));  // (unpacked again from here on)
+        // forwards: what a factor's change is worth, the state before (less x, which a gate that is not a factor takes as much from)
+        float worth[kSteps][V];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            float f[V];
+            unpack<T>(in.w[k], f);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const float before = h[v];
-                h[v] = onward<FACTORS>(a[k][v], h[v], b[k][v]);
-                b[k][v] = m.cut >> k & 1 ? 0.f : before;
+                const float before = DOCS && (m.cut >> k & 1) ? 0.f : h[v];
+                worth[k][v] = FACTORS ? before : before - f[v];
+                h[v] = onward<FACTORS>(a[k][v], h[v], FACTORS ? f[v] : rest[k][v] * f[v]);
             }
+        }
         // backwards
 #pragma unroll
-        for (int k = kSteps - 1; k >= 0; --k)
+        for (int k = kSteps - 1; k >= 0; --k) {
+            float dx[V], dg[V], ds[V], own[V];
+            unpack<T>(out_grad.w[k], ds);
+#pragma unroll
+            for (int v = 0; v < V; ++v) own[v] = a[k][v];
+            if (DOCS && !FACTORS && (m.cut >> k & 1)) {  // where the state before was dropped, the gate still weighs x
+                float gs[V], again;
+                unpack<T>(gate.w[k], gs);
+#pragma unroll
+                for (int v = 0; v < V; ++v) sigmoids<T>(gs[v], own[v], again);
+            }
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const float here = l[v] + (float)d.r[k].v[v], in = (float)x.r[k].v[v];
+                const float here = l[v] + ds[v];
                 l[v] = onward<FACTORS>(a[k][v], here, 0.f);
-                float dx = here, dg = here * b[k][v];
-                if (!FACTORS) {
-                    float own_a, rest;
-                    sigmoids<T>((float)g.r[k].v[v], own_a, rest);
-                    dx = here * rest;
-                    dg = dx * (b[k][v] - in) * own_a;
-                }
-                const bool live = m.live >> k & 1;
-                x.r[k].v[v] = (T)(live ? dx : 0.f);
-                g.r[k].v[v] = (T)(live ? dg : 0.f);
+                dx[v] = FACTORS ? here : here * rest[k][v];
+                dg[v] = FACTORS ? here * worth[k][v] : dx[v] * worth[k][v] * own[v];
             }
-        x.store(p.x_grad, p.x_grad_at, batch, t, c, p.length, p.channels);
-        g.store(p.gates_grad, p.gates_grad_at, batch, t, c, p.length, p.channels);
+            x.w[k] = pack<T>(dx);
+            g.w[k] = pack<T>(dg);
+        }
+        hide(m, x);
+        hide(m, g);
+    };
+    const Side<T> x_side(p.x, p.x_at, seat), g_side(p.gates, p.gates_at, seat), d_side(p.out_grad, p.out_grad_at, seat);
+    const Side<T> dx_side(p.x_grad, p.x_grad_at, seat), dg_side(p.gates_grad, p.gates_grad_at, seat);
+    struct Tile {
+        Steps<T> x, g, d;
+        float state[V];
+        Documents documents;
+    };
+    const int used = seat.used();
+    auto load = [&](Tile& s, int i) {
+        const bool there = i >= 0;
+        i = max(i, 0);
+        const int begin = seat.first + i * kTile;
+        x_side.load(s.x, seat, i, p.length - begin, there);
+        g_side.load(s.g, seat, i, p.length - begin, there);
+        d_side.load(s.d, seat, i, p.length - begin, there);
+        const float* state = p.states + seat.batch * p.states_at.b + (int64_t)(begin / kBlock) * p.states_at.t + seat.c;
+#pragma unroll
+        for (int v = 0; v < V; ++v) s.state[v] = state[seat.lone ? 0 : v];
+        if (DOCS) s.documents.load(p, seat.batch, begin + seat.own);
+    };
+    for (int i = seat.tiles - 1; i >= used; --i) {  // behind the sequence
+        const Steps<T> none = {};
+        dx_side.store(none, seat, i, p.length - seat.first - i * kTile);
+        dg_side.store(none, seat, i, p.length - seat.first - i * kTile);
     }
-    if (p.initial_grad && own == 0) store_state<V>(p.initial_grad, batch * p.initial_grad_b, c, p.channels, carry);
+    Tile one;
+    if (used > 0) load(one, used - 1);
+    for (int i = used - 1; i >= 0; --i) {
+        const int begin = seat.first + i * kTile, count = min(max(seat.length - begin - seat.own, 0), kSteps);
+        Marks m = {(1u << count) - 1, 0, count};
+        if (DOCS) m = one.documents.marks(count);
+        Tile next;
+        gradients(one.x, one.g, one.d, one.state, m, [&] { load(next, i - 1); });
+        dx_side.store(one.x, seat, i, p.length - begin);
+        dg_side.store(one.g, seat, i, p.length - begin);
+        one = next;
+    }
+    if (p.initial_grad && seat.own == 0 && seat.range == 0) store_state<V>(p.initial_grad, seat.batch * p.initial_grad_b, seat.c, p.channels, carry);
 }
 
-template <class T, int V>
-void launch_recurrence(const char* op, const RecurrenceParams& p, bool backward, bool factors, int64_t blocks, hipStream_t stream) {
-    launch(op, backward ? (factors ? recurrence_backward_kernel<T, V, true> : recurrence_backward_kernel<T, V, false>)
-                        : (factors ? recurrence_kernel<T, V, true> : recurrence_kernel<T, V, false>), (unsigned)blocks, kThreads, stream, p);
+// What each range of positions does to the state before it (to the gradient behind it where BACK): the map of all its positions.  A
+// thread goes through its share of them by itself, and all meet once.
+template <class T, int LANES, bool FACTORS, bool DOCS, bool BACK>
+__global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_range_kernel(const RecurrenceParams p) {
+    constexpr int V = kPack<T>, kWaves = Team<LANES>::kWaves;
+    const Seat<T, LANES> seat(p);
+    if (!seat.there(p.ranges - 1)) return;
+    const int range = seat.range + BACK;  // the last one has none behind it, the first one none before it
+    const int first = range * p.tiles * kTile + seat.own * p.tiles;  // this thread's first position, of tiles * kSteps
+    const bool whole = !seat.lone && (range + 1) * p.tiles * kTile <= p.length;
+    float A[V], B[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) A[v] = 1, B[v] = 0;
+    auto compose = [&](const Steps<T>& x, const Steps<T>& g, const Marks& m) {
+        float a[kSteps][V], b[kSteps][V];
+        maps<T, FACTORS>(x, g, a, b);
+        if (BACK) {
+            // b is the gradient that joins here: what comes before it is all that is scaled, h -> a (h + d)
+            Steps<T> d = x;
+            hide(m, d);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) unpack<T>(d.w[k], b[k]);
+        }
+        if (!m.plain()) {
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    a[k][v] = m.cut >> k & 1 ? 0.f : k < m.count ? a[k][v] : 1.f;
+                    if (!BACK) b[k][v] = m.live >> k & 1 ? b[k][v] : 0.f;
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int k = BACK ? kSteps - 1 - i : i;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                B[v] = BACK ? onward<FACTORS>(a[k][v], B[v] + b[k][v], 0.f) : onward<FACTORS>(a[k][v], B[v], b[k][v]);
+                A[v] = together<FACTORS>(A[v], a[k][v]);
+            }
+        }
+    };
+    const Rows other_at = BACK ? p.out_grad_at : p.x_at;
+    const char* other = (const char*)(BACK ? p.out_grad : p.x) + (seat.batch * other_at.b + seat.c) * (int64_t)sizeof(T);
+    const char* gates = (const char*)p.gates + (seat.batch * p.gates_at.b + seat.c) * (int64_t)sizeof(T);
+    const int64_t other_step = other_at.t * (int64_t)sizeof(T), gates_step = p.gates_at.t * (int64_t)sizeof(T);
+    auto load = [&](Steps<T>& s, const char* from, int64_t step, int t) {
+        if (whole) {
+            from += t * step;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) s.w[k] = ((const Word<T>*)(from + k * step))->w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                const char* at = from + min(t + k, p.length - 1) * step;
+                s.w[k] = seat.lone ? *(const unsigned short*)at : ((const Word<T>*)at)->w;
+            }
+        }
+    };
+    for (int i = 0; i < p.tiles; ++i) {
+        const int t = first + (BACK ? p.tiles - 1 - i : i) * kSteps, count = min(max(seat.length - t, 0), kSteps);
+        Steps<T> x, g;
+        load(x, other, other_step, t);
+        load(g, gates, gates_step, t);
+        Marks m = {(1u << count) - 1, 0, count};
+        if (DOCS) {
+            Documents d;
+            d.load(p, seat.batch, t);
+            m = d.marks(count);
+        }
+        compose(x, g, m);
+    }
+    __shared__ float2 parts[kWaves][LANES * V];
+    float preA, preB;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        across<LANES, FACTORS, BACK>(seat.lane, A[v], B[v], preA, preB);
+        if (seat.lane < LANES) parts[seat.wave][seat.slot + v] = make_float2(A[v], B[v]);
+    }
+    __syncthreads();
+    if (seat.own != 0) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        float a = 1, b = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            const float2 part = parts[BACK ? kWaves - 1 - i : i][seat.slot + v];
+            b = onward<FACTORS>(part.x, b, part.y);
+            a = together<FACTORS>(a, part.x);
+        }
+        if (seat.c + v < p.channels) p.carry[(int64_t)range * p.batch * p.channels + seat.state + v] = make_float2(a, b);
+    }
 }
+
+template <class T, int LANES, bool FACTORS, bool DOCS>
+void launch_recurrence(const char* op, const RecurrenceParams& p, bool backward, hipStream_t stream) {
+    const auto blocks = [&](int ranges) { return (unsigned)(((int64_t)p.groups * p.batch * ranges + 7) / 8 * 8); };
+    constexpr int threads = Team<LANES>::kThreads;
+    if constexpr (LANES == kNarrow)  // (rows are wide where there is no need of ranges)
+        if (p.ranges > 1)
+            launch(op, backward ? recurrence_range_kernel<T, LANES, FACTORS, DOCS, true> : recurrence_range_kernel<T, LANES, FACTORS, DOCS, false>,
+                   blocks(p.ranges - 1), threads, stream, p);
+    launch(op, backward ? recurrence_backward_kernel<T, LANES, FACTORS, DOCS> : recurrence_kernel<T, LANES, FACTORS, DOCS>, blocks(p.ranges), threads, stream, p);
+}
+
+template <class T, int LANES>
+void launch_recurrence(const char* op, const RecurrenceParams& p, bool backward, bool factors, hipStream_t stream) {
+    if (factors && p.documents) launch_recurrence<T, LANES, true, true>(op, p, backward, stream);
+    else if (factors) launch_recurrence<T, LANES, true, false>(op, p, backward, stream);
+    else if (p.documents) launch_recurrence<T, LANES, false, true>(op, p, backward, stream);
+    else launch_recurrence<T, LANES, false, false>(op, p, backward, stream);
+}
+
+// How channels are cut into rows and positions into ranges.
+struct Cut {
+    int lanes, groups, tiles, ranges;  // tiles: of a range
+    Cut(const adhip_array& x) {
+        const int64_t v = 4 / type_bytes(x.type), channels = x.dims[2], batch = std::max<int64_t>(x.dims[0], 1);
+        lanes = (channels + kWide * v - 1) / (kWide * v) * batch >= kFull ? kWide : kNarrow;
+        groups = (int)((channels + lanes * v - 1) / (lanes * v));
+        const int64_t all = (x.dims[1] + kTile - 1) / kTile, blocks = std::max<int64_t>(groups * batch, 1);
+        const int64_t want = lanes == kWide ? 1 : std::max<int64_t>(1, std::min<int64_t>(kFull / blocks, all / 2));
+        tiles = (int)std::max<int64_t>(1, (all + want - 1) / want);
+        ranges = (int)std::max<int64_t>(1, (all + tiles - 1) / tiles);
+    }
+    size_t workspace(const adhip_array& x) const { return ranges == 1 ? 0 : (size_t)ranges * (size_t)x.dims[0] * (size_t)x.dims[2] * sizeof(float2); }
+};
 
 // Shape and type of x: [batch, length, channels].
 void check_x(const char* op, const adhip_array& x) {
@@ -425,15 +778,26 @@ void recurrence(const char* op, const adhip_recurrence_args& g, bool backward, h
     } else {
         p.out = g.out.data, p.initial = (const float*)g.initial.data, p.final = (float*)g.final.data;
     }
+    const Cut cut(g.x);
     p.length = (int)length;
     p.channels = (int)channels;
-    const int v = g.x.type == ADHIP_BF16 ? 2 : 1;
-    p.groups = (int)((channels + kLanes * v - 1) / (kLanes * v));
+    p.batch = (int)batch;
+    p.groups = cut.groups;
+    p.ranges = cut.ranges;
+    p.tiles = cut.tiles;
     const int64_t blocks = batch * p.groups;
-    ADHIP_CHECK(fits_launch(blocks, kThreads), "%s: %lld sequences of %lld channels are too many for one call", op, (long long)batch, (long long)channels);
+    ADHIP_CHECK(fits_launch(blocks + 8, Team<kWide>::kThreads), "%s: %lld sequences of %lld channels are too many for one call", op, (long long)batch, (long long)channels);
     if (blocks == 0) return;
-    if (g.x.type == ADHIP_BF16) launch_recurrence<bf16, 2>(op, p, backward, g.factors != 0, blocks, stream);
-    else launch_recurrence<float, 1>(op, p, backward, g.factors != 0, blocks, stream);
+    ADHIP_CHECK(cut.workspace(g.x) == 0 || (g.workspace && (uintptr_t)g.workspace % 16 == 0 && g.workspace_bytes >= cut.workspace(g.x)),
+                "%s: the workspace has %zu bytes, %zu are wanted, aligned to 16", op, g.workspace ? g.workspace_bytes : (size_t)0, cut.workspace(g.x));
+    p.carry = (float2*)g.workspace;
+    for (const Rows* at : {&p.x_at, &p.gates_at, &p.out_at, &p.out_grad_at, &p.x_grad_at, &p.gates_grad_at})
+        ADHIP_CHECK(at->t <= (1 << 21), "%s: positions %lld elements apart, at most 2^21 are wanted", op, (long long)at->t);
+    const bool factors = g.factors != 0, wide = cut.lanes == kWide;
+    if (g.x.type == ADHIP_BF16 && wide) launch_recurrence<bf16, kWide>(op, p, backward, factors, stream);
+    else if (g.x.type == ADHIP_BF16) launch_recurrence<bf16, kNarrow>(op, p, backward, factors, stream);
+    else if (wide) launch_recurrence<float, kWide>(op, p, backward, factors, stream);
+    else launch_recurrence<float, kNarrow>(op, p, backward, factors, stream);
 }
 
 }  // namespace
@@ -446,7 +810,7 @@ int adhip_recurrence_workspace(adhip_ctx* ctx, const adhip_recurrence_args* args
         const char* op = "adhip_recurrence_workspace";
         ADHIP_CHECK(args && bytes, "%s: no arguments", op);
         adhip::check_x(op, args->x);
-        *bytes = 0;
+        *bytes = adhip::Cut(args->x).workspace(args->x);
     });
 }
 

@@ -301,7 +301,8 @@ int adhip_layer_norm_backward(adhip_ctx* ctx, const adhip_layer_norm_args* args,
  * or document.
  * states (f32 [batch, ceil(length / 256), channels]; may be left out) receives the state before every 256th position, for the
  * backward pass.  out may be x or gates themselves, under the same strides.
- * workspace: adhip_recurrence_workspace() bytes, aligned to 16, used until the call's kernels are done; needs no more where it is 0. */
+ * Positions lie at most 2^21 elements apart.
+ * workspace: adhip_recurrence_workspace() bytes, aligned to 16, used until the call's kernels are done; may be left out where that is 0. */
 #define ADHIP_RECURRENCE_BLOCK 256
 typedef struct adhip_recurrence_args {
     adhip_array x, gates, out, initial, final, states, lengths, documents;
