@@ -25,6 +25,8 @@ constexpr int kSteps = 8;                       // consecutive positions of a th
 template <int LANES>
 struct Team {
     static constexpr int kThreads = kTile / kSteps * LANES, kWaves = kThreads / 64, kSpread = 64 / LANES;
+    // A sequence shorter than a tile takes no more wavefronts than it has positions for.
+    static int threads(int length) { return std::min(kThreads, (std::max(length, 1) + kSteps * kSpread - 1) / (kSteps * kSpread) * 64); }
 };
 constexpr unsigned kAll = (1u << kSteps) - 1;
 constexpr int kNarrow = 16, kWide = 32;         // lanes of a row of channels
@@ -309,6 +311,35 @@ __device__ __forceinline__ void across(int lane, float& A, float& B, float& preA
     }
 }
 
+// A state carried over whole ranges, from `r` on up to, but not, `end`.  The maps are loaded eight at once: there may be many.
+template <class T, int LANES, bool FACTORS>
+__device__ __forceinline__ void over_ranges(const RecurrenceParams& p, const Seat<T, LANES>& seat, int r, int end, int way, float (&h)[kPack<T>]) {
+    constexpr int kAtOnce = 8;
+    const int64_t range = (int64_t)p.batch * p.channels;
+    while (r != end) {
+        float2 m[kAtOnce][kPack<T>];
+        const int n = min(abs(end - r), kAtOnce);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+            for (int v = 0; v < kPack<T>; ++v) m[i][v] = p.carry[(r + way * min(i, n - 1)) * range + seat.state + (seat.lone ? 0 : v)];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+            for (int v = 0; v < kPack<T>; ++v)
+                if (i < n) h[v] = onward<FACTORS>(m[i][v].x, h[v], m[i][v].y);
+        r += way * n;
+    }
+}
+
+// What wavefronts that are not there do to a state: nothing.
+template <int WAVES, int PARTS>
+__device__ __forceinline__ void fill_absent(float2 (&parts)[2][WAVES][PARTS]) {
+    const int waves = blockDim.x / 64;
+    for (int i = threadIdx.x; i < (WAVES - waves) * PARTS; i += blockDim.x)
+        parts[0][waves + i / PARTS][i % PARTS] = parts[1][waves + i / PARTS][i % PARTS] = make_float2(1, 0);
+}
+
 template <class T, int LANES, bool FACTORS, bool DOCS>
 __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const RecurrenceParams p) {
     constexpr int V = kPack<T>, kWaves = Team<LANES>::kWaves;
@@ -316,15 +347,10 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const
     if (!seat.there(p.ranges)) return;
     const int lane = seat.lane, wave = seat.wave, slot = seat.slot;
     __shared__ float2 parts[2][kWaves][LANES * V];  // (by turns: the other one's barrier stands between readers and writers)
+    fill_absent(parts);
     float carry[V];
     load_state<V>(p.initial, seat.batch * p.initial_b, seat.c, p.channels, carry);
-    for (int r = 0; r < seat.range; ++r)
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (seat.c + v < p.channels) {
-                const float2 m = p.carry[(int64_t)r * p.batch * p.channels + seat.state + v];
-                carry[v] = onward<FACTORS>(m.x, carry[v], m.y);
-            }
+    over_ranges<T, LANES, FACTORS>(p, seat, 0, seat.range, 1, carry);
     int turn = 0;
     // From the maps of a tile to its states, and the state behind it.
     auto states = [&](const float (&a)[kSteps][V], const float (&b)[kSteps][V], int begin, Steps<T>& o) {
@@ -407,15 +433,14 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
     const int lane = seat.lane, wave = seat.wave, slot = seat.slot;
     __shared__ float2 parts[2][kWaves][LANES * V];
     __shared__ float back_parts[2][kWaves][LANES * V];
+    fill_absent(parts);
+    for (int i = blockDim.x + threadIdx.x; i < Team<LANES>::kThreads; i += blockDim.x)
+        if (i % 64 < LANES)
+#pragma unroll
+            for (int v = 0; v < V; ++v) back_parts[0][i / 64][i % 64 * V + v] = back_parts[1][i / 64][i % 64 * V + v] = 0;
     float carry[V];  // the gradient of the state behind a tile
     load_state<V>(p.final_grad, seat.batch * p.final_grad_b, seat.c, p.channels, carry);
-    for (int r = p.ranges - 1; r > seat.range; --r)
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (seat.c + v < p.channels) {
-                const float2 m = p.carry[(int64_t)r * p.batch * p.channels + seat.state + v];
-                carry[v] = onward<FACTORS>(m.x, carry[v], m.y);
-            }
+    over_ranges<T, LANES, FACTORS>(p, seat, p.ranges - 1, seat.range, -1, carry);
     int turn = 0;
     // From a tile's inputs to the gradients of x and gates, in their places.  `more` is called as soon as the inputs are in
     // other registers.  What one instruction makes of them again (the halves of a pack, b = rest x) is not kept from the first walk to
@@ -675,15 +700,70 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_range_kernel
     }
 }
 
+// Few positions, as a decoder takes them one by one: a lane goes through those of its channels by itself.  A lone last channel belongs to
+// one lane alone (in place, a pack of two would read what its neighbour may already have written).
+template <class T, bool FACTORS>
+__global__ __launch_bounds__(256) void recurrence_step_kernel(const RecurrenceParams p) {
+    constexpr int V = kPack<T>;
+    const unsigned packs = (unsigned)((p.channels + V - 1) / V);
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, batch = at / packs;
+    if (batch >= p.batch) return;
+    const int c = (int)(at - batch * packs) * V;
+    const bool lone = c + V > p.channels;
+    const int length = p.lengths ? min(max(p.lengths[batch * p.lengths_b], 0), p.length) : p.length;
+    const auto address = [&](const void* from, const Rows& rows, int t) { return (char*)from + (batch * rows.b + t * rows.t + c) * (int64_t)sizeof(T); };
+    Steps<T> x = {}, g = {};
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+        if (k < p.length) {
+            const char *from = address(p.x, p.x_at, k), *gate = address(p.gates, p.gates_at, k);
+            x.w[k] = lone ? *(const unsigned short*)from : ((const Word<T>*)from)->w;
+            g.w[k] = lone ? *(const unsigned short*)gate : ((const Word<T>*)gate)->w;
+        }
+    float h[V];
+    load_state<V>(p.initial, batch * p.initial_b, c, p.channels, h);
+    if (p.states) store_state<V>(p.states, batch * p.states_at.b, c, p.channels, h);
+    Marks m = {(1u << length) - 1, 0, length};
+    if (p.documents) {
+        Documents d;
+        d.load(p, batch, 0);
+        m = d.marks(length);
+    }
+    float a[kSteps][V], b[kSteps][V];
+    maps<T, FACTORS>(x, g, a, b);
+    mark<V>(m, a, b);
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+        if (k < p.length) {
+            float o[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                h[v] = onward<FACTORS>(a[k][v], h[v], b[k][v]);
+                o[v] = m.live >> k & 1 ? h[v] : 0.f;
+            }
+            char* to = address(p.out, p.out_at, k);
+            const unsigned w = pack<T>(o);
+            if (lone) *(unsigned short*)to = (unsigned short)w;
+            else ((Word<T>*)to)->w = w;
+        }
+    if (p.final) store_state<V>(p.final, batch * p.final_b, c, p.channels, h);
+}
+
+// Where there are workgroups enough, wide rows bring whole cache lines (forward and f32 backward 5 to 10 % faster).  The backward pass of bf16,
+// and of documents, has no registers for two sets of them: 128 a thread, with the spills that come of it, against twice as many.
+constexpr bool wide_pays(int type, bool backward, bool documents) { return !backward || (type == ADHIP_F32 && !documents); }
+
 template <class T, int LANES, bool FACTORS, bool DOCS>
 void launch_recurrence(const char* op, const RecurrenceParams& p, bool backward, hipStream_t stream) {
+    const unsigned threads = (unsigned)Team<LANES>::threads(p.length);
     const auto blocks = [&](int ranges) { return (unsigned)(((int64_t)p.groups * p.batch * ranges + 7) / 8 * 8); };
-    constexpr int threads = Team<LANES>::kThreads;
-    if constexpr (LANES == kNarrow)  // (rows are wide where there is no need of ranges)
-        if (p.ranges > 1)
-            launch(op, backward ? recurrence_range_kernel<T, LANES, FACTORS, DOCS, true> : recurrence_range_kernel<T, LANES, FACTORS, DOCS, false>,
-                   blocks(p.ranges - 1), threads, stream, p);
-    launch(op, backward ? recurrence_backward_kernel<T, LANES, FACTORS, DOCS> : recurrence_kernel<T, LANES, FACTORS, DOCS>, blocks(p.ranges), threads, stream, p);
+    if (p.ranges > 1)
+        launch(op, backward ? recurrence_range_kernel<T, LANES, FACTORS, DOCS, true> : recurrence_range_kernel<T, LANES, FACTORS, DOCS, false>,
+               blocks(p.ranges - 1), Team<LANES>::kThreads, stream, p);
+    if (!backward) launch(op, recurrence_kernel<T, LANES, FACTORS, DOCS>, blocks(p.ranges), threads, stream, p);
+    {
+        if (backward) launch(op, recurrence_backward_kernel<T, LANES, FACTORS, DOCS>, blocks(p.ranges), threads, stream, p);
+    }
 }
 
 template <class T, int LANES>
@@ -697,12 +777,13 @@ void launch_recurrence(const char* op, const RecurrenceParams& p, bool backward,
 // How channels are cut into rows and positions into ranges.
 struct Cut {
     int lanes, groups, tiles, ranges;  // tiles: of a range
-    Cut(const adhip_array& x) {
+    Cut(const adhip_array& x, bool wide) {
         const int64_t v = 4 / type_bytes(x.type), channels = x.dims[2], batch = std::max<int64_t>(x.dims[0], 1);
-        lanes = (channels + kWide * v - 1) / (kWide * v) * batch >= kFull ? kWide : kNarrow;
-        groups = (int)((channels + lanes * v - 1) / (lanes * v));
-        const int64_t all = (x.dims[1] + kTile - 1) / kTile, blocks = std::max<int64_t>(groups * batch, 1);
-        const int64_t want = lanes == kWide ? 1 : std::max<int64_t>(1, std::min<int64_t>(kFull / blocks, all / 2));
+        const auto blocks = [&](int lanes) { return (channels + lanes * v - 1) / (lanes * v) * batch; };
+        lanes = wide && blocks(kNarrow) > kFull ? kWide : kNarrow;
+        groups = (int)(blocks(lanes) / batch);
+        const int64_t all = (x.dims[1] + kTile - 1) / kTile;
+        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kFull / std::max<int64_t>(blocks(lanes), 1), all / 2));
         tiles = (int)std::max<int64_t>(1, (all + want - 1) / want);
         ranges = (int)std::max<int64_t>(1, (all + tiles - 1) / tiles);
     }
@@ -778,7 +859,9 @@ void recurrence(const char* op, const adhip_recurrence_args& g, bool backward, h
     } else {
         p.out = g.out.data, p.initial = (const float*)g.initial.data, p.final = (float*)g.final.data;
     }
-    const Cut cut(g.x);
+    for (const Rows* at : {&p.x_at, &p.gates_at, &p.out_at, &p.out_grad_at, &p.x_grad_at, &p.gates_grad_at})
+        ADHIP_CHECK(at->t <= (1 << 21), "%s: positions %lld elements apart, at most 2^21 are wanted", op, (long long)at->t);
+    const Cut cut(g.x, wide_pays(g.x.type, backward, g.documents.data != nullptr));
     p.length = (int)length;
     p.channels = (int)channels;
     p.batch = (int)batch;
@@ -786,14 +869,21 @@ void recurrence(const char* op, const adhip_recurrence_args& g, bool backward, h
     p.ranges = cut.ranges;
     p.tiles = cut.tiles;
     const int64_t blocks = batch * p.groups;
+    const bool factors = g.factors != 0, wide = cut.lanes == kWide;
+    if (!backward && length >= 1 && length <= kSteps) {
+        const int64_t v = 4 / type_bytes(g.x.type), lanes = batch * ((channels + v - 1) / v);
+        ADHIP_CHECK(fits_launch((lanes + 255) / 256, 256), "%s: %lld sequences of %lld channels are too many for one call", op, (long long)batch, (long long)channels);
+        if (lanes == 0) return;
+        launch(op, g.x.type == ADHIP_BF16 ? (factors ? recurrence_step_kernel<bf16, true> : recurrence_step_kernel<bf16, false>)
+                                          : (factors ? recurrence_step_kernel<float, true> : recurrence_step_kernel<float, false>),
+               (unsigned)((lanes + 255) / 256), 256, stream, p);
+        return;
+    }
     ADHIP_CHECK(fits_launch(blocks + 8, Team<kWide>::kThreads), "%s: %lld sequences of %lld channels are too many for one call", op, (long long)batch, (long long)channels);
     if (blocks == 0) return;
     ADHIP_CHECK(cut.workspace(g.x) == 0 || (g.workspace && (uintptr_t)g.workspace % 16 == 0 && g.workspace_bytes >= cut.workspace(g.x)),
                 "%s: the workspace has %zu bytes, %zu are wanted, aligned to 16", op, g.workspace ? g.workspace_bytes : (size_t)0, cut.workspace(g.x));
     p.carry = (float2*)g.workspace;
-    for (const Rows* at : {&p.x_at, &p.gates_at, &p.out_at, &p.out_grad_at, &p.x_grad_at, &p.gates_grad_at})
-        ADHIP_CHECK(at->t <= (1 << 21), "%s: positions %lld elements apart, at most 2^21 are wanted", op, (long long)at->t);
-    const bool factors = g.factors != 0, wide = cut.lanes == kWide;
     if (g.x.type == ADHIP_BF16 && wide) launch_recurrence<bf16, kWide>(op, p, backward, factors, stream);
     else if (g.x.type == ADHIP_BF16) launch_recurrence<bf16, kNarrow>(op, p, backward, factors, stream);
     else if (wide) launch_recurrence<float, kWide>(op, p, backward, factors, stream);
@@ -810,7 +900,7 @@ int adhip_recurrence_workspace(adhip_ctx* ctx, const adhip_recurrence_args* args
         const char* op = "adhip_recurrence_workspace";
         ADHIP_CHECK(args && bytes, "%s: no arguments", op);
         adhip::check_x(op, args->x);
-        *bytes = adhip::Cut(args->x).workspace(args->x);
+        *bytes = std::max(adhip::Cut(args->x, true).workspace(args->x), adhip::Cut(args->x, false).workspace(args->x));
     });
 }
 

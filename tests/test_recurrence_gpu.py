@@ -57,7 +57,8 @@ def check(dev, a, what, *, factors=False, backward=True, **how):
 
 
 SHAPES = [(1, 1, 1), (2, 1, 5), (3, 2, 33), (2, 7, 31), (1, 8, 32), (2, 9, 17), (1, 32, 16), (3, 33, 64), (2, 64, 40), (1, 255, 48), (1, 256, 16),
-          (2, 257, 33), (1, 511, 64), (1, 513, 130), (2, 700, 9), (1, 1025, 65), (300, 3, 7), (1, 5, 2000)]
+          (2, 257, 33), (1, 511, 64), (1, 513, 130), (2, 700, 9), (1, 1025, 65), (300, 3, 7), (1, 5, 2000), (40, 20, 65), (5, 100, 131), (3, 8, 4097),
+          (70, 17, 1025), (3, 40, 3001), (2, 300, 4097)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
