@@ -14,10 +14,11 @@
 namespace adhip {
 namespace {
 
-constexpr int kElements = 16;      // of a row that a lane holds
-constexpr int kGradThreads = 1024;
-constexpr int kGradBlocks = 256;   // a compute unit each: more would leave more partial sums of the weights' gradients
-constexpr int64_t kMostSize = 1024 * kElements;
+constexpr int kElements = 16;          // of a row that a lane holds at most
+constexpr int kThreads = 256;          // of a workgroup that rows of one wavefront and less share
+constexpr int kWaves = 16;             // of a row at most, and of a workgroup of the backward pass
+constexpr int kGradBlocks = 256;       // a compute unit each: more would leave more partial sums of the weights' gradients
+constexpr int64_t kMostSize = kWaves * 64 * kElements;
 
 struct Place {
     int64_t s[3];  // strides of the dims that number the rows
@@ -30,6 +31,7 @@ struct NormParams {
     Place x_at, added_at, total_at, out_at, out_grad_at, total_grad_at, x_grad_at;
     unsigned rows, n1, n2;  // row number (i0 n1 + i1) n2 + i2
     int size, padded;       // padded: of a row of partial sums
+    int waves, groups;      // wavefronts that share a row, and rows that a workgroup has at once
     float eps, centered;    // centered: 1 or 0
 };
 
@@ -52,11 +54,11 @@ struct __attribute__((packed, aligned(sizeof(T)))) Loose {
     T v[N];
 };
 
-// V elements of a row from e on; zeros behind its end.
-template <class T, int V>
+// V elements of a row from e on; zeros behind its end.  Rows that fill their lanes have none (FULL).
+template <class T, int V, bool FULL>
 __device__ __forceinline__ void load_row(const void* row, int64_t at, int e, int size, float (&f)[V]) {
     const T* x = (const T*)row + at + e;
-    if (e + V <= size) {
+    if (FULL || e + V <= size) {
         const Loose<T, V> r = *(const Loose<T, V>*)x;
 #pragma unroll
         for (int k = 0; k < V; ++k) f[k] = (float)r.v[k];
@@ -66,10 +68,10 @@ __device__ __forceinline__ void load_row(const void* row, int64_t at, int e, int
     }
 }
 
-template <class T, int V>
+template <class T, int V, bool FULL>
 __device__ __forceinline__ void store_row(void* row, int64_t at, int e, int size, const float (&f)[V]) {
     T* x = (T*)row + at + e;
-    if (e + V <= size) {
+    if (FULL || e + V <= size) {
         Loose<T, V> r;
 #pragma unroll
         for (int k = 0; k < V; ++k) r.v[k] = (T)f[k];
@@ -103,54 +105,66 @@ __device__ __forceinline__ float lanes_sum(float x) {
     return x;
 }
 
-// Sums of a and b over the lanes of a row.  More than a wavefront meet in LDS, in one of two places by turns: between a
-// place's readers and its next writers stands the other place's barrier.
-template <int LANES, int THREADS>
-struct RowSums {
-    static constexpr int kWaves = THREADS / 64, kOfRow = LANES / 64;
+// The lanes of a row: 16 of a wavefront, or all of 1 to 16 wavefronts.
+template <int LANES>
+struct Team {
+    int waves, wave, group, lane;  // lane: of the row's
     int turn = 0;
-    __device__ __forceinline__ void operator()(float& a, float& b) {
+    __device__ __forceinline__ Team(const NormParams& p) {
+        waves = p.waves;
+        wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        if (LANES == 64) {
+            group = waves == 1 ? wave : wave / waves;
+            lane = (wave - group * waves) * 64 + (threadIdx.x & 63);
+        } else {
+            group = threadIdx.x / LANES;
+            lane = threadIdx.x % LANES;
+        }
+    }
+    __device__ __forceinline__ int lanes() const { return LANES == 64 ? waves * 64 : LANES; }
+    // Sums of a and b over the row.  Those of several wavefronts meet in LDS, in one of two places by turns: between a place's
+    // readers and its next writers stands the other place's barrier.
+    __device__ __forceinline__ void sum(float& a, float& b) {
         a = lanes_sum<LANES>(a);
         b = lanes_sum<LANES>(b);
-        if constexpr (LANES > 64) {
-            __shared__ float2 parts[2][kWaves];
-            const int wave = threadIdx.x >> 6;
-            if ((threadIdx.x & 63) == 0) parts[turn][wave] = make_float2(a, b);
-            __syncthreads();
-            const int first = wave / kOfRow * kOfRow;
-            a = b = 0;
-#pragma unroll
-            for (int i = 0; i < kOfRow; ++i) {
-                const float2 s = parts[turn][first + i];
-                a += s.x;
-                b += s.y;
-            }
-            turn ^= 1;
+        if (LANES < 64 || waves == 1) return;
+        __shared__ float2 parts[2][kWaves];
+        if ((threadIdx.x & 63) == 0) parts[turn][wave] = make_float2(a, b);
+        __syncthreads();
+        a = b = 0;
+        for (int i = 0; i < waves; ++i) {
+            const float2 s = parts[turn][group * waves + i];
+            a += s.x;
+            b += s.y;
         }
+        turn ^= 1;
     }
 };
 
-template <class T, class W, int LANES>
-__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(const NormParams p) {
-    constexpr int kThreads = LANES < 256 ? 256 : LANES, V = 16 / sizeof(T), C = kElements / V;
-    const int lane = threadIdx.x % LANES;
-    RowSums<LANES, kThreads> sums;
+template <class T, class W, int LANES, int C, bool FULL>
+__global__ __launch_bounds__(LANES == 64 ? kWaves * 64 : kThreads) void norm_kernel(const NormParams p) {
+    constexpr int V = 16 / sizeof(T);
+    Team<LANES> team(p);
+    const int lanes = team.lanes();
     const float per = 1.f / (float)p.size;
-    for (unsigned row = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES; row < p.rows; row += gridDim.x * (kThreads / LANES)) {
+    // (all lanes of a workgroup go round equally often: they meet at barriers)
+    for (unsigned first = blockIdx.x * p.groups; first < p.rows; first += gridDim.x * p.groups) {
+        const unsigned row = min(first + team.group, p.rows - 1);
+        const bool there = first + team.group < p.rows;  // (a row too many reads the last one, and writes nothing)
         const RowIndex index(p, row);
         float x[C][V];
 #pragma unroll
-        for (int c = 0; c < C; ++c) load_row<T, V>(p.x, index.at(p.x_at), (c * LANES + lane) * V, p.size, x[c]);
+        for (int c = 0; c < C; ++c) load_row<T, V, FULL>(p.x, index.at(p.x_at), (c * lanes + team.lane) * V, p.size, x[c]);
         if (p.added) {
+            float y[C][V];
+#pragma unroll
+            for (int c = 0; c < C; ++c) load_row<T, V, FULL>(p.added, index.at(p.added_at), (c * lanes + team.lane) * V, p.size, y[c]);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const int e = (c * LANES + lane) * V;
-                float y[V];
-                load_row<T, V>(p.added, index.at(p.added_at), e, p.size, y);
                 // rounded to the arrays' type as it is kept: what is normed here is what the backward pass reads
 #pragma unroll
-                for (int k = 0; k < V; ++k) x[c][k] = (float)(T)(x[c][k] + y[k]);
-                store_row<T, V>(p.total, index.at(p.total_at), e, p.size, x[c]);
+                for (int k = 0; k < V; ++k) x[c][k] = (float)(T)(x[c][k] + y[c][k]);
+                if (there) store_row<T, V, FULL>(p.total, index.at(p.total_at), (c * lanes + team.lane) * V, p.size, x[c]);
             }
         }
         float sum = 0, none = 0;
@@ -160,7 +174,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(const N
             for (int k = 0; k < V; ++k) sum += x[c][k];
         float mean = 0;
         if (p.centered != 0.f) {
-            sums(sum, none);
+            team.sum(sum, none);
             mean = sum * per;
         }
         float squares = 0;
@@ -168,30 +182,31 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(const N
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                x[c][k] = (c * LANES + lane) * V + k < p.size ? x[c][k] - mean : 0.f;
+                x[c][k] = FULL || (c * lanes + team.lane) * V + k < p.size ? x[c][k] - mean : 0.f;
                 squares = __builtin_fmaf(x[c][k], x[c][k], squares);
             }
         none = 0;
-        sums(squares, none);
+        team.sum(squares, none);
         const float root = 1.f / sqrtf(squares * per + p.eps);
-        if (p.stats && lane == 0) *(float2*)(p.stats + 2 * (int64_t)row) = make_float2(mean, root);
+        if (!there) continue;
+        if (p.stats && team.lane == 0) *(float2*)(p.stats + 2 * (int64_t)row) = make_float2(mean, root);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int e = (c * LANES + lane) * V;
+            const int e = (c * lanes + team.lane) * V;
             float w[V];
 #pragma unroll
             for (int k = 0; k < V; ++k) x[c][k] *= root;
             if (p.weight) {
-                load_row<W, V>(p.weight, 0, e, p.size, w);
+                load_row<W, V, FULL>(p.weight, 0, e, p.size, w);
 #pragma unroll
                 for (int k = 0; k < V; ++k) x[c][k] *= w[k];
             }
             if (p.bias) {
-                load_row<W, V>(p.bias, 0, e, p.size, w);
+                load_row<W, V, FULL>(p.bias, 0, e, p.size, w);
 #pragma unroll
                 for (int k = 0; k < V; ++k) x[c][k] += w[k];
             }
-            store_row<T, V>(p.out, index.at(p.out_at), e, p.size, x[c]);
+            store_row<T, V, FULL>(p.out, index.at(p.out_at), e, p.size, x[c]);
         }
     }
 }
@@ -199,37 +214,76 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_kernel(const N
 // With n the normed row and u = out_grad weight:
 //     x_grad = root (u - mean(u) - n mean(u n)) + total_grad      (without the mean of u where the norm takes no mean)
 //     weight_grad = sum over rows of out_grad n,  bias_grad = sum over rows of out_grad
-template <class T, class W, int LANES, bool SUMS>
-__global__ __launch_bounds__(kGradThreads) void norm_backward_kernel(const NormParams p) {
-    constexpr int V = 16 / sizeof(T), C = kElements / V, kRows = kGradThreads / LANES;
-    const int lane = threadIdx.x % LANES;
-    RowSums<LANES, kGradThreads> sums;
+// Where rows fill their lanes (FULL) the next one is asked for as soon as this one is in other registers; loads without a branch are
+// loads that the compiler can count, so it waits for those of this row alone.
+template <class T, class W, int LANES, int C, bool FULL, bool SUMS, bool ADDS>
+__global__ __launch_bounds__(kWaves * 64) void norm_backward_kernel(const NormParams p) {
+    constexpr int V = 16 / sizeof(T);
+    Team<LANES> team(p);
+    const int lanes = team.lanes();
     const float per = 1.f / (float)p.size;
     float dw[C][V] = {}, db[C][V] = {};
-    // (all lanes of a workgroup go round equally often: they meet at barriers)
-    for (unsigned first = blockIdx.x * kRows; first < p.rows; first += gridDim.x * kRows) {
-        const unsigned row = first + threadIdx.x / LANES;
-        const bool there = row < p.rows;
-        const RowIndex index(p, there ? row : 0);
-        float n[C][V], u[C][V];
-        float mean = 0, root = 0;
-        if (there) {
-            const float2 s = *(const float2*)(p.stats + 2 * (int64_t)row);
-            mean = s.x, root = s.y;
-        }
-        float sum = 0, along = 0;
+    struct Row {
+        Loose<T, V> x[C], d[C], more[ADDS ? C : 1];
+        float2 stats;
+    } raw;
+    const auto element = [&](int c) { return (c * lanes + team.lane) * V; };
+    const auto ask = [&](Row& r, unsigned row) {
+        const RowIndex index(p, row);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int e = (c * LANES + lane) * V, size = there ? p.size : 0;
-            float w[V];
-            load_row<T, V>(p.x, index.at(p.x_at), e, size, n[c]);
-            load_row<T, V>(p.out_grad, index.at(p.out_grad_at), e, size, u[c]);
+            r.x[c] = *(const Loose<T, V>*)((const T*)p.x + index.at(p.x_at) + element(c));
+            r.d[c] = *(const Loose<T, V>*)((const T*)p.out_grad + index.at(p.out_grad_at) + element(c));
+            if (ADDS) r.more[c] = *(const Loose<T, V>*)((const T*)p.total_grad + index.at(p.total_grad_at) + element(c));
+        }
+        r.stats = *(const float2*)(p.stats + 2 * (int64_t)row);
+    };
+    const unsigned step = gridDim.x * p.groups;
+    if (FULL) ask(raw, min(blockIdx.x * p.groups + team.group, p.rows - 1));
+    // (all lanes of a workgroup go round equally often: they meet at barriers)
+    for (unsigned first = blockIdx.x * p.groups; first < p.rows; first += step) {
+        const unsigned row = first + team.group;
+        const bool there = row < p.rows;
+        const RowIndex index(p, there ? row : 0);
+        float n[C][V], u[C][V], more[ADDS ? C : 1][V], w[C][V];
+        float mean, root;
+        if (FULL) {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    n[c][k] = (float)raw.x[c].v[k];
+                    u[c][k] = there ? (float)raw.d[c].v[k] : 0.f;
+                    if (ADDS) more[c][k] = (float)raw.more[c].v[k];
+                }
+            mean = raw.stats.x, root = raw.stats.y;
+        } else {
+            const int size = there ? p.size : 0;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                load_row<T, V, false>(p.x, index.at(p.x_at), element(c), size, n[c]);
+                load_row<T, V, false>(p.out_grad, index.at(p.out_grad_at), element(c), size, u[c]);
+                if (ADDS) load_row<T, V, false>(p.total_grad, index.at(p.total_grad_at), element(c), size, more[c]);
+            }
+            mean = root = 0;
+            if (there) {
+                const float2 s = *(const float2*)(p.stats + 2 * (int64_t)row);
+                mean = s.x, root = s.y;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
             if (p.weight) {
-                load_row<W, V>(p.weight, 0, e, p.size, w);
+                load_row<W, V, FULL>(p.weight, 0, element(c), p.size, w[c]);
             } else {
 #pragma unroll
-                for (int k = 0; k < V; ++k) w[k] = 1.f;
+                for (int k = 0; k < V; ++k) w[c][k] = 1.f;
             }
+        }
+        if (FULL) ask(raw, min(row + step, p.rows - 1));
+        float sum = 0, along = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 n[c][k] = (n[c][k] - mean) * root;
@@ -237,71 +291,55 @@ __global__ __launch_bounds__(kGradThreads) void norm_backward_kernel(const NormP
                     dw[c][k] = __builtin_fmaf(u[c][k], n[c][k], dw[c][k]);
                     db[c][k] += u[c][k];
                 }
-                u[c][k] *= w[k];
+                u[c][k] *= w[c][k];
                 sum += u[c][k];
                 along = __builtin_fmaf(u[c][k], n[c][k], along);
             }
-        }
-        sums(sum, along);
+        team.sum(sum, along);
         sum *= per * p.centered;
         along *= per;
         if (there) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const int e = (c * LANES + lane) * V;
 #pragma unroll
                 for (int k = 0; k < V; ++k) u[c][k] = root * (u[c][k] - sum - n[c][k] * along);
-                if (p.total_grad) {
-                    float g[V];
-                    load_row<T, V>(p.total_grad, index.at(p.total_grad_at), e, p.size, g);
+                if (ADDS)
 #pragma unroll
-                    for (int k = 0; k < V; ++k) u[c][k] += g[k];
-                }
-                store_row<T, V>(p.x_grad, index.at(p.x_grad_at), e, p.size, u[c]);
+                    for (int k = 0; k < V; ++k) u[c][k] += more[c][k];
+                store_row<T, V, FULL>(p.x_grad, index.at(p.x_grad_at), element(c), p.size, u[c]);
             }
         }
     }
     if constexpr (SUMS) {
-        // The rows' sums of one workgroup: of a wavefront's groups of 16 lanes by exchange, of wavefronts (or of the sets of them
-        // that share rows) pairwise in LDS.  Lane `lane` of the first of them is left with the columns that it had all along.
-        if constexpr (LANES == 16) {
+        // The sums of a workgroup: those of a wavefront's groups of 16 lanes by exchange, then all that have the same columns in LDS,
+        // one after the other.
+        __shared__ float meet[kWaves * 64 * V];
+        const int across = LANES == 64 ? lanes * V : LANES * V, rows = LANES == 64 ? p.groups : kWaves;
+        const int mine = LANES == 64 ? team.group : team.wave;
+        float* const part = p.part + (int64_t)blockIdx.x * 2 * p.padded;
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    for (float* s : {&dw[c][k], &db[c][k]}) {
-                        *s += __shfl_xor(*s, 16);
-                        *s += __shfl_xor(*s, 32);
-                    }
-                }
-        }
-        if constexpr (LANES < kGradThreads) {
-            constexpr int kSet = LANES < 64 ? 64 : LANES, kSets = kGradThreads / kSet;
-            __shared__ float meet[kSets / 2][kElements][kSet];
-            const int set = threadIdx.x / kSet, at = threadIdx.x % kSet;
-            for (int half = kSets / 2; half >= 1; half /= 2)
-                for (auto* s : {&dw, &db}) {
-                    __syncthreads();
-                    if (set >= half && set < 2 * half)
-#pragma unroll
-                        for (int c = 0; c < C; ++c)
-#pragma unroll
-                            for (int k = 0; k < V; ++k) meet[set - half][c * V + k][at] = (*s)[c][k];
-                    __syncthreads();
-                    if (set < half)
-#pragma unroll
-                        for (int c = 0; c < C; ++c)
-#pragma unroll
-                            for (int k = 0; k < V; ++k) (*s)[c][k] += meet[set][c * V + k][at];
-                }
-        }
-        if (threadIdx.x < LANES)
+        for (int which = 0; which < 2; ++which)
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const int e = (c * LANES + lane) * V;
-                float* part = p.part + (int64_t)blockIdx.x * 2 * p.padded;
-                store_row<float, V>(part, 0, e, p.size, dw[c]);
-                store_row<float, V>(part, p.padded, e, p.size, db[c]);
+                float s[V];
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    s[k] = which ? db[c][k] : dw[c][k];
+                    if (LANES == 16) {
+                        s[k] += __shfl_xor(s[k], 16);
+                        s[k] += __shfl_xor(s[k], 32);
+                    }
+                }
+                __syncthreads();
+                if (LANES == 64 || (threadIdx.x & 63) < LANES)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) meet[mine * across + team.lane * V + k] = s[k];
+                __syncthreads();
+                for (int i = threadIdx.x; i < across; i += blockDim.x) {
+                    float sum = 0;
+                    for (int r = 0; r < rows; ++r) sum += meet[r * across + i];
+                    if (c * across + i < p.padded) part[which * p.padded + c * across + i] = sum;
+                }
             }
     }
 }
@@ -336,38 +374,61 @@ __global__ __launch_bounds__(256) void norm_sums_kernel(const float* part, int p
     }
 }
 
-// Lanes that share a row.
-int lanes_of(int64_t size) { return size <= 16 * kElements ? 16 : size <= 64 * kElements ? 64 : size <= 256 * kElements ? 256 : 1024; }
+// How rows are shared out: 16 lanes each, or 1 to 16 wavefronts; packs of 16 bytes a lane; whether rows fill their lanes.
+struct Share {
+    int lanes, packs, waves, groups, grad_groups;
+    bool full;
+    Share(int type, int64_t size) {
+        const int v = 16 / type_bytes(type), most = kElements / v;
+        lanes = size <= 16 * kElements ? 16 : 64;
+        packs = most;
+        full = false;
+        // two packs a lane, or one, that rows fill exactly (of bf16 rather one: two and a residual's gradient pass the registers)
+        for (int i : {0, 1}) {
+            const int c = type == ADHIP_BF16 ? 2 - i : 1 + i;
+            const int64_t unit = (int64_t)lanes * v * c;
+            if (lanes == 16 ? size == unit : size % unit == 0 && size / unit <= kWaves) packs = c, full = true;
+        }
+        waves = lanes == 16 ? 1 : (int)((size + 64 * v * packs - 1) / (64 * v * packs));
+        groups = lanes == 16 ? kThreads / 16 : std::max(1, kThreads / 64 / waves);
+        grad_groups = lanes == 16 ? kWaves * 4 : kWaves / waves;
+    }
+    int threads(bool backward) const { return lanes == 16 ? (backward ? kWaves * 64 : kThreads) : (backward ? grad_groups : groups) * waves * 64; }
+};
 
 int padded_of(int64_t size) { return (int)((size + 3) / 4 * 4); }
 
-int64_t grad_blocks(int64_t rows, int64_t size) {
-    const int64_t at_once = kGradThreads / lanes_of(size);
+int64_t grad_blocks(int type, int64_t rows, int64_t size) {
+    const int64_t at_once = Share(type, size).grad_groups;
     return std::min<int64_t>((rows + at_once - 1) / at_once, kGradBlocks);
 }
 
-size_t workspace_of(int64_t rows, int64_t size) { return (size_t)grad_blocks(rows, size) * 2 * (size_t)padded_of(size) * sizeof(float); }
+size_t workspace_of(int type, int64_t rows, int64_t size) { return (size_t)grad_blocks(type, rows, size) * 2 * (size_t)padded_of(size) * sizeof(float); }
 
-template <class T, class W, bool SUMS>
-void launch_backward(const char* op, const NormParams& p, unsigned blocks, hipStream_t stream) {
-    const int lanes = lanes_of(p.size);
-    launch(op, lanes == 16 ? norm_backward_kernel<T, W, 16, SUMS> : lanes == 64 ? norm_backward_kernel<T, W, 64, SUMS>
-               : lanes == 256 ? norm_backward_kernel<T, W, 256, SUMS> : norm_backward_kernel<T, W, 1024, SUMS>, blocks, kGradThreads, stream, p);
+template <class T, class W, int LANES, int C, bool FULL>
+void launch_norm(const char* op, const NormParams& p, const Share& share, bool backward, bool sums, unsigned blocks, hipStream_t stream) {
+    const unsigned threads = (unsigned)share.threads(backward);
+    if (!backward)
+        launch(op, norm_kernel<T, W, LANES, C, FULL>, blocks, threads, stream, p);
+    else if (sums && p.total_grad)
+        launch(op, norm_backward_kernel<T, W, LANES, C, FULL, true, true>, blocks, threads, stream, p);
+    else if (sums)
+        launch(op, norm_backward_kernel<T, W, LANES, C, FULL, true, false>, blocks, threads, stream, p);
+    else if (p.total_grad)
+        launch(op, norm_backward_kernel<T, W, LANES, C, FULL, false, true>, blocks, threads, stream, p);
+    else
+        launch(op, norm_backward_kernel<T, W, LANES, C, FULL, false, false>, blocks, threads, stream, p);
 }
 
 template <class T, class W>
-void launch_norm(const char* op, const NormParams& p, bool backward, bool sums, unsigned blocks, hipStream_t stream) {
-    if (backward) {
-        if (sums) launch_backward<T, W, true>(op, p, blocks, stream);
-        else launch_backward<T, W, false>(op, p, blocks, stream);
-        return;
-    }
-    const int lanes = lanes_of(p.size), threads = std::max(256, lanes);
-    const int64_t at_once = threads / lanes;
-    // (more rows than a launch holds go round)
-    const int64_t all = std::min<int64_t>((p.rows + at_once - 1) / at_once, 0xffffffffu / threads);
-    launch(op, lanes == 16 ? norm_kernel<T, W, 16> : lanes == 64 ? norm_kernel<T, W, 64> : lanes == 256 ? norm_kernel<T, W, 256> : norm_kernel<T, W, 1024>,
-           (unsigned)all, threads, stream, p);
+void launch_norm(const char* op, const NormParams& p, const Share& share, bool backward, bool sums, unsigned blocks, hipStream_t stream) {
+    constexpr int most = kElements * sizeof(T) / 16;
+    if (share.lanes == 16 && !share.full) launch_norm<T, W, 16, most, false>(op, p, share, backward, sums, blocks, stream);
+    else if (share.lanes == 16 && share.packs == 1) launch_norm<T, W, 16, 1, true>(op, p, share, backward, sums, blocks, stream);
+    else if (share.lanes == 16) launch_norm<T, W, 16, 2, true>(op, p, share, backward, sums, blocks, stream);
+    else if (!share.full) launch_norm<T, W, 64, most, false>(op, p, share, backward, sums, blocks, stream);
+    else if (share.packs == 1) launch_norm<T, W, 64, 1, true>(op, p, share, backward, sums, blocks, stream);
+    else launch_norm<T, W, 64, 2, true>(op, p, share, backward, sums, blocks, stream);
 }
 
 struct Named {
@@ -441,8 +502,8 @@ void layer_norm(const char* op, const adhip_layer_norm_args& g, bool backward, h
     if (backward) {
         if (g.weight_grad.data) check_vector(op, "weight_grad", g.weight_grad, size, true);
         if (g.bias_grad.data) check_vector(op, "bias_grad", g.bias_grad, size, true);
-        ADHIP_CHECK(!sums || rows == 0 || (g.workspace && (uintptr_t)g.workspace % 16 == 0 && g.workspace_bytes >= workspace_of(rows, size)),
-                    "%s: the workspace has %zu bytes, %zu are wanted, aligned to 16", op, g.workspace ? g.workspace_bytes : (size_t)0, workspace_of(rows, size));
+        ADHIP_CHECK(!sums || rows == 0 || (g.workspace && (uintptr_t)g.workspace % 16 == 0 && g.workspace_bytes >= workspace_of(g.x.type, rows, size)),
+                    "%s: the workspace has %zu bytes, %zu are wanted, aligned to 16", op, g.workspace ? g.workspace_bytes : (size_t)0, workspace_of(g.x.type, rows, size));
     }
     p.rows = (unsigned)rows;
     p.size = (int)size;
@@ -486,13 +547,18 @@ void layer_norm(const char* op, const adhip_layer_norm_args& g, bool backward, h
     p.n2 = used >= 3 ? (unsigned)dims[used - 3] : 1;
 
     if (rows > 0) {
-        const unsigned blocks = (unsigned)grad_blocks(rows, size);
-        if (g.x.type == ADHIP_F32) launch_norm<float, float>(op, p, backward, sums, blocks, stream);
-        else if (w_type == ADHIP_F32) launch_norm<bf16, float>(op, p, backward, sums, blocks, stream);
-        else launch_norm<bf16, bf16>(op, p, backward, sums, blocks, stream);
+        const Share share(g.x.type, size);
+        p.waves = share.waves;
+        p.groups = backward ? share.grad_groups : share.groups;
+        // (more rows than a launch holds go round)
+        const int64_t all = std::min<int64_t>((rows + p.groups - 1) / p.groups, 0xffffffffu / (unsigned)share.threads(false));
+        const unsigned blocks = (unsigned)(backward ? grad_blocks(g.x.type, rows, size) : all);
+        if (g.x.type == ADHIP_F32) launch_norm<float, float>(op, p, share, backward, sums, blocks, stream);
+        else if (w_type == ADHIP_F32) launch_norm<bf16, float>(op, p, share, backward, sums, blocks, stream);
+        else launch_norm<bf16, bf16>(op, p, share, backward, sums, blocks, stream);
     }
     if (sums)
-        launch(op, norm_sums_kernel, dim3((unsigned)((size + 63) / 64), 2), 256, stream, (const float*)g.workspace, rows > 0 ? (int)grad_blocks(rows, size) : 0,
+        launch(op, norm_sums_kernel, dim3((unsigned)((size + 63) / 64), 2), 256, stream, (const float*)g.workspace, rows > 0 ? (int)grad_blocks(g.x.type, rows, size) : 0,
                (int)size, p.padded, g.weight_grad.data, g.bias_grad.data, g.weight_grad.type == ADHIP_BF16, g.bias_grad.type == ADHIP_BF16);
 }
 
@@ -505,7 +571,8 @@ int adhip_layer_norm_workspace(adhip_ctx* ctx, const adhip_layer_norm_args* args
     return adhip::context_guarded(ctx, [&] {
         const char* op = "adhip_layer_norm_workspace";
         ADHIP_CHECK(args && bytes, "%s: no arguments", op);
-        *bytes = adhip::workspace_of(adhip::check_rows(op, args->x), args->x.dims[args->x.rank - 1]);
+        const int64_t rows = adhip::check_rows(op, args->x);
+        *bytes = adhip::workspace_of(args->x.type, rows, args->x.dims[args->x.rank - 1]);
     });
 }
 
