@@ -10,6 +10,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
+#include <vector>
 
 #pragma clang fp contract(off)
 
@@ -232,6 +234,13 @@ void gradients(const char* op, const adhip_gradients_args& g, bool clip, hipStre
         ADHIP_CHECK(t.count == 0 || (t.g && (t.out || !clip)), "%s: an array of gradient %lld is missing", op, (long long)i);
         ADHIP_CHECK((uintptr_t)t.g % w == 0 && (!clip || (uintptr_t)t.out % w == 0), "%s: an array of gradient %lld is not aligned to its type", op,
                     (long long)i);
+    }
+    if (clip) {  // a gradient that is listed twice would be scaled twice, at once
+        std::vector<std::pair<uintptr_t, uintptr_t>> outs;
+        for (int64_t i = 0; i < g.n_tensors; ++i)
+            if (g.tensors[i].count) outs.emplace_back((uintptr_t)g.tensors[i].out, (uintptr_t)g.tensors[i].out + g.tensors[i].count * type_bytes((int)g.tensors[i].type));
+        std::sort(outs.begin(), outs.end());
+        for (size_t i = 1; i < outs.size(); ++i) ADHIP_CHECK(outs[i].first >= outs[i - 1].second, "%s: two clipped gradients share memory", op);
     }
     double* const partial = (double*)g.workspace;
     float* const factor = g.factor || !clip ? g.factor : (float*)(partial + blocks);

@@ -879,7 +879,7 @@ void recurrence(const char* op, const adhip_recurrence_args& g, bool backward, h
                (unsigned)((lanes + 255) / 256), 256, stream, p);
         return;
     }
-    ADHIP_CHECK(fits_launch(blocks + 8, Team<kWide>::kThreads), "%s: %lld sequences of %lld channels are too many for one call", op, (long long)batch, (long long)channels);
+    ADHIP_CHECK(fits_launch(blocks * cut.ranges + 8, (unsigned)(wide ? Team<kWide>::threads(p.length) : Team<kNarrow>::threads(p.length))), "%s: %lld sequences of %lld channels are too many for one call", op, (long long)batch, (long long)channels);
     if (blocks == 0) return;
     ADHIP_CHECK(cut.workspace(g.x) == 0 || (g.workspace && (uintptr_t)g.workspace % 16 == 0 && g.workspace_bytes >= cut.workspace(g.x)),
                 "%s: the workspace has %zu bytes, %zu are wanted, aligned to 16", op, g.workspace ? g.workspace_bytes : (size_t)0, cut.workspace(g.x));

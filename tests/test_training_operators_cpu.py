@@ -203,6 +203,10 @@ def test_recurrence_refusals(dev):
     no("lengths is f32", x, x, x, lengths=Array(3))
     no("documents is", x, x, x, documents=Array(3, 301, dtype="int32"))
     no("documents is f32", x, x, x, documents=Array(3, 300))
+    far = Array(3, 300, 40, stride=(1 << 40, (1 << 21) + 1, 1))
+    no("2\\^21", far, x, x)
+    no("2\\^21", x, far, x)
+    no("2\\^21", x, x, far)
     no("extents below", Array(1, 1 << 30, 1), Array(1, 1 << 30, 1), Array(1, 1 << 30, 1))
     refused(dev, "in device memory", ops.recurrence, x, torch.zeros(3, 300, 40), x)
 
@@ -220,13 +224,43 @@ def test_recurrence_backward_refusals(dev):
     no("gates_grad is bf16", x, x, states, x, x, Array(3, 300, 40, dtype="bfloat16"))
     no("final_grad is", x, x, states, x, x, x, final_grad=Array(3, 39))
     no("initial_grad share memory", x, x, states, x, x, x, initial_grad=Array(3, 40, stride=(0, 1)))
+    far = Array(3, 300, 40, stride=(1 << 40, (1 << 21) + 1, 1))
+    no("2\\^21", x, x, states, far, x, x)
+    no("2\\^21", x, x, states, x, far, x)
+    no("2\\^21", x, x, states, x, x, far)
+
+
+def test_recurrence_workspaces_and_launches(dev):
+    """Few channels over many positions are cut into ranges, whose maps a workspace holds; a call without one is refused.  Both passes
+    take what one question said, and launches fit."""
+    for dtype in ("float32", "bfloat16"):
+        for B, L, C in ((1, 1, 1), (1, 9, 1), (1, 256, 64), (1, 5000, 20), (2, 30000, 300), (1, 100000, 8192), (1, 1 << 20, 1), (4, 3000, 4096),
+                        (300, 700, 65), (1 << 20, 20, 33), (70000, 1, 1000), (1, 512, 64)):
+            x, states, state = Array(B, L, C, dtype=dtype), Array(B, ops.recurrence_blocks(L), C), Array(B, C)
+            need = ops.recurrence_workspace(dev, x, backward=True)
+            assert need % 8 == 0 and need <= 256 * 8 * max(B * C, 8192)
+            room = Array(need, dtype="float8_e4m3fn") if need else None
+            for how in (dict(), dict(documents=Array(B, L, dtype="int32")), dict(factors=True)):
+                ops.recurrence(dev, x, x, x, states=states, final=state, workspace=room, **how)
+                ops.recurrence_backward(dev, x, x, states, x, x, x, workspace=room, **how)
+                for gx, gy, gz, threads in dev.launches():
+                    assert 1 <= gx * threads < 1 << 32 and (gy, gz) == (1, 1)
+    x = Array(1, 5000, 20)
+    need = ops.recurrence_workspace(dev, x)
+    assert need > 0 and ops.recurrence_workspace(dev, Array(4, 3000, 4096)) == 0
+    refused(dev, "workspace has 0 bytes", ops.recurrence, x, x, x)
+    refused(dev, "workspace has", ops.recurrence, x, x, x, workspace=Array(need - 1, dtype="float8_e4m3fn"))
+    refused(dev, "aligned to 16", ops.recurrence, x, x, x, workspace=Array(need, dtype="int32", at=4104))
+    refused(dev, "workspace has 0 bytes", ops.recurrence_backward, x, x, Array(1, 20, 20), x, x, x)
+    refused(dev, "too many", ops.recurrence, *[Array(1 << 29, 9, 64, dtype="bfloat16")] * 3)
+    refused(dev, "too many", ops.recurrence, *[Array(1 << 29, 1, 1 << 20, dtype="bfloat16")] * 3)
 
 
 # ---- the norm over gradients --------------------------------------------------------------------------------------------
 
 
 def test_gradient_refusals(dev):
-    gs, norm = [Array(5, 7), Array(9, dtype="bfloat16")], Array(1)
+    gs, norm = [Array(5, 7), Array(9, dtype="bfloat16", at=8192)], Array(1)
     need = ops.gradient_norm_workspace(dev, gs)
     good = dict(limit=1.0, factor=Array(1), workspace=Array(need, dtype="float8_e4m3fn"))
     ops.clip_gradients(dev, gs, norm, **good)
@@ -251,13 +285,19 @@ def test_gradient_refusals(dev):
     no("workspace has 0 bytes", gs, norm, workspace=None)
     no("workspace has", gs, norm, workspace=Array(need - 1, dtype="float8_e4m3fn"))
     no("aligned to 8", gs, norm, workspace=Array(need, dtype="int32", at=4100))
+    # a list that names a gradient twice, or a part of one
+    no("share memory", gs[:1] * 2, norm, workspace=ROOM)
+    no("share memory", [Array(100, at=4096), Array(100, at=4096 + 396)], norm, workspace=ROOM)
+    ops.clip_gradients(dev, [Array(100, at=4096), Array(100, at=4096 + 400), Array(0, at=4096)], norm, limit=1.0, workspace=ROOM)
+    ops.gradient_norm(dev, gs[:1] * 2, norm, workspace=ROOM)
+    assert len(dev.launches()) == 2
     refused(dev, "in device memory", ops.gradient_norm, [torch.zeros(3)], norm, workspace=ROOM)
     refused(dev, "in device memory", ops.gradient_norm, gs, torch.zeros(1), workspace=ROOM)
     refused(dev, "in device memory", ops.clip_gradients, gs, norm, limit=1.0, gradients_out=[torch.zeros(5, 7), gs[1]], workspace=ROOM)
 
 
 def test_gradient_launches_fit(dev):
-    many = [Array(1 + 300 * i) for i in range(1000)]
+    many = [Array(1 + 300 * i, at=4096 + (i << 21)) for i in range(1000)]
     room = Array(ops.gradient_norm_workspace(dev, many), dtype="float8_e4m3fn")
     ops.clip_gradients(dev, many, Array(1), limit=1.0, workspace=room)
     seen = dev.launches()
