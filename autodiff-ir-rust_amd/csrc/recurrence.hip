@@ -749,21 +749,23 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(const RecurrencePa
     if (p.final) store_state<V>(p.final, batch * p.final_b, c, p.channels, h);
 }
 
-// Where there are workgroups enough, wide rows bring whole cache lines (forward and f32 backward 5 to 10 % faster).  The backward pass of bf16,
-// and of documents, has no registers for two sets of them: 128 a thread, with the spills that come of it, against twice as many.
+// Wide rows bring whole cache lines: 5 to 10 % forward and backward in f32.  The backward pass of bf16, and that of documents, does not fit the 128
+// registers that their 1024 threads have: 16 x 1000 positions of 4000 channels in bf16 with documents 390 us wide and 216 narrow.
 constexpr bool wide_pays(int type, bool backward, bool documents) { return !backward || (type == ADHIP_F32 && !documents); }
 
 template <class T, int LANES, bool FACTORS, bool DOCS>
 void launch_recurrence(const char* op, const RecurrenceParams& p, bool backward, hipStream_t stream) {
     const unsigned threads = (unsigned)Team<LANES>::threads(p.length);
     const auto blocks = [&](int ranges) { return (unsigned)(((int64_t)p.groups * p.batch * ranges + 7) / 8 * 8); };
-    if (p.ranges > 1)
-        launch(op, backward ? recurrence_range_kernel<T, LANES, FACTORS, DOCS, true> : recurrence_range_kernel<T, LANES, FACTORS, DOCS, false>,
-               blocks(p.ranges - 1), Team<LANES>::kThreads, stream, p);
-    if (!backward) launch(op, recurrence_kernel<T, LANES, FACTORS, DOCS>, blocks(p.ranges), threads, stream, p);
-    {
-        if (backward) launch(op, recurrence_backward_kernel<T, LANES, FACTORS, DOCS>, blocks(p.ranges), threads, stream, p);
+    if (!backward) {
+        if (p.ranges > 1) launch(op, recurrence_range_kernel<T, LANES, FACTORS, DOCS, false>, blocks(p.ranges - 1), Team<LANES>::kThreads, stream, p);
+        launch(op, recurrence_kernel<T, LANES, FACTORS, DOCS>, blocks(p.ranges), threads, stream, p);
     }
+    if constexpr (LANES == kNarrow || wide_pays(sizeof(T) == 4 ? ADHIP_F32 : ADHIP_BF16, true, DOCS))
+        if (backward) {
+            if (p.ranges > 1) launch(op, recurrence_range_kernel<T, LANES, FACTORS, DOCS, true>, blocks(p.ranges - 1), Team<LANES>::kThreads, stream, p);
+            launch(op, recurrence_backward_kernel<T, LANES, FACTORS, DOCS>, blocks(p.ranges), threads, stream, p);
+        }
 }
 
 template <class T, int LANES>
@@ -774,16 +776,21 @@ void launch_recurrence(const char* op, const RecurrenceParams& p, bool backward,
     else launch_recurrence<T, LANES, false, false>(op, p, backward, stream);
 }
 
-// How channels are cut into rows and positions into ranges.
+// How channels are cut into rows and positions into ranges.  Compute units left without a workgroup are given ranges of positions, at
+// the price of a kernel that reads them before (8191 positions of 1000 channels in f32, forward and backward: 248 us in one range, 120 in four), of
+// two tiles or more each.  Rows are wide where narrow ones would give some compute units two workgroups (4 x 2049 of 2560 in bf16: 47 us
+// narrow, 39 wide; 2 x 8192 of 4096, where they give each one: 290 narrow, 386 wide), and where there are ranges of four
+// tiles and more to make up for them (the first example in eight: 109 us; 4096 positions of 1024 channels in bf16, two tiles each: 36 narrow, 38 wide).
 struct Cut {
     int lanes, groups, tiles, ranges;  // tiles: of a range
     Cut(const adhip_array& x, bool wide) {
         const int64_t v = 4 / type_bytes(x.type), channels = x.dims[2], batch = std::max<int64_t>(x.dims[0], 1);
-        const auto blocks = [&](int lanes) { return (channels + lanes * v - 1) / (lanes * v) * batch; };
-        lanes = wide && blocks(kNarrow) > kFull ? kWide : kNarrow;
-        groups = (int)(blocks(lanes) / batch);
         const int64_t all = (x.dims[1] + kTile - 1) / kTile;
-        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kFull / std::max<int64_t>(blocks(lanes), 1), all / 2));
+        const auto blocks = [&](int lanes) { return std::max<int64_t>((channels + lanes * v - 1) / (lanes * v) * batch, 1); };
+        const bool many = blocks(kNarrow) > kFull, long_ranges = 2 * blocks(kNarrow) <= kFull && all * blocks(kWide) >= 4 * kFull;
+        lanes = wide && (many || long_ranges) ? kWide : kNarrow;
+        groups = (int)((channels + lanes * v - 1) / (lanes * v));
+        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kFull / blocks(lanes), all / 2));
         tiles = (int)std::max<int64_t>(1, (all + want - 1) / want);
         ranges = (int)std::max<int64_t>(1, (all + tiles - 1) / tiles);
     }

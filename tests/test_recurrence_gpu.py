@@ -78,6 +78,25 @@ def test_long_sequences_of_few_channels(hip_device, shape, factors, dtype):
     check(hip_device, inputs(*shape, dtype, factors=factors, seed=2, slow=6.0), f"{shape}, {dtype}", factors=factors)
 
 
+@pytest.mark.parametrize("dtype,C", [("f32", 930), ("bf16", 1857)])
+@pytest.mark.parametrize("factors", [False, True])
+@pytest.mark.parametrize("masked", [False, True])
+def test_long_ranges_of_wide_rows(hip_device, masked, factors, dtype, C):
+    """Channels in rows of 128 bytes (of bf16, the last one alone in its row) and positions in ranges."""
+    masks = dict(documents=0.002, lengths=[8700]) if masked else {}
+    a = inputs(1, 9001, C, dtype, factors=factors, seed=3, slow=5.0, **masks)
+    assert ops.recurrence_workspace(hip_device, a["x"]) > 0
+    check(hip_device, a, f"9001 x {C}, {dtype}", factors=factors)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("masked", [False, True])
+def test_many_sequences_of_several_tiles(hip_device, masked, dtype):
+    """Rows of 128 bytes without ranges."""
+    masks = dict(documents=0.01, lengths=[700, 530, 0, 1, 256, 699]) if masked else {}
+    check(hip_device, inputs(6, 700, 1473, dtype, seed=3, **masks), f"many, {dtype}")
+
+
 MASKS = {
     "lengths": dict(lengths=[700, 0, 256]),
     "lengths out of range": dict(lengths=[9999, -3, 1]),
