@@ -42,7 +42,7 @@ struct RecurrenceParams {
     const float *initial, *final_grad;
     float *states, *final, *initial_grad;
     const int *lengths, *documents;
-    float2* carry;  // [ranges, batch, channels]: what a range does to a state
+    float2* carry;  // [ranges, batch, channels]: what a range does to a state; forward, the last one's place holds the state before all
     Rows x_at, gates_at, out_at, out_grad_at, x_grad_at, gates_grad_at, states_at, documents_at;
     int64_t initial_b, final_b, final_grad_b, initial_grad_b, lengths_b;
     int length, channels, groups;  // groups: of channels that a workgroup takes
@@ -349,8 +349,17 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const
     __shared__ float2 parts[2][kWaves][LANES * V];  // (by turns: the other one's barrier stands between readers and writers)
     fill_absent(parts);
     float carry[V];
-    load_state<V>(p.initial, seat.batch * p.initial_b, seat.c, p.channels, carry);
-    over_ranges<T, LANES, FACTORS>(p, seat, 0, seat.range, 1, carry);
+    if (p.ranges == 1) {
+        load_state<V>(p.initial, seat.batch * p.initial_b, seat.c, p.channels, carry);
+    } else {
+        // (final may be initial, and the last range may be done before the first one begins: the state was put aside)
+        float2 kept[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) kept[v] = p.carry[(int64_t)(p.ranges - 1) * p.batch * p.channels + seat.state + (seat.lone ? 0 : v)];
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = kept[v].y;
+        over_ranges<T, LANES, FACTORS>(p, seat, 0, seat.range, 1, carry);
+    }
     int turn = 0;
     // From the maps of a tile to its states, and the state behind it.
     auto states = [&](const float (&a)[kSteps][V], const float (&b)[kSteps][V], int begin, Steps<T>& o) {
@@ -687,6 +696,13 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_range_kernel
     }
     __syncthreads();
     if (seat.own != 0) return;
+    if (!BACK && range == 0) {
+        float initial[V];
+        load_state<V>(p.initial, seat.batch * p.initial_b, seat.c, p.channels, initial);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (seat.c + v < p.channels) p.carry[(int64_t)(p.ranges - 1) * p.batch * p.channels + seat.state + v] = make_float2(0, initial[v]);
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         float a = 1, b = 0;

@@ -251,6 +251,21 @@ def test_in_place(hip_device, L, dtype):
         assert torch.equal(g[to[0]], want["x_grad"]) and torch.equal(g[to[1]], want["gates_grad"]) and torch.equal(g["initial"], want["initial_grad"])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("L,C", [(600, 300), (5000, 40), (9001, 930)])
+def test_a_state_in_place_over_long_sequences(hip_device, L, C, dtype):
+    """The last range of positions writes the state that the first one begins with."""
+    a = {n: to_gpu(x) for n, x in inputs(1, L, C, dtype, factors=True, seed=4, slow=8.0).items()}
+    room = torch.empty(ops.recurrence_workspace(hip_device, a["x"]) + 16, dtype=torch.uint8, device="cuda")
+    out, final = torch.empty_like(a["x"]), torch.empty_like(a["initial"])
+    for _ in range(3):
+        ops.recurrence(hip_device, a["x"], a["gates"], out, factors=True, initial=a["initial"], final=final, workspace=room, stream=here())
+        state, again = a["initial"].clone(), torch.empty_like(out)
+        ops.recurrence(hip_device, a["x"], a["gates"], again, factors=True, initial=state, final=state, workspace=room, stream=here())
+        assert torch.equal(out, again) and torch.equal(final, state)
+        a["initial"] = state
+
+
 @pytest.mark.parametrize("factors", [False, True])
 def test_no_positions_and_no_sequences(hip_device, factors):
     a = inputs(2, 0, 40, "f32", factors=factors)
