@@ -23,7 +23,6 @@ constexpr int kThreads = 256;
 constexpr int kChunk = 8192;     // elements of a workgroup
 constexpr int kSmall = 1024;     // elements of a wavefront where one workgroup does everything,
 constexpr int kSmallChunks = 64; // and how many such chunks there may be
-constexpr int64_t kLastCache = 256 << 20;  // bytes
 constexpr int64_t kBlocks = 0xffffffffu / kThreads;  // workgroups of a launch: it holds fewer than 2^32 threads
 
 struct GradientLaunch {
@@ -145,7 +144,6 @@ __global__ __launch_bounds__(kFinish) void gradient_norm_kernel(const double* pa
 // PAST: written past the caches, which hold what is read again instead.
 template <class T, int V, int THREADS, bool PAST>
 __device__ __forceinline__ void scale_chunk(const T* g, T* out, int64_t begin, int64_t end, float scale) {
-    typedef unsigned Quad __attribute__((ext_vector_type(4)));
     int64_t i = begin + (int64_t)(threadIdx.x % THREADS) * V;
     if constexpr (V > 1) {
         constexpr int U = 4;
@@ -157,7 +155,7 @@ __device__ __forceinline__ void scale_chunk(const T* g, T* out, int64_t begin, i
             for (int u = 0; u < U; ++u) {
 #pragma unroll
                 for (int k = 0; k < V; ++k) r[u].v[k] = (T)((float)r[u].v[k] * scale);
-                if (PAST) __builtin_nontemporal_store(*(const Quad*)&r[u], (Quad*)(out + i + u * THREADS * V));
+                if (PAST) store_past((Word16*)(out + i + u * THREADS * V), *(const Word16*)&r[u]);
                 else *(Pack<T, V>*)(out + i + u * THREADS * V) = r[u];
             }
         }
@@ -293,9 +291,8 @@ void gradients(const char* op, const adhip_gradients_args& g, bool clip, hipStre
     }
     each_launch(kChunk, [&](const GradientLaunch& a) { launch(op, gradient_squares_kernel, a.first[a.n], kThreads, stream, a); });
     launch(op, gradient_norm_kernel, 1, kFinish, stream, partial, blocks, norm);
-    // Gradients and what is made of them, where the last cache does not hold both: then what is written goes past it, and the
-    // gradients are still there when they are read again (and the next step's find no lines that have to be written first).
-    // 38 M in f32: 76 us instead of 91.
+    // Where the last cache does not hold gradients and what is made of them, what is written goes past it, and the gradients are still
+    // there when they are read again.  38 M in f32: 76 us instead of 91.
     const bool past = bytes > kLastCache;
     if (clip)
         each_launch(kChunk, [&](const GradientLaunch& a) {

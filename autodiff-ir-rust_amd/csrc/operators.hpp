@@ -24,6 +24,10 @@ void launch(const char* op, void (*kernel)(P...), dim3 grid, unsigned threads, h
     if (e != hipSuccess) throw Error(strf("%s: the launch failed: %s", op, hipGetErrorString(e)));
 }
 
+// The last cache before memory.  A call whose arrays pass it together leaves nothing there for the next one; written past it, its results
+// cost no room for what is still to be read, and the next call finds no lines that have to be written back first.
+constexpr int64_t kLastCache = 256 << 20;  // bytes
+
 inline int type_bytes(int type) { return type == ADHIP_BF16 ? 2 : type == ADHIP_E4M3 ? 1 : 4; }
 inline const char* type_name(int type) {
     static const char* const names[] = {"f32", "bf16", "int32", "e4m3"};
@@ -119,5 +123,13 @@ template <class T, int N>
 struct __attribute__((aligned(sizeof(T) * N))) Pack {
     T v[N];
 };
+
+// 4 and 16 bytes written past the caches, to addresses that are aligned to two.
+typedef unsigned Word4 __attribute__((aligned(2)));
+typedef unsigned Word16 __attribute__((ext_vector_type(4), aligned(2)));
+template <class W>
+__device__ __forceinline__ void store_past(W* to, W w) {
+    __builtin_nontemporal_store(w, to);
+}
 
 }  // namespace adhip

@@ -47,6 +47,7 @@ struct RecurrenceParams {
     int64_t initial_b, final_b, final_grad_b, initial_grad_b, lengths_b;
     int length, channels, groups;  // groups: of channels that a workgroup takes
     int batch, ranges, tiles;      // of positions, and tiles of a range
+    bool past;                     // results go past the caches
 };
 
 // Operand of a wait for all memory operations of a wavefront, and of nothing else.
@@ -167,8 +168,11 @@ struct Seat {
     bool lone;
     __device__ __forceinline__ Seat(const RecurrenceParams& p) {
         lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), slot = (lane & (LANES - 1)) * V;
-        // Workgroups go to the eight dies in turn: neighbours of a row, whose channels share cache lines, go to one die.
-        unsigned at = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+        // Workgroups go to the eight dies in turn: of 256, which run at a time, neighbours of a row, whose channels share cache lines,
+        // go to one die, and together they cover whole rows (8 x 2048 positions of 4096 channels in bf16: 315 us with neighbours of all
+        // workgroups on one die, 276 so).
+        const unsigned window = blockIdx.x / kFull * kFull, of = blockIdx.x % kFull, die = min(gridDim.x - window, (unsigned)kFull) / 8;
+        unsigned at = window + of % 8 * die + of / 8;
         const unsigned group = at % (unsigned)p.groups;
         at /= (unsigned)p.groups;
         batch = at % (unsigned)p.batch;
@@ -222,11 +226,16 @@ struct Side {
         }
     }
     template <int LANES>
-    __device__ __forceinline__ void store(const Steps<T>& s, const Seat<T, LANES>& seat, int i, int rows) const {
+    __device__ __forceinline__ void store(const Steps<T>& s, const Seat<T, LANES>& seat, int i, int rows, bool past) const {
         char* to = tile + (int64_t)i * kTile * step;
         if (rows >= kTile && !seat.lone) {
+            if (past) {
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) ((Word<T>*)(row_of(to + k * step) + (off + lane)))->w = s.w[k];
+                for (int k = 0; k < kSteps; ++k) store_past((Word4*)(row_of(to + k * step) + (off + lane)), s.w[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) ((Word<T>*)(row_of(to + k * step) + (off + lane)))->w = s.w[k];
+            }
             return;
         }
 #pragma unroll
@@ -422,14 +431,14 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const
         Steps<T> o;
         states(a, b, begin, o);
         hide(m, o);
-        o_side.store(o, seat, i, p.length - begin);
+        o_side.store(o, seat, i, p.length - begin, p.past);
     }
     for (int i = used; i < seat.tiles; ++i) {  // behind the sequence
         const int begin = seat.first + i * kTile;
         if (p.states && seat.own == 0)
             store_state<V>(p.states, seat.batch * p.states_at.b + (int64_t)(begin / kBlock) * p.states_at.t, seat.c, p.channels, carry);
         Steps<T> o = {};
-        o_side.store(o, seat, i, p.length - begin);
+        o_side.store(o, seat, i, p.length - begin, p.past);
     }
     if (p.final && seat.own == 0 && seat.range == p.ranges - 1) store_state<V>(p.final, seat.batch * p.final_b, seat.c, p.channels, carry);
 }
@@ -452,8 +461,8 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
     over_ranges<T, LANES, FACTORS>(p, seat, p.ranges - 1, seat.range, -1, carry);
     int turn = 0;
     // From a tile's inputs to the gradients of x and gates, in their places.  `more` is called as soon as the inputs are in
-    // other registers.  What one instruction makes of them again (the halves of a pack, b = rest x) is not kept from the first walk to
-    // the second: registers decide how many wavefronts there are.
+    // other registers.  What one instruction makes of them again (b = rest x, with wide rows, whose threads have 128 registers, also the
+    // halves of a pack) is not kept from the first walk to the second.
     auto gradients = [&](Steps<T>& x, Steps<T>& g, Steps<T>& d, const float (&state)[V], const Marks& m, auto&& more) {
         float a[kSteps][V], rest[kSteps][V], A[V], B[V], preA[V], preB[V], back[V], behindA[V], behindB[V], h[V], l[V];
         hide(m, x);
@@ -534,8 +543,9 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
             l[v] = onward<FACTORS>(behindA[v], l[v], behindB[v]);
         }
         turn ^= 1;
+        if constexpr (LANES == kWide)  // (unpacked again from here on)
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) asm volatile("" : "+v"(in.w[k]), "+v"(out_grad.w[k]));  // (unpacked again from here on)
+            for (int k = 0; k < kSteps; ++k) asm volatile("" : "+v"(in.w[k]), "+v"(out_grad.w[k]));
         // forwards: what a factor's change is worth, the state before (less x, which a gate that is not a factor takes as much from)
         float worth[kSteps][V];
 #pragma unroll
@@ -597,8 +607,8 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
     };
     for (int i = seat.tiles - 1; i >= used; --i) {  // behind the sequence
         const Steps<T> none = {};
-        dx_side.store(none, seat, i, p.length - seat.first - i * kTile);
-        dg_side.store(none, seat, i, p.length - seat.first - i * kTile);
+        dx_side.store(none, seat, i, p.length - seat.first - i * kTile, p.past);
+        dg_side.store(none, seat, i, p.length - seat.first - i * kTile, p.past);
     }
     Tile one;
     if (used > 0) load(one, used - 1);
@@ -608,8 +618,8 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
         if (DOCS) m = one.documents.marks(count);
         Tile next;
         gradients(one.x, one.g, one.d, one.state, m, [&] { load(next, i - 1); });
-        dx_side.store(one.x, seat, i, p.length - begin);
-        dg_side.store(one.g, seat, i, p.length - begin);
+        dx_side.store(one.x, seat, i, p.length - begin, p.past);
+        dg_side.store(one.g, seat, i, p.length - begin, p.past);
         one = next;
     }
     if (p.initial_grad && seat.own == 0 && seat.range == 0) store_state<V>(p.initial_grad, seat.batch * p.initial_grad_b, seat.c, p.channels, carry);
@@ -891,6 +901,8 @@ void recurrence(const char* op, const adhip_recurrence_args& g, bool backward, h
     p.groups = cut.groups;
     p.ranges = cut.ranges;
     p.tiles = cut.tiles;
+    // (4 x 2048 positions of 4096 channels in f32, both passes: 223 us past the caches, 239 through them)
+    p.past = (backward ? 5 : 3) * batch * length * channels * type_bytes(g.x.type) > kLastCache;
     const int64_t blocks = batch * p.groups;
     const bool factors = g.factors != 0, wide = cut.lanes == kWide;
     if (!backward && length >= 1 && length <= kSteps) {
