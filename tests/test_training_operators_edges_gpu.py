@@ -190,3 +190,64 @@ def test_gradients_beyond_32_bits(hip_device):
     ops.clip_gradients(hip_device, [g], norm, limit=6.5, factor=factor, workspace=room, stream=here())
     assert float(norm) == 13.0 and float(factor) == 0.5
     assert g[-4:].tolist() == [0.0, 1.5, 2.0, 6.0]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_past_the_caches(hip_device, dtype):
+    """A call whose arrays pass the last cache writes past it; the same rows in calls of a quarter do not, and give the same bits."""
+    rows, size = (16000, 4099) if dtype == "f32" else (32000, 4096)
+    t = TYPES[dtype]
+    x, added, dy, dt = (torch.randn((rows, size), device="cuda").to(t) for _ in range(4))
+    w = torch.randn(size, device="cuda")
+    stats = torch.empty((rows, 2), device="cuda")
+
+    def both(x, added, dy, dt, stats):
+        total, out, dx, dw = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x), torch.empty(size, device="cuda")
+        room = torch.empty(ops.layer_norm_workspace(hip_device, x), dtype=torch.uint8, device="cuda")
+        ops.layer_norm(hip_device, x, out, weight=w, added=added, total=total, stats=stats, stream=here())
+        ops.layer_norm_backward(hip_device, total, stats, dy, dx, weight=w, weight_grad=dw, total_grad=dt, workspace=room, stream=here())
+        return total, out, dx, dw
+
+    assert rows * size * x.element_size() * 4 > 1 << 28 > rows * size * x.element_size()
+    whole = both(x, added, dy, dt, stats)
+    parts = [both(*(a.reshape(4, rows // 4, -1)[i] for a in (x, added, dy, dt, stats))) for i in range(4)]
+    for i in range(3):
+        assert torch.equal(whole[i], torch.cat([part[i] for part in parts]))
+    assert torch.allclose(whole[3], sum(part[3] for part in parts), rtol=1e-4, atol=1e-4 * rows ** 0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,L,C", [(1, 1300, 60001), (9, 700, 7000), (1, 300000, 150)])
+def test_recurrences_past_the_caches(hip_device, B, L, C, dtype):
+    """Channels are independent: some of a call that passes the last cache, against their restatement."""
+    t = TYPES[dtype]
+    L = L if dtype == "bf16" or L < 100000 else L // 2
+    x, gates, dout = (torch.randn((B, L, C), device="cuda").to(t) for _ in range(3))
+    assert 3 * x.numel() * x.element_size() > 1 << 28 or 5 * x.numel() * x.element_size() > 1 << 28
+    out, dx, dg = (torch.empty_like(x) for _ in range(3))
+    states = torch.empty((B, ops.recurrence_blocks(L), C), device="cuda")
+    room = torch.empty(ops.recurrence_workspace(hip_device, x, backward=True) + 16, dtype=torch.uint8, device="cuda")
+    ops.recurrence(hip_device, x, gates, out, states=states, workspace=room, stream=here())
+    ops.recurrence_backward(hip_device, x, gates, states, dout, dx, dg, workspace=room, stream=here())
+    some = [0, 1, C // 3, C - 2, C - 1]
+    if L <= 20000:
+        pick = lambda a: a[..., some].cpu()  # noqa: E731
+        first = last = 0
+    else:  # the beginning of the long one (its states fade within some hundred positions), and its end backwards
+        first, last = 0, 3000
+        pick = lambda a: a[:, :3000, some].cpu()  # noqa: E731
+    want, bound = oracle.recurrence(pick(x), pick(gates), out_grad=pick(dout))
+    assert_within(out[:, first:last or L, some], want["out"], bound["out"], "out")
+    end = (last - 400) if last else L  # the gradient of what lies behind the part has faded 400 positions before its end: a < 0.98^400
+    for n, got in (("x_grad", dx), ("gates_grad", dg)):
+        assert_within(got[:, :end, some], want[n][:, :end], bound[n][:, :end] + (1e-3 * want[n].abs().max() if last else 0), n)
+
+
+def test_gradients_past_the_caches(hip_device):
+    g = [torch.randn(n, device="cuda") for n in (30_000_001, 8_000_000, 5)]
+    out, norm, factor = [torch.full_like(x, 7.0) for x in g], torch.empty(1, device="cuda"), torch.empty(1, device="cuda")
+    room = torch.empty(ops.gradient_norm_workspace(hip_device, g), dtype=torch.uint8, device="cuda")
+    ops.clip_gradients(hip_device, g, norm, limit=1.0, factor=factor, gradients_out=out, workspace=room, stream=here())
+    assert all(torch.equal(o, x * factor) for x, o in zip(g, out))
+    want = torch.sqrt(sum((x.double() ** 2).sum() for x in g))
+    assert abs(float(norm) / float(want) - 1) <= 2.0 ** -23
