@@ -124,10 +124,12 @@ struct __attribute__((aligned(sizeof(T) * N))) Pack {
     T v[N];
 };
 
-// 4 and 16 bytes written past the caches, to addresses that are aligned to two.
+// 4, 8 and 16 bytes written past the caches, to addresses that are aligned to two.
 typedef unsigned Word4 __attribute__((aligned(2)));
+typedef unsigned Word8 __attribute__((ext_vector_type(2), aligned(2)));
 typedef unsigned Word16 __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ void store_past(Word4* to, unsigned w) { __builtin_nontemporal_store(w, to); }
+__device__ __forceinline__ void store_past(Word8* to, Word8 w) { __builtin_nontemporal_store(w, to); }
 __device__ __forceinline__ void store_past(Word16* to, Word16 w) { __builtin_nontemporal_store(w, to); }
 
 }  // namespace adhip
