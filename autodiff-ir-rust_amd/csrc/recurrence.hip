@@ -229,7 +229,7 @@ struct Side {
     __device__ __forceinline__ void store(const Steps<T>& s, const Seat<T, LANES>& seat, int i, int rows, bool past) const {
         char* to = tile + (int64_t)i * kTile * step;
         if (rows >= kTile && !seat.lone) {
-            if (past) {
+            if (LANES == kWide && past) {
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) store_past((Word4*)(row_of(to + k * step) + (off + lane)), s.w[k]);
             } else {
@@ -901,10 +901,11 @@ void recurrence(const char* op, const adhip_recurrence_args& g, bool backward, h
     p.groups = cut.groups;
     p.ranges = cut.ranges;
     p.tiles = cut.tiles;
-    // (4 x 2048 positions of 4096 channels in f32, both passes: 223 us past the caches, 239 through them)
-    p.past = (backward ? 5 : 3) * batch * length * channels * type_bytes(g.x.type) > kLastCache;
     const int64_t blocks = batch * p.groups;
     const bool factors = g.factors != 0, wide = cut.lanes == kWide;
+    // (4 x 2048 positions of 4096 channels in f32, both passes: 223 us past the caches, 239 through them.  Half lines, as narrow rows write them,
+    // cost a quarter more traffic past the caches, at the same time.)
+    p.past = wide && (backward ? 5 : 3) * batch * length * channels * type_bytes(g.x.type) > kLastCache;
     if (!backward && length >= 1 && length <= kSteps) {
         const int64_t v = 4 / type_bytes(g.x.type), lanes = batch * ((channels + v - 1) / v);
         ADHIP_CHECK(fits_launch((lanes + 255) / 256, 256), "%s: %lld sequences of %lld channels are too many for one call", op, (long long)batch, (long long)channels);
