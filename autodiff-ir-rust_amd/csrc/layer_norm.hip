@@ -1,11 +1,13 @@
 // Layer norm (Ba et al. 2016), and without the mean RMS norm (Zhang and Sennrich 2019), of the rows of an array, with the
 // residual that is added on the way; the backward pass with the sums over rows that are the weights' gradients.
 //
-// Memory bounds it: a row is read once, stays in the registers of the lanes that share it (16, 64, 256 or 1024 of them, up to 16
+// Memory bounds it: a row is read once, stays in the registers of the lanes that share it (16 of them, or 1 to 16 whole wavefronts, up to 16
 // elements each), and its results are written once.  Mean and squared deviations are two sums one after the other over those
 // registers, so a mean that is large against the deviations costs no bits.  In the backward pass a lane keeps the same columns of all
 // rows that it meets, so the weights' gradients add up in its registers; a workgroup adds its lanes' sums in LDS, and a small second
 // kernel the workgroups', always in the same order.
+// 16384 rows of 4096 in bf16 with a residual: forward 99 us (5.4 TB/s), backward 108 (5.0) and 5 for the last sums; 131072 rows of 128: 13.4, 20.2
+// and 3.8; 3001 rows of 1023 in f32 with a residual: 12.2, 16.2 and 3.9.
 #include "operators.hpp"
 
 #include <algorithm>
@@ -17,7 +19,7 @@ namespace {
 constexpr int kElements = 16;          // of a row that a lane holds at most
 constexpr int kThreads = 256;          // of a workgroup that rows of one wavefront and less share
 constexpr int kWaves = 16;             // of a row at most, and of a workgroup of the backward pass
-constexpr int kGradBlocks = 256;       // a compute unit each: more would leave more partial sums of the weights' gradients
+constexpr int kGradBlocks = 256;       // a compute unit each: twice as many of half the size leave twice the partial sums (245 us became 297)
 constexpr int64_t kMostSize = kWaves * 64 * kElements;
 
 struct Place {
@@ -388,7 +390,9 @@ struct Share {
         lanes = size <= 16 * kElements ? 16 : 64;
         packs = most;
         full = false;
-        // two packs a lane, or one, that rows fill exactly (of bf16 rather one: two and a residual's gradient pass the registers)
+        // Two packs a lane, or one, that rows fill exactly.  Of bf16 rather one: two, and a residual's gradient, pass the registers (16384 rows
+        // of 4096, both passes: 211 us with one, 254 with two).  Of f32 rather two, which halve the wavefronts that have to meet (8192
+        // rows: 211 with two, 232 with one).
         for (int i : {0, 1}) {
             const int c = type == ADHIP_BF16 ? 2 - i : 1 + i;
             const int64_t unit = (int64_t)lanes * v * c;

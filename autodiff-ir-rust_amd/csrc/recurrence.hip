@@ -10,6 +10,10 @@
 // knows, out of registers.  From tile to tile only the state is carried, so inputs are read once.  The backward pass needs the
 // states again: the forward pass leaves one every 256 positions, from which a tile of them is recomputed beside the gradients,
 // instead of reading all outputs, which are rounded.
+//
+// 2 x 8192 positions of 4096 channels in bf16: forward 108 us, backward 181 (3.7 TB/s; two arrays copied into a third in this pattern, 64 bytes of
+// rows 8 KB apart, take 107), of 4032 channels 96 and 174; 4 x 2048 of 4096 in f32, 128 bytes of a row: 85 and 137 (4.8, 4.9 TB/s).  Vector units are
+// busy 0.4 of the time: 22 instructions an element forward and 40 backward.  One position of 256 x 8192 channels: 13 us.
 #include "operators.hpp"
 
 #include <algorithm>
