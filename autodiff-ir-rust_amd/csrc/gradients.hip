@@ -11,7 +11,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <utility>
 #include <vector>
 
 #pragma clang fp contract(off)
@@ -234,12 +233,27 @@ void gradients(const char* op, const adhip_gradients_args& g, bool clip, hipStre
         ADHIP_CHECK((uintptr_t)t.g % w == 0 && (!clip || (uintptr_t)t.out % w == 0), "%s: an array of gradient %lld is not aligned to its type", op,
                     (long long)i);
     }
-    if (clip) {  // a gradient that is listed twice would be scaled twice, at once
-        std::vector<std::pair<uintptr_t, uintptr_t>> outs;
+    if (clip) {  // a gradient that is listed twice would be scaled twice, at once; one where another is written may be read too late
+        struct Span {
+            uintptr_t begin, end;
+            int64_t i;
+        };
+        const auto span = [&](const void* a, int64_t i) {
+            return Span{(uintptr_t)a, (uintptr_t)a + (uintptr_t)g.tensors[i].count * type_bytes((int)g.tensors[i].type), i};
+        };
+        std::vector<Span> outs;
         for (int64_t i = 0; i < g.n_tensors; ++i)
-            if (g.tensors[i].count) outs.emplace_back((uintptr_t)g.tensors[i].out, (uintptr_t)g.tensors[i].out + g.tensors[i].count * type_bytes((int)g.tensors[i].type));
-        std::sort(outs.begin(), outs.end());
-        for (size_t i = 1; i < outs.size(); ++i) ADHIP_CHECK(outs[i].first >= outs[i - 1].second, "%s: two clipped gradients share memory", op);
+            if (g.tensors[i].count) outs.push_back(span(g.tensors[i].out, i));
+        std::sort(outs.begin(), outs.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+        for (size_t k = 1; k < outs.size(); ++k) ADHIP_CHECK(outs[k].begin >= outs[k - 1].end, "%s: two clipped gradients share memory", op);
+        for (int64_t i = 0; i < g.n_tensors; ++i) {
+            if (g.tensors[i].count == 0) continue;
+            const Span in = span(g.tensors[i].g, i);
+            // (the first of them that ends behind the gradient's begin; its own, in place, is the only one that it meets)
+            const auto out = std::partition_point(outs.begin(), outs.end(), [&](const Span& o) { return o.end <= in.begin; });
+            ADHIP_CHECK(out == outs.end() || out->begin >= in.end || (out->i == i && out->begin == in.begin),
+                        "%s: gradient %lld lies where another clipped one is written", op, (long long)i);
+        }
     }
     double* const partial = (double*)g.workspace;
     float* const factor = g.factor || !clip ? g.factor : (float*)(partial + blocks);

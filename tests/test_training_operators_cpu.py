@@ -292,6 +292,20 @@ def test_gradient_refusals(dev):
     ops.gradient_norm(dev, gs[:1] * 2, norm, workspace=ROOM)
     assert len(dev.launches()) == 2
     refused(dev, "in device memory", ops.gradient_norm, [torch.zeros(3)], norm, workspace=ROOM)
+    # a gradient where another clipped one is written, or where its own one is written a little apart
+    x, y, z = Array(100, at=4096), Array(100, at=4496), Array(100, at=4896)
+    lies = "lies where another"
+    no(lies, [x, y], norm, gradients_out=[y, x], workspace=ROOM)
+    no(lies, [x, y], norm, gradients_out=[Array(100, at=8192), x], workspace=ROOM)
+    no(lies, [x, x], norm, gradients_out=[z, x], workspace=ROOM)
+    no(lies, [x], norm, gradients_out=[Array(100, at=4096 + 4)], workspace=ROOM)
+    no(lies, [Array(100, at=4096 + 4)], norm, gradients_out=[x], workspace=ROOM)
+    no(lies, [Array(200, at=4096)], norm, gradients_out=[Array(200, at=4496)], workspace=ROOM)
+    for outs in ([z, Array(100, at=8192)], [x, z], [z, y]):
+        ops.clip_gradients(dev, [x, y], norm, limit=1.0, gradients_out=outs, workspace=ROOM)
+        assert len(dev.launches()) == 1
+    ops.clip_gradients(dev, [x, x], norm, limit=1.0, gradients_out=[y, z], workspace=ROOM)
+    assert len(dev.launches()) == 1
     refused(dev, "in device memory", ops.gradient_norm, gs, torch.zeros(1), workspace=ROOM)
     refused(dev, "in device memory", ops.clip_gradients, gs, norm, limit=1.0, gradients_out=[torch.zeros(5, 7), gs[1]], workspace=ROOM)
 
