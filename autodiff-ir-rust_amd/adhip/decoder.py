@@ -218,6 +218,8 @@ class DecoderRecurrence(DecoderLayer):
 
 
 def main(kind: str = "attention"):
+    if kind not in ("attention", "recurrence"):
+        raise SystemExit(f"{kind}: attention or recurrence is wanted")
     from . import HipDevice
     rng = np.random.default_rng(0)
     x = rng.standard_normal((2, 512, 256)).astype(np.float32)

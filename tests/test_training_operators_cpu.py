@@ -8,7 +8,7 @@ import subprocess
 import pytest
 import torch
 
-from adhip import operators as ops
+from adhip import decoder, operators as ops
 from adhip.device import library_path
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -334,6 +334,11 @@ def test_adamw_factor_refusals(dev):
 
 
 # ---- without a context, and the C structs ---------------------------------------------------------------------------------
+def test_the_decoder_names_its_layers():
+    with pytest.raises(SystemExit, match="attention or recurrence"):
+        decoder.main("convolution")
+
+
 
 
 def test_calls_without_a_context_or_arguments_are_errors(dev):
