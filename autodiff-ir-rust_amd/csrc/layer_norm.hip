@@ -490,6 +490,7 @@ void layer_norm(const char* op, const adhip_layer_norm_args& g, bool backward, h
         if (arrays[i].output) check_distinct(op, arrays[i].name, a);
     }
     // weights: of x's type or f32, both alike
+    ADHIP_CHECK(!adds || rows == 0 || g.total.data != g.out.data, "%s: total and out are one array", op);
     const int w_type = g.weight.data ? g.weight.type : g.bias.data && !backward ? g.bias.type : ADHIP_F32;
     if (g.weight.data) check_vector(op, "weight", g.weight, size, false);
     if (g.bias.data && !backward) check_vector(op, "bias", g.bias, size, false);

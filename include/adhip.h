@@ -267,7 +267,7 @@ int adhip_attention_backward(adhip_ctx* ctx, const adhip_attention_args* args, v
  *     out = (t - mean) root weight + bias
  * weight and bias [size] are f32 or of x's type, both alike; no weight is a weight of 1, no bias a bias of 0.  Not centered and
  * without a bias it is RMS norm.  stats (f32, x's leading dims and 2, packed, aligned to 8 bytes; may be left out) receives mean and root.  total and out
- * may be x or added themselves, under the same strides (out not beside a total that is the same array). */
+ * may be x or added themselves, under the same strides (out and total are two arrays). */
 typedef struct adhip_layer_norm_args {
     adhip_array x, added, total, out, weight, bias, stats;
     /* backward only */

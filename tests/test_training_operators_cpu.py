@@ -119,6 +119,7 @@ def test_layer_norm_refusals(dev):
     no("total has 0 dims", x, x, added=x)
     no("added has 0 dims", x, x, total=x)
     no("added is", x, x, added=Array(6, 41), total=x)
+    no("total and out are one array", x, x, added=x, total=x)
     no("weight is", x, x, weight=Array(41))
     no("weight and bias are bf16", x, x, weight=Array(40, dtype="bfloat16"), bias=None)
     no("one type is wanted", x, x, bias=Array(40, dtype="bfloat16"))
