@@ -259,11 +259,12 @@ __global__ __launch_bounds__(kWaves * 64) void norm_backward_kernel(const NormPa
             for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    n[c][k] = (float)raw.x[c].v[k];
+                    // (a row that is not there read the last one, or what x_grad put in its place, and must not show in the sums)
+                    n[c][k] = there ? (float)raw.x[c].v[k] : 0.f;
                     u[c][k] = there ? (float)raw.d[c].v[k] : 0.f;
                     if (ADDS) more[c][k] = (float)raw.more[c].v[k];
                 }
-            mean = raw.stats.x, root = raw.stats.y;
+            mean = there ? raw.stats.x : 0.f, root = there ? raw.stats.y : 0.f;
         } else {
             const int size = there ? p.size : 0;
 #pragma unroll
@@ -489,8 +490,8 @@ void layer_norm(const char* op, const adhip_layer_norm_args& g, bool backward, h
         check_packed_rows(op, arrays[i].name, a);
         if (arrays[i].output) check_distinct(op, arrays[i].name, a);
     }
-    // weights: of x's type or f32, both alike
     ADHIP_CHECK(!adds || rows == 0 || g.total.data != g.out.data, "%s: total and out are one array", op);
+    // weights: of x's type or f32, both alike
     const int w_type = g.weight.data ? g.weight.type : g.bias.data && !backward ? g.bias.type : ADHIP_F32;
     if (g.weight.data) check_vector(op, "weight", g.weight, size, false);
     if (g.bias.data && !backward) check_vector(op, "bias", g.bias, size, false);

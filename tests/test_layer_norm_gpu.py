@@ -147,6 +147,23 @@ def test_in_place(hip_device, size, dtype):
     assert torch.equal(g["out_grad"], want["x_grad"]) and torch.equal(dw, want["weight_grad"])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,size", [(1, 256), (3, 512), (257, 128), (16 * 256 + 1, 512), (513, 4096)])
+def test_a_last_row_in_place_that_is_not_finite(hip_device, rows, size, dtype):
+    """What x_grad puts in the place of the last row is not read by those that have no row."""
+    a = inputs((rows, size), dtype, "f32", seed=rows)
+    a["total_grad"][-1] = float("inf")
+    want = run(hip_device, a)
+    room = torch.empty(ops.layer_norm_workspace(hip_device, want["total"]), dtype=torch.uint8, device="cuda")
+    dw, db = torch.empty(size, device="cuda"), torch.empty(size, device="cuda")
+    g = {n: a[n].cuda() for n in ("weight", "out_grad", "total_grad")}
+    ops.layer_norm_backward(hip_device, want["total"], want["stats"], g["out_grad"], want["total"], weight=g["weight"], weight_grad=dw, bias_grad=db,
+                            total_grad=g["total_grad"], workspace=room, stream=here())
+    torch.cuda.synchronize()
+    assert torch.equal(want["total"], want["x_grad"]) and want["x_grad"][-1].isinf().all()
+    assert dw.isfinite().all() and torch.equal(dw, want["weight_grad"]) and torch.equal(db, want["bias_grad"])
+
+
 def test_gradients_that_are_not_asked_for(hip_device):
     a = inputs((9, 300), "f32", "f32")
     want = run(hip_device, a, adds=False)

@@ -292,7 +292,6 @@ def test_gradient_refusals(dev):
     ops.clip_gradients(dev, [Array(100, at=4096), Array(100, at=4096 + 400), Array(0, at=4096)], norm, limit=1.0, workspace=ROOM)
     ops.gradient_norm(dev, gs[:1] * 2, norm, workspace=ROOM)
     assert len(dev.launches()) == 2
-    refused(dev, "in device memory", ops.gradient_norm, [torch.zeros(3)], norm, workspace=ROOM)
     # a gradient where another clipped one is written, or where its own one is written a little apart
     x, y, z = Array(100, at=4096), Array(100, at=4496), Array(100, at=4896)
     lies = "lies where another"
@@ -307,6 +306,7 @@ def test_gradient_refusals(dev):
         assert len(dev.launches()) == 1
     ops.clip_gradients(dev, [x, x], norm, limit=1.0, gradients_out=[y, z], workspace=ROOM)
     assert len(dev.launches()) == 1
+    refused(dev, "in device memory", ops.gradient_norm, [torch.zeros(3)], norm, workspace=ROOM)
     refused(dev, "in device memory", ops.gradient_norm, gs, torch.zeros(1), workspace=ROOM)
     refused(dev, "in device memory", ops.clip_gradients, gs, norm, limit=1.0, gradients_out=[torch.zeros(5, 7), gs[1]], workspace=ROOM)
 
@@ -334,12 +334,12 @@ def test_adamw_factor_refusals(dev):
     refused(dev, "in device memory", ops.adamw, one, one, one, one, factor=torch.ones(1), **how)
 
 
-# ---- without a context, and the C structs ---------------------------------------------------------------------------------
 def test_the_decoder_names_its_layers():
     with pytest.raises(SystemExit, match="attention or recurrence"):
         decoder.main("convolution")
 
 
+# ---- without a context, and the C structs ---------------------------------------------------------------------------------
 
 
 def test_calls_without_a_context_or_arguments_are_errors(dev):
