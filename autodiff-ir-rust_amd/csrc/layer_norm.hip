@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace adhip {
 namespace {
@@ -57,36 +58,43 @@ struct __attribute__((packed, aligned(sizeof(T)))) Loose {
     T v[N];
 };
 
-// V elements of a row from e on; zeros behind its end.  Rows that fill their lanes have none (FULL).
+// Where a pack of V elements that begins at `at` lies.  In rows that do not fill their lanes (FULL) one that would pass the end is moved
+// back to it: its first `skip` elements belong to another lane, all V to a lane behind the end.  So every lane makes the same loads, with
+// no branch between them, and rows of at least V elements are wanted.
+template <int V, bool FULL>
+struct Spot {
+    int e, skip;
+    __device__ __forceinline__ Spot(int at, int size) : e(FULL ? at : min(at, size - V)), skip(FULL ? 0 : at - e) {}
+    __device__ __forceinline__ bool has(int k) const { return FULL || k >= skip; }
+};
+
 template <class T, int V, bool FULL>
-__device__ __forceinline__ void load_row(const void* row, int64_t at, int e, int size, float (&f)[V]) {
-    const T* x = (const T*)row + at + e;
-    if (FULL || e + V <= size) {
-        const Loose<T, V> r = *(const Loose<T, V>*)x;
+__device__ __forceinline__ void load_row(const void* row, int64_t at, const Spot<V, FULL>& spot, float (&f)[V]) {
+    const Loose<T, V> r = *(const Loose<T, V>*)((const T*)row + at + spot.e);
 #pragma unroll
-        for (int k = 0; k < V; ++k) f[k] = (float)r.v[k];
-    } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) f[k] = e + k < size ? (float)x[k] : 0.f;
-    }
+    for (int k = 0; k < V; ++k) f[k] = spot.has(k) ? (float)r.v[k] : 0.f;
 }
 
 template <class T, int V, bool FULL>
-__device__ __forceinline__ void store_row(void* row, int64_t at, int e, int size, bool past, const float (&f)[V]) {
-    T* x = (T*)row + at + e;
-    if (FULL || e + V <= size) {
+__device__ __forceinline__ void store_row(void* row, int64_t at, const Spot<V, FULL>& spot, bool past, const float (&f)[V]) {
+    T* x = (T*)row + at + spot.e;
+    if (FULL || spot.skip == 0) {
         Loose<T, V> r;
 #pragma unroll
         for (int k = 0; k < V; ++k) r.v[k] = (T)f[k];
-        Word16 w;
-        static_assert(sizeof r == sizeof w, "a lane's pack");
-        __builtin_memcpy(&w, &r, sizeof w);
-        if (past) store_past((Word16*)x, w);
-        else *(Word16*)x = w;
+        if constexpr (V == 1) {
+            *(Loose<T, V>*)x = r;
+        } else {
+            Word16 w;
+            static_assert(sizeof r == sizeof w, "a lane's pack");
+            __builtin_memcpy(&w, &r, sizeof w);
+            if (past) store_past((Word16*)x, w);
+            else *(Word16*)x = w;
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < V; ++k)
-            if (e + k < size) x[k] = (T)f[k];
+            if (spot.has(k)) x[k] = (T)f[k];
     }
 }
 
@@ -148,30 +156,54 @@ struct Team {
     }
 };
 
-template <class T, class W, int LANES, int C, bool FULL>
+// A workgroup takes several rows one after the other: the next one, whose loads no branch divides, is asked for as soon as this one is in
+// other registers, and weight and bias stay in registers.
+template <class T, class W, int V, int LANES, int C, bool FULL, bool ADDS>
 __global__ __launch_bounds__(LANES == 64 ? kWaves * 64 : kThreads) void norm_kernel(const NormParams p) {
-    constexpr int V = 16 / sizeof(T);
     Team<LANES> team(p);
     const int lanes = team.lanes();
     const float per = 1.f / (float)p.size;
+    const auto spot = [&](int c) { return Spot<V, FULL>((c * lanes + team.lane) * V, p.size); };
+    struct Row {
+        Loose<T, V> x[C], added[ADDS ? C : 1];
+    } raw;
+    const auto ask = [&](unsigned row) {
+        const RowIndex index(p, row);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            raw.x[c] = *(const Loose<T, V>*)((const T*)p.x + index.at(p.x_at) + spot(c).e);
+            if (ADDS) raw.added[c] = *(const Loose<T, V>*)((const T*)p.added + index.at(p.added_at) + spot(c).e);
+        }
+    };
+    const unsigned step = gridDim.x * p.groups;
+    ask(min(blockIdx.x * p.groups + team.group, p.rows - 1));
+    Loose<W, V> weight[C], bias[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if (p.weight) weight[c] = *(const Loose<W, V>*)((const W*)p.weight + spot(c).e);
+        if (p.bias) bias[c] = *(const Loose<W, V>*)((const W*)p.bias + spot(c).e);
+    }
     // (all lanes of a workgroup go round equally often: they meet at barriers)
-    for (unsigned first = blockIdx.x * p.groups; first < p.rows; first += gridDim.x * p.groups) {
+    for (unsigned first = blockIdx.x * p.groups; first < p.rows; first += step) {
         const unsigned row = min(first + team.group, p.rows - 1);
         const bool there = first + team.group < p.rows;  // (a row too many reads the last one, and writes nothing)
         const RowIndex index(p, row);
-        float x[C][V];
+        float x[C][V], added[ADDS ? C : 1][V];
 #pragma unroll
-        for (int c = 0; c < C; ++c) load_row<T, V, FULL>(p.x, index.at(p.x_at), (c * lanes + team.lane) * V, p.size, x[c]);
-        if (p.added) {
-            float y[C][V];
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int c = 0; c < C; ++c) load_row<T, V, FULL>(p.added, index.at(p.added_at), (c * lanes + team.lane) * V, p.size, y[c]);
+            for (int k = 0; k < V; ++k) {
+                x[c][k] = spot(c).has(k) ? (float)raw.x[c].v[k] : 0.f;
+                if (ADDS) added[c][k] = spot(c).has(k) ? (float)raw.added[c].v[k] : 0.f;
+            }
+        ask(min(first + step + team.group, p.rows - 1));
+        if (ADDS) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 // rounded to the arrays' type as it is kept: what is normed here is what the backward pass reads
 #pragma unroll
-                for (int k = 0; k < V; ++k) x[c][k] = (float)(T)(x[c][k] + y[c][k]);
-                if (there) store_row<T, V, FULL>(p.total, index.at(p.total_at), (c * lanes + team.lane) * V, p.size, p.past, x[c]);
+                for (int k = 0; k < V; ++k) x[c][k] = (float)(T)(x[c][k] + added[c][k]);
+                if (there) store_row<T>(p.total, index.at(p.total_at), spot(c), p.past, x[c]);
             }
         }
         float sum = 0, none = 0;
@@ -189,7 +221,7 @@ __global__ __launch_bounds__(LANES == 64 ? kWaves * 64 : kThreads) void norm_ker
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                x[c][k] = FULL || (c * lanes + team.lane) * V + k < p.size ? x[c][k] - mean : 0.f;
+                x[c][k] = spot(c).has(k) ? x[c][k] - mean : 0.f;
                 squares = __builtin_fmaf(x[c][k], x[c][k], squares);
             }
         none = 0;
@@ -199,21 +231,15 @@ __global__ __launch_bounds__(LANES == 64 ? kWaves * 64 : kThreads) void norm_ker
         if (p.stats && team.lane == 0) *(float2*)(p.stats + 2 * (int64_t)row) = make_float2(mean, root);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int e = (c * lanes + team.lane) * V;
-            float w[V];
 #pragma unroll
             for (int k = 0; k < V; ++k) x[c][k] *= root;
-            if (p.weight) {
-                load_row<W, V, FULL>(p.weight, 0, e, p.size, w);
+            if (p.weight)
 #pragma unroll
-                for (int k = 0; k < V; ++k) x[c][k] *= w[k];
-            }
-            if (p.bias) {
-                load_row<W, V, FULL>(p.bias, 0, e, p.size, w);
+                for (int k = 0; k < V; ++k) x[c][k] *= (float)weight[c].v[k];
+            if (p.bias)
 #pragma unroll
-                for (int k = 0; k < V; ++k) x[c][k] += w[k];
-            }
-            store_row<T, V, FULL>(p.out, index.at(p.out_at), e, p.size, p.past, x[c]);
+                for (int k = 0; k < V; ++k) x[c][k] += (float)bias[c].v[k];
+            store_row<T>(p.out, index.at(p.out_at), spot(c), p.past, x[c]);
         }
     }
 }
@@ -222,10 +248,9 @@ __global__ __launch_bounds__(LANES == 64 ? kWaves * 64 : kThreads) void norm_ker
 //     x_grad = root (u - mean(u) - n mean(u n)) + total_grad      (without the mean of u where the norm takes no mean)
 //     weight_grad = sum over rows of out_grad n,  bias_grad = sum over rows of out_grad
 // Where rows fill their lanes (FULL) the next one is asked for as soon as this one is in other registers; loads without a branch are
-// loads that the compiler can count, so it waits for those of this row alone.
-template <class T, class W, int LANES, int C, bool FULL, bool SUMS, bool ADDS>
+// loads that the compiler can count, so it waits for those of this row alone.  Others take twice the registers already.
+template <class T, class W, int V, int LANES, int C, bool FULL, bool SUMS, bool ADDS>
 __global__ __launch_bounds__(kWaves * 64) void norm_backward_kernel(const NormParams p) {
-    constexpr int V = 16 / sizeof(T);
     Team<LANES> team(p);
     const int lanes = team.lanes();
     const float per = 1.f / (float)p.size;
@@ -234,61 +259,49 @@ __global__ __launch_bounds__(kWaves * 64) void norm_backward_kernel(const NormPa
         Loose<T, V> x[C], d[C], more[ADDS ? C : 1];
         float2 stats;
     } raw;
-    const auto element = [&](int c) { return (c * lanes + team.lane) * V; };
+    const auto spot = [&](int c) { return Spot<V, FULL>((c * lanes + team.lane) * V, p.size); };
     const auto ask = [&](Row& r, unsigned row) {
         const RowIndex index(p, row);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            r.x[c] = *(const Loose<T, V>*)((const T*)p.x + index.at(p.x_at) + element(c));
-            r.d[c] = *(const Loose<T, V>*)((const T*)p.out_grad + index.at(p.out_grad_at) + element(c));
-            if (ADDS) r.more[c] = *(const Loose<T, V>*)((const T*)p.total_grad + index.at(p.total_grad_at) + element(c));
+            r.x[c] = *(const Loose<T, V>*)((const T*)p.x + index.at(p.x_at) + spot(c).e);
+            r.d[c] = *(const Loose<T, V>*)((const T*)p.out_grad + index.at(p.out_grad_at) + spot(c).e);
+            if (ADDS) r.more[c] = *(const Loose<T, V>*)((const T*)p.total_grad + index.at(p.total_grad_at) + spot(c).e);
         }
         r.stats = *(const float2*)(p.stats + 2 * (int64_t)row);
     };
     const unsigned step = gridDim.x * p.groups;
-    if (FULL) ask(raw, min(blockIdx.x * p.groups + team.group, p.rows - 1));
+    constexpr bool AHEAD = FULL || C * V <= 8;  // (of others the registers do not hold two rows)
+    if (AHEAD) ask(raw, min(blockIdx.x * p.groups + team.group, p.rows - 1));
     // (all lanes of a workgroup go round equally often: they meet at barriers)
     for (unsigned first = blockIdx.x * p.groups; first < p.rows; first += step) {
         const unsigned row = first + team.group;
         const bool there = row < p.rows;
         const RowIndex index(p, there ? row : 0);
         float n[C][V], u[C][V], more[ADDS ? C : 1][V], w[C][V];
-        float mean, root;
-        if (FULL) {
+        if (!AHEAD) ask(raw, min(row, p.rows - 1));
+        // (a row that is not there read the last one, or what x_grad put in its place, and must not show in the sums)
+        const float mean = there ? raw.stats.x : 0.f, root = there ? raw.stats.y : 0.f;
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    // (a row that is not there read the last one, or what x_grad put in its place, and must not show in the sums)
-                    n[c][k] = there ? (float)raw.x[c].v[k] : 0.f;
-                    u[c][k] = there ? (float)raw.d[c].v[k] : 0.f;
-                    if (ADDS) more[c][k] = (float)raw.more[c].v[k];
-                }
-            mean = there ? raw.stats.x : 0.f, root = there ? raw.stats.y : 0.f;
-        } else {
-            const int size = there ? p.size : 0;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                load_row<T, V, false>(p.x, index.at(p.x_at), element(c), size, n[c]);
-                load_row<T, V, false>(p.out_grad, index.at(p.out_grad_at), element(c), size, u[c]);
-                if (ADDS) load_row<T, V, false>(p.total_grad, index.at(p.total_grad_at), element(c), size, more[c]);
+            for (int k = 0; k < V; ++k) {
+                // what does not count has n = 0, whatever mean and root are
+                const bool counts = there && spot(c).has(k);
+                n[c][k] = counts ? (float)raw.x[c].v[k] : mean;
+                u[c][k] = counts ? (float)raw.d[c].v[k] : 0.f;
+                if (ADDS) more[c][k] = (float)raw.more[c].v[k];
             }
-            mean = root = 0;
-            if (there) {
-                const float2 s = *(const float2*)(p.stats + 2 * (int64_t)row);
-                mean = s.x, root = s.y;
-            }
-        }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             if (p.weight) {
-                load_row<W, V, FULL>(p.weight, 0, element(c), p.size, w[c]);
+                load_row<W>(p.weight, 0, spot(c), w[c]);
             } else {
 #pragma unroll
                 for (int k = 0; k < V; ++k) w[c][k] = 1.f;
             }
         }
-        if (FULL) ask(raw, min(row + step, p.rows - 1));
+        if (AHEAD) ask(raw, min(row + step, p.rows - 1));
         float sum = 0, along = 0;
 #pragma unroll
         for (int c = 0; c < C; ++c)
@@ -314,7 +327,7 @@ __global__ __launch_bounds__(kWaves * 64) void norm_backward_kernel(const NormPa
                 if (ADDS)
 #pragma unroll
                     for (int k = 0; k < V; ++k) u[c][k] += more[c][k];
-                store_row<T, V, FULL>(p.x_grad, index.at(p.x_grad_at), element(c), p.size, p.past, u[c]);
+                store_row<T>(p.x_grad, index.at(p.x_grad_at), spot(c), p.past, u[c]);
             }
         }
     }
@@ -340,7 +353,8 @@ __global__ __launch_bounds__(kWaves * 64) void norm_backward_kernel(const NormPa
                 }
                 if (LANES == 64 || (threadIdx.x & 63) < LANES)
 #pragma unroll
-                    for (int k = 0; k < V; ++k) meet[(mine * 2 * C + which * C + c) * across + team.lane * V + k] = s[k];
+                    for (int k = 0; k < V; ++k)
+                        if (spot(c).has(k)) meet[(mine * 2 + which) * C * across + spot(c).e + k] = s[k];
             }
         __syncthreads();
         const int columns = C * across;
@@ -348,7 +362,7 @@ __global__ __launch_bounds__(kWaves * 64) void norm_backward_kernel(const NormPa
             for (int i = threadIdx.x; i < columns; i += blockDim.x) {
                 float sum = 0;
                 for (int r = 0; r < rows; ++r) sum += meet[(r * 2 + which) * columns + i];
-                if (i < p.padded) part[which * p.padded + i] = sum;
+                if (i < p.size) part[which * p.padded + i] = sum;
             }
     }
 }
@@ -386,11 +400,15 @@ __global__ __launch_bounds__(256) void norm_sums_kernel(const float* part, int p
 // How rows are shared out: 16 lanes each, or 1 to 16 wavefronts; packs of 16 bytes a lane; whether rows fill their lanes.
 struct Share {
     int lanes, packs, waves, groups, grad_groups;
-    bool full;
+    bool full, narrow;  // narrow: rows shorter than a pack, an element a lane
     Share(int type, int64_t size) {
-        const int v = 16 / type_bytes(type), most = kElements / v;
-        lanes = size <= 16 * kElements ? 16 : 64;
-        packs = most;
+        const int v = 16 / type_bytes(type);
+        narrow = size < v;
+        // One pack where the lanes hold a row so, two otherwise, and four of f32 where 16 wavefronts of two do not.  With fewer elements a lane
+        // more rows are under way: 30001 rows of 250 in f32, both passes: 55 us, and 71 by 16 lanes of four packs; 32072 rows of 500 in bf16:
+        // 17, and 22 with two.  With one pack a lane, more wavefronts meet in longer rows: 20001 rows of 3001 in bf16: 79 us, and 59 with two.
+        lanes = size <= 16 * 2 * v ? 16 : 64;
+        packs = size <= lanes * v ? 1 : size <= kWaves * 64 * 2 * v ? 2 : 4;
         full = false;
         // Two packs a lane, or one, that rows fill exactly.  Of bf16 rather one: two, and a residual's gradient, pass the registers (16384 rows
         // of 4096, both passes: 211 us with one, 254 with two).  Of f32 rather two, which halve the wavefronts that have to meet (8192
@@ -416,30 +434,41 @@ int64_t grad_blocks(int type, int64_t rows, int64_t size) {
 
 size_t workspace_of(int type, int64_t rows, int64_t size) { return (size_t)grad_blocks(type, rows, size) * 2 * (size_t)padded_of(size) * sizeof(float); }
 
-template <class T, class W, int LANES, int C, bool FULL>
+template <class T, class W, int V, int LANES, int C, bool FULL>
 void launch_norm(const char* op, const NormParams& p, const Share& share, bool backward, bool sums, unsigned blocks, hipStream_t stream) {
     const unsigned threads = (unsigned)share.threads(backward);
     if (!backward)
-        launch(op, norm_kernel<T, W, LANES, C, FULL>, blocks, threads, stream, p);
+        launch(op, p.added ? norm_kernel<T, W, V, LANES, C, FULL, true> : norm_kernel<T, W, V, LANES, C, FULL, false>, blocks, threads, stream, p);
     else if (sums && p.total_grad)
-        launch(op, norm_backward_kernel<T, W, LANES, C, FULL, true, true>, blocks, threads, stream, p);
+        launch(op, norm_backward_kernel<T, W, V, LANES, C, FULL, true, true>, blocks, threads, stream, p);
     else if (sums)
-        launch(op, norm_backward_kernel<T, W, LANES, C, FULL, true, false>, blocks, threads, stream, p);
+        launch(op, norm_backward_kernel<T, W, V, LANES, C, FULL, true, false>, blocks, threads, stream, p);
     else if (p.total_grad)
-        launch(op, norm_backward_kernel<T, W, LANES, C, FULL, false, true>, blocks, threads, stream, p);
+        launch(op, norm_backward_kernel<T, W, V, LANES, C, FULL, false, true>, blocks, threads, stream, p);
     else
-        launch(op, norm_backward_kernel<T, W, LANES, C, FULL, false, false>, blocks, threads, stream, p);
+        launch(op, norm_backward_kernel<T, W, V, LANES, C, FULL, false, false>, blocks, threads, stream, p);
 }
+
+template <auto X>
+using Is = std::integral_constant<decltype(X), X>;
 
 template <class T, class W>
 void launch_norm(const char* op, const NormParams& p, const Share& share, bool backward, bool sums, unsigned blocks, hipStream_t stream) {
-    constexpr int most = kElements * sizeof(T) / 16;
-    if (share.lanes == 16 && !share.full) launch_norm<T, W, 16, most, false>(op, p, share, backward, sums, blocks, stream);
-    else if (share.lanes == 16 && share.packs == 1) launch_norm<T, W, 16, 1, true>(op, p, share, backward, sums, blocks, stream);
-    else if (share.lanes == 16) launch_norm<T, W, 16, 2, true>(op, p, share, backward, sums, blocks, stream);
-    else if (!share.full) launch_norm<T, W, 64, most, false>(op, p, share, backward, sums, blocks, stream);
-    else if (share.packs == 1) launch_norm<T, W, 64, 1, true>(op, p, share, backward, sums, blocks, stream);
-    else launch_norm<T, W, 64, 2, true>(op, p, share, backward, sums, blocks, stream);
+    constexpr int V = 16 / sizeof(T);
+    const auto go = [&](auto lanes, auto packs, auto full) {
+        launch_norm<T, W, V, lanes(), packs(), full()>(op, p, share, backward, sums, blocks, stream);
+    };
+    const auto with_lanes = [&](auto lanes) {
+        if (share.full && share.packs == 1) return go(lanes, Is<1>(), Is<true>());
+        if (share.full) return go(lanes, Is<2>(), Is<true>());
+        if (share.packs == 1) return go(lanes, Is<1>(), Is<false>());
+        if constexpr (lanes() == 64 && V == 4)
+            if (share.packs == 4) return go(lanes, Is<4>(), Is<false>());
+        go(lanes, Is<2>(), Is<false>());
+    };
+    if (share.narrow) launch_norm<T, W, 1, 16, 1, false>(op, p, share, backward, sums, blocks, stream);
+    else if (share.lanes == 16) with_lanes(Is<16>());
+    else with_lanes(Is<64>());
 }
 
 struct Named {
@@ -564,8 +593,12 @@ void layer_norm(const char* op, const adhip_layer_norm_args& g, bool backward, h
         const Share share(g.x.type, size);
         p.waves = share.waves;
         p.groups = backward ? share.grad_groups : share.groups;
-        // (more rows than a launch holds go round)
-        const int64_t all = std::min<int64_t>((rows + p.groups - 1) / p.groups, 0xffffffffu / (unsigned)share.threads(false));
+        // A forward workgroup takes several rows, two at least where there are more than the chip has at once, in four times as many workgroups
+        // as it holds, and eight times with a residual (16384 rows of 4096 in bf16: 52 us, with a residual 96; the other way round 56 and 98; a
+        // row each 76 and 98).
+        const int64_t each = (rows + p.groups - 1) / p.groups, at_once = 256 * 2048 / share.threads(false);
+        const int64_t rounds = std::max<int64_t>((each - 1) / (at_once * (adds ? 8 : 4)) + 1, each > 2 * at_once ? 2 : 1);
+        const int64_t all = (each + rounds - 1) / rounds;
         const unsigned blocks = (unsigned)(backward ? grad_blocks(g.x.type, rows, size) : all);
         if (g.x.type == ADHIP_F32) launch_norm<float, float>(op, p, share, backward, sums, blocks, stream);
         else if (w_type == ADHIP_F32) launch_norm<bf16, float>(op, p, share, backward, sums, blocks, stream);

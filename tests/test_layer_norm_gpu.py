@@ -85,6 +85,21 @@ def test_a_mean_that_is_large_against_the_deviations(hip_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [1, 2, 4, 8, 32, 64])
+def test_a_mean_whose_product_with_the_root_passes_the_range(hip_device, size, dtype):
+    """Rows of 2^80 alone (a sum and a mean that are exact) have no deviation, and a root of 1e15: mean times root is infinite, and lanes
+    behind the end of the rows must not bring it into the sums."""
+    a = inputs((5, size), dtype, "f32", seed=size)
+    a["x"] = torch.full_like(a["x"], 2.0**80)
+    got = run(hip_device, a, eps=1e-30, adds=False)
+    assert torch.equal(got["out"].cpu(), a["bias"].expand(5, size).to(TYPES[dtype])) and got["x_grad"].isfinite().all()
+    assert (got["weight_grad"] == 0).all()
+    # five addends, added in some order: four roundings of sums that are at most the sum of magnitudes
+    exact = a["out_grad"].double().sum(0)
+    assert ((got["bias_grad"].cpu() - exact).abs() <= 4 * 2.0**-24 * a["out_grad"].double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_rows_of_equal_values(hip_device, dtype):
     """No deviation: the root is that of eps alone."""
     a = inputs((3, 64), dtype, "f32")
