@@ -121,6 +121,19 @@ __device__ __forceinline__ float together(float a, float b) {
     return FACTORS && (a == 0.f || b == 0.f) ? 0.f : a * b;
 }
 
+// The same with the factor of one position, which is finite: a comparison that serves both (4 x 2049 positions of 2560 channels in bf16,
+// factors: forward 48 us, with the other two 51; both passes 146 and 158).
+template <bool FACTORS>
+__device__ __forceinline__ float step(float a, float h, float b) {
+    const float r = __builtin_fmaf(a, h, b);
+    return FACTORS && a == 0.f ? b : r;
+}
+template <bool FACTORS>
+__device__ __forceinline__ float grown(float A, float a) {
+    const float r = A * a;
+    return FACTORS && a == 0.f ? 0.f : r;
+}
+
 // Which of K positions from t on count (live), and where the state before is dropped (cut); positions from `count` on pass it on.
 struct Marks {
     unsigned live, cut;
@@ -345,13 +358,35 @@ __device__ __forceinline__ void over_ranges(const RecurrenceParams& p, const Sea
     }
 }
 
-// What wavefronts that are not there do to a state: nothing.
-template <int WAVES, int PARTS>
-__device__ __forceinline__ void fill_absent(float2 (&parts)[2][WAVES][PARTS]) {
-    const int waves = blockDim.x / 64;
-    for (int i = threadIdx.x; i < (WAVES - waves) * PARTS; i += blockDim.x)
-        parts[0][waves + i / PARTS][i % PARTS] = parts[1][waves + i / PARTS][i % PARTS] = make_float2(1, 0);
+// A state carried over the maps of whole wavefronts, from `w` on up to, but not, `end`, four loads at once.  `map` reads one.  A wavefront
+// goes over those before it alone, and of a pack's two channels a thread over one: with all of both, where 16 wavefronts share wide rows,
+// a third of all instructions (4 x up to 2049 positions of 2560 channels: 41 us, with all 44; 256 x 16 of 1024, both passes: 40 and 48).
+template <bool FACTORS, class M>
+__device__ __forceinline__ float over_waves(int w, int end, int way, float h, M&& map) {
+    constexpr int kAtOnce = 4;
+    while (w != end) {
+        float2 m[kAtOnce];
+        const int n = min(abs(end - w), kAtOnce);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) m[i] = map(w + way * min(i, n - 1));
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (i < n) h = onward<FACTORS>(m[i].x, h, m[i].y);
+        w += way * n;
+    }
+    return h;
 }
+
+// Of the threads of a wavefront that have the same two channels one half carries states over wavefronts for the one, the other half for
+// the other: `pick` is a thread's own, and this gives both to both.
+template <int LANES>
+__device__ __forceinline__ void share(int pick, float at, float (&h)[2]) {
+    const float other = __shfl_xor(at, LANES);
+    h[0] = pick ? other : at;
+    h[1] = pick ? at : other;
+}
+template <int LANES>
+__device__ __forceinline__ void share(int, float at, float (&h)[1]) { h[0] = at; }
 
 template <class T, int LANES, bool FACTORS, bool DOCS>
 __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const RecurrenceParams p) {
@@ -360,7 +395,8 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const
     if (!seat.there(p.ranges)) return;
     const int lane = seat.lane, wave = seat.wave, slot = seat.slot;
     __shared__ float2 parts[2][kWaves][LANES * V];  // (by turns: the other one's barrier stands between readers and writers)
-    fill_absent(parts);
+    __shared__ float carried[2][LANES * V];         // the state before a tile: who needs it reads it, and the last wavefront leaves the next one
+    const int waves = blockDim.x / 64, pick = lane / LANES % V;
     float carry[V];
     if (p.ranges == 1) {
         load_state<V>(p.initial, seat.batch * p.initial_b, seat.c, p.channels, carry);
@@ -373,6 +409,9 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const
         for (int v = 0; v < V; ++v) carry[v] = kept[v].y;
         over_ranges<T, LANES, FACTORS>(p, seat, 0, seat.range, 1, carry);
     }
+    if (seat.own == 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) carried[0][slot + v] = carry[v];
     int turn = 0;
     // From the maps of a tile to its states, and the state behind it.
     auto states = [&](const float (&a)[kSteps][V], const float (&b)[kSteps][V], int begin, Steps<T>& o) {
@@ -382,21 +421,19 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const
             A[v] = a[0][v], B[v] = b[0][v];
 #pragma unroll
             for (int k = 1; k < kSteps; ++k) {
-                A[v] = together<FACTORS>(A[v], a[k][v]);
-                B[v] = onward<FACTORS>(a[k][v], B[v], b[k][v]);
+                A[v] = grown<FACTORS>(A[v], a[k][v]);
+                B[v] = step<FACTORS>(a[k][v], B[v], b[k][v]);
             }
             across<LANES, FACTORS, false>(lane, A[v], B[v], preA[v], preB[v]);
             if (lane < LANES) parts[turn][wave][slot + v] = make_float2(A[v], B[v]);
         }
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float2 part = parts[turn][w][slot + v];
-                if (w == wave) h[v] = carry[v];
-                carry[v] = onward<FACTORS>(part.x, carry[v], part.y);
-            }
+        const float at = over_waves<FACTORS>(0, wave, 1, carried[turn][slot + pick], [&](int w) { return parts[turn][w][slot + pick]; });
+        if (wave == waves - 1 && lane < LANES * V) {
+            const float2 part = parts[turn][wave][slot + pick];
+            carried[turn ^ 1][slot + pick] = onward<FACTORS>(part.x, at, part.y);
+        }
+        share<LANES>(pick, at, h);
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = onward<FACTORS>(preA[v], h[v], preB[v]);
         turn ^= 1;
@@ -404,7 +441,7 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = onward<FACTORS>(a[k][v], h[v], b[k][v]);
+            for (int v = 0; v < V; ++v) h[v] = step<FACTORS>(a[k][v], h[v], b[k][v]);
             o.w[k] = pack<T>(h);
         }
     };
@@ -437,6 +474,9 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const
         hide(m, o);
         o_side.store(o, seat, i, p.length - begin, p.past);
     }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = carried[turn][slot + v];
     for (int i = used; i < seat.tiles; ++i) {  // behind the sequence
         const int begin = seat.first + i * kTile;
         if (p.states && seat.own == 0)
@@ -455,14 +495,14 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
     const int lane = seat.lane, wave = seat.wave, slot = seat.slot;
     __shared__ float2 parts[2][kWaves][LANES * V];
     __shared__ float back_parts[2][kWaves][LANES * V];
-    fill_absent(parts);
-    for (int i = blockDim.x + threadIdx.x; i < Team<LANES>::kThreads; i += blockDim.x)
-        if (i % 64 < LANES)
-#pragma unroll
-            for (int v = 0; v < V; ++v) back_parts[0][i / 64][i % 64 * V + v] = back_parts[1][i / 64][i % 64 * V + v] = 0;
-    float carry[V];  // the gradient of the state behind a tile
+    __shared__ float carried[2][LANES * V];  // the gradient of the state behind a tile, as forwards
+    const int waves = blockDim.x / 64, pick = lane / LANES % V;
+    float carry[V];
     load_state<V>(p.final_grad, seat.batch * p.final_grad_b, seat.c, p.channels, carry);
     over_ranges<T, LANES, FACTORS>(p, seat, p.ranges - 1, seat.range, -1, carry);
+    if (seat.own == 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) carried[0][slot + v] = carry[v];
     int turn = 0;
     // From a tile's inputs to the gradients of x and gates, in their places.  `more` is called as soon as the inputs are in
     // other registers.  What one instruction makes of them again (b = rest x, with wide rows, whose threads have 128 registers, also the
@@ -504,8 +544,8 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
             put_in(k, b);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                A[v] = together<FACTORS>(A[v], a[k][v]);
-                B[v] = onward<FACTORS>(a[k][v], B[v], b[v]);
+                A[v] = grown<FACTORS>(A[v], a[k][v]);
+                B[v] = step<FACTORS>(a[k][v], B[v], b[v]);
             }
         }
 #pragma unroll
@@ -513,7 +553,7 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
             float f[V];
             unpack<T>(out_grad.w[k], f);
 #pragma unroll
-            for (int v = 0; v < V; ++v) back[v] = onward<FACTORS>(a[k][v], back[v] + f[v], 0.f);
+            for (int v = 0; v < V; ++v) back[v] = step<FACTORS>(a[k][v], back[v] + f[v], 0.f);
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -526,21 +566,13 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
             }
         }
         __syncthreads();
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = state[v];
-        for (int w = 0; w < wave; ++w)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float2 part = parts[turn][w][slot + v];
-                h[v] = onward<FACTORS>(part.x, h[v], part.y);
-            }
-#pragma unroll 4
-        for (int w = kWaves - 1; w >= 0; --w)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                if (w == wave) l[v] = carry[v];
-                carry[v] = onward<FACTORS>(parts[turn][w][slot + v].x, carry[v], back_parts[turn][w][slot + v]);
-            }
+        const int mine = slot + pick;
+        const float before = over_waves<FACTORS>(0, wave, 1, pick ? state[V - 1] : state[0], [&](int w) { return parts[turn][w][mine]; });
+        const float behind = over_waves<FACTORS>(waves - 1, wave, -1, carried[turn][mine],
+                                                 [&](int w) { return make_float2(parts[turn][w][mine].x, back_parts[turn][w][mine]); });
+        if (wave == 0 && lane < LANES * V) carried[turn ^ 1][mine] = onward<FACTORS>(parts[turn][0][mine].x, behind, back_parts[turn][0][mine]);
+        share<LANES>(pick, before, h);
+        share<LANES>(pick, behind, l);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             h[v] = onward<FACTORS>(preA[v], h[v], preB[v]);
@@ -560,7 +592,7 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
             for (int v = 0; v < V; ++v) {
                 const float before = DOCS && (m.cut >> k & 1) ? 0.f : h[v];
                 worth[k][v] = FACTORS ? before : before - f[v];
-                h[v] = onward<FACTORS>(a[k][v], h[v], FACTORS ? f[v] : rest[k][v] * f[v]);
+                h[v] = step<FACTORS>(a[k][v], h[v], FACTORS ? f[v] : rest[k][v] * f[v]);
             }
         }
         // backwards
@@ -579,7 +611,7 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float here = l[v] + ds[v];
-                l[v] = onward<FACTORS>(a[k][v], here, 0.f);
+                l[v] = step<FACTORS>(a[k][v], here, 0.f);
                 dx[v] = FACTORS ? here : here * rest[k][v];
                 dg[v] = FACTORS ? here * worth[k][v] : dx[v] * worth[k][v] * own[v];
             }
@@ -626,7 +658,11 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
         dg_side.store(one.g, seat, i, p.length - begin, p.past);
         one = next;
     }
-    if (p.initial_grad && seat.own == 0 && seat.range == 0) store_state<V>(p.initial_grad, seat.batch * p.initial_grad_b, seat.c, p.channels, carry);
+    if (!p.initial_grad || seat.range != 0) return;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = carried[turn][slot + v];
+    if (seat.own == 0) store_state<V>(p.initial_grad, seat.batch * p.initial_grad_b, seat.c, p.channels, carry);
 }
 
 // What each range of positions does to the state before it (to the gradient behind it where BACK): the map of all its positions.  A
@@ -666,8 +702,8 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_range_kernel
             const int k = BACK ? kSteps - 1 - i : i;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                B[v] = BACK ? onward<FACTORS>(a[k][v], B[v] + b[k][v], 0.f) : onward<FACTORS>(a[k][v], B[v], b[k][v]);
-                A[v] = together<FACTORS>(A[v], a[k][v]);
+                B[v] = BACK ? step<FACTORS>(a[k][v], B[v] + b[k][v], 0.f) : step<FACTORS>(a[k][v], B[v], b[k][v]);
+                A[v] = grown<FACTORS>(A[v], a[k][v]);
             }
         }
     };
@@ -768,7 +804,7 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(const RecurrencePa
             float o[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                h[v] = onward<FACTORS>(a[k][v], h[v], b[k][v]);
+                h[v] = step<FACTORS>(a[k][v], h[v], b[k][v]);
                 o[v] = m.live >> k & 1 ? h[v] : 0.f;
             }
             char* to = address(p.out, p.out_at, k);

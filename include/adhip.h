@@ -296,7 +296,7 @@ int adhip_layer_norm_backward(adhip_ctx* ctx, const adhip_layer_norm_args* args,
  * to 0 .. length): positions behind a sequence's length leave the state as it is.  documents (int32 [batch, length]): the state
  * begins at 0 at every position whose document is not that of the position before (the first position goes on from initial), and is 0 behind a
  * position of a document below 0.  Positions behind lengths or of documents below 0 give out = 0 and gradients 0, whatever x,
- * gates and out_grad hold there; everything else must be finite (gates may be infinite).  A factor of 0 drops the state before it, whatever
+ * gates and out_grad hold there; everything else must be finite (gates that are no factors may be infinite).  A factor of 0 drops the state before it, whatever
  * that is.  Factors are multiplied over runs of positions: where such a product passes 2^128, results may be infinite or NaN up to the next factor of 0
  * or document.
  * states (f32 [batch, ceil(length / 256), channels]; may be left out) receives the state before every 256th position, for the
