@@ -213,22 +213,23 @@ def test_recurrence_refusals(dev):
 
 
 def test_recurrence_backward_refusals(dev):
-    x, state, states = Array(3, 300, 40), Array(3, 40), Array(3, 2, 40)
+    x, y, state, states = Array(3, 300, 40), Array(3, 300, 40, at=1 << 20), Array(3, 40), Array(3, 2, 40)
     good = dict(final_grad=state, initial_grad=state, workspace=ROOM)
-    ops.recurrence_backward(dev, x, x, states, x, x, x, **good)
+    ops.recurrence_backward(dev, x, x, states, x, x, y, **good)
     assert dev.launches()
     no = lambda what, *args, **how: refused(dev, what, ops.recurrence_backward, *args, **{**good, **how})  # noqa: E731
+    no("one array", x, x, states, x, y, y)
     no("states has 0 dims", x, x, None, x, x, x)
     no("states is", x, x, Array(3, 1, 40), x, x, x)
     no("out_grad is", x, x, states, Array(3, 300, 39), x, x)
     no("x_grad share memory", x, x, states, x, Array(3, 300, 40, stride=(0, 40, 1)), x)
     no("gates_grad is bf16", x, x, states, x, x, Array(3, 300, 40, dtype="bfloat16"))
-    no("final_grad is", x, x, states, x, x, x, final_grad=Array(3, 39))
-    no("initial_grad share memory", x, x, states, x, x, x, initial_grad=Array(3, 40, stride=(0, 1)))
+    no("final_grad is", x, x, states, x, x, y, final_grad=Array(3, 39))
+    no("initial_grad share memory", x, x, states, x, x, y, initial_grad=Array(3, 40, stride=(0, 1)))
     far = Array(3, 300, 40, stride=(1 << 40, (1 << 21) + 1, 1))
-    no("2\\^21", x, x, states, far, x, x)
-    no("2\\^21", x, x, states, x, far, x)
-    no("2\\^21", x, x, states, x, x, far)
+    no("2\\^21", x, x, states, far, x, y)
+    no("2\\^21", x, x, states, x, far, y)
+    no("2\\^21", x, x, states, x, y, far)
 
 
 def test_recurrence_workspaces_and_launches(dev):
@@ -243,7 +244,7 @@ def test_recurrence_workspaces_and_launches(dev):
             room = Array(need, dtype="float8_e4m3fn") if need else None
             for how in (dict(), dict(documents=Array(B, L, dtype="int32")), dict(factors=True)):
                 ops.recurrence(dev, x, x, x, states=states, final=state, workspace=room, **how)
-                ops.recurrence_backward(dev, x, x, states, x, x, x, workspace=room, **how)
+                ops.recurrence_backward(dev, x, x, states, x, x, Array(B, L, C, dtype=dtype, at=1 << 50), workspace=room, **how)
                 for gx, gy, gz, threads in dev.launches():
                     assert 1 <= gx * threads < 1 << 32 and (gy, gz) == (1, 1)
     x = Array(1, 5000, 20)
