@@ -52,6 +52,7 @@ struct RecurrenceParams {
     int length, channels, groups;  // groups: of channels that a workgroup takes
     int batch, ranges, tiles;      // of positions, and tiles of a range
     bool past;                     // results go past the caches
+    bool near;                     // neighbouring workgroups share cache lines
 };
 
 // Operand of a wait for all memory operations of a wavefront, and of nothing else.
@@ -184,10 +185,14 @@ struct Seat {
     __device__ __forceinline__ Seat(const RecurrenceParams& p) {
         lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), slot = (lane & (LANES - 1)) * V;
         // Workgroups go to the eight dies in turn: of 256, which run at a time, neighbours of a row, whose channels share cache lines,
-        // go to one die, and together they cover whole rows (8 x 2048 positions of 4096 channels in bf16: 315 us with neighbours of all
-        // workgroups on one die, 276 so).
-        const unsigned window = blockIdx.x / kFull * kFull, of = blockIdx.x % kFull, die = min(gridDim.x - window, (unsigned)kFull) / 8;
-        unsigned at = window + of % 8 * die + of / 8;
+        // go to one die, and together they cover whole rows (2 x 8192 positions of 4096 channels in bf16, both passes: 285 us, and 319 without; 8191
+        // of 1000 in f32 104 and 125).  Where rows of workgroups are whole lines there is nothing to share (4 x 2048 of 4096 in f32: 224 us so, 214
+        // without).
+        unsigned at = blockIdx.x;
+        if (p.near) {
+            const unsigned window = at / kFull * kFull, of = at % kFull, die = min(gridDim.x - window, (unsigned)kFull) / 8;
+            at = window + of % 8 * die + of / 8;
+        }
         const unsigned group = at % (unsigned)p.groups;
         at /= (unsigned)p.groups;
         batch = at % (unsigned)p.batch;
@@ -832,8 +837,8 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(const RecurrencePa
     if (p.final) store_state<V>(p.final, batch * p.final_b, c, p.channels, h);
 }
 
-// Wide rows bring whole cache lines: 5 to 10 % forward and backward in f32.  The backward pass of bf16, and that of documents, does not fit the 128
-// registers that their 1024 threads have: 16 x 1000 positions of 4000 channels in bf16 with documents 390 us wide and 216 narrow.
+// Wide rows bring whole cache lines: a tenth and more, forward and backward in f32.  The backward pass of bf16, and that of documents, does not fit
+// the 128 registers that their 1024 threads have: 16 x 1000 positions of 4000 channels in bf16 with documents 275 us wide and 184 narrow.
 constexpr bool wide_pays(int type, bool backward, bool documents) { return !backward || (type == ADHIP_F32 && !documents); }
 
 template <class T, int LANES, bool FACTORS, bool DOCS>
@@ -860,10 +865,10 @@ void launch_recurrence(const char* op, const RecurrenceParams& p, bool backward,
 }
 
 // How channels are cut into rows and positions into ranges.  Compute units left without a workgroup are given ranges of positions, at
-// the price of a kernel that reads them before (8191 positions of 1000 channels in f32, forward and backward: 248 us in one range, 120 in four), of
-// two tiles or more each.  Rows are wide where narrow ones would give some compute units two workgroups (4 x 2049 of 2560 in bf16: 47 us
-// narrow, 39 wide; 2 x 8192 of 4096, where they give each one: 290 narrow, 386 wide), and where there are ranges of four
-// tiles and more to make up for them (the first example in eight: 109 us; 4096 positions of 1024 channels in bf16, two tiles each: 36 narrow, 38 wide).
+// the price of a kernel that reads them before (8191 positions of 1000 channels in f32, forward and backward: 185 us in one range, 107 in four), of
+// two tiles or more each.  Rows are wide where narrow ones would give some compute units two workgroups (4 x 2049 of 2560 in bf16: 56 us
+// narrow, 44 wide; 2 x 8192 of 4096, where they give each one: 285 narrow, 328 wide), and where there are ranges of four
+// tiles and more to make up for them (the first example in eight: 103 us; 4096 positions of 1024 channels in bf16, two tiles each, forward: 16 narrow, 20 wide).
 struct Cut {
     int lanes, groups, tiles, ranges;  // tiles: of a range
     Cut(const adhip_array& x, bool wide) {
@@ -960,6 +965,11 @@ void recurrence(const char* op, const adhip_recurrence_args& g, bool backward, h
     p.tiles = cut.tiles;
     const int64_t blocks = batch * p.groups;
     const bool factors = g.factors != 0, wide = cut.lanes == kWide;
+    const auto whole_lines = [&](const adhip_array& a) {
+        const int64_t w = type_bytes(a.type);
+        return (uintptr_t)a.data % 128 == 0 && a.strides[0] * w % 128 == 0 && a.strides[1] * w % 128 == 0;
+    };
+    p.near = !wide || !whole_lines(g.x) || !whole_lines(g.gates);
     // (4 x 2048 positions of 4096 channels in f32, both passes: 223 us past the caches, 239 through them.  Half lines, as narrow rows write them,
     // cost a quarter more traffic past the caches, at the same time.)
     p.past = wide && (backward ? 5 : 3) * batch * length * channels * type_bytes(g.x.type) > kLastCache;
