@@ -6,8 +6,8 @@
 // registers, so a mean that is large against the deviations costs no bits.  In the backward pass a lane keeps the same columns of all
 // rows that it meets, so the weights' gradients add up in its registers; a workgroup adds its lanes' sums in LDS, and a small second
 // kernel the workgroups', always in the same order.
-// 16384 rows of 4096 in bf16 with a residual: forward 99 us (5.4 TB/s), backward 108 (5.0) and 5 for the last sums; 131072 rows of 128: 13.4, 20.2
-// and 3.8; 3001 rows of 1023 in f32 with a residual: 12.2, 16.2 and 3.9.
+// 16384 rows of 4096 in bf16 with a residual: forward 92 us (5.9 TB/s), backward 107 (5.0) and 5 for the last sums; 131072 rows of 128: 12.5, 18.1
+// and 3.9; 3001 rows of 1023 in f32 with a residual: 10.8, 14.6 and 3.8.  Results past the caches gain nothing here.
 #include "operators.hpp"
 
 #include <algorithm>
@@ -20,7 +20,7 @@ namespace {
 constexpr int kElements = 16;          // of a row that a lane holds at most
 constexpr int kThreads = 256;          // of a workgroup that rows of one wavefront and less share
 constexpr int kWaves = 16;             // of a row at most, and of a workgroup of the backward pass
-constexpr int kGradBlocks = 256;       // a compute unit each: twice as many of half the size leave twice the partial sums (245 us became 297)
+constexpr int kGradBlocks = 256;       // a compute unit each: twice as many leave twice the partial sums (202 us become 208)
 constexpr int64_t kMostSize = kWaves * 64 * kElements;
 
 struct Place {
@@ -36,7 +36,6 @@ struct NormParams {
     int size, padded;       // padded: of a row of partial sums
     int waves, groups;      // wavefronts that share a row, and rows that a workgroup has at once
     float eps, centered;    // centered: 1 or 0
-    bool past;              // results go past the caches
 };
 
 struct RowIndex {
@@ -76,7 +75,7 @@ __device__ __forceinline__ void load_row(const void* row, int64_t at, const Spot
 }
 
 template <class T, int V, bool FULL>
-__device__ __forceinline__ void store_row(void* row, int64_t at, const Spot<V, FULL>& spot, bool past, const float (&f)[V]) {
+__device__ __forceinline__ void store_row(void* row, int64_t at, const Spot<V, FULL>& spot, const float (&f)[V]) {
     T* x = (T*)row + at + spot.e;
     if (FULL || spot.skip == 0) {
         Loose<T, V> r;
@@ -84,12 +83,11 @@ __device__ __forceinline__ void store_row(void* row, int64_t at, const Spot<V, F
         for (int k = 0; k < V; ++k) r.v[k] = (T)f[k];
         if constexpr (V == 1) {
             *(Loose<T, V>*)x = r;
-        } else {
+        } else {  // (as one store of 16 bytes)
             Word16 w;
             static_assert(sizeof r == sizeof w, "a lane's pack");
             __builtin_memcpy(&w, &r, sizeof w);
-            if (past) store_past((Word16*)x, w);
-            else *(Word16*)x = w;
+            *(Word16*)x = w;
         }
     } else {
 #pragma unroll
@@ -203,7 +201,7 @@ __global__ __launch_bounds__(LANES == 64 ? kWaves * 64 : kThreads) void norm_ker
                 // rounded to the arrays' type as it is kept: what is normed here is what the backward pass reads
 #pragma unroll
                 for (int k = 0; k < V; ++k) x[c][k] = (float)(T)(x[c][k] + added[c][k]);
-                if (there) store_row<T>(p.total, index.at(p.total_at), spot(c), p.past, x[c]);
+                if (there) store_row<T>(p.total, index.at(p.total_at), spot(c), x[c]);
             }
         }
         float sum = 0, none = 0;
@@ -239,7 +237,7 @@ __global__ __launch_bounds__(LANES == 64 ? kWaves * 64 : kThreads) void norm_ker
             if (p.bias)
 #pragma unroll
                 for (int k = 0; k < V; ++k) x[c][k] += (float)bias[c].v[k];
-            store_row<T>(p.out, index.at(p.out_at), spot(c), p.past, x[c]);
+            store_row<T>(p.out, index.at(p.out_at), spot(c), x[c]);
         }
     }
 }
@@ -271,7 +269,7 @@ __global__ __launch_bounds__(kWaves * 64) void norm_backward_kernel(const NormPa
         r.stats = *(const float2*)(p.stats + 2 * (int64_t)row);
     };
     const unsigned step = gridDim.x * p.groups;
-    constexpr bool AHEAD = FULL || C * V <= 8;  // (of others the registers do not hold two rows)
+    constexpr bool AHEAD = FULL || C * V <= 8;  // (of others the registers do not hold two rows; 12001 of 1030 in f32: 62 us, and 73 without)
     if (AHEAD) ask(raw, min(blockIdx.x * p.groups + team.group, p.rows - 1));
     // (all lanes of a workgroup go round equally often: they meet at barriers)
     for (unsigned first = blockIdx.x * p.groups; first < p.rows; first += step) {
@@ -327,7 +325,7 @@ __global__ __launch_bounds__(kWaves * 64) void norm_backward_kernel(const NormPa
                 if (ADDS)
 #pragma unroll
                     for (int k = 0; k < V; ++k) u[c][k] += more[c][k];
-                store_row<T>(p.x_grad, index.at(p.x_grad_at), spot(c), p.past, u[c]);
+                store_row<T>(p.x_grad, index.at(p.x_grad_at), spot(c), u[c]);
             }
         }
     }
@@ -411,8 +409,8 @@ struct Share {
         packs = size <= lanes * v ? 1 : size <= kWaves * 64 * 2 * v ? 2 : 4;
         full = false;
         // Two packs a lane, or one, that rows fill exactly.  Of bf16 rather one: two, and a residual's gradient, pass the registers (16384 rows
-        // of 4096, both passes: 211 us with one, 254 with two).  Of f32 rather two, which halve the wavefronts that have to meet (8192
-        // rows: 211 with two, 232 with one).
+        // of 4096, both passes: 202 us with one, 242 with two).  Of f32 rather two, which halve the wavefronts that have to meet (8192
+        // rows: 206 with two, 226 with one).
         for (int i : {0, 1}) {
             const int c = type == ADHIP_BF16 ? 2 - i : 1 + i;
             const int64_t unit = (int64_t)lanes * v * c;
@@ -551,8 +549,6 @@ void layer_norm(const char* op, const adhip_layer_norm_args& g, bool backward, h
     p.padded = padded_of(size);
     p.eps = (float)g.eps;
     p.centered = g.centered ? 1.f : 0.f;
-    // (16384 rows of 4096 in bf16 with a residual, both passes: 198 us past the caches, 211 through them)
-    p.past = n * rows * size * type_bytes(g.x.type) > kLastCache;
     p.x = g.x.data;
     p.weight = g.weight.data;
     p.stats = (float*)g.stats.data;

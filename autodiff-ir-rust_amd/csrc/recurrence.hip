@@ -11,9 +11,10 @@
 // states again: the forward pass leaves one every 256 positions, from which a tile of them is recomputed beside the gradients,
 // instead of reading all outputs, which are rounded.
 //
-// 2 x 8192 positions of 4096 channels in bf16: forward 108 us, backward 181 (3.7 TB/s; two arrays copied into a third in this pattern, 64 bytes of
-// rows 8 KB apart, take 107), of 4032 channels 96 and 174; 4 x 2048 of 4096 in f32, 128 bytes of a row: 85 and 137 (4.8, 4.9 TB/s).  Vector units are
-// busy 0.4 of the time: 22 instructions an element forward and 40 backward.  One position of 256 x 8192 channels: 13 us.
+// 2 x 8192 positions of 4096 channels in bf16: forward 108 us, backward 178 (3.8 TB/s; two arrays copied into a third in this pattern, 64 bytes of
+// rows 8 KB apart, take 107), of 4032 channels 90 and 151; 4 x 2048 of 4096 in f32, 128 bytes of a row: 80 and 134 (5.0 TB/s).  One position of
+// 256 x 8192 channels: 12 us.  A compute unit with one workgroup of wide rows is bound by its instructions: a tile of 256 positions of 64 channels
+// takes it 2.5 us.
 #include "operators.hpp"
 
 #include <algorithm>
@@ -970,7 +971,7 @@ void recurrence(const char* op, const adhip_recurrence_args& g, bool backward, h
         return (uintptr_t)a.data % 128 == 0 && a.strides[0] * w % 128 == 0 && a.strides[1] * w % 128 == 0;
     };
     p.near = !wide || !whole_lines(g.x) || !whole_lines(g.gates);
-    // (4 x 2048 positions of 4096 channels in f32, both passes: 223 us past the caches, 239 through them.  Half lines, as narrow rows write them,
+    // (4 x 2048 positions of 4096 channels in f32, both passes: 215 us past the caches, 232 through them.  Half lines, as narrow rows write them,
     // cost a quarter more traffic past the caches, at the same time.)
     p.past = wide && (backward ? 5 : 3) * batch * length * channels * type_bytes(g.x.type) > kLastCache;
     if (!backward && length >= 1 && length <= kSteps) {
