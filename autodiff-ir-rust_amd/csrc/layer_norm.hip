@@ -245,8 +245,8 @@ __global__ __launch_bounds__(LANES == 64 ? kWaves * 64 : kThreads) void norm_ker
 // With n the normed row and u = out_grad weight:
 //     x_grad = root (u - mean(u) - n mean(u n)) + total_grad      (without the mean of u where the norm takes no mean)
 //     weight_grad = sum over rows of out_grad n,  bias_grad = sum over rows of out_grad
-// Where rows fill their lanes (FULL) the next one is asked for as soon as this one is in other registers; loads without a branch are
-// loads that the compiler can count, so it waits for those of this row alone.  Others take twice the registers already.
+// The next row is asked for as soon as this one is in other registers (AHEAD); loads without a branch are loads that the compiler can
+// count, so it waits for those of this row alone.
 template <class T, class W, int V, int LANES, int C, bool FULL, bool SUMS, bool ADDS>
 __global__ __launch_bounds__(kWaves * 64) void norm_backward_kernel(const NormParams p) {
     Team<LANES> team(p);

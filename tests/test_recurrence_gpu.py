@@ -97,6 +97,22 @@ def test_many_sequences_of_several_tiles(hip_device, masked, dtype):
     check(hip_device, inputs(6, 700, 1473, dtype, seed=3, **masks), f"many, {dtype}")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,L,lines", [(1, 9001, 29), (9, 530, 32)])
+def test_rows_of_whole_cache_lines(hip_device, B, L, lines, dtype):
+    """Workgroups that share no cache lines are numbered otherwise: the same bits as in rows that begin off a line."""
+    C = lines * (32 if dtype == "f32" else 64)
+    a = inputs(B, L, C, dtype, seed=3, slow=5.0)
+    check(hip_device, a, f"{B} x {L} x {C}, {dtype}")
+    plain = run(hip_device, a)
+    for n in ("x", "gates", "out_grad"):
+        wide = torch.zeros((B, L, C + 3), dtype=a[n].dtype)
+        wide[..., 1:-2] = a[n]
+        a[n] = wide[..., 1:-2]
+    got = run(hip_device, a, like=torch.empty_like)
+    assert all(torch.equal(got[n], plain[n]) for n in plain)
+
+
 MASKS = {
     "lengths": dict(lengths=[700, 0, 256]),
     "lengths out of range": dict(lengths=[9999, -3, 1]),
