@@ -139,6 +139,17 @@ def test_long_masks(hip_device, factors, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("off", [-1, 0, 1])
+@pytest.mark.parametrize("every", [64, 1024])
+def test_documents_that_begin_where_ranges_do(hip_device, every, off, dtype):
+    """The last and the first one of a range decide what it does to a state."""
+    a = inputs(2, 4500, 18, dtype, seed=6, slow=6.0, lengths=[4500, 2305])
+    a["documents"] = ((torch.arange(4500) - off) // every).to(torch.int32).expand(2, 4500).contiguous()
+    a["documents"][:, 2304:2306] = -1
+    check(hip_device, a, f"every {every} and {off}, {dtype}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("factors", [False, True])
 @pytest.mark.parametrize("L", [600, 5, 4100])
 def test_hidden_positions_may_hold_anything(hip_device, L, factors, dtype):
