@@ -538,7 +538,7 @@ def recurrence(dev, x, gates, out, *, factors: bool = False, initial=None, final
 def recurrence_backward(dev, x, gates, states, out_grad, x_grad, gates_grad, *, factors: bool = False, final_grad=None, initial_grad=None,
                         lengths=None, documents=None, workspace=None, stream: Optional[int] = None) -> None:
     """Gradients of x, gates and, where it is given, initial from `recurrence`'s states and the gradients of out and, where it is
-    given, final; the other arguments as there."""
+    given, final (initial_grad and final_grad may be one array); the other arguments as there."""
     args = b"".join((_array(x), _array(gates), _NONE * 3, _array(states), _array(lengths), _array(documents), _array(out_grad),
                      _array(final_grad), _array(x_grad), _array(gates_grad), _array(initial_grad),
                      _RECURRENCE_TAIL.pack(bool(factors), *_room(workspace))))

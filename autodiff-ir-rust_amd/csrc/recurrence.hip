@@ -47,7 +47,7 @@ struct RecurrenceParams {
     const float *initial, *final_grad;
     float *states, *final, *initial_grad;
     const int *lengths, *documents;
-    float2* carry;  // [ranges, batch, channels]: what a range does to a state; forward, the last one's place holds the state before all
+    float2* carry;  // [ranges, batch, channels]: what a range does to a state (to a gradient); one place holds what all begin with
     Rows x_at, gates_at, out_at, out_grad_at, x_grad_at, gates_grad_at, states_at, documents_at;
     int64_t initial_b, final_b, final_grad_b, initial_grad_b, lengths_b;
     int length, channels, groups;  // groups: of channels that a workgroup takes
@@ -375,6 +375,28 @@ __device__ __forceinline__ void over_ranges(const RecurrenceParams& p, const Sea
     }
 }
 
+// The range whose map nobody asks for: the last one's, and backwards the first one's.  Its place holds the state (the gradient) that all begin
+// with, put aside before any range writes: final may be initial and initial_grad final_grad, and the range that writes them may be done
+// before another one begins.
+template <bool BACK>
+__device__ __forceinline__ int64_t aside(const RecurrenceParams& p) {
+    return BACK ? 0 : (int64_t)(p.ranges - 1) * p.batch * p.channels;
+}
+
+// The state before a range's first position, and backwards the gradient behind its last one.
+template <class T, int LANES, bool FACTORS, bool BACK>
+__device__ __forceinline__ void first_state(const RecurrenceParams& p, const Seat<T, LANES>& seat, const float* given, int64_t given_b,
+                                            float (&h)[kPack<T>]) {
+    constexpr int V = kPack<T>;
+    if (p.ranges == 1) return load_state<V>(given, seat.batch * given_b, seat.c, p.channels, h);
+    float2 kept[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) kept[v] = p.carry[aside<BACK>(p) + seat.state + (seat.lone ? 0 : v)];
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = kept[v].y;
+    over_ranges<T, LANES, FACTORS>(p, seat, BACK ? p.ranges - 1 : 0, seat.range, BACK ? -1 : 1, h);
+}
+
 // A state carried over the maps of whole wavefronts, from `w` on up to, but not, `end`, four loads at once.  `map` reads one.  A wavefront
 // goes over those before it alone, and of a pack's two channels a thread over one: with all of both, where 16 wavefronts share wide rows,
 // a third of all instructions (4 x up to 2049 positions of 2560 channels: 41 us, with all 44; 256 x 16 of 1024, both passes: 40 and 48).
@@ -411,17 +433,7 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_kernel(const
     __shared__ float carried[2][LANES * V];         // the state before a tile: who needs it reads it, and the last wavefront leaves the next one
     const int waves = blockDim.x / 64, pick = lane / LANES % V;
     float carry[V];
-    if (p.ranges == 1) {
-        load_state<V>(p.initial, seat.batch * p.initial_b, seat.c, p.channels, carry);
-    } else {
-        // (final may be initial, and the last range may be done before the first one begins: the state was put aside)
-        float2 kept[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) kept[v] = p.carry[(int64_t)(p.ranges - 1) * p.batch * p.channels + seat.state + (seat.lone ? 0 : v)];
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = kept[v].y;
-        over_ranges<T, LANES, FACTORS>(p, seat, 0, seat.range, 1, carry);
-    }
+    first_state<T, LANES, FACTORS, false>(p, seat, p.initial, p.initial_b, carry);
     if (seat.own == 0)
 #pragma unroll
         for (int v = 0; v < V; ++v) carried[0][slot + v] = carry[v];
@@ -512,8 +524,7 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_backward_ker
     __shared__ float carried[2][LANES * V];  // the gradient of the state behind a tile, as forwards
     const int waves = blockDim.x / 64, pick = lane / LANES % V;
     float carry[V];
-    load_state<V>(p.final_grad, seat.batch * p.final_grad_b, seat.c, p.channels, carry);
-    over_ranges<T, LANES, FACTORS>(p, seat, p.ranges - 1, seat.range, -1, carry);
+    first_state<T, LANES, FACTORS, true>(p, seat, p.final_grad, p.final_grad_b, carry);
     if (seat.own == 0)
 #pragma unroll
         for (int v = 0; v < V; ++v) carried[0][slot + v] = carry[v];
@@ -780,12 +791,12 @@ __global__ __launch_bounds__(Team<LANES>::kThreads) void recurrence_range_kernel
     }
     __syncthreads();
     if (seat.own != 0) return;
-    if (!BACK && range == 0) {
-        float initial[V];
-        load_state<V>(p.initial, seat.batch * p.initial_b, seat.c, p.channels, initial);
+    if (seat.range == 0) {
+        float given[V];
+        load_state<V>(BACK ? p.final_grad : p.initial, seat.batch * (BACK ? p.final_grad_b : p.initial_b), seat.c, p.channels, given);
 #pragma unroll
         for (int v = 0; v < V; ++v)
-            if (seat.c + v < p.channels) p.carry[(int64_t)(p.ranges - 1) * p.batch * p.channels + seat.state + v] = make_float2(0, initial[v]);
+            if (seat.c + v < p.channels) p.carry[aside<BACK>(p) + seat.state + v] = make_float2(0, given[v]);
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {

@@ -317,7 +317,8 @@ int adhip_recurrence_workspace(adhip_ctx* ctx, const adhip_recurrence_args* args
 int adhip_recurrence(adhip_ctx* ctx, const adhip_recurrence_args* args, void* stream);
 /* Gradients of x, gates and, where asked for, initial, from x, gates, the forward call's states, the gradient of out and, where it
  * is given, that of final ([batch, channels]); lengths, documents and factors as there.  x_grad and gates_grad may be x, gates or out_grad
- * themselves, under the same strides.  out, initial and final are not looked at.  The order of additions is fixed. */
+ * themselves, under the same strides, and initial_grad may be final_grad itself (a gradient that is carried from call to call).
+ * out, initial and final are not looked at.  The order of additions is fixed. */
 int adhip_recurrence_backward(adhip_ctx* ctx, const adhip_recurrence_args* args, void* stream);
 
 #ifdef __cplusplus
