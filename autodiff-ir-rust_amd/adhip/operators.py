@@ -502,7 +502,8 @@ def layer_norm(dev, x, out, *, weight=None, bias=None, eps: float = 1e-5, center
 def layer_norm_backward(dev, x, stats, out_grad, x_grad, *, weight=None, weight_grad=None, bias_grad=None, centered: bool = True,
                         total_grad=None, workspace=None, stream: Optional[int] = None) -> None:
     """Gradients from what `layer_norm` normed (x, or total where something was added) and its stats.  total_grad, the gradient that
-    reaches the sum by another way, is added to x_grad; weight_grad and bias_grad, where they are given, take a workspace."""
+    reaches the sum by another way, is added to x_grad; weight_grad and bias_grad, where they are given, are two arrays (one for both
+    holds bias_grad alone) and take a workspace."""
     args = b"".join((_array(x), _NONE * 3, _array(weight), _NONE, _array(stats), _array(out_grad), _array(total_grad), _array(x_grad),
                      _array(weight_grad), _array(bias_grad), _NORM_TAIL.pack(1.0, bool(centered), *_room(workspace))))
     _check(dev, _lib(dev).adhip_layer_norm_backward(dev._ctx, args, _stream(dev, stream)), "adhip_layer_norm_backward")

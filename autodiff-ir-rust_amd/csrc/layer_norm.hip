@@ -538,9 +538,16 @@ void layer_norm(const char* op, const adhip_layer_norm_args& g, bool backward, h
         ADHIP_CHECK((uintptr_t)g.stats.data % 8 == 0, "%s: stats is not aligned to 8 bytes", op);
     }
     const bool sums = backward && (g.weight_grad.data || g.bias_grad.data);
+    bool one_sum = false;  // one array for both holds bias_grad: nobody writes weight_grad there before or after it
     if (backward) {
         if (g.weight_grad.data) check_vector(op, "weight_grad", g.weight_grad, size, true);
         if (g.bias_grad.data) check_vector(op, "bias_grad", g.bias_grad, size, true);
+        if (g.weight_grad.data && g.bias_grad.data) {
+            const char *w = (const char*)g.weight_grad.data, *b = (const char*)g.bias_grad.data;
+            one_sum = w == b && g.weight_grad.type == g.bias_grad.type;
+            ADHIP_CHECK(one_sum || w + size * type_bytes(g.weight_grad.type) <= b || b + size * type_bytes(g.bias_grad.type) <= w,
+                        "%s: weight_grad and bias_grad share memory", op);
+        }
         ADHIP_CHECK(!sums || rows == 0 || (g.workspace && (uintptr_t)g.workspace % 16 == 0 && g.workspace_bytes >= workspace_of(g.x.type, rows, size)),
                     "%s: the workspace has %zu bytes, %zu are wanted, aligned to 16", op, g.workspace ? g.workspace_bytes : (size_t)0, workspace_of(g.x.type, rows, size));
     }
@@ -602,7 +609,7 @@ void layer_norm(const char* op, const adhip_layer_norm_args& g, bool backward, h
     }
     if (sums)
         launch(op, norm_sums_kernel, dim3((unsigned)((size + 63) / 64), 2), 256, stream, (const float*)g.workspace, rows > 0 ? (int)grad_blocks(g.x.type, rows, size) : 0,
-               (int)size, p.padded, g.weight_grad.data, g.bias_grad.data, g.weight_grad.type == ADHIP_BF16, g.bias_grad.type == ADHIP_BF16);
+               (int)size, p.padded, one_sum ? nullptr : g.weight_grad.data, g.bias_grad.data, g.weight_grad.type == ADHIP_BF16, g.bias_grad.type == ADHIP_BF16);
 }
 
 }  // namespace

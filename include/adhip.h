@@ -284,8 +284,8 @@ int adhip_layer_norm(adhip_ctx* ctx, const adhip_layer_norm_args* args, void* st
  * total_grad (may be left out), a gradient that reaches t by another way, is added to it.  Where something was added x_grad is the gradient of both x and
  * added.  x_grad may be out_grad, total_grad or x itself, under the same strides.  weight_grad and bias_grad ([size], f32 or bf16, each may be left out)
  * are sums over all rows in 32 bits, added in an order that only the shape decides; with either a workspace of
- * adhip_layer_norm_workspace() bytes, aligned to 16, is used until the call's kernels are done.  added, total, out and bias are
- * not looked at. */
+ * adhip_layer_norm_workspace() bytes, aligned to 16, is used until the call's kernels are done.  The two share no memory; one array
+ * given for both holds bias_grad alone.  added, total, out and bias are not looked at. */
 int adhip_layer_norm_backward(adhip_ctx* ctx, const adhip_layer_norm_args* args, void* stream);
 
 /* A gated linear recurrence over positions, each channel by itself.  x, gates and out are [batch, length, channels] (f32 or

@@ -1,5 +1,5 @@
 // What a hand-written kernel's source needs of HIP to be compiled for the host and run there, workgroup by workgroup in the order of
-// their numbers: on its include path this file stands in for the real one.  The threads of a workgroup are contexts of one thread of the
+// their numbers, or in the opposite one: on its include path this file stands in for the real one.  The threads of a workgroup are contexts of one thread of the
 // host; those of a wavefront go from one exchange between lanes to the next together, and wavefronts from barrier to barrier.
 #pragma once
 #include <ucontext.h>
@@ -31,6 +31,10 @@ struct alignas(8) float2 {
     float x, y;
 };
 inline float2 make_float2(float x, float y) { return {x, y}; }
+struct alignas(16) float4 {
+    float x, y, z, w;
+};
+inline float4 make_float4(float x, float y, float z, float w) { return {x, y, z, w}; }
 
 inline dim3 threadIdx, blockIdx, blockDim, gridDim;
 
@@ -113,12 +117,16 @@ inline void run_workgroup(unsigned n) {
     }
 }
 
+extern bool last_first;  // the order of workgroups
+
 inline hipError_t run(const std::function<void()>& kernel, dim3 grid, dim3 block) {
     body = &kernel;
     gridDim = grid, blockDim = block;
-    for (blockIdx.y = 0; blockIdx.y < grid.y; ++blockIdx.y)
-        for (blockIdx.x = 0; blockIdx.x < grid.x; ++blockIdx.x) run_workgroup(block.x);
-    blockIdx.y = 0;
+    for (uint64_t i = 0, n = (uint64_t)grid.x * grid.y; i < n; ++i) {
+        const uint64_t at = last_first ? n - 1 - i : i;
+        blockIdx = dim3((unsigned)(at % grid.x), (unsigned)(at / grid.x), 0);
+        run_workgroup(block.x);
+    }
     return hipSuccess;
 }
 
@@ -126,6 +134,16 @@ struct Two {
     int v[2];
     int operator[](int i) const { return v[i]; }
 };
+// Where a lane's value comes from under those controls of the data-parallel primitives that kernels here use.
+inline int from_lane(int x, int control) {
+    const int* all = exchange(x);
+    const int lane = (int)(threadIdx.x & 63);
+    if (control < 0x100) return all[(lane & ~3) | (control >> 2 * (lane & 3) & 3)];  // any of four lanes
+    if (control == 0x140) return all[lane ^ 15];                                    // sixteen mirrored
+    if (control == 0x141) return all[lane ^ 7];                                     // eight mirrored
+    fprintf(stderr, "control 0x%x is not known here\n", control);
+    abort();
+}
 inline Two swap_lanes(int x, unsigned off) {
     const int* all = exchange(x);
     return {{all[(threadIdx.x & 63) & ~off], all[(threadIdx.x & 63) | off]}};
@@ -143,6 +161,10 @@ inline uint64_t __ballot(bool x) {
     for (int i = 0; i < 64; ++i) r |= (uint64_t)(all[i] != 0) << i;
     return r;
 }
+inline float __shfl_xor(float x, int off) {
+    const int* all = host_hip::exchange(__builtin_bit_cast(int, x));
+    return __builtin_bit_cast(float, all[(threadIdx.x & 63) ^ off]);
+}
 inline int atomicMin(int* a, int x) { const int was = *a; *a = x < was ? x : was; return was; }
 inline int atomicMax(int* a, int x) { const int was = *a; *a = x > was ? x : was; return was; }
 template <class T>
@@ -155,5 +177,6 @@ inline float __uint_as_float(unsigned x) { return __builtin_bit_cast(float, x); 
 #define __builtin_amdgcn_s_waitcnt(x) ((void)0)
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
 #define __builtin_amdgcn_rcpf(x) (1.f / (x))
+#define __builtin_amdgcn_update_dpp(old, x, control, rows, banks, bound) host_hip::from_lane(x, control)
 #define __builtin_amdgcn_permlane16_swap(a, b, ...) host_hip::swap_lanes(a, 16)
 #define __builtin_amdgcn_permlane32_swap(a, b, ...) host_hip::swap_lanes(a, 32)

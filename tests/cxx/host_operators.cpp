@@ -10,6 +10,11 @@ namespace {
 std::string last;
 }
 
+namespace host_hip {
+bool last_first = false;
+}
+extern "C" void host_last_workgroup_first(int yes) { host_hip::last_first = yes; }
+
 namespace adhip {
 int context_guarded(adhip_ctx* ctx, const std::function<void()>& f) {
     if (!ctx) return 2;

@@ -1,6 +1,6 @@
 """Runs hand-written operators on the host, kernels and all: their source compiles as ordinary C++ with a stand-in for HIP
 (cxx/host_hip) under which a workgroup's threads run as contexts of one thread, and workgroups one after the other in the order of their
-numbers.  What depends on the order in which workgroups run, and what an access touches, shows here without a GPU."""
+numbers or in the opposite one.  What depends on the order in which workgroups run, and what an access touches, shows here without a GPU."""
 import os
 import re
 import subprocess
@@ -36,6 +36,15 @@ class HostDevice:
 
     def last_error(self):
         return self._lib.adhip_last_error(self._ctx).decode()
+
+    def in_both_orders(self, f):
+        """What f gives with workgroups in the order of their numbers, and with the last one first."""
+        results = []
+        for last_first in (0, 1):
+            self._lib.host_last_workgroup_first(last_first)
+            results.append(f())
+        self._lib.host_last_workgroup_first(0)
+        return results
 
 
 class HostArray:
