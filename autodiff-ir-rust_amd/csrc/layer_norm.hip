@@ -519,6 +519,12 @@ void layer_norm(const char* op, const adhip_layer_norm_args& g, bool backward, h
         if (arrays[i].output) check_distinct(op, arrays[i].name, a);
     }
     ADHIP_CHECK(!adds || rows == 0 || g.total.data != g.out.data, "%s: total and out are one array", op);
+    for (int i = 0; i < n; ++i)
+        for (int j = i + 1; j < n; ++j) {
+            const Named &a = arrays[i], &b = arrays[j];  // (inputs come first)
+            if (b.output && !a.output) check_in_place(op, a.name, *a.a, b.name, *b.a);
+            else if (b.output) check_apart(op, a.name, *a.a, b.name, *b.a);
+        }
     // weights: of x's type or f32, both alike
     const int w_type = g.weight.data ? g.weight.type : g.bias.data && !backward ? g.bias.type : ADHIP_F32;
     if (g.weight.data) check_vector(op, "weight", g.weight, size, false);

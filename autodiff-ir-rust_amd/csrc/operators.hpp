@@ -104,6 +104,78 @@ inline void check_distinct(const char* op, const char* name, const adhip_array& 
     }
 }
 
+// Whether two arrays of packed rows share memory: whether a row of one and a row of the other are less than a row apart.  The distance of
+// rows is a sum over the dims' strides, each times an index (a difference of two, where both arrays have the stride); the search goes
+// from the largest stride on and leaves out what the smaller ones cannot make up for, so distinct elements leave it one or two ways at each.
+// Where thousands of ways (of arrays that interleave under unlike strides) do not tell, none is found.
+class SharedMemory {
+    using Wide = __int128;  // (two arrays may reach 2^62 bytes each)
+    struct Term {
+        Wide stride, least, most;
+    } terms[8];
+    int n = 0, ways = 1 << 16;
+    Wide below, above;  // rows meet at distances between the two
+
+    void add(int64_t stride, int64_t least, int64_t most) {
+        if (stride == 0) return;
+        int i = 0;
+        while (i < n && terms[i].stride > stride) ++i;
+        if (i < n && terms[i].stride == stride) {
+            terms[i].least += least, terms[i].most += most;
+            return;
+        }
+        for (int j = n++; j > i; --j) terms[j] = terms[j - 1];
+        terms[i] = {stride, least, most};
+    }
+    static Wide reach(const adhip_array& a) {
+        int64_t r = a.dims[a.rank - 1];
+        for (int d = 0; d + 1 < a.rank; ++d) r += (a.dims[d] - 1) * a.strides[d];
+        return r;
+    }
+    static Wide floor_div(Wide a, Wide b) { return a / b - (a % b < 0); }
+    bool meets(int i, Wide at) {
+        Wide least = 0, most = 0;
+        for (int j = i; j < n; ++j) least += terms[j].least * terms[j].stride, most += terms[j].most * terms[j].stride;
+        if (--ways < 0 || at + least >= above || at + most <= below) return false;
+        if (i == n) return true;
+        const Term t = terms[i];
+        least -= t.least * t.stride, most -= t.most * t.stride;
+        const Wide from = floor_div(below - at - most, t.stride) + 1, to = -floor_div(at + least - above, t.stride) - 1;
+        for (Wide k = from > t.least ? from : t.least; k <= (to < t.most ? to : t.most) && ways > 0; ++k)
+            if (meets(i + 1, at + k * t.stride)) return true;
+        return false;
+    }
+
+public:
+    bool found = false;
+    SharedMemory(const adhip_array& a, const adhip_array& b) {
+        const int64_t aw = type_bytes(a.type), bw = type_bytes(b.type);
+        for (const adhip_array* x : {&a, &b})
+            for (int d = 0; d < x->rank; ++d)
+                if (x->dims[d] == 0) return;
+        const Wide at = (Wide)(uintptr_t)b.data - (Wide)(uintptr_t)a.data;
+        above = a.dims[a.rank - 1] * aw, below = -(Wide)(b.dims[b.rank - 1] * bw);
+        if (at >= reach(a) * aw || -at >= reach(b) * bw) return;  // (as a rule)
+        for (int d = 0; d + 1 < b.rank; ++d)
+            if (b.dims[d] > 1) add(b.strides[d] * bw, 0, b.dims[d] - 1);
+        for (int d = 0; d + 1 < a.rank; ++d)
+            if (a.dims[d] > 1) add(a.strides[d] * aw, 1 - a.dims[d], 0);
+        found = meets(0, at);
+    }
+};
+
+// What may be written where it is read, element by element, or apart from it: an input and an output of one shape and type.
+inline void check_in_place(const char* op, const char* in_name, const adhip_array& in, const char* out_name, const adhip_array& out) {
+    bool same = in.data == out.data;
+    for (int d = 0; d < in.rank; ++d) same = same && (in.strides[d] == out.strides[d] || in.dims[d] <= 1);
+    ADHIP_CHECK(same || !SharedMemory(in, out).found, "%s: %s and %s share memory, but not element by element", op, out_name, in_name);
+}
+
+// Two outputs.
+inline void check_apart(const char* op, const char* a_name, const adhip_array& a, const char* b_name, const adhip_array& b) {
+    ADHIP_CHECK(!SharedMemory(a, b).found, "%s: %s and %s share memory", op, a_name, b_name);
+}
+
 // The largest power of two, at most `most`, that divides an array's address and all its strides but the last (extents of
 // one aside), in elements: how many elements a lane may take at once from a multiple of it.
 inline int vector_elements(const adhip_array& a, int most) {

@@ -267,7 +267,7 @@ int adhip_attention_backward(adhip_ctx* ctx, const adhip_attention_args* args, v
  *     out = (t - mean) root weight + bias
  * weight and bias [size] are f32 or of x's type, both alike; no weight is a weight of 1, no bias a bias of 0.  Not centered and
  * without a bias it is RMS norm.  stats (f32, x's leading dims and 2, packed, aligned to 8 bytes; may be left out) receives mean and root.  total and out
- * may be x or added themselves, under the same strides (out and total are two arrays). */
+ * may be x or added themselves, under the same strides; otherwise they share no memory with these, nor with one another. */
 typedef struct adhip_layer_norm_args {
     adhip_array x, added, total, out, weight, bias, stats;
     /* backward only */
@@ -282,7 +282,7 @@ int adhip_layer_norm_workspace(adhip_ctx* ctx, const adhip_layer_norm_args* args
 int adhip_layer_norm(adhip_ctx* ctx, const adhip_layer_norm_args* args, void* stream);
 /* Gradients, from x (what was normed: `total` where something was added), stats, weight and the gradient of out.  x_grad is that of t;
  * total_grad (may be left out), a gradient that reaches t by another way, is added to it.  Where something was added x_grad is the gradient of both x and
- * added.  x_grad may be out_grad, total_grad or x itself, under the same strides.  weight_grad and bias_grad ([size], f32 or bf16, each may be left out)
+ * added.  x_grad may be out_grad, total_grad or x itself, under the same strides; otherwise it shares no memory with them.  weight_grad and bias_grad ([size], f32 or bf16, each may be left out)
  * are sums over all rows in 32 bits, added in an order that only the shape decides; with either a workspace of
  * adhip_layer_norm_workspace() bytes, aligned to 16, is used until the call's kernels are done.  The two share no memory; one array
  * given for both holds bias_grad alone.  added, total, out and bias are not looked at. */
