@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 namespace adhip {
 namespace {
@@ -942,6 +943,27 @@ int64_t check_state(const char* op, const char* name, const adhip_array& a, cons
     return a.strides[0];
 }
 
+// What is written takes the place of an input, element by element, or shares no memory with any.
+void check_shared(const char* op, const adhip_recurrence_args& g, bool backward) {
+    const auto in_place = [&](const char* in_name, const adhip_array& in, const char* out_name, const adhip_array& out) {
+        if (in.data && out.data) check_in_place(op, in_name, in, out_name, out);
+    };
+    if (backward) {
+        ADHIP_CHECK(g.x.dims[1] == 0 || g.x_grad.data != g.gates_grad.data, "%s: x_grad and gates_grad are one array", op);
+        for (const auto& [out_name, out] : {std::pair("x_grad", &g.x_grad), std::pair("gates_grad", &g.gates_grad)}) {
+            in_place("x", g.x, out_name, *out);
+            in_place("gates", g.gates, out_name, *out);
+            in_place("out_grad", g.out_grad, out_name, *out);
+        }
+        check_apart(op, "x_grad", g.x_grad, "gates_grad", g.gates_grad);
+        in_place("final_grad", g.final_grad, "initial_grad", g.initial_grad);
+    } else {
+        in_place("x", g.x, "out", g.out);
+        in_place("gates", g.gates, "out", g.out);
+        in_place("initial", g.initial, "final", g.final);
+    }
+}
+
 void recurrence(const char* op, const adhip_recurrence_args& g, bool backward, hipStream_t stream) {
     check_x(op, g.x);
     const int64_t batch = g.x.dims[0], length = g.x.dims[1], channels = g.x.dims[2];
@@ -1007,6 +1029,7 @@ void recurrence(const char* op, const adhip_recurrence_args& g, bool backward, h
         const int64_t v = 4 / type_bytes(g.x.type), lanes = batch * ((channels + v - 1) / v);
         ADHIP_CHECK(fits_launch((lanes + 255) / 256, 256), "%s: %lld sequences of %lld channels are too many for one call", op, (long long)batch, (long long)channels);
         if (lanes == 0) return;
+        check_shared(op, g, backward);
         launch(op, g.x.type == ADHIP_BF16 ? (factors ? recurrence_step_kernel<bf16, true> : recurrence_step_kernel<bf16, false>)
                                           : (factors ? recurrence_step_kernel<float, true> : recurrence_step_kernel<float, false>),
                (unsigned)((lanes + 255) / 256), 256, stream, p);
@@ -1016,7 +1039,7 @@ void recurrence(const char* op, const adhip_recurrence_args& g, bool backward, h
     if (blocks == 0) return;
     ADHIP_CHECK(cut.workspace(g.x) == 0 || (g.workspace && (uintptr_t)g.workspace % 16 == 0 && g.workspace_bytes >= cut.workspace(g.x)),
                 "%s: the workspace has %zu bytes, %zu are wanted, aligned to 16", op, g.workspace ? g.workspace_bytes : (size_t)0, cut.workspace(g.x));
-    ADHIP_CHECK(!backward || length == 0 || g.x_grad.data != g.gates_grad.data, "%s: x_grad and gates_grad are one array", op);
+    check_shared(op, g, backward);
     p.carry = (float2*)g.workspace;
     if (g.x.type == ADHIP_BF16 && wide) launch_recurrence<bf16, kWide>(op, p, backward, factors, stream);
     else if (g.x.type == ADHIP_BF16) launch_recurrence<bf16, kNarrow>(op, p, backward, factors, stream);

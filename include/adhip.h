@@ -300,7 +300,8 @@ int adhip_layer_norm_backward(adhip_ctx* ctx, const adhip_layer_norm_args* args,
  * that is.  Factors are multiplied over runs of positions: where such a product passes 2^128, results may be infinite or NaN up to the next factor of 0
  * or document.
  * states (f32 [batch, ceil(length / 256), channels]; may be left out) receives the state before every 256th position, for the
- * backward pass.  out may be x or gates themselves, under the same strides.
+ * backward pass.  out may be x or gates themselves, under the same strides; otherwise it shares no memory with them, nor final
+ * with initial.
  * Positions lie at most 2^21 elements apart.
  * workspace: adhip_recurrence_workspace() bytes, aligned to 16, used until the call's kernels are done; may be left out where that is 0. */
 #define ADHIP_RECURRENCE_BLOCK 256
@@ -317,7 +318,8 @@ int adhip_recurrence_workspace(adhip_ctx* ctx, const adhip_recurrence_args* args
 int adhip_recurrence(adhip_ctx* ctx, const adhip_recurrence_args* args, void* stream);
 /* Gradients of x, gates and, where asked for, initial, from x, gates, the forward call's states, the gradient of out and, where it
  * is given, that of final ([batch, channels]); lengths, documents and factors as there.  x_grad and gates_grad may be x, gates or out_grad
- * themselves, under the same strides, and initial_grad may be final_grad itself (a gradient that is carried from call to call).
+ * themselves, under the same strides, and initial_grad may be final_grad itself (a gradient that is carried from call to call);
+ * otherwise they share no memory with these, nor x_grad and gates_grad with one another.
  * out, initial and final are not looked at.  The order of additions is fixed. */
 int adhip_recurrence_backward(adhip_ctx* ctx, const adhip_recurrence_args* args, void* stream);
 

@@ -82,3 +82,35 @@ def test_arrays_that_reach_far(dev):  # noqa: F811
     ops.layer_norm(dev, x, Array(1 << 20, 3, 64, stride=(1 << 38, 64, 1), at=(1 << 40) + 4 * 192))
     assert len(dev.launches()) == 2
     refused(dev, "share memory", ops.layer_norm, x, Array(1 << 20, 3, 64, stride=(1 << 38, 64, 1), at=(1 << 40) + 4 * ((1 << 57) + 191)))
+
+
+def test_recurrences_that_share_memory(dev):  # noqa: F811
+    one = lambda at, stride=(12000, 40, 1): Array(3, 300, 40, stride=stride, at=4096 + 4 * at)  # noqa: E731
+    state = lambda at, stride=(40, 1): Array(3, 40, stride=stride, at=4096 + 4 * at)  # noqa: E731
+    x, far, apart, wide = one(0), one(100000), one(200000), (24000, 80, 1)
+    for where in (one(40), one(-39), one(12000), one(0, wide), one(36000 - 1)):
+        refused(dev, "out and x share memory", ops.recurrence, x, far, where)
+        refused(dev, "out and gates share memory", ops.recurrence, far, x, where)
+        backward = lambda *a: refused(dev, f"{a[0]} share memory", ops.recurrence_backward, a[1], a[2], Array(3, 2, 40), *a[3:])  # noqa: E731
+        backward("x_grad and x", x, far, far, where, apart)
+        backward("x_grad and gates", far, x, far, where, apart)
+        backward("x_grad and out_grad", far, far, x, where, apart)
+        backward("gates_grad and x", x, far, far, apart, where)
+        backward("gates_grad and gates", far, x, far, apart, where)
+        backward("gates_grad and out_grad", far, far, x, apart, where)
+        if where.data_ptr() != x.data_ptr():
+            backward("x_grad and gates_grad", far, far, far, x, where)
+    backward("x_grad and gates_grad", far, far, far, one(0, wide), one(80 * 299 + 39))
+    for L in (300, 4):
+        y = Array(3, L, 40, at=1 << 30)
+        for where in (state(40), state(-1), state(0, (80, 1))):
+            refused(dev, "final and initial share memory", ops.recurrence, y, y, y, initial=state(0), final=where)
+            refused(dev, "initial_grad and final_grad share memory", ops.recurrence_backward, y, y, Array(3, -(-L // 256), 40), y, y,
+                    Array(3, L, 40, at=1 << 40), final_grad=state(0), initial_grad=where)
+    refused(dev, "out and x share memory", ops.recurrence, Array(3, 1, 40), far.__class__(3, 1, 40, at=1 << 30), Array(3, 1, 40, at=4096 + 4 * 40))
+    # halves of one array of gradients, and the ones of inputs that lie like that
+    left, right = one(0, wide), one(40, wide)
+    ops.recurrence(dev, left, right, left)
+    ops.recurrence_backward(dev, far, far, Array(3, 2, 40), far, left, right)
+    ops.recurrence_backward(dev, left, right, Array(3, 2, 40), far, right, left, final_grad=state(1 << 20), initial_grad=state((1 << 20) + 120))
+    assert len(dev.launches()) == 3
