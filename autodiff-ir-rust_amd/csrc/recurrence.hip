@@ -930,7 +930,7 @@ Rows check_like(const char* op, const char* name, const adhip_array& a, const ad
     check_dims(op, name, a, {x.dims[0], x.dims[1], x.dims[2]});
     check_packed_rows(op, name, a);
     if (output) check_distinct(op, name, a);
-    return {a.strides[0], a.strides[1]};
+    return {a.strides[0], a.dims[1] > 1 ? a.strides[1] : 0};  // (one position alone is not apart from any)
 }
 
 // f32 [batch, channels], which need not be given.

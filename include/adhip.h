@@ -302,7 +302,7 @@ int adhip_layer_norm_backward(adhip_ctx* ctx, const adhip_layer_norm_args* args,
  * states (f32 [batch, ceil(length / 256), channels]; may be left out) receives the state before every 256th position, for the
  * backward pass.  out may be x or gates themselves, under the same strides; otherwise it shares no memory with them, nor final
  * with initial.
- * Positions lie at most 2^21 elements apart.
+ * Positions, where there are two and more, lie at most 2^21 elements apart.
  * workspace: adhip_recurrence_workspace() bytes, aligned to 16, used until the call's kernels are done; may be left out where that is 0. */
 #define ADHIP_RECURRENCE_BLOCK 256
 typedef struct adhip_recurrence_args {

@@ -34,7 +34,7 @@ def run(dev, a, *, factors=False, in_place=False):
     """Both passes; with `in_place` the state and its gradient are carried in one array each."""
     x, (B, L, C) = a["x"], a["x"].shape
     new = lambda *s: torch.full(s, 7.0)  # noqa: E731
-    r = {n: torch.full_like(x, 7.0) for n in ("out", "x_grad", "gates_grad")} | {"states": new(B, ops.recurrence_blocks(L), C)}
+    r = {n: torch.full_like(x, 7.0).as_strided(x.shape, x.stride()) for n in ("out", "x_grad", "gates_grad")} | {"states": new(B, ops.recurrence_blocks(L), C)}
     initial, final_grad = a["initial"].clone(), a["final_grad"].clone()
     r["final"], r["initial_grad"] = (initial, final_grad) if in_place else (new(B, C), new(B, C))
     h = {n: host.seen(t) for n, t in {**a, **r, "initial": initial, "final_grad": final_grad}.items()}
@@ -72,3 +72,14 @@ def test_states_and_their_gradients_are_carried_in_place(dev, B, L, C, masked, f
     for carried in dev.in_both_orders(lambda: run(dev, a, factors=factors, in_place=True)):
         for n in apart:
             assert torch.equal(apart[n], carried[n]), n
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_position_has_no_distance_to_speak_of(dev, dtype):
+    """One token of arrays that have all sequences of a position beside one another, however many those are."""
+    a = inputs(3, 1, 40, dtype)
+    want = run(dev, a)
+    for n in ("x", "gates", "out_grad"):
+        a[n] = a[n].as_strided((3, 1, 40), (40, 1 << 40, 1))
+    got = run(dev, a)
+    assert all(torch.equal(got[n], want[n]) for n in want)
