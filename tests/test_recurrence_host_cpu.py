@@ -83,3 +83,33 @@ def test_one_position_has_no_distance_to_speak_of(dev, dtype):
         a[n] = a[n].as_strided((3, 1, 40), (40, 1 << 40, 1))
     got = run(dev, a)
     assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("factors", [False, True])
+@pytest.mark.parametrize("L,C", [(L, C) for L in (4, 300, 1100) for C in (33, 35)])
+def test_channels_that_fill_no_pack_in_place(dev, L, C, factors):
+    """The last pack of a row that begins before its place, and a last channel alone in its workgroup."""
+    a = inputs(2, L, C, "bf16", factors=factors)
+    want = run(dev, a, factors=factors)
+
+    def forward(to):
+        g = {n: None if t is None else t.clone() for n, t in a.items()}
+        h = {n: host.seen(t) for n, t in g.items()}
+        ops.recurrence(dev, h["x"], h["gates"], h[to], factors=factors, initial=h["initial"], final=h["initial"], stream=0,
+                       workspace=host.room(ops.recurrence_workspace(dev, h["x"])))
+        return g[to], g["initial"]
+
+    def backward(to):
+        g = {n: None if t is None else t.clone() for n, t in a.items()}
+        h = {n: host.seen(t) for n, t in g.items()}
+        ops.recurrence_backward(dev, h["x"], h["gates"], host.seen(want["states"]), h["out_grad"], h[to[0]], h[to[1]], factors=factors,
+                                final_grad=h["final_grad"], initial_grad=h["final_grad"], stream=0,
+                                workspace=host.room(ops.recurrence_workspace(dev, h["x"], backward=True)))
+        return g[to[0]], g[to[1]], g["final_grad"]
+
+    for to in ("x", "gates"):
+        for out, final in dev.in_both_orders(lambda: forward(to)):
+            assert torch.equal(out, want["out"]) and torch.equal(final, want["final"])
+    for to in (("x", "gates"), ("out_grad", "x"), ("gates", "out_grad")):
+        for got in dev.in_both_orders(lambda: backward(to)):
+            assert all(torch.equal(g, want[n]) for g, n in zip(got, ("x_grad", "gates_grad", "initial_grad")))
