@@ -30,7 +30,7 @@ struct GradientLaunch {
     void* out[kTensors];
     int64_t count[kTensors];
     unsigned first[kTensors + 1];                            // the workgroup that begins each tensor
-    unsigned bf16s[kTensors / 32], aligned[kTensors / 32];   // bit i: tensor i is bf16; it can be read 16 bytes at once
+    unsigned bf16s[kTensors / 32];                           // bit i: tensor i is bf16
     int n;
     float grad_scale;
     const float* factor;
@@ -67,26 +67,26 @@ __device__ __forceinline__ int tensor_of(const GradientLaunch& a, unsigned block
     return lo;
 }
 
-// THREADS with consecutive numbers share a chunk.
-template <class T, int V, int THREADS>
+// THREADS with consecutive numbers share a chunk, in packs of 16 bytes that begin at any element: the address, which for views of odd sizes in one
+// buffer is anything, decides over no bit (38 M in bf16 off an aligned address: clipped in 47 us as aligned, and 61 by single elements).
+template <class T, int THREADS>
 __device__ __forceinline__ double square_chunk(const T* g, int64_t begin, int64_t end) {
+    constexpr int V = 16 / sizeof(T);
     double s[2] = {0, 0};
     int64_t i = begin + (int64_t)(threadIdx.x % THREADS) * V;
-    if (V > 1) {
-        // whole packs, four of them under way
-        constexpr int U = 4;
-        for (; i + (U - 1) * THREADS * V + V <= end; i += U * THREADS * V) {
-            Pack<T, V> r[U];
+    // whole packs, four of them under way
+    constexpr int U = 4;
+    for (; i + (U - 1) * THREADS * V + V <= end; i += U * THREADS * V) {
+        Loose<T, V> r[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) r[u] = *(const Pack<T, V>*)(g + i + u * THREADS * V);
+        for (int u = 0; u < U; ++u) r[u] = *(const Loose<T, V>*)(g + i + u * THREADS * V);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const double x = (float)r[u].v[k];
-                    s[k & 1] = __builtin_fma(x, x, s[k & 1]);
-                }
-        }
+            for (int k = 0; k < V; ++k) {
+                const double x = (float)r[u].v[k];
+                s[k & 1] = __builtin_fma(x, x, s[k & 1]);
+            }
     }
     for (; i < end; i += THREADS * V)
 #pragma unroll
@@ -98,17 +98,12 @@ __device__ __forceinline__ double square_chunk(const T* g, int64_t begin, int64_
     return s[0] + s[1];
 }
 
-template <class T, int THREADS>
-__device__ __forceinline__ double squares(const void* g, int64_t begin, int64_t end, bool aligned) {
-    return aligned ? square_chunk<T, 16 / sizeof(T), THREADS>((const T*)g, begin, end) : square_chunk<T, 1, THREADS>((const T*)g, begin, end);
-}
-
 template <int THREADS, int CHUNK>
 __device__ __forceinline__ double squares_of(const GradientLaunch& a, unsigned chunk) {
     const int t = tensor_of(a, chunk);
     const int64_t begin = (int64_t)(chunk - a.first[t]) * CHUNK, end = min(begin + CHUNK, a.count[t]);
-    const bool aligned = a.aligned[t >> 5] >> (t & 31) & 1;
-    return a.bf16s[t >> 5] >> (t & 31) & 1 ? squares<bf16, THREADS>(a.g[t], begin, end, aligned) : squares<float, THREADS>(a.g[t], begin, end, aligned);
+    return a.bf16s[t >> 5] >> (t & 31) & 1 ? square_chunk<bf16, THREADS>((const bf16*)a.g[t], begin, end)
+                                           : square_chunk<float, THREADS>((const float*)a.g[t], begin, end);
 }
 
 __global__ __launch_bounds__(kThreads) void gradient_squares_kernel(const GradientLaunch a) {
@@ -142,22 +137,23 @@ __global__ __launch_bounds__(kFinish) void gradient_norm_kernel(const double* pa
 }
 
 // PAST: written past the caches, which hold what is read again instead.
-template <class T, int V, int THREADS, bool PAST>
+template <class T, int THREADS, bool PAST>
 __device__ __forceinline__ void scale_chunk(const T* g, T* out, int64_t begin, int64_t end, float scale) {
+    constexpr int V = 16 / sizeof(T);
     int64_t i = begin + (int64_t)(threadIdx.x % THREADS) * V;
-    if constexpr (V > 1) {
-        constexpr int U = 4;
-        for (; i + (U - 1) * THREADS * V + V <= end; i += U * THREADS * V) {
-            Pack<T, V> r[U];
+    constexpr int U = 4;
+    for (; i + (U - 1) * THREADS * V + V <= end; i += U * THREADS * V) {
+        Loose<T, V> r[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) r[u] = *(const Pack<T, V>*)(g + i + u * THREADS * V);
+        for (int u = 0; u < U; ++u) r[u] = *(const Loose<T, V>*)(g + i + u * THREADS * V);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int k = 0; k < V; ++k) r[u].v[k] = (T)((float)r[u].v[k] * scale);
-                if (PAST) store_past((Word16*)(out + i + u * THREADS * V), *(const Word16*)&r[u]);
-                else *(Pack<T, V>*)(out + i + u * THREADS * V) = r[u];
-            }
+            for (int k = 0; k < V; ++k) r[u].v[k] = (T)((float)r[u].v[k] * scale);
+            Word16 w;  // (as one store of 16 bytes)
+            __builtin_memcpy(&w, &r[u], sizeof w);
+            if (PAST) store_past((Word16*)(out + i + u * THREADS * V), w);
+            else *(Word16*)(out + i + u * THREADS * V) = w;
         }
     }
     for (; i < end; i += THREADS * V)
@@ -166,21 +162,14 @@ __device__ __forceinline__ void scale_chunk(const T* g, T* out, int64_t begin, i
             if (i + k < end) out[i + k] = (T)((float)g[i + k] * scale);
 }
 
-template <class T, int THREADS, bool PAST>
-__device__ __forceinline__ void scaled(const void* g, void* out, int64_t begin, int64_t end, bool aligned, float scale) {
-    if (aligned) scale_chunk<T, 16 / sizeof(T), THREADS, PAST>((const T*)g, (T*)out, begin, end, scale);
-    else scale_chunk<T, 1, THREADS, false>((const T*)g, (T*)out, begin, end, scale);
-}
-
 template <int THREADS, int CHUNK, bool PAST>
 __device__ __forceinline__ void scale_of(const GradientLaunch& a, unsigned chunk, float scale) {
     const int t = tensor_of(a, chunk);
     // in place, a scale of one leaves every number as it is
     if (scale == 1.f && a.out[t] == a.g[t]) return;
     const int64_t begin = (int64_t)(chunk - a.first[t]) * CHUNK, end = min(begin + CHUNK, a.count[t]);
-    const bool aligned = a.aligned[t >> 5] >> (t & 31) & 1;
-    if (a.bf16s[t >> 5] >> (t & 31) & 1) scaled<bf16, THREADS, PAST>(a.g[t], a.out[t], begin, end, aligned, scale);
-    else scaled<float, THREADS, PAST>(a.g[t], a.out[t], begin, end, aligned, scale);
+    if (a.bf16s[t >> 5] >> (t & 31) & 1) scale_chunk<bf16, THREADS, PAST>((const bf16*)a.g[t], (bf16*)a.out[t], begin, end, scale);
+    else scale_chunk<float, THREADS, PAST>((const float*)a.g[t], (float*)a.out[t], begin, end, scale);
 }
 
 template <bool PAST>
@@ -269,7 +258,7 @@ void gradients(const char* op, const adhip_gradients_args& g, bool clip, hipStre
             a.partial += a.first[a.n];
             a.n = 0;
             a.first[0] = 0;
-            for (int k = 0; k < kTensors / 32; ++k) a.bf16s[k] = a.aligned[k] = 0;
+            for (unsigned& bits : a.bf16s) bits = 0;
         };
         for (int64_t i = 0; i < g.n_tensors; ++i) {
             const adhip_gradient& t = g.tensors[i];
@@ -281,7 +270,6 @@ void gradients(const char* op, const adhip_gradients_args& g, bool clip, hipStre
                 a.out[a.n] = clip ? (char*)t.out + at * width : nullptr;
                 a.count[a.n] = std::min(t.count - at, own * chunk);
                 if (t.type == ADHIP_BF16) a.bf16s[a.n >> 5] |= 1u << (a.n & 31);
-                if ((uintptr_t)t.g % 16 == 0 && (!clip || (uintptr_t)t.out % 16 == 0)) a.aligned[a.n >> 5] |= 1u << (a.n & 31);
                 at += own * chunk;
                 ++a.n;
                 a.first[a.n] = a.first[a.n - 1] + (unsigned)own;

@@ -51,12 +51,6 @@ struct RowIndex {
     __device__ __forceinline__ int64_t at(const Place& p) const { return i0 * p.s[0] + i1 * p.s[1] + i2 * p.s[2]; }
 };
 
-// 16 bytes that begin at any element: global memory takes such accesses, at the cost of one more line where they cross one.
-template <class T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) Loose {
-    T v[N];
-};
-
 // Where a pack of V elements that begins at `at` lies.  In rows that do not fill their lanes (FULL) one that would pass the end is moved
 // back to it: its first `skip` elements belong to another lane, all V to a lane behind the end.  So every lane makes the same loads, with
 // no branch between them, and rows of at least V elements are wanted.

@@ -196,6 +196,12 @@ struct __attribute__((aligned(sizeof(T) * N))) Pack {
     T v[N];
 };
 
+// 16 bytes that begin at any element: global memory takes such accesses, at the cost of one more line where they cross one.
+template <class T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+    T v[N];
+};
+
 // 4, 8 and 16 bytes written past the caches, to addresses that are aligned to two.
 typedef unsigned Word4 __attribute__((aligned(2)));
 typedef unsigned Word8 __attribute__((ext_vector_type(2), aligned(2)));

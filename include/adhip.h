@@ -200,7 +200,7 @@ int adhip_adamw_scaled(adhip_ctx* ctx, const adhip_adamw_args* args, const float
 
 /* The norm over all gradients of a step, and clipping by it.
  *     norm = |grad_scale| sqrt(sum over all tensors of g g),    factor = 1 where norm <= limit, limit / norm otherwise
- * with the sum in 64 bits, added in an order that only the tensors' sizes, types and alignment decide.  norm and factor are f32 numbers in device memory
+ * with the sum in 64 bits, added in an order that only the tensors' sizes and types decide.  norm and factor are f32 numbers in device memory
  * (factor may be NULL).  adhip_clip_gradients also writes  out = g (grad_scale factor)  of each tensor, rounded once; `out`
  * may be `g` itself; otherwise it shares memory with no gradient and no other `out`.  A gradient that is not finite shows: a NaN makes norm, factor and every clipped gradient NaN; an infinity
  * makes the norm infinite and, under a finite limit, the factor 0 (and itself NaN).  Gradients are ADHIP_F32 or ADHIP_BF16,

@@ -165,6 +165,10 @@ inline float __shfl_xor(float x, int off) {
     const int* all = host_hip::exchange(__builtin_bit_cast(int, x));
     return __builtin_bit_cast(float, all[(threadIdx.x & 63) ^ off]);
 }
+inline double __shfl_xor(double x, int off) {
+    const uint64_t w = __builtin_bit_cast(uint64_t, x), low = (unsigned)host_hip::exchange((int)w)[(threadIdx.x & 63) ^ off];
+    return __builtin_bit_cast(double, low | (uint64_t)(unsigned)host_hip::exchange((int)(w >> 32))[(threadIdx.x & 63) ^ off] << 32);
+}
 inline int atomicMin(int* a, int x) { const int was = *a; *a = x < was ? x : was; return was; }
 inline int atomicMax(int* a, int x) { const int was = *a; *a = x > was ? x : was; return was; }
 template <class T>

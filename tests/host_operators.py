@@ -61,6 +61,12 @@ class HostArray:
     def data_ptr(self):
         return self.t.data_ptr()
 
+    def numel(self):
+        return self.t.numel()
+
+    def is_contiguous(self):
+        return self.t.is_contiguous()
+
 
 def build(work, *names):
     """A device whose operators are those of csrc/<name>.hip."""
