@@ -51,6 +51,8 @@ class DecoderLayer:
             raise ValueError(f"target is {list(target.shape)}, x {list(x.shape)}")
         if not clip >= 0.0:
             raise ValueError(f"clip {clip}: a limit above zero is wanted, or 0 for none")
+        if documents is not None:
+            documents = ops._host_values(documents, "int32").reshape(batch, length)
         rows = batch * length
         self.dev, self.rate, self.decay, self.clip, self.steps = dev, rate, decay, clip, 0
         rng = np.random.default_rng(seed)
@@ -97,7 +99,7 @@ class DecoderLayer:
             self.arrays[n] = ops.program_array(self.weigh, t.val().id)
 
         a = self.arrays
-        self.documents = None if documents is None else ops.DeviceArray.of(dev, np.asarray(documents, np.int32).reshape(batch, length))
+        self.documents = None if documents is None else ops.DeviceArray.of(dev, documents)
         self.norm = norm
         if norm:
             # the mixed positions as they are normed, and the gradient that comes back through the norm
