@@ -518,7 +518,7 @@ def recurrence_blocks(length: int) -> int:
 
 
 def recurrence_workspace(dev, x, *, backward: bool = False) -> int:
-    """Bytes of workspace that `recurrence`, and with `backward` also `recurrence_backward`, take on arrays of x's shape."""
+    """Bytes of workspace that `recurrence` and `recurrence_backward` take on arrays of x's shape: one size serves both, whatever `backward` is."""
     need = ctypes.c_size_t()
     args = _array(x, True) + _RECURRENCE_X
     _check(dev, _lib(dev).adhip_recurrence_workspace(dev._ctx, args, bool(backward), ctypes.byref(need)), "adhip_recurrence_workspace")

@@ -481,7 +481,7 @@ int64_t check_rows(const char* op, const adhip_array& x) {
     return rows;
 }
 
-void check_vector(const char* op, const char* name, const adhip_array& a, int64_t size, bool output) {
+void check_vector(const char* op, const char* name, const adhip_array& a, int64_t size) {
     ADHIP_CHECK(a.type == ADHIP_F32 || a.type == ADHIP_BF16, "%s: %s is %s, f32 or bf16 is wanted", op, name, type_name(a.type));
     check_array(op, name, a, a.type, 1);
     check_dims(op, name, a, {size});
@@ -521,8 +521,8 @@ void layer_norm(const char* op, const adhip_layer_norm_args& g, bool backward, h
         }
     // weights: of x's type or f32, both alike
     const int w_type = g.weight.data ? g.weight.type : g.bias.data && !backward ? g.bias.type : ADHIP_F32;
-    if (g.weight.data) check_vector(op, "weight", g.weight, size, false);
-    if (g.bias.data && !backward) check_vector(op, "bias", g.bias, size, false);
+    if (g.weight.data) check_vector(op, "weight", g.weight, size);
+    if (g.bias.data && !backward) check_vector(op, "bias", g.bias, size);
     ADHIP_CHECK(w_type == ADHIP_F32 || w_type == g.x.type, "%s: weight and bias are %s, f32 or the type of x is wanted", op, type_name(w_type));
     ADHIP_CHECK(backward || !g.weight.data || !g.bias.data || g.weight.type == g.bias.type, "%s: weight is %s and bias %s, one type is wanted", op,
                 type_name(g.weight.type), type_name(g.bias.type));
@@ -540,8 +540,8 @@ void layer_norm(const char* op, const adhip_layer_norm_args& g, bool backward, h
     const bool sums = backward && (g.weight_grad.data || g.bias_grad.data);
     bool one_sum = false;  // one array for both holds bias_grad: nobody writes weight_grad there before or after it
     if (backward) {
-        if (g.weight_grad.data) check_vector(op, "weight_grad", g.weight_grad, size, true);
-        if (g.bias_grad.data) check_vector(op, "bias_grad", g.bias_grad, size, true);
+        if (g.weight_grad.data) check_vector(op, "weight_grad", g.weight_grad, size);
+        if (g.bias_grad.data) check_vector(op, "bias_grad", g.bias_grad, size);
         if (g.weight_grad.data && g.bias_grad.data) {
             const char *w = (const char*)g.weight_grad.data, *b = (const char*)g.bias_grad.data;
             one_sum = w == b && g.weight_grad.type == g.bias_grad.type;

@@ -313,7 +313,7 @@ typedef struct adhip_recurrence_args {
     void* workspace;
     size_t workspace_bytes;
 } adhip_recurrence_args;
-/* Only the shape and type of x are looked at. */
+/* Only the shape and type of x are looked at; one size serves both passes, whatever `backward` is. */
 int adhip_recurrence_workspace(adhip_ctx* ctx, const adhip_recurrence_args* args, int backward, size_t* bytes);
 int adhip_recurrence(adhip_ctx* ctx, const adhip_recurrence_args* args, void* stream);
 /* Gradients of x, gates and, where asked for, initial, from x, gates, the forward call's states, the gradient of out and, where it
