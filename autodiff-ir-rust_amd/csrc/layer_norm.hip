@@ -3,11 +3,11 @@
 //
 // Memory bounds it: a row is read once, stays in the registers of the lanes that share it (16 of them, or 1 to 16 whole wavefronts, up to 16
 // elements each), and its results are written once.  Mean and squared deviations are two sums one after the other over those
-// registers, so a mean that is large against the deviations costs no bits.  In the backward pass a lane keeps the same columns of all
+// registers, so a mean that is large against the deviations costs them its own rounding alone.  In the backward pass a lane keeps the same columns of all
 // rows that it meets, so the weights' gradients add up in its registers; a workgroup adds its lanes' sums in LDS, and a small second
 // kernel the workgroups', always in the same order.
-// 16384 rows of 4096 in bf16 with a residual: forward 92 us (5.9 TB/s), backward 107 (5.0) and 5 for the last sums; 131072 rows of 128: 12.5, 18.1
-// and 3.9; 3001 rows of 1023 in f32 with a residual: 10.8, 14.6 and 3.8.  Results past the caches gain nothing here.
+// 16384 rows of 4096 in bf16 with a residual: forward 92 us (5.9 TB/s), backward 107 (5.0) and 5 for the last sums; 131072 rows of 128: 15, 19
+// and 4; 3001 rows of 1023 in f32 with a residual: 14.5, 15.7 and 3.8, and 10.8 and 14.6 from the last cache.  Results past the caches gain nothing here.
 #include "operators.hpp"
 
 #include <algorithm>

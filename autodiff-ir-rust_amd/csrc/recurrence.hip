@@ -11,10 +11,10 @@
 // states again: the forward pass leaves one every 256 positions, from which a tile of them is recomputed beside the gradients,
 // instead of reading all outputs, which are rounded.
 //
-// 2 x 8192 positions of 4096 channels in bf16: forward 108 us, backward 178 (3.8 TB/s; two arrays copied into a third in this pattern, 64 bytes of
-// rows 8 KB apart, take 107), of 4032 channels 90 and 151; 4 x 2048 of 4096 in f32, 128 bytes of a row: 80 and 134 (5.0 TB/s).  One position of
-// 256 x 8192 channels: 12 us.  A compute unit with one workgroup of wide rows is bound by its instructions: a tile of 256 positions of 64 channels
-// takes it 2.5 us.
+// 2 x 8192 positions of 4096 channels in bf16: forward 108 us, backward 179 (3.8 TB/s; in this pattern, 64 bytes of rows 8 KB apart, two
+// arrays copied into a third take 107, three into two 186), of 4032 channels 90 and 151; 4 x 2048 of 4096 in f32, 128 bytes of a row: 80 and 134 (5.0 TB/s).  One position of
+// 256 x 8192 channels: 12 us.  A compute unit with one workgroup of wide rows takes 5.0 us for a tile of 256 positions of 64 channels from memory and 4.1 from the last
+// cache (4 x 2049 of 2560 in bf16, factors: 45 and 37 us): its vector units issue 61 % of the latter's cycles, 25 instructions an element.
 #include "operators.hpp"
 
 #include <algorithm>
