@@ -113,7 +113,7 @@ class SharedMemory {
     struct Term {
         Wide stride, least, most;
     } terms[8];
-    int n = 0, ways = 1 << 16;
+    int n = 0, ways = 1 << 13;
     Wide below, above;  // rows meet at distances between the two
 
     void add(int64_t stride, int64_t least, int64_t most) {
